@@ -245,6 +245,127 @@ WARP_API int warp_moe_route(const float *logits, int T, int E, int K, int score_
 WARP_API int warp_rmsnorm(const float *x, const float *w, float *o, int rows, int n,
                           float eps, void *stream);
 
+/* ---- attention: rotary positions, paged keys and values ------------------------------
+ *
+ * The attention half of a decoder block, between the trunk matmul that makes
+ * q, k and v and the one that takes the result.  All strides count elements;
+ * the head_dim values of one (token, head) are contiguous. */
+
+typedef enum { WARP_T_F32 = 0, WARP_T_F16 = 1, WARP_T_BF16 = 2 } warp_type;
+
+/* Pages of keys and values: element (page, slot, head, d) of k is at
+ * k + page*k_page + slot*k_slot + head*k_head + d, and v alike, so pages may
+ * be laid out [slot][head] or [head][slot].  page_size is a power of two from
+ * 16 to 4096; type is WARP_T_F16 or WARP_T_BF16; base addresses and strides are
+ * multiples of 16 bytes.  Slot number n is slot n % page_size of page
+ * n / page_size. */
+typedef struct {
+    void *k, *v;
+    int type, page_size, kv_heads, head_dim;
+    int64_t pages;
+    int64_t k_page, k_slot, k_head;
+    int64_t v_page, v_slot, v_head;
+} warp_kv_pages;
+
+/* Queries and keys (and values) of `tokens` tokens on their way to attention:
+ *   - with q_norm / k_norm (fp32 [head_dim]; NULL for none) each head's row is
+ *     normed first, x * 1/sqrt(mean(x^2) + eps) * w;
+ *   - the first rot_dim dimensions are rotated: pair i by the angle
+ *     positions[t] * inv_freq[i] (inv_freq fp64 [rot_dim/2], radians a
+ *     position), where pair i is (i, i + rot_dim/2), or (2i, 2i+1) with
+ *     interleaved set; cos and sin are multiplied by rot_scale.  The angle is
+ *     reduced in 64 bits, so far positions lose nothing;
+ *   - the rest passes through.
+ * type is that of q, k and v, out_type that of the results: the same type, or
+ * any type when type is WARP_T_F32.  Arithmetic is fp32, rounded once.
+ * q_out [tokens][q_heads][head_dim] is contiguous; it may be q itself when
+ * the types and the layout agree, and so may k_out.  head_dim is even, 2..256,
+ * rot_dim even, 0..head_dim.  tokens 0 is no work. */
+typedef struct {
+    int tokens, q_heads, kv_heads, head_dim;
+    int type, out_type;
+    const void *q, *k, *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    void *q_out, *k_out;
+    const float *q_norm, *k_norm;
+    float eps;
+    const double *inv_freq;
+    int rot_dim, interleaved;
+    float rot_scale;
+    const int32_t *positions;
+} warp_rope_desc;
+
+/* Norm and rotation of q and k in one launch into q_out and k_out (q or k may
+ * be NULL with 0 heads).  v is not used. */
+WARP_API int warp_qk_norm_rope(const warp_rope_desc *d, void *stream);
+
+/* The same launch with the keys' results and the values written to the pages:
+ * token t's go to slot slots[t] (int64, device; a negative one stores
+ * nothing).  out_type is the pages' type; k_out is not used; q may be NULL
+ * with q_heads 0.  A slot past the pages is not written and is reported by
+ * warp_attn_status.  Two tokens with the same slot: one of them is stored. */
+WARP_API int warp_kv_append(const warp_rope_desc *d, const warp_kv_pages *c,
+                            const int64_t *slots, void *stream);
+
+/* The step's plan for warp_kv_append, made once for all layers.  Request b's
+ * new tokens are q_start[b]..q_start[b+1]-1 (int32 [batch+1]) and are the last
+ * of its kv_len[b] own keys (int32, the new ones counted); own key j is in
+ * slot j % page_size of page pages[b*pages_row + j / page_size].  Writes for
+ * token t positions[t] = base + j and slots[t]; base is the length of a prefix
+ * that the requests share (warp_paged_attention), else 0.  A token whose j is
+ * negative or past the row's pages_per_row pages gets slot -1, and so does one
+ * of no request. */
+WARP_API int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int batch, int tokens,
+                           const int32_t *pages, int64_t pages_row, int pages_per_row,
+                           int page_size, int base, int32_t *positions, int64_t *slots,
+                           void *stream);
+
+/* Attention of `tokens` queries over paged keys and values.
+ *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j
+ * Request b owns tokens q_start[b]..q_start[b+1]-1 and kv_len[b] keys in the
+ * pages of its row of the page table (as in warp_kv_slots); query head h reads
+ * kv head h / (q_heads / kv_heads).  With causal set, the i-th of the
+ * request's n queries sees own keys j <= kv_len - n + i; else all (cross
+ * attention to states of another length).  With prefix_len > 0 every query
+ * also sees the prefix_len keys of prefix_pages, before its own; where the
+ * requests' rows are few they are computed together, so that the prefix is
+ * read once for the batch.  A query that sees no key gets zeros, and what is
+ * in slots past a length (NaN, infinities) has no effect.
+ * type is that of q, out and the pages (WARP_T_F16 or WARP_T_BF16); head_dim
+ * is 64 or 128.  The products take their operands in that type and accumulate
+ * in fp32; softmax statistics are fp32, and its weights are rounded to `type`
+ * for the second product.  max_q and max_kv are host bounds on the requests'
+ * queries and own keys; what exceeds them, or a page number outside the pages,
+ * is left out and reported by warp_attn_status.
+ * scratch: warp_attn_scratch(d, c) bytes of device memory, 256-byte aligned,
+ * free again when the stream has passed the call.  No host synchronisation;
+ * capturable. */
+typedef struct {
+    int batch, tokens, q_heads, kv_heads, head_dim, type;
+    const void *q;
+    int64_t q_token, q_head;
+    void *out;                  /* [tokens][q_heads][head_dim], contiguous */
+    const int32_t *q_start, *kv_len;
+    const int32_t *pages;
+    int64_t pages_row;
+    int pages_per_row;
+    int max_q, max_kv;
+    int causal;
+    float scale;
+    const int32_t *prefix_pages;
+    int prefix_len;
+} warp_attn_desc;
+
+WARP_API int64_t warp_attn_scratch(const warp_attn_desc *d, const warp_kv_pages *c);
+WARP_API int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *c, void *scratch,
+                                  void *stream);
+
+/* What the kernels above left out since the last clear: WARP_OK, WARP_E_ARG
+ * (a slot or page number outside the pages, a length over its bound) or
+ * WARP_E_TIMEOUT (a bounded wait gave up; that launch's output is
+ * incomplete).  Synchronises the device; clear = 1 resets. */
+WARP_API int warp_attn_status(int clear);
+
 /* ---- resident MoE layer ---------------------------------------------------------- */
 
 typedef struct warp_moe_layer warp_moe_layer;

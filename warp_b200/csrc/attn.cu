@@ -1,0 +1,620 @@
+// attn.cu — attention over paged keys and values for few query rows a key
+// head: single-token decoding and short chunks.
+//
+// The rows of one CTA are 16 (token, head) pairs that read the same kv head,
+// so each key and value is read once for the heads that share it.  With few
+// rows a key the work is a stream of K and V at a handful of operations a
+// byte: bound by memory.  The running maximum m and sum l make one pass of it:
+//     m' = max(m, max_j x_j),  p_j = 2^(x_j - m'),
+//     l' = l 2^(m - m') + sum p_j,  o' = o 2^(m - m') + sum p_j v_j
+// with x = scale * log2(e) * q.k.  Key ranges are independent until they are
+// joined the same way, which is done for the warps of a CTA in shared memory
+// and for the parts of a long range by attn_join_kernel.
+//
+// Each warp streams its own tiles of 16 keys (every fourth of the CTA's range)
+// through a private ring of shared memory filled by cp.async, so the loop has
+// no barrier between warps.  Both products are mma.sync m16n8k16: S = Q K^T with Q held
+// in registers, then O += P V with the accumulators of S repacked as P.
+#include "attn.cuh"
+
+#include <math.h>
+
+namespace warp {
+
+constexpr int kADWarps = 4;
+constexpr int kADStages = 3;
+constexpr int kADRows = 16;
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4],
+                                                 uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
+                                                        uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// 16 bytes, or zeros where `live` is false (the source is then not read).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const uint32_t *)&h;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t *)&h;
+}
+
+template <typename T> struct F16Bits;
+template <> struct F16Bits<__half> { static constexpr uint32_t exp = 0x7c00u, one = 0x3c00u; };
+template <> struct F16Bits<__nv_bfloat16> { static constexpr uint32_t exp = 0x7f80u, one = 0x3f80u; };
+
+// A weight of zero does not hide a value that is not finite (0 * inf is NaN),
+// so where a tile holds keys that only some of its rows see, such values are
+// taken out of the B operand (b0, b1) and counted for each row by products of
+// the rows' visibility with indicators instead: what sees a NaN or both
+// infinities becomes NaN, what sees one infinity becomes it.
+template <typename T>
+__device__ __forceinline__ void mend_values(uint32_t &b0, uint32_t &b1, const uint32_t (&seen)[4],
+                                            float (&o)[4]) {
+    constexpr uint32_t E = F16Bits<T>::exp, one = F16Bits<T>::one;
+    const auto odd = [](uint32_t x) { return (x & E) == E || (x >> 16 & E) == E; };
+    if (!__any_sync(~0u, odd(b0) || odd(b1))) return;
+    float n_nan[4] = {}, n_pos[4] = {}, n_neg[4] = {};
+    uint32_t is[3][2] = {};
+    auto part = [&](uint32_t &b, int w) {
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+            const uint32_t x = b >> h & 0xffffu;
+            if ((x & E) != E) continue;
+            b &= ~(0xffffu << h);
+            is[(x & 0x7fffu) != E ? 0 : x >> 15 ? 2 : 1][w] |= one << h;
+        }
+    };
+    part(b0, 0);
+    part(b1, 1);
+    mma16816<T>(n_nan, seen, is[0][0], is[0][1]);
+    mma16816<T>(n_pos, seen, is[1][0], is[1][1]);
+    mma16816<T>(n_neg, seen, is[2][0], is[2][1]);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (n_pos[e] > 0.f) o[e] += INFINITY;
+        if (n_neg[e] > 0.f) o[e] -= INFINITY;
+        if (n_nan[e] > 0.f) o[e] = NAN;
+    }
+}
+
+// How many parts a range of `tiles` key tiles is split into, `each` tiles a part.
+__device__ __forceinline__ int attn_parts(int tiles, int each) {
+    return (tiles + each - 1) / each;
+}
+
+template <int D> struct ADLay {
+    static constexpr int row_bytes = D * 2;
+    static constexpr int tile_bytes = kAttnTile * row_bytes;
+    static constexpr int stage_bytes = 2 * tile_bytes;          // K, then V
+    static constexpr int warp_bytes = kADStages * stage_bytes;
+    static constexpr int ring = kADWarps * warp_bytes;
+    // the warps' results when the ring is done with: o [warp][16][D + 4], m and l
+    static constexpr int o_pitch = D + 4;
+    static constexpr int join = kADWarps * kADRows * (o_pitch + 2) * 4;
+    static constexpr int bytes = ring > join ? ring : join;
+};
+
+// PACKED: rows are those of all the batch's tokens, keys the shared prefix
+// (one "request" for the batch).  Otherwise rows and keys of one request, with
+// the prefix's keys in front where there is one that is not computed apart.
+template <typename T, int D, bool PACKED>
+__global__ void __launch_bounds__(kADWarps * 32, 2) attn_rows_kernel(const AttnArgs a) {
+    using Lay = ADLay<D>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int kvh = blockIdx.y;
+    AttnReq rq;
+    int part, row0, pre_tiles, own_tiles;
+    if (PACKED) {
+        rq = {0, a.tokens, 0};
+        part = blockIdx.x % a.prefix_parts;
+        row0 = (blockIdx.x / a.prefix_parts) * kADRows;
+    } else {
+        rq = attn_req(a, blockIdx.z);
+        const int tiles_max = (a.packed ? 0 : (a.prefix_len + kAttnTile - 1) / kAttnTile) +
+                              (a.max_kv + kAttnTile - 1) / kAttnTile;
+        const int parts_max = max(1, attn_parts(tiles_max, a.split_tiles));
+        part = blockIdx.x % parts_max;
+        row0 = (blockIdx.x / parts_max) * kADRows;
+    }
+    const int rows = rq.n * a.group;
+    if (row0 >= rows) return;
+    const int n_pre = PACKED || !a.packed ? a.prefix_len : 0;
+    pre_tiles = (n_pre + kAttnTile - 1) / kAttnTile;
+    // own keys that the tile's last row sees
+    const int last_row = min(rows, row0 + kADRows) - 1;
+    int own_seen = rq.len;
+    if (!PACKED && a.causal)
+        own_seen = max(0, min(rq.len, rq.len - rq.n + last_row / a.group + 1));
+    own_tiles = PACKED ? 0 : (own_seen + kAttnTile - 1) / kAttnTile;
+    // parts are counted by the request's keys, whatever a tile's rows see, so
+    // that the join knows their number
+    const int all_tiles = pre_tiles + (PACKED ? 0 : (rq.len + kAttnTile - 1) / kAttnTile);
+    const int each = PACKED ? a.prefix_split_tiles : a.split_tiles;
+    const int parts = max(1, attn_parts(all_tiles, each));
+    if (part >= parts) return;
+    const int tile0 = part * each;
+    const int tile1 = min(tile0 + each, pre_tiles + own_tiles);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int32_t *own_pages = PACKED ? nullptr : a.pages + (int64_t)blockIdx.z * a.pages_row;
+    const T *kp = (const T *)a.kp + (int64_t)kvh * a.k_head;
+    const T *vp = (const T *)a.vp + (int64_t)kvh * a.v_head;
+    const uint32_t ring = smem_u32(smem) + warp * Lay::warp_bytes;
+
+    // Page numbers of the warp's next 32 tiles, one a lane.
+    int page_of = 0;
+    auto pages_at = [&](int first) {
+        const int i = first + lane * kADWarps;
+        if (i < tile1)
+            page_of = i < pre_tiles ? attn_page(a, a.prefix_pages, i * kAttnTile)
+                                    : attn_page(a, own_pages, (i - pre_tiles) * kAttnTile);
+    };
+    // tile i (the n-th of this warp) into its ring stage
+    auto fetch = [&](int i, int n) {
+        if (n % 32 == 0) pages_at(i);
+        const int64_t page = __shfl_sync(~0u, page_of, n % 32);
+        if (i < tile1) {
+            const bool pre = i < pre_tiles;
+            const int j0 = (pre ? i : i - pre_tiles) * kAttnTile;
+            const int live = (pre ? n_pre : own_seen) - j0;
+            const int64_t off = j0 & ((1 << a.page_shift) - 1);
+            const T *ks = kp + page * a.k_page + off * a.k_slot;
+            const T *vs = vp + page * a.v_page + off * a.v_slot;
+            const uint32_t dst = ring + (n % kADStages) * Lay::stage_bytes;
+            constexpr int CH = D / 8;                   // 16-byte pieces of a row
+#pragma unroll
+            for (int c = lane; c < kAttnTile * CH; c += 32) {
+                const int r = c / CH, p = c % CH;
+                const uint32_t at = dst + r * Lay::row_bytes + ((p ^ (r & 7)) << 4);
+                cp_async16_or_zero(at, ks + r * a.k_slot + p * 8, r < live);
+                cp_async16_or_zero(at + Lay::tile_bytes, vs + r * a.v_slot + p * 8, r < live);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int n = 0; n < kADStages - 1; n++) fetch(tile0 + warp + n * kADWarps, n);
+
+    // Q: the A operand, 16 rows x D
+    uint32_t qf[D / 16][4];
+    const int rlo = row0 + lane / 4, rhi = rlo + 8;
+    {
+        const T *qlo = nullptr, *qhi = nullptr;
+        if (rlo < rows)
+            qlo = (const T *)a.q + (int64_t)(rq.t0 + rlo / a.group) * a.q_token +
+                  (int64_t)(kvh * a.group + rlo % a.group) * a.q_head;
+        if (rhi < rows)
+            qhi = (const T *)a.q + (int64_t)(rq.t0 + rhi / a.group) * a.q_token +
+                  (int64_t)(kvh * a.group + rhi % a.group) * a.q_head;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+            const int c = k * 16 + (lane % 4) * 2;
+            qf[k][0] = qlo ? *(const uint32_t *)(qlo + c) : 0u;
+            qf[k][1] = qhi ? *(const uint32_t *)(qhi + c) : 0u;
+            qf[k][2] = qlo ? *(const uint32_t *)(qlo + c + 8) : 0u;
+            qf[k][3] = qhi ? *(const uint32_t *)(qhi + c + 8) : 0u;
+        }
+    }
+    // own keys that the thread's two rows and the tile's first row see
+    int see_lo = own_seen, see_hi = own_seen, see_first = own_seen;
+    if (!PACKED && a.causal) {
+        see_first = rq.len - rq.n + row0 / a.group + 1;
+        see_lo = rq.len - rq.n + rlo / a.group + 1;
+        see_hi = rq.len - rq.n + rhi / a.group + 1;
+    }
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+
+    int n = 0;
+    for (int i = tile0 + warp; i < tile1; i += kADWarps, n++) {
+        fetch(i + (kADStages - 1) * kADWarps, n + kADStages - 1);
+        cp_async_wait<kADStages - 1>();
+        __syncwarp();
+        const uint32_t kb = ring + (n % kADStages) * Lay::stage_bytes;
+        const uint32_t vb = kb + Lay::tile_bytes;
+
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+            uint32_t b[4];
+            const int r = (lane & 7) + (lane >> 4) * 8, p = k * 2 + ((lane >> 3) & 1);
+            ldsm4(b, kb + r * Lay::row_bytes + ((p ^ (r & 7)) << 4));
+            mma16816<T>(s[0], qf[k], b[0], b[1]);
+            mma16816<T>(s[1], qf[k], b[2], b[3]);
+        }
+        const bool pre = i < pre_tiles;
+        const int j0 = (pre ? i : i - pre_tiles) * kAttnTile;
+        const int lim_lo = pre ? n_pre - j0 : min(see_lo, own_seen) - j0;
+        const int lim_hi = pre ? n_pre - j0 : min(see_hi, own_seen) - j0;
+        float mx_lo = m_lo, mx_hi = m_hi;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int j = t * 8 + (lane % 4) * 2 + e;
+                s[t][e] = j < lim_lo ? s[t][e] * a.scale_log2 : -INFINITY;
+                s[t][2 + e] = j < lim_hi ? s[t][2 + e] * a.scale_log2 : -INFINITY;
+                mx_lo = fmaxf(mx_lo, s[t][e]);
+                mx_hi = fmaxf(mx_hi, s[t][2 + e]);
+            }
+#pragma unroll
+        for (int x = 1; x <= 2; x <<= 1) {
+            mx_lo = fmaxf(mx_lo, __shfl_xor_sync(~0u, mx_lo, x));
+            mx_hi = fmaxf(mx_hi, __shfl_xor_sync(~0u, mx_hi, x));
+        }
+        if (__any_sync(~0u, mx_lo > m_lo || mx_hi > m_hi)) {
+            const float w_lo = mx_lo == -INFINITY ? 1.f : ex2(m_lo - mx_lo);
+            const float w_hi = mx_hi == -INFINITY ? 1.f : ex2(m_hi - mx_hi);
+            l_lo *= w_lo;
+            l_hi *= w_hi;
+#pragma unroll
+            for (int d = 0; d < D / 8; d++) {
+                o[d][0] *= w_lo;
+                o[d][1] *= w_lo;
+                o[d][2] *= w_hi;
+                o[d][3] *= w_hi;
+            }
+            m_lo = mx_lo;
+            m_hi = mx_hi;
+        }
+        const float z_lo = m_lo == -INFINITY ? 0.f : m_lo, z_hi = m_hi == -INFINITY ? 0.f : m_hi;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                s[t][e] = ex2(s[t][e] - z_lo);
+                s[t][2 + e] = ex2(s[t][2 + e] - z_hi);
+                l_lo += s[t][e];
+                l_hi += s[t][2 + e];
+            }
+        uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]),
+                         pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+        // a tile that some of the rows see only in part
+        const bool cut = !PACKED && !pre && min(own_seen, j0 + kAttnTile) > see_first;
+        uint32_t seen[4];
+        if (cut) {
+            const int c = (lane % 4) * 2;
+            seen[0] = pack2<T>(c < lim_lo, c + 1 < lim_lo);
+            seen[1] = pack2<T>(c < lim_hi, c + 1 < lim_hi);
+            seen[2] = pack2<T>(c + 8 < lim_lo, c + 9 < lim_lo);
+            seen[3] = pack2<T>(c + 8 < lim_hi, c + 9 < lim_hi);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) {
+            uint32_t b[4];
+            const int r = (lane & 7) + ((lane >> 3) & 1) * 8, c = d * 2 + (lane >> 4);
+            ldsm4t(b, vb + r * Lay::row_bytes + ((c ^ (r & 7)) << 4));
+            if (cut) {
+                mend_values<T>(b[0], b[1], seen, o[2 * d]);
+                mend_values<T>(b[2], b[3], seen, o[2 * d + 1]);
+            }
+            mma16816<T>(o[2 * d], p, b[0], b[1]);
+            mma16816<T>(o[2 * d + 1], p, b[2], b[3]);
+        }
+        __syncwarp();                       // the stage is free for the next fetch
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+        l_lo += __shfl_xor_sync(~0u, l_lo, x);
+        l_hi += __shfl_xor_sync(~0u, l_hi, x);
+    }
+    __syncthreads();
+    // join the warps
+    float *so = (float *)smem;
+    float *sm = so + kADWarps * kADRows * Lay::o_pitch, *sl = sm + kADWarps * kADRows;
+    {
+        float *mine = so + warp * kADRows * Lay::o_pitch;
+        const int r = lane / 4;
+#pragma unroll
+        for (int d = 0; d < D / 8; d++) {
+            const int c = d * 8 + (lane % 4) * 2;
+            *(float2 *)(mine + r * Lay::o_pitch + c) = make_float2(o[d][0], o[d][1]);
+            *(float2 *)(mine + (r + 8) * Lay::o_pitch + c) = make_float2(o[d][2], o[d][3]);
+        }
+        if (lane % 4 == 0) {
+            sm[warp * kADRows + r] = m_lo;
+            sm[warp * kADRows + r + 8] = m_hi;
+            sl[warp * kADRows + r] = l_lo;
+            sl[warp * kADRows + r + 8] = l_hi;
+        }
+    }
+    __syncthreads();
+    constexpr int TPR = D / 4;                          // threads a row, 4 values each
+    const bool direct = !PACKED && !a.packed && parts == 1;
+#pragma unroll
+    for (int r = threadIdx.x / TPR; r < kADRows; r += kADWarps * 32 / TPR) {
+        if (row0 + r >= rows) break;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kADWarps; w++) M = fmaxf(M, sm[w * kADRows + r]);
+        const float z = M == -INFINITY ? 0.f : M;
+        float l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int c = (threadIdx.x % TPR) * 4;
+#pragma unroll
+        for (int w = 0; w < kADWarps; w++) {
+            const float f = ex2(sm[w * kADRows + r] - z);
+            l += f * sl[w * kADRows + r];
+            const float4 x = *(const float4 *)(so + (w * kADRows + r) * Lay::o_pitch + c);
+            v.x += f * x.x;
+            v.y += f * x.y;
+            v.z += f * x.z;
+            v.w += f * x.w;
+        }
+        const int64_t row = (int64_t)(rq.t0 + (row0 + r) / a.group) * a.q_heads +
+                            kvh * a.group + (row0 + r) % a.group;
+        if (direct) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint2 w;
+            w.x = pack2<T>(v.x * inv, v.y * inv);
+            w.y = pack2<T>(v.z * inv, v.w * inv);
+            *(uint2 *)((T *)a.out + row * D + c) = w;
+        } else {
+            const int64_t slot = (int64_t)(PACKED ? part : a.prefix_parts + part) * a.tokens *
+                                     a.q_heads + row;
+            *(float4 *)(a.part_o + slot * D + c) = v;
+            if (c == 0) a.part_ml[slot] = make_float2(M, l);
+        }
+    }
+}
+
+// Joins the parts of each row: a warp a (token, head).  Rows whose request has
+// one part were written by their CTA.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+    const int lane = threadIdx.x % 32;
+    const int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const int64_t rows = (int64_t)a.tokens * a.q_heads;
+    if (row >= rows) return;
+    const int t = (int)(row / a.q_heads);
+    // the token's request: the last one that starts at or before it
+    int b = -1;
+    for (int i0 = 0; i0 < a.batch; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned hit = __ballot_sync(~0u, i < a.batch && a.q_start[i] <= t);
+        if (hit) b = i0 + 31 - __clz(hit);
+        if (hit != ~0u) break;
+    }
+    if (b < 0) return;
+    const AttnReq rq = attn_req(a, b);
+    if (t >= rq.t0 + rq.n) return;
+    const int own = (a.packed ? 0 : (a.prefix_len + kAttnTile - 1) / kAttnTile) +
+                    (rq.len + kAttnTile - 1) / kAttnTile;
+    int parts = max(1, attn_parts(own, a.split_tiles));
+    if (!a.packed && parts == 1) return;
+    parts += a.prefix_parts;
+    constexpr int V = D / 32;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = 0.f;
+    float M = -INFINITY, l = 0.f;
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+        const int p = p0 + lane;
+        const float2 ml = p < parts ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f);
+        float m = fmaxf(M, ml.x);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
+        const float z = m == -INFINITY ? 0.f : m;
+        const float keep = ex2(M - z), w = ex2(ml.x - z);
+        l = l * keep + w * ml.y;            // a lane's own parts
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] *= keep;
+        M = m;
+        const int here = min(32, parts - p0);
+        for (int k = 0; k < here; k++) {
+            const float f = __shfl_sync(~0u, w, k);
+            const float *src = a.part_o + ((p0 + k) * rows + row) * D + lane * V;
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += f * src[i];
+        }
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *dst = (T *)a.out + row * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *(uint32_t *)(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+}
+
+// ------------------------------------------------------------ host side --
+
+struct AttnPlan {
+    int packed, prefix_parts, prefix_split_tiles;
+    int split_tiles, parts;                 // own parts at most
+    int64_t o_bytes, ml_bytes;
+    int max_q, max_kv;                      // the host's bounds, no wider than tokens and pages
+};
+
+static int tiles_of(int64_t keys) { return (int)((keys + kAttnTile - 1) / kAttnTile); }
+
+// Key tiles a CTA: enough CTAs to fill the card twice over where there are
+// keys enough, no fewer than 16 tiles (4 a warp).
+static int pick_split(int64_t tiles, int64_t ctas) {
+    const int64_t want = 2 * 2 * 148;
+    ctas = ctas < 1 ? 1 : ctas;
+    int64_t parts = (want + ctas - 1) / ctas;
+    parts = parts < 1 ? 1 : parts > 256 ? 256 : parts;
+    int64_t each = (tiles + parts - 1) / parts;
+    if (each < 16) each = 16;
+    return (int)each;
+}
+
+static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
+    AttnPlan p = {};
+    p.max_q = d->max_q < d->tokens ? d->max_q : d->tokens;
+    const int64_t held = (int64_t)d->pages_per_row * c->page_size;
+    p.max_kv = d->max_kv < held ? d->max_kv : (int)held;
+    const int group = d->q_heads / d->kv_heads;
+    // The prefix apart, for all rows at once, where a request's rows alone
+    // would leave a row tile mostly empty.
+    p.packed = d->prefix_len > 0 && d->batch > 1 &&
+               (int64_t)d->tokens * group <= (int64_t)128 * d->batch;
+    const int64_t row_tiles = ((int64_t)p.max_q * group + kADRows - 1) / kADRows;
+    const int64_t own = tiles_of(p.max_kv) + (p.packed ? 0 : tiles_of(d->prefix_len));
+    p.split_tiles = pick_split(own, (int64_t)d->batch * d->kv_heads * row_tiles);
+    p.parts = own ? (int)((own + p.split_tiles - 1) / p.split_tiles) : 1;
+    if (p.packed) {
+        const int64_t tiles = tiles_of(d->prefix_len);
+        const int64_t rt = ((int64_t)d->tokens * group + kADRows - 1) / kADRows;
+        p.prefix_split_tiles = pick_split(tiles, rt * d->kv_heads);
+        p.prefix_parts = (int)((tiles + p.prefix_split_tiles - 1) / p.prefix_split_tiles);
+    }
+    const int all = p.prefix_parts + (p.packed || p.parts > 1 ? p.parts : 0);
+    const int64_t rows = (int64_t)d->tokens * d->q_heads;
+    p.o_bytes = (all * rows * d->head_dim * 4 + 255) / 256 * 256;
+    p.ml_bytes = (all * rows * 8 + 255) / 256 * 256;
+    return p;
+}
+
+static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
+    const char *who = "warp_paged_attention";
+    WARP_ARG(d, "%s: NULL description", who);
+    const int rc = kv_pages_check(c, who);
+    if (rc) return rc;
+    WARP_ARG(d->batch >= 0 && d->tokens >= 0 && d->max_q >= 0 && d->max_kv >= 0 &&
+                 d->prefix_len >= 0 && d->pages_per_row >= 0 && d->pages_row >= 0,
+             "%s: negative size", who);
+    WARP_ARG(d->q_heads >= 1 && d->kv_heads >= 1 && d->q_heads % d->kv_heads == 0,
+             "%s: %d query heads over %d kv heads", who, d->q_heads, d->kv_heads);
+    WARP_ARG(d->head_dim == 64 || d->head_dim == 128, "%s: head_dim %d is not 64 or 128", who,
+             d->head_dim);
+    WARP_ARG(c->kv_heads == d->kv_heads && c->head_dim == d->head_dim && c->type == d->type,
+             "%s: the pages hold %d heads of %d (type %d), the queries want %d of %d (type %d)",
+             who, c->kv_heads, c->head_dim, c->type, d->kv_heads, d->head_dim, d->type);
+    WARP_ARG(d->scale > 0.f && isfinite(d->scale), "%s: scale %g is not positive", who,
+             (double)d->scale);
+    WARP_ARG(d->kv_heads <= 65535 && d->batch <= 65535, "%s: more than 65535 requests or kv heads",
+             who);
+    WARP_ARG(d->max_kv < (1 << 30) && d->prefix_len < (1 << 30), "%s: more than 2^30 keys", who);
+    WARP_ARG((int64_t)d->tokens * d->q_heads < (int64_t)1 << 30, "%s: more than 2^30 rows", who);
+    return WARP_OK;
+}
+
+template <typename T, int D>
+static int attn_launch(const AttnArgs &a, const AttnPlan &p, cudaStream_t st) {
+    using Lay = ADLay<D>;
+    static bool attr_done = false;                      // per instantiation, per process
+    if (!attr_done) {
+        cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<T, D, false>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             Lay::bytes);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attn_rows_kernel<T, D, true>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::bytes);
+        if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
+        attr_done = true;
+    }
+    if (a.packed) {
+        const int64_t rt = ((int64_t)a.tokens * a.group + kADRows - 1) / kADRows;
+        attn_rows_kernel<T, D, true>
+            <<<dim3((unsigned)(rt * p.prefix_parts), a.kv_heads, 1), kADWarps * 32, Lay::bytes,
+               st>>>(a);
+        WARP_CHECK_LAUNCH("attn_rows_kernel (prefix)");
+    }
+    const int64_t rt = ((int64_t)a.max_q * a.group + kADRows - 1) / kADRows;
+    attn_rows_kernel<T, D, false>
+        <<<dim3((unsigned)(rt * p.parts), a.kv_heads, a.batch), kADWarps * 32, Lay::bytes, st>>>(a);
+    WARP_CHECK_LAUNCH("attn_rows_kernel");
+    if (a.packed || p.parts > 1) {
+        attn_join_kernel<T, D>
+            <<<cdiv((size_t)a.tokens * a.q_heads, 8), 256, 0, st>>>(a);
+        WARP_CHECK_LAUNCH("attn_join_kernel");
+    }
+    return WARP_OK;
+}
+
+}  // namespace warp
+
+extern "C" int64_t warp_attn_scratch(const warp_attn_desc *d, const warp_kv_pages *c) {
+    const int rc = warp::attn_check(d, c);
+    if (rc) return rc;
+    const warp::AttnPlan p = warp::attn_plan(d, c);
+    return p.o_bytes + p.ml_bytes;
+}
+
+extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *c, void *scratch,
+                                    void *stream) {
+    int rc = warp::attn_check(d, c);
+    if (rc) return rc;
+    if (d->tokens == 0 || d->batch == 0 || d->max_q == 0) return WARP_OK;
+    const char *who = "warp_paged_attention";
+    WARP_ARG(d->q && d->out && d->q_start && d->kv_len, "%s: NULL pointer", who);
+    WARP_ARG(d->pages || d->pages_per_row == 0, "%s: NULL page table", who);
+    WARP_ARG(d->prefix_pages || d->prefix_len == 0, "%s: NULL prefix page table", who);
+    WARP_ARG(((uintptr_t)d->q & 15) == 0 && ((uintptr_t)d->out & 15) == 0 && d->q_token % 8 == 0 &&
+                 d->q_head % 8 == 0,
+             "%s: queries and results must be 16-byte aligned, strides multiples of 16 bytes", who);
+    const warp::AttnPlan p = warp::attn_plan(d, c);
+    WARP_ARG(p.o_bytes + p.ml_bytes == 0 || (scratch && ((uintptr_t)scratch & 255) == 0),
+             "%s: scratch must be 256-byte aligned", who);
+    warp::AttnArgs a = {};
+    a.q = d->q, a.kp = c->k, a.vp = c->v, a.out = d->out;
+    a.q_token = d->q_token, a.q_head = d->q_head;
+    a.k_page = c->k_page, a.k_slot = c->k_slot, a.k_head = c->k_head;
+    a.v_page = c->v_page, a.v_slot = c->v_slot, a.v_head = c->v_head;
+    a.q_start = d->q_start, a.kv_len = d->kv_len;
+    a.pages = d->pages, a.prefix_pages = d->prefix_pages, a.pages_row = d->pages_row;
+    a.pages_per_row = d->pages_per_row, a.page_shift = __builtin_ctz(c->page_size);
+    a.n_pages = (int)c->pages;
+    a.batch = d->batch, a.tokens = d->tokens;
+    a.q_heads = d->q_heads, a.kv_heads = d->kv_heads, a.group = d->q_heads / d->kv_heads;
+    a.max_q = p.max_q, a.max_kv = p.max_kv, a.causal = d->causal != 0;
+    a.prefix_len = d->prefix_len;
+    a.scale_log2 = d->scale * 1.4426950408889634f;
+    a.part_o = (float *)scratch;
+    a.part_ml = (float2 *)((char *)scratch + p.o_bytes);
+    a.packed = p.packed, a.prefix_parts = p.prefix_parts;
+    a.split_tiles = p.split_tiles, a.prefix_split_tiles = p.prefix_split_tiles;
+    rc = warp::attn_err_word(&a.err);
+    if (rc) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (d->type == WARP_T_F16)
+        return d->head_dim == 64 ? warp::attn_launch<__half, 64>(a, p, st)
+                                 : warp::attn_launch<__half, 128>(a, p, st);
+    return d->head_dim == 64 ? warp::attn_launch<__nv_bfloat16, 64>(a, p, st)
+                             : warp::attn_launch<__nv_bfloat16, 128>(a, p, st);
+}

@@ -1,0 +1,86 @@
+// attn.cuh — what the attention kernels share: element types, the error word
+// behind warp_attn_status, and the checks of a page description.
+#pragma once
+#include "common.cuh"
+
+namespace warp {
+
+// Bits of the error word.
+constexpr unsigned kAttnBadSlot = 1u;     // a slot outside the pages
+constexpr unsigned kAttnBadPage = 2u;     // a page number outside the pages
+constexpr unsigned kAttnBadLen = 4u;      // a length over its host bound
+constexpr unsigned kAttnTimeout = 8u;     // a bounded wait gave up
+
+// Device address of the error word (one per device).
+int attn_err_word(unsigned **out);
+
+int kv_pages_check(const warp_kv_pages *c, const char *who);
+
+template <typename T> struct AttnType;
+template <> struct AttnType<float> {
+    static __device__ __forceinline__ float up(float x) { return x; }
+    static __device__ __forceinline__ float down(float x) { return x; }
+};
+template <> struct AttnType<__half> {
+    static __device__ __forceinline__ float up(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
+};
+template <> struct AttnType<__nv_bfloat16> {
+    static __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+};
+
+// One attention call as its kernels see it.
+struct AttnArgs {
+    const void *q, *kp, *vp;
+    void *out;
+    int64_t q_token, q_head;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    const int32_t *q_start, *kv_len, *pages, *prefix_pages;
+    int64_t pages_row;
+    int pages_per_row, page_shift, n_pages;
+    int batch, tokens, q_heads, kv_heads, group;
+    int max_q, max_kv, causal, prefix_len;
+    float scale_log2;                       // scale * log2(e)
+    unsigned *err;
+    // Partial results of split key ranges: o [part][token][head][D] not yet
+    // divided by l, and (m, l) with m the running maximum in the log2 domain.
+    // Parts 0..prefix_parts-1 are the shared prefix's where it is computed for
+    // the whole batch at once (`packed`), the requests' own parts follow.
+    float *part_o;
+    float2 *part_ml;
+    int packed, prefix_parts;
+    int split_tiles;                        // key tiles of a request's part
+    int prefix_split_tiles;                 // and of a part of the prefix
+};
+
+// Request b as the host's bounds leave it: its first token, its queries and
+// its own keys.
+struct AttnReq { int t0, n, len; };
+
+__device__ __forceinline__ AttnReq attn_req(const AttnArgs &a, int b) {
+    AttnReq r;
+    const int s = a.q_start[b], e = a.q_start[b + 1], l = a.kv_len[b];
+    r.t0 = min(max(s, 0), a.tokens);
+    r.n = min(min(max(e - s, 0), a.max_q), a.tokens - r.t0);
+    r.len = (int)min((int64_t)min(max(l, 0), a.max_kv),
+                     (int64_t)a.pages_per_row << a.page_shift);
+    if (threadIdx.x == 0 && (r.t0 != s || r.n != e - s || r.len != l))
+        atomicOr(a.err, kAttnBadLen);
+    return r;
+}
+
+// The page of own or prefix key j; a number outside the pages is reported and
+// read as page 0.
+__device__ __forceinline__ int attn_page(const AttnArgs &a, const int32_t *table, int j) {
+    const int p = table[j >> a.page_shift];
+    if ((unsigned)p < (unsigned)a.n_pages) return p;
+    atomicOr(a.err, kAttnBadPage);
+    return 0;
+}
+
+// Keys come in tiles of kAttnTile; the prefix's last tile and a request's last
+// one may be partly filled, and a tile never mixes the two.
+constexpr int kAttnTile = 16;
+
+}  // namespace warp

@@ -1,0 +1,387 @@
+// rope.cu — per-head norm and rotary positions of queries and keys, with the
+// keys and values written to a paged cache in the same pass.
+//
+// One row is the head_dim values of one (token, head).  With a the angle of
+// pair i at the token's position,
+//     (x0, x1) -> (x0 cos a - x1 sin a, x0 sin a + x1 cos a),
+// after x -> x / sqrt(mean(x^2) + eps) * w where a norm is asked for.  Nothing
+// is read twice, so the kernel is bound by memory: one read of q, k, v and one
+// write of the results.
+//
+// A thread owns a "unit" of 2*VEC values of a row: the two VEC-wide vectors
+// whose elements are each other's partners (half layout: VEC values of the
+// first half and the VEC values rot_dim/2 further on; interleaved: 2*VEC
+// neighbours), so that the rotation needs no exchange between threads.  A
+// row's units sit on neighbouring lanes, and the norm's sum is a butterfly over them.
+#include "attn.cuh"
+
+namespace warp {
+
+__device__ unsigned g_attn_err;
+
+int attn_err_word(unsigned **out) {
+    const cudaError_t e = cudaGetSymbolAddress((void **)out, g_attn_err);
+    return e == cudaSuccess ? WARP_OK : cuda_fail(e, "attention error word");
+}
+
+int kv_pages_check(const warp_kv_pages *c, const char *who) {
+    WARP_ARG(c && c->k && c->v, "%s: NULL pages", who);
+    WARP_ARG(c->type == WARP_T_F16 || c->type == WARP_T_BF16,
+             "%s: pages must be fp16 or bf16 (type %d)", who, c->type);
+    WARP_ARG(c->page_size >= 16 && c->page_size <= 4096 && !(c->page_size & (c->page_size - 1)),
+             "%s: page_size %d is not a power of two in 16..4096", who, c->page_size);
+    WARP_ARG(c->pages >= 1 && c->pages < ((int64_t)1 << 31), "%s: %lld pages", who,
+             (long long)c->pages);
+    WARP_ARG(c->kv_heads >= 1 && c->head_dim >= 2, "%s: kv_heads %d, head_dim %d", who,
+             c->kv_heads, c->head_dim);
+    WARP_ARG((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, "%s: pages must be 16-byte aligned",
+             who);
+    const int64_t st[6] = {c->k_page, c->k_slot, c->k_head, c->v_page, c->v_slot, c->v_head};
+    for (int i = 0; i < 6; i++)
+        WARP_ARG(st[i] >= 0 && (st[i] & 7) == 0,
+                 "%s: page strides must be non-negative multiples of 16 bytes", who);
+    return WARP_OK;
+}
+
+struct RopeArgs {
+    const void *q, *k, *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    void *q_out, *k_out;                    // contiguous [tokens][heads][D]
+    const float *q_norm, *k_norm;
+    const double *inv_freq;
+    const int32_t *positions;
+    const int64_t *slots;                   // non-NULL: append to the pages
+    void *kp, *vp;
+    int64_t k_page, k_slot, k_ph, v_page, v_slot, v_ph;
+    int64_t n_slots;
+    unsigned *err;
+    float eps, rot_scale;
+    int tokens, q_heads, kv_heads, D, rot, interleaved, page_shift;
+    int rows;                               // rows a token: q, then k, then v (append)
+    int rows_per_cta;
+};
+
+template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) RopeVec {
+    T x[N];
+};
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeMaxPairs = 128;          // head_dim up to 256
+
+// L lanes a row, UPL units a lane.
+template <typename TI, typename TO, int VEC, int L, int UPL>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
+    __shared__ float2 cs[kRopeMaxPairs];
+    const int t = blockIdx.x;
+    const int row0 = blockIdx.y * a.rows_per_cta;
+    const int row1 = min(a.rows, row0 + a.rows_per_cta);
+    const int half = a.rot / 2;
+    // The angle in turns, reduced in 64 bits: what is left is a fraction of a
+    // turn that fp32 holds to 2^-25, whatever the position.
+    if ((int)threadIdx.x < half) {
+        double turns = (double)a.positions[t] * a.inv_freq[threadIdx.x] * 0.15915494309189533577;
+        turns -= rint(turns);
+        float s, c;
+        sincospif(2.0f * (float)turns, &s, &c);
+        cs[threadIdx.x] = make_float2(c * a.rot_scale, s * a.rot_scale);
+    }
+    int64_t slot = -1;
+    if (a.slots) {
+        slot = a.slots[t];
+        if (slot >= a.n_slots) {
+            if (threadIdx.x == 0) atomicOr(a.err, kAttnBadSlot);
+            slot = -1;
+        }
+    }
+    __syncthreads();
+
+    constexpr int RPP = kRopeThreads / L;   // rows in flight
+    const int lane = threadIdx.x % L;
+    const int units = a.D / (2 * VEC), rot_units = a.rot / (2 * VEC);
+    for (int base = row0; base < row1; base += RPP) {
+        const int r = base + (int)threadIdx.x / L;
+        const bool live = r < row1;
+        // whose row: 0 q, 1 k, 2 v
+        const int rr = live ? r : row0;
+        const int who = rr < a.q_heads ? 0 : rr < a.q_heads + a.kv_heads ? 1 : 2;
+        const int h = who == 0 ? rr : who == 1 ? rr - a.q_heads : rr - a.q_heads - a.kv_heads;
+        const TI *src = who == 0 ? (const TI *)a.q + t * a.q_token + h * a.q_head
+                      : who == 1 ? (const TI *)a.k + t * a.k_token + h * a.k_head
+                                 : (const TI *)a.v + t * a.v_token + h * a.v_head;
+        float x0[UPL][VEC], x1[UPL][VEC];
+        int at0[UPL], at1[UPL];             // where the unit's two vectors start
+#pragma unroll
+        for (int n = 0; n < UPL; n++) {
+            const int u = lane + n * L;
+            // rotated units first; behind them the rest of the row, two vectors a unit
+            if (u < rot_units && !a.interleaved) {
+                at0[n] = u * VEC;
+                at1[n] = half + u * VEC;
+            } else {
+                at0[n] = u * 2 * VEC;
+                at1[n] = at0[n] + VEC;
+            }
+            if (live && u < units) {
+                const RopeVec<TI, VEC> v0 = *(const RopeVec<TI, VEC> *)(src + at0[n]);
+                const RopeVec<TI, VEC> v1 = *(const RopeVec<TI, VEC> *)(src + at1[n]);
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    x0[n][i] = AttnType<TI>::up(v0.x[i]);
+                    x1[n][i] = AttnType<TI>::up(v1.x[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) x0[n][i] = x1[n][i] = 0.f;
+            }
+        }
+        const float *w = who == 0 ? a.q_norm : who == 1 ? a.k_norm : nullptr;
+        if (a.q_norm || a.k_norm) {         // the same branch for the whole warp
+            float ss = 0.f;
+#pragma unroll
+            for (int n = 0; n < UPL; n++)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) ss += x0[n][i] * x0[n][i] + x1[n][i] * x1[n][i];
+#pragma unroll
+            for (int o = L / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+            if (w) {
+                const float inv = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+                for (int n = 0; n < UPL; n++) {
+                    if (lane + n * L >= units) continue;
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        x0[n][i] *= inv * __ldg(w + at0[n] + i);
+                        x1[n][i] *= inv * __ldg(w + at1[n] + i);
+                    }
+                }
+            }
+        }
+        if (!live) continue;
+        TO *dst;
+        if (who == 0) {
+            dst = (TO *)a.q_out + ((int64_t)t * a.q_heads + h) * a.D;
+        } else if (a.slots) {
+            if (slot < 0) continue;
+            const int64_t page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
+            dst = who == 1 ? (TO *)a.kp + page * a.k_page + off * a.k_slot + h * a.k_ph
+                           : (TO *)a.vp + page * a.v_page + off * a.v_slot + h * a.v_ph;
+        } else {
+            dst = (TO *)a.k_out + ((int64_t)t * a.kv_heads + h) * a.D;
+        }
+#pragma unroll
+        for (int n = 0; n < UPL; n++) {
+            const int u = lane + n * L;
+            if (u >= units) continue;
+            if (u < rot_units && who != 2) {
+                if (a.interleaved) {
+                    // pairs are neighbours: (x0[0], x0[1]) ..., then x1's
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        // value i of the unit's 2*VEC, pair u*VEC + i
+                        float &p = 2 * i < VEC ? x0[n][(2 * i) % VEC] : x1[n][(2 * i) % VEC];
+                        float &q = 2 * i + 1 < VEC ? x0[n][(2 * i + 1) % VEC]
+                                                   : x1[n][(2 * i + 1) % VEC];
+                        const float2 c = cs[u * VEC + i];
+                        const float y0 = p * c.x - q * c.y, y1 = p * c.y + q * c.x;
+                        p = y0;
+                        q = y1;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        const float2 c = cs[u * VEC + i];
+                        const float y0 = x0[n][i] * c.x - x1[n][i] * c.y;
+                        const float y1 = x0[n][i] * c.y + x1[n][i] * c.x;
+                        x0[n][i] = y0;
+                        x1[n][i] = y1;
+                    }
+                }
+            }
+            RopeVec<TO, VEC> v0, v1;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                v0.x[i] = AttnType<TO>::down(x0[n][i]);
+                v1.x[i] = AttnType<TO>::down(x1[n][i]);
+            }
+            *(RopeVec<TO, VEC> *)(dst + at0[n]) = v0;
+            *(RopeVec<TO, VEC> *)(dst + at1[n]) = v1;
+        }
+    }
+}
+
+template <typename TI, typename TO, int VEC, int L, int UPL>
+static int rope_launch(RopeArgs &a, cudaStream_t st) {
+    constexpr int RPP = kRopeThreads / L;
+    a.rows_per_cta = RPP;
+    rope_kernel<TI, TO, VEC, L, UPL>
+        <<<dim3(a.tokens, cdiv(a.rows, a.rows_per_cta)), kRopeThreads, 0, st>>>(a);
+    WARP_CHECK_LAUNCH("rope_kernel");
+    return WARP_OK;
+}
+
+// The widest vectors that the row's parts, addresses and strides allow.
+template <typename TI, typename TO>
+static int rope_vec(RopeArgs &a, cudaStream_t st) {
+    auto fits = [&](int vec) {
+        const uintptr_t ib = vec * sizeof(TI) < 16 ? vec * sizeof(TI) : 16;
+        const uintptr_t ob = vec * sizeof(TO) < 16 ? vec * sizeof(TO) : 16;
+        if (a.rot % (2 * vec) || a.D % (2 * vec)) return false;
+        uintptr_t in = 0, out = (uintptr_t)a.q_out | (uintptr_t)a.k_out;
+        auto add = [&](const void *p, int64_t s0, int64_t s1) {
+            if (p) in |= (uintptr_t)p | (uintptr_t)(s0 * sizeof(TI)) | (uintptr_t)(s1 * sizeof(TI));
+        };
+        add(a.q, a.q_token, a.q_head);
+        add(a.k, a.k_token, a.k_head);
+        if (a.slots) add(a.v, a.v_token, a.v_head);
+        return in % ib == 0 && out % ob == 0;
+    };
+    const int units = a.D / 16;
+    if (fits(8)) {
+        if (units <= 4) return rope_launch<TI, TO, 8, 4, 1>(a, st);
+        if (units <= 8) return rope_launch<TI, TO, 8, 8, 1>(a, st);
+        return rope_launch<TI, TO, 8, 16, 1>(a, st);
+    }
+    if (fits(2)) return rope_launch<TI, TO, 2, 32, 2>(a, st);
+    return rope_launch<TI, TO, 1, 32, 4>(a, st);
+}
+
+static int rope_run(const warp_rope_desc *d, const warp_kv_pages *c, const int64_t *slots,
+                    const char *who, cudaStream_t st) {
+    WARP_ARG(d, "%s: NULL description", who);
+    WARP_ARG(d->tokens >= 0 && d->q_heads >= 0 && d->kv_heads >= 0, "%s: negative size", who);
+    WARP_ARG(d->head_dim >= 2 && d->head_dim <= 256 && d->head_dim % 2 == 0,
+             "%s: head_dim %d is not even in 2..256", who, d->head_dim);
+    WARP_ARG(d->rot_dim >= 0 && d->rot_dim <= d->head_dim && d->rot_dim % 2 == 0,
+             "%s: rot_dim %d is not even in 0..%d", who, d->rot_dim, d->head_dim);
+    WARP_ARG(d->type >= WARP_T_F32 && d->type <= WARP_T_BF16 && d->out_type >= WARP_T_F32 &&
+                 d->out_type <= WARP_T_BF16 && (d->type == d->out_type || d->type == WARP_T_F32),
+             "%s: type %d to out_type %d (the same type, or from fp32)", who, d->type,
+             d->out_type);
+    const int rows = d->q_heads + (c ? 2 : 1) * d->kv_heads;
+    WARP_ARG(rows <= 65536, "%s: %d heads", who, rows);
+    if (d->tokens == 0 || rows == 0) return WARP_OK;
+    WARP_ARG(d->positions || d->rot_dim == 0, "%s: NULL positions", who);
+    WARP_ARG(d->inv_freq || d->rot_dim == 0, "%s: NULL inv_freq", who);
+    WARP_ARG(!d->q_heads || (d->q && d->q_out), "%s: NULL queries", who);
+    WARP_ARG(!d->kv_heads || (d->k && (c ? d->v != nullptr : d->k_out != nullptr)),
+             "%s: NULL keys or values", who);
+    RopeArgs a = {};
+    a.q = d->q_heads ? d->q : nullptr;
+    a.k = d->kv_heads ? d->k : nullptr;
+    a.q_token = d->q_token, a.q_head = d->q_head;
+    a.k_token = d->k_token, a.k_head = d->k_head;
+    a.q_out = d->q_heads ? d->q_out : nullptr;
+    a.q_norm = d->q_norm, a.k_norm = d->k_norm;
+    a.inv_freq = d->inv_freq, a.positions = d->positions;
+    a.eps = d->eps, a.rot_scale = d->rot_scale;
+    a.tokens = d->tokens, a.q_heads = d->q_heads, a.kv_heads = d->kv_heads;
+    a.D = d->head_dim, a.rot = d->rot_dim, a.interleaved = d->interleaved != 0;
+    a.rows = rows;
+    if (c) {
+        const int rc = kv_pages_check(c, who);
+        if (rc) return rc;
+        WARP_ARG(slots, "%s: NULL slots", who);
+        WARP_ARG(c->kv_heads == d->kv_heads && c->head_dim == d->head_dim,
+                 "%s: the pages hold %d heads of %d, the keys are %d of %d", who, c->kv_heads,
+                 c->head_dim, d->kv_heads, d->head_dim);
+        WARP_ARG(c->type == d->out_type, "%s: out_type %d is not the pages' %d", who, d->out_type,
+                 c->type);
+        a.v = d->v, a.v_token = d->v_token, a.v_head = d->v_head;
+        a.slots = slots;
+        a.kp = c->k, a.vp = c->v;
+        a.k_page = c->k_page, a.k_slot = c->k_slot, a.k_ph = c->k_head;
+        a.v_page = c->v_page, a.v_slot = c->v_slot, a.v_ph = c->v_head;
+        a.n_slots = c->pages * c->page_size;
+        a.page_shift = __builtin_ctz(c->page_size);
+        const int er = attn_err_word(&a.err);
+        if (er) return er;
+    } else {
+        a.k_out = d->kv_heads ? d->k_out : nullptr;
+    }
+    if (d->type == WARP_T_F16) return rope_vec<__half, __half>(a, st);
+    if (d->type == WARP_T_BF16) return rope_vec<__nv_bfloat16, __nv_bfloat16>(a, st);
+    return d->out_type == WARP_T_F16    ? rope_vec<float, __half>(a, st)
+           : d->out_type == WARP_T_BF16 ? rope_vec<float, __nv_bfloat16>(a, st)
+                                        : rope_vec<float, float>(a, st);
+}
+
+// One thread a token; its request by bisection of q_start.  A few microseconds
+// once a step, for all layers.
+__global__ void kv_slots_kernel(const int32_t *__restrict__ q_start,
+                                const int32_t *__restrict__ kv_len, int batch, int tokens,
+                                const int32_t *__restrict__ pages, int64_t pages_row,
+                                int pages_per_row, int page_shift, int base,
+                                int32_t *__restrict__ positions, int64_t *__restrict__ slots) {
+    const int t = blockIdx.x * blockDim.x + threadIdx.x;
+    if (t >= tokens) return;
+    int lo = 0, hi = batch;                 // the last b with q_start[b] <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (q_start[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int first = q_start[lo], end = q_start[lo + 1];
+    int64_t slot = -1;
+    int32_t pos = 0;
+    if (t >= first && t < end) {
+        const int64_t j = (int64_t)kv_len[lo] - end + t;
+        pos = (int32_t)(base + j);
+        if (j >= 0 && (j >> page_shift) < pages_per_row)
+            slot = ((int64_t)pages[lo * pages_row + (j >> page_shift)] << page_shift) +
+                   (j & ((1 << page_shift) - 1));
+    }
+    positions[t] = pos;
+    slots[t] = slot;
+}
+
+}  // namespace warp
+
+extern "C" int warp_qk_norm_rope(const warp_rope_desc *d, void *stream) {
+    return warp::rope_run(d, nullptr, nullptr, "warp_qk_norm_rope", (cudaStream_t)stream);
+}
+
+extern "C" int warp_kv_append(const warp_rope_desc *d, const warp_kv_pages *c,
+                              const int64_t *slots, void *stream) {
+    WARP_ARG(c, "warp_kv_append: NULL pages");
+    return warp::rope_run(d, c, slots, "warp_kv_append", (cudaStream_t)stream);
+}
+
+extern "C" int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int batch, int tokens,
+                             const int32_t *pages, int64_t pages_row, int pages_per_row,
+                             int page_size, int base, int32_t *positions, int64_t *slots,
+                             void *stream) {
+    WARP_ARG(batch >= 0 && tokens >= 0 && pages_per_row >= 0 && pages_row >= 0 && base >= 0,
+             "warp_kv_slots: negative size");
+    WARP_ARG(page_size >= 16 && page_size <= 4096 && !(page_size & (page_size - 1)),
+             "warp_kv_slots: page_size %d is not a power of two in 16..4096", page_size);
+    if (tokens == 0) return WARP_OK;
+    WARP_ARG(batch >= 1 && q_start && kv_len && positions && slots && (pages || !pages_per_row),
+             "warp_kv_slots: NULL pointer or no request");
+    warp::kv_slots_kernel<<<warp::cdiv(tokens, 256), 256, 0, (cudaStream_t)stream>>>(
+        q_start, kv_len, batch, tokens, pages, pages_row, pages_per_row,
+        __builtin_ctz(page_size), base, positions, slots);
+    WARP_CHECK_LAUNCH("kv_slots_kernel");
+    return WARP_OK;
+}
+
+extern "C" int warp_attn_status(int clear) {
+    unsigned v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, warp::g_attn_err, sizeof(v));
+    if (e != cudaSuccess) return warp::cuda_fail(e, "warp_attn_status");
+    if (clear && v) {
+        const unsigned z = 0;
+        e = cudaMemcpyToSymbol(warp::g_attn_err, &z, sizeof(z));
+        if (e != cudaSuccess) return warp::cuda_fail(e, "warp_attn_status");
+    }
+    if (v & warp::kAttnTimeout) {
+        warp::set_error("attention: a tensor-core wait gave up (flags 0x%x)", v);
+        return WARP_E_TIMEOUT;
+    }
+    if (v) {
+        warp::set_error("attention:%s%s%s",
+                        v & warp::kAttnBadSlot ? " a slot outside the pages;" : "",
+                        v & warp::kAttnBadPage ? " a page number outside the pages;" : "",
+                        v & warp::kAttnBadLen ? " a length over its bound" : "");
+        return WARP_E_ARG;
+    }
+    return WARP_OK;
+}

@@ -44,6 +44,12 @@ SIGNATURES = {
     "warp_qwen_route": (I, [P, I, I, I, I, P, P, P]),
     "warp_moe_route": (I, [P, I, I, I, I, P, I, F, P, P, P]),
     "warp_rmsnorm": (I, [P, P, P, I, I, F, P]),
+    "warp_qk_norm_rope": (I, [P, P]),
+    "warp_kv_append": (I, [P, P, P, P]),
+    "warp_kv_slots": (I, [P, P, I, I, P, I64, I, I, I, P, P, P]),
+    "warp_attn_scratch": (I64, [P, P]),
+    "warp_paged_attention": (I, [P, P, P, P]),
+    "warp_attn_status": (I, [I]),
     "warp_moe_layer_create": (I, [P, I, P]),
     "warp_moe_layer_destroy": (None, [P]),
     "warp_moe_layer_status": (I, [P, P]),
@@ -88,6 +94,38 @@ class VqJob(ctypes.Structure):
         ("y", P), ("rec", P), ("rec_bytes", SZ), ("idx_off", ctypes.c_uint32),
         ("sc_off", ctypes.c_uint32), ("lut", P), ("lut_bytes", SZ),
         ("lut_off", ctypes.c_uint32), ("m", I), ("nv", I), ("stages", I), ("entries", I),
+    ]
+
+
+class KVPages(ctypes.Structure):
+    """warp_kv_pages (include/warp_cuda.h)."""
+    _fields_ = [
+        ("k", P), ("v", P), ("type", I), ("page_size", I), ("kv_heads", I), ("head_dim", I),
+        ("pages", I64), ("k_page", I64), ("k_slot", I64), ("k_head", I64),
+        ("v_page", I64), ("v_slot", I64), ("v_head", I64),
+    ]
+
+
+class RopeDesc(ctypes.Structure):
+    """warp_rope_desc (include/warp_cuda.h)."""
+    _fields_ = [
+        ("tokens", I), ("q_heads", I), ("kv_heads", I), ("head_dim", I),
+        ("type", I), ("out_type", I), ("q", P), ("k", P), ("v", P),
+        ("q_token", I64), ("q_head", I64), ("k_token", I64), ("k_head", I64),
+        ("v_token", I64), ("v_head", I64), ("q_out", P), ("k_out", P),
+        ("q_norm", P), ("k_norm", P), ("eps", F), ("inv_freq", P),
+        ("rot_dim", I), ("interleaved", I), ("rot_scale", F), ("positions", P),
+    ]
+
+
+class AttnDesc(ctypes.Structure):
+    """warp_attn_desc (include/warp_cuda.h)."""
+    _fields_ = [
+        ("batch", I), ("tokens", I), ("q_heads", I), ("kv_heads", I), ("head_dim", I),
+        ("type", I), ("q", P), ("q_token", I64), ("q_head", I64), ("out", P),
+        ("q_start", P), ("kv_len", P), ("pages", P), ("pages_row", I64), ("pages_per_row", I),
+        ("max_q", I), ("max_kv", I), ("causal", I), ("scale", F),
+        ("prefix_pages", P), ("prefix_len", I),
     ]
 
 

@@ -12,10 +12,20 @@ Names follow the reference functions whose arithmetic each call computes:
     qwen_moe_route  waste_qwen_moe_route    (src/qwen_moe.c:10-44)
     MoELayer        qwen_moe_layer / moe_layer (model.c:8180, 5488)
 
+The attention half of a decoder block, which the reference computes per model
+family on the CPU, is served by operators of its own shape:
+
+    rope_inv_freq   rotary frequencies, plain or stretched for long contexts
+    qk_norm_rope    norms of queries and keys for each head, and the rotation
+    kv_slots        where a step's tokens go in the pages, once for all layers
+    kv_append       qk_norm_rope with keys and values written to the pages
+    paged_attention attention over the pages, with or without a shared prefix
+
 Every tensor argument must already be on the CUDA device; calls are
 asynchronous on torch's current stream.  A failure raises ffi.WarpError.
 """
 import ctypes
+import math
 
 import torch
 
@@ -160,6 +170,246 @@ def rmsnorm(x, w=None, eps=1e-6, out=None):
     ffi.check(ffi.load().warp_rmsnorm(_p(x2), _p(w), _p(out), x2.shape[0], x2.shape[1],
                                       eps, _stream()))
     return out
+
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def rope_inv_freq(rot_dim, base=10000.0, scaling="none", factor=1.0, trained=None,
+                  beta_fast=32.0, beta_slow=1.0, device=None):
+    """(inv_freq, rot_scale): fp64 radians a position for each of rot_dim/2
+    pairs, base^(-2i/rot_dim), and the factor on cos and sin.  scaling:
+
+        "none"    as it is
+        "linear"  positions divided by `factor`
+        "ntk"     base * factor^(rot_dim/(rot_dim-2))
+        "yarn"    pairs that turn more than beta_fast times over `trained`
+                  positions as they are, fewer than beta_slow divided by
+                  `factor`, a ramp between; rot_scale 0.1 ln(factor) + 1
+    """
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and at least 2")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if scaling != "none" and not factor >= 1.0:
+        raise ValueError("factor must be at least 1")
+    if scaling == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs rot_dim above 2")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = float(base) ** -(torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        if not trained:
+            raise ValueError("yarn scaling needs the trained context length")
+
+        def pair(turns):
+            return rot_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+        lo = max(0, math.floor(pair(beta_fast)))
+        hi = min(rot_dim - 1, math.ceil(pair(beta_slow)))
+        i = torch.arange(rot_dim // 2, dtype=torch.float64)
+        ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        f = f * (1 - ramp) + f / factor * ramp
+        scale = 0.1 * math.log(factor) + 1.0
+    return f.to(device), scale
+
+
+def _heads3(x, name):
+    if x.dim() != 3 or x.dtype not in _TYPES:
+        raise ValueError(f"{name} must be [tokens][heads][head_dim], fp32, fp16 or bf16")
+    # the stride of an axis of one entry has no meaning, and may be anything
+    if x.shape[2] > 1 and x.stride(2) != 1:
+        raise ValueError(f"{name}: the values of a head must be contiguous")
+    return (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+
+
+def _of(x, dtype, name, shape=None, device=None):
+    if x.dtype != dtype or not x.is_contiguous() or (shape is not None and x.shape != shape):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor"
+                         + (f" of shape {tuple(shape)}" if shape is not None else ""))
+    return x
+
+
+def _rope_desc(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
+               out_dtype):
+    _cuda(q, k, v, positions, inv_freq, q_norm, k_norm)
+    d = ffi.RopeDesc()
+    x = q if q is not None else k
+    if x is None:
+        raise ValueError("neither queries nor keys")
+    T, _, D = x.shape if x.dim() == 3 else (0, 0, 0)
+    d.tokens, d.head_dim = T, D
+    d.type, d.out_type = _TYPES.get(x.dtype, -1), _TYPES.get(out_dtype, -1)
+    if q is not None:
+        d.q_token, d.q_head = _heads3(q, "q")
+        d.q, d.q_heads = q.data_ptr(), q.shape[1]
+    if k is not None:
+        d.k_token, d.k_head = _heads3(k, "k")
+        d.k, d.kv_heads = k.data_ptr(), k.shape[1]
+        if k.shape[0] != T or k.shape[2] != D or k.dtype != x.dtype:
+            raise ValueError("k must have q's tokens, head_dim and dtype")
+    if v is not None:
+        d.v_token, d.v_head = _heads3(v, "v")
+        d.v = v.data_ptr()
+        if k is None or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("v must have k's shape and dtype")
+    if inv_freq is not None:
+        _of(inv_freq, torch.float64, "inv_freq")
+        _of(positions, torch.int32, "positions", (T,))
+        d.inv_freq, d.positions = inv_freq.data_ptr(), positions.data_ptr()
+        d.rot_dim = 2 * inv_freq.numel()
+    if q_norm is not None:
+        d.q_norm = _of(q_norm, torch.float32, "q_norm", (D,)).data_ptr()
+    if k_norm is not None:
+        d.k_norm = _of(k_norm, torch.float32, "k_norm", (D,)).data_ptr()
+    d.eps, d.interleaved, d.rot_scale = eps, int(interleaved), rot_scale
+    return d
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6,
+                 interleaved=False, rot_scale=1.0, out_dtype=None):
+    """Per-head RMSNorm (with q_norm / k_norm, fp32 [head_dim]) and rotary
+    positions of queries and keys in one launch (warp_qk_norm_rope).
+
+    q [T][Hq][D] and k [T][Hk][D], any strides with contiguous heads (parts of
+    one projection's rows, say); either may be None.  positions int32 [T];
+    inv_freq fp64 [R/2] rotates the first R dimensions (rope_inv_freq; None:
+    no rotation).  Returns contiguous (q_out, k_out) in out_dtype: the inputs'
+    own, or any for fp32 inputs."""
+    x = q if q is not None else k
+    out_dtype = out_dtype or (x.dtype if x is not None else None)
+    d = _rope_desc(q, k, None, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
+                   out_dtype)
+    q_out = k_out = None
+    if q is not None:
+        q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        d.q_out = q_out.data_ptr()
+    if k is not None:
+        k_out = torch.empty(k.shape, dtype=out_dtype, device=k.device)
+        d.k_out = k_out.data_ptr()
+    ffi.check(ffi.load().warp_qk_norm_rope(ctypes.byref(d), _stream()))
+    return q_out, k_out
+
+
+def _pages(k_pages, v_pages):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must be [pages][page_size][kv_heads][head_dim] "
+                         "of one shape and dtype")
+    n, size, heads, dim = k_pages.shape
+    if dim > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
+        raise ValueError("the values of a head must be contiguous in the pages")
+    c = ffi.KVPages()
+    c.k, c.v, c.type = k_pages.data_ptr(), v_pages.data_ptr(), _TYPES.get(k_pages.dtype, -1)
+    c.pages, c.page_size, c.kv_heads, c.head_dim = n, size, heads, dim
+    one = [s if e > 1 else 0 for s, e in zip(k_pages.stride(), k_pages.shape)]
+    c.k_page, c.k_slot, c.k_head = one[:3]
+    one = [s if e > 1 else 0 for s, e in zip(v_pages.stride(), v_pages.shape)]
+    c.v_page, c.v_slot, c.v_head = one[:3]
+    return c
+
+
+def kv_append(q, k, v, k_pages, v_pages, slots, positions, inv_freq, q_norm=None, k_norm=None,
+              eps=1e-6, interleaved=False, rot_scale=1.0):
+    """qk_norm_rope with the keys' results and the values written to the pages
+    in the same launch (warp_kv_append); returns q's result, in the pages'
+    dtype (None for q None).
+
+    k_pages / v_pages [pages][page_size][Hk][D], fp16 or bf16, any strides with
+    contiguous heads (a transposed [pages][Hk][page_size][D], say); slots int64
+    [T]: token t's slot (page * page_size + offset; negative: not stored), as
+    kv_slots makes them."""
+    _cuda(k_pages, v_pages, slots)
+    c = _pages(k_pages, v_pages)
+    if k is None or v is None:
+        raise ValueError("kv_append needs keys and values")
+    d = _rope_desc(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
+                   k_pages.dtype)
+    _of(slots, torch.int64, "slots", (d.tokens,))
+    q_out = None
+    if q is not None:
+        q_out = torch.empty(q.shape, dtype=k_pages.dtype, device=q.device)
+        d.q_out = q_out.data_ptr()
+    ffi.check(ffi.load().warp_kv_append(ctypes.byref(d), ctypes.byref(c), _p(slots), _stream()))
+    return q_out
+
+
+def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
+    """(positions int32 [T], slots int64 [T]) of a step's tokens for kv_append
+    (warp_kv_slots): q_start int32 [B+1], kv_len int32 [B] own keys with the
+    new ones counted, pages int32 [B][n]; base: the shared prefix's length."""
+    _cuda(q_start, kv_len, pages)
+    B = kv_len.numel()
+    _of(kv_len, torch.int32, "kv_len", (B,))
+    _of(q_start, torch.int32, "q_start", (B + 1,))
+    row, wide = _page_table(pages, B)
+    positions = torch.empty(tokens, dtype=torch.int32, device=q_start.device)
+    slots = torch.empty(tokens, dtype=torch.int64, device=q_start.device)
+    ffi.check(ffi.load().warp_kv_slots(_p(q_start), _p(kv_len), B, tokens, _p(pages), row, wide,
+                                       page_size, base, _p(positions), _p(slots), _stream()))
+    return positions, slots
+
+
+def _page_table(pages, batch):
+    if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != batch or \
+            (pages.shape[1] > 1 and pages.stride(1) != 1):
+        raise ValueError("pages must be int32 [batch][pages a request], rows contiguous")
+    return (pages.stride(0) if batch > 1 else 0), pages.shape[1]
+
+
+def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale=None,
+                    causal=True, prefix_pages=None, prefix_len=0, out=None):
+    """Attention of ragged queries over paged keys and values
+    (warp_paged_attention).
+
+    q [T][Hq][D] fp16 or bf16, D 64 or 128; k_pages / v_pages as for
+    kv_append, Hq a multiple of Hk.  Request b owns tokens q_start[b] ..
+    q_start[b+1]-1 and kv_len[b] keys in the pages of pages[b] (all int32 on
+    the device); max_q and max_kv bound both on the host.  causal: the queries
+    are the request's last positions; False: every query sees every key.  With
+    prefix_len, all queries also see the first prefix_len keys of prefix_pages
+    (int32 [n]), before their own.  A query that sees nothing gets zeros.
+    scale: 1/sqrt(D) by default.  Returns [T][Hq][D] in q's dtype."""
+    _cuda(q, k_pages, v_pages, pages, kv_len, q_start, prefix_pages)
+    c = _pages(k_pages, v_pages)
+    d = ffi.AttnDesc()
+    d.q_token, d.q_head = _heads3(q, "q")
+    T, Hq, D = q.shape
+    B = kv_len.numel()
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and dtype")
+    _of(kv_len, torch.int32, "kv_len", (B,))
+    _of(q_start, torch.int32, "q_start", (B + 1,))
+    d.pages_row, d.pages_per_row = _page_table(pages, B)
+    d.batch, d.tokens, d.q_heads, d.kv_heads, d.head_dim = B, T, Hq, c.kv_heads, D
+    d.type = _TYPES[q.dtype]
+    d.q, d.out, d.pages = q.data_ptr(), out.data_ptr(), pages.data_ptr()
+    d.q_start, d.kv_len = q_start.data_ptr(), kv_len.data_ptr()
+    d.max_q, d.max_kv, d.causal = max_q, max_kv, int(causal)
+    d.scale = 1.0 / math.sqrt(D) if scale is None else scale
+    if prefix_len:
+        if prefix_pages is None or prefix_len > prefix_pages.numel() * c.page_size:
+            raise ValueError("prefix_pages hold fewer than prefix_len keys")
+        d.prefix_pages = _of(prefix_pages, torch.int32, "prefix_pages").data_ptr()
+        d.prefix_len = prefix_len
+    lib = ffi.load()
+    need = lib.warp_attn_scratch(ctypes.byref(d), ctypes.byref(c))
+    if need < 0:
+        ffi.check(need)
+    # from torch's allocator: ordered by the stream, and private to a graph
+    # where one is being captured
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ffi.check(lib.warp_paged_attention(ctypes.byref(d), ctypes.byref(c), _p(scratch), _stream()))
+    return out
+
+
+def attn_status(clear=True):
+    """Raises if an attention kernel left something out (a page or slot out of
+    range, a length over its bound, a wait that gave up) since the last clear."""
+    ffi.check(ffi.load().warp_attn_status(int(clear)))
 
 
 class MoELayer:
