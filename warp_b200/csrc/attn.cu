@@ -62,22 +62,6 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src
                  ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *(const uint32_t *)&h;
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *(const uint32_t *)&h;
-}
-
 template <typename T> struct F16Bits;
 template <> struct F16Bits<__half> { static constexpr uint32_t exp = 0x7c00u, one = 0x3c00u; };
 template <> struct F16Bits<__nv_bfloat16> { static constexpr uint32_t exp = 0x7f80u, one = 0x3f80u; };
@@ -117,11 +101,6 @@ __device__ __forceinline__ void mend_values(uint32_t &b0, uint32_t &b1, const ui
     }
 }
 
-// How many parts a range of `tiles` key tiles is split into, `each` tiles a part.
-__device__ __forceinline__ int attn_parts(int tiles, int each) {
-    return (tiles + each - 1) / each;
-}
-
 template <int D> struct ADLay {
     static constexpr int row_bytes = D * 2;
     static constexpr int tile_bytes = kAttnTile * row_bytes;
@@ -157,7 +136,7 @@ __global__ void __launch_bounds__(kADWarps * 32, 2) attn_rows_kernel(const AttnA
         row0 = (blockIdx.x / parts_max) * kADRows;
     }
     const int rows = rq.n * a.group;
-    if (row0 >= rows) return;
+    if (row0 >= rows || (!PACKED && rows > a.rows_small)) return;
     const int n_pre = PACKED || !a.packed ? a.prefix_len : 0;
     pre_tiles = (n_pre + kAttnTile - 1) / kAttnTile;
     // own keys that the tile's last row sees
@@ -422,9 +401,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     if (b < 0) return;
     const AttnReq rq = attn_req(a, b);
     if (t >= rq.t0 + rq.n) return;
-    const int own = (a.packed ? 0 : (a.prefix_len + kAttnTile - 1) / kAttnTile) +
-                    (rq.len + kAttnTile - 1) / kAttnTile;
-    int parts = max(1, attn_parts(own, a.split_tiles));
+    const bool wide = rq.n * a.group > a.rows_small;
+    const int tile = wide ? kAttnWide : kAttnTile;
+    const int own = (a.packed ? 0 : (a.prefix_len + tile - 1) / tile) + (rq.len + tile - 1) / tile;
+    int parts = max(1, attn_parts(own, wide ? a.wide_each : a.split_tiles));
     if (!a.packed && parts == 1) return;
     parts += a.prefix_parts;
     constexpr int V = D / 32;
@@ -463,24 +443,41 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 // ------------------------------------------------------------ host side --
 
 struct AttnPlan {
-    int packed, prefix_parts, prefix_split_tiles;
-    int split_tiles, parts;                 // own parts at most
+    int packed, packed_wide, prefix_parts, prefix_each;
+    int rows_small;
+    int each, parts;                        // own parts at most, attn_rows_kernel
+    int wide_each, wide_parts;              // and attn_umma_kernel (0 parts: not run)
+    int small_tiles;                        // row tiles a request, attn_rows_kernel (0: not run)
+    int join;
     int64_t o_bytes, ml_bytes;
     int max_q, max_kv;                      // the host's bounds, no wider than tokens and pages
 };
 
-static int tiles_of(int64_t keys) { return (int)((keys + kAttnTile - 1) / kAttnTile); }
+static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Key tiles a CTA: enough CTAs to fill the card twice over where there are
-// keys enough, no fewer than 16 tiles (4 a warp).
+// Key tiles a part of attn_rows_kernel: CTAs enough to fill the card twice
+// over where there are keys enough, no fewer than 16 tiles (4 a warp).
 static int pick_split(int64_t tiles, int64_t ctas) {
     const int64_t want = 2 * 2 * 148;
     ctas = ctas < 1 ? 1 : ctas;
-    int64_t parts = (want + ctas - 1) / ctas;
-    parts = parts < 1 ? 1 : parts > 256 ? 256 : parts;
-    int64_t each = (tiles + parts - 1) / parts;
-    if (each < 16) each = 16;
-    return (int)each;
+    int64_t parts = up(want, ctas);
+    parts = parts > 256 ? 256 : parts;
+    const int64_t each = up(tiles, parts);
+    return (int)(each < 16 ? 16 : each);
+}
+
+// Key tiles a part of attn_umma_kernel, one CTA an SM: the split with the
+// fewest tiles in a row on the busiest SM, counting a part's start, end and
+// join as the like of three tiles.
+static int pick_wide(int64_t tiles, int64_t ctas) {
+    ctas = ctas < 1 ? 1 : ctas;
+    int64_t best = tiles < 1 ? 1 : tiles, cost = up(ctas, 148) * (tiles + 3);
+    for (int64_t parts = 2; parts <= 64 && parts * 2 <= tiles; parts++) {
+        const int64_t each = up(tiles, parts);
+        const int64_t now = up(ctas * up(tiles, each), 148) * (each + 3) + 3;
+        if (now < cost) best = each, cost = now;
+    }
+    return (int)best;
 }
 
 static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
@@ -488,25 +485,40 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     p.max_q = d->max_q < d->tokens ? d->max_q : d->tokens;
     const int64_t held = (int64_t)d->pages_per_row * c->page_size;
     p.max_kv = d->max_kv < held ? d->max_kv : (int)held;
-    const int group = d->q_heads / d->kv_heads;
+    const int64_t group = d->q_heads / d->kv_heads;
     // The prefix apart, for all rows at once, where a request's rows alone
     // would leave a row tile mostly empty.
-    p.packed = d->prefix_len > 0 && d->batch > 1 &&
-               (int64_t)d->tokens * group <= (int64_t)128 * d->batch;
-    const int64_t row_tiles = ((int64_t)p.max_q * group + kADRows - 1) / kADRows;
-    const int64_t own = tiles_of(p.max_kv) + (p.packed ? 0 : tiles_of(d->prefix_len));
-    p.split_tiles = pick_split(own, (int64_t)d->batch * d->kv_heads * row_tiles);
-    p.parts = own ? (int)((own + p.split_tiles - 1) / p.split_tiles) : 1;
-    if (p.packed) {
-        const int64_t tiles = tiles_of(d->prefix_len);
-        const int64_t rt = ((int64_t)d->tokens * group + kADRows - 1) / kADRows;
-        p.prefix_split_tiles = pick_split(tiles, rt * d->kv_heads);
-        p.prefix_parts = (int)((tiles + p.prefix_split_tiles - 1) / p.prefix_split_tiles);
+    p.packed = d->prefix_len > 0 && d->batch > 1 && d->tokens * group <= (int64_t)128 * d->batch;
+    const int pre = p.packed ? 0 : d->prefix_len;
+    const int64_t rows = p.max_q * group;
+    // A single request's rows are known to be more than a few: all of them wide.
+    p.rows_small = d->batch == 1 && rows > kADRows ? 0 : kADRows;
+    if (rows > p.rows_small) {
+        const int64_t pairs = up(rows, 256) * d->batch, by_tokens = up(d->tokens * group, 256);
+        const int64_t ctas = pairs < by_tokens + d->batch - 1 ? pairs : by_tokens + d->batch - 1;
+        const int64_t tiles = up(p.max_kv, kAttnWide) + up(pre, kAttnWide);
+        p.wide_each = pick_wide(tiles, ctas * d->kv_heads);
+        p.wide_parts = tiles ? (int)up(tiles, p.wide_each) : 1;
     }
-    const int all = p.prefix_parts + (p.packed || p.parts > 1 ? p.parts : 0);
-    const int64_t rows = (int64_t)d->tokens * d->q_heads;
-    p.o_bytes = (all * rows * d->head_dim * 4 + 255) / 256 * 256;
-    p.ml_bytes = (all * rows * 8 + 255) / 256 * 256;
+    if (p.rows_small) {
+        const int64_t tiles = up(p.max_kv, kAttnTile) + up(pre, kAttnTile);
+        p.small_tiles = (int)up(rows < p.rows_small ? rows : p.rows_small, kADRows);
+        p.each = pick_split(tiles, (int64_t)d->batch * d->kv_heads * p.small_tiles);
+        p.parts = tiles ? (int)up(tiles, p.each) : 1;
+    }
+    if (p.packed) {
+        const int64_t all = d->tokens * group;
+        p.packed_wide = all > kADRows;
+        const int64_t tiles = up(d->prefix_len, p.packed_wide ? kAttnWide : kAttnTile);
+        p.prefix_each = p.packed_wide ? pick_wide(tiles, up(all, 256) * d->kv_heads)
+                                      : pick_split(tiles, up(all, kADRows) * d->kv_heads);
+        p.prefix_parts = (int)up(tiles, p.prefix_each);
+    }
+    const int own = p.parts > p.wide_parts ? p.parts : p.wide_parts;
+    p.join = p.packed || own > 1;
+    const int64_t all = p.join ? p.prefix_parts + own : 0, out = (int64_t)d->tokens * d->q_heads;
+    p.o_bytes = up(all * out * d->head_dim * 4, 256) * 256;
+    p.ml_bytes = up(all * out * 8, 256) * 256;
     return p;
 }
 
@@ -548,18 +560,19 @@ static int attn_launch(const AttnArgs &a, const AttnPlan &p, cudaStream_t st) {
         if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
         attr_done = true;
     }
-    if (a.packed) {
-        const int64_t rt = ((int64_t)a.tokens * a.group + kADRows - 1) / kADRows;
+    if (p.packed && !p.packed_wide) {
         attn_rows_kernel<T, D, true>
-            <<<dim3((unsigned)(rt * p.prefix_parts), a.kv_heads, 1), kADWarps * 32, Lay::bytes,
-               st>>>(a);
+            <<<dim3((unsigned)(up((int64_t)a.tokens * a.group, kADRows) * p.prefix_parts),
+                    a.kv_heads, 1), kADWarps * 32, Lay::bytes, st>>>(a);
         WARP_CHECK_LAUNCH("attn_rows_kernel (prefix)");
     }
-    const int64_t rt = ((int64_t)a.max_q * a.group + kADRows - 1) / kADRows;
-    attn_rows_kernel<T, D, false>
-        <<<dim3((unsigned)(rt * p.parts), a.kv_heads, a.batch), kADWarps * 32, Lay::bytes, st>>>(a);
-    WARP_CHECK_LAUNCH("attn_rows_kernel");
-    if (a.packed || p.parts > 1) {
+    if (p.small_tiles) {
+        attn_rows_kernel<T, D, false>
+            <<<dim3(p.small_tiles * p.parts, a.kv_heads, a.batch), kADWarps * 32, Lay::bytes,
+               st>>>(a);
+        WARP_CHECK_LAUNCH("attn_rows_kernel");
+    }
+    if (p.join) {
         attn_join_kernel<T, D>
             <<<cdiv((size_t)a.tokens * a.q_heads, 8), 256, 0, st>>>(a);
         WARP_CHECK_LAUNCH("attn_join_kernel");
@@ -608,10 +621,15 @@ extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages
     a.part_o = (float *)scratch;
     a.part_ml = (float2 *)((char *)scratch + p.o_bytes);
     a.packed = p.packed, a.prefix_parts = p.prefix_parts;
-    a.split_tiles = p.split_tiles, a.prefix_split_tiles = p.prefix_split_tiles;
+    a.rows_small = p.rows_small;
+    a.split_tiles = p.each, a.wide_each = p.wide_each, a.wide_parts = p.wide_parts;
+    a.prefix_split_tiles = a.prefix_wide_each = p.prefix_each;
     rc = warp::attn_err_word(&a.err);
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
+    if (p.packed_wide) rc = warp::attn_umma(a, c, true, st);
+    if (!rc && p.wide_parts) rc = warp::attn_umma(a, c, false, st);
+    if (rc) return rc;
     if (d->type == WARP_T_F16)
         return d->head_dim == 64 ? warp::attn_launch<__half, 64>(a, p, st)
                                  : warp::attn_launch<__half, 128>(a, p, st);

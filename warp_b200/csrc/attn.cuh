@@ -50,8 +50,13 @@ struct AttnArgs {
     float *part_o;
     float2 *part_ml;
     int packed, prefix_parts;
+    // Requests with more rows a kv head than rows_small go to attn_umma_kernel,
+    // which counts keys in tiles of kAttnWide; the others to attn_rows_kernel.
+    int rows_small;
     int split_tiles;                        // key tiles of a request's part
     int prefix_split_tiles;                 // and of a part of the prefix
+    int wide_each, wide_parts;              // the same for attn_umma_kernel: wide tiles
+    int prefix_wide_each;                   // of a part, and parts at most
 };
 
 // Request b as the host's bounds leave it: its first token, its queries and
@@ -82,5 +87,31 @@ __device__ __forceinline__ int attn_page(const AttnArgs &a, const int32_t *table
 // Keys come in tiles of kAttnTile; the prefix's last tile and a request's last
 // one may be partly filled, and a tile never mixes the two.
 constexpr int kAttnTile = 16;
+constexpr int kAttnWide = 128;
+
+// How many parts a range of `tiles` key tiles is split into, `each` tiles a part.
+__device__ __forceinline__ int attn_parts(int tiles, int each) {
+    return (tiles + each - 1) / each;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const uint32_t *)&h;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t *)&h;
+}
+
+// The tensor-core kernel: the requests with many rows, or (packed) the shared
+// prefix for all rows of the batch.
+int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, cudaStream_t st);
 
 }  // namespace warp
