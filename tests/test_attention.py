@@ -128,6 +128,17 @@ def test_attention_nothing_to_do(lib):
         assert lib.warp_paged_attention(ctypes.byref(d), ctypes.byref(kv_pages()), None, None) == 0
 
 
+@pytest.mark.parametrize("fmt, cls", [("KV_PAGES", "KVPages"), ("ROPE_DESC", "RopeDesc"),
+                                      ("ATTN_DESC", "AttnDesc")])
+def test_packed_descriptions_match_the_structures(fmt, cls):
+    fmt, cls = getattr(ffi, fmt), getattr(ffi, cls)
+    values = list(range(1, len(cls._fields_) + 1))
+    raw = fmt.pack(*values)
+    assert fmt.size == ctypes.sizeof(cls)
+    d = cls.from_buffer_copy(raw)
+    assert [getattr(d, name) for name, _ in cls._fields_] == values
+
+
 def test_slots_refusals(lib):
     p = ctypes.c_void_p(256)
     assert lib.warp_kv_slots(p, p, 1, 1, p, 4, 4, 12, 0, p, p, None) == -1

@@ -5,6 +5,7 @@ never falls back to anything: a missing or unloadable library raises.
 """
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libwarp_cuda.so")
@@ -127,6 +128,14 @@ class AttnDesc(ctypes.Structure):
         ("max_q", I), ("max_kv", I), ("causal", I), ("scale", F),
         ("prefix_pages", P), ("prefix_len", I),
     ]
+
+
+# The three descriptions above as struct formats (native alignment), for
+# callers that fill one per call: packing is several times cheaper than setting
+# a Structure's fields one by one.
+KV_PAGES = struct.Struct("@PP4iq6q")
+ROPE_DESC = struct.Struct("@6iPPP6qPPPPfPiifP")
+ATTN_DESC = struct.Struct("@6iPqqPPPPqiiiifPi0P")
 
 
 _lib = None

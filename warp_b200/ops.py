@@ -38,7 +38,8 @@ def _p(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # torch.cuda.current_stream().cuda_stream without the Stream object around it
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _cuda(*ts):
@@ -216,56 +217,81 @@ def rope_inv_freq(rot_dim, base=10000.0, scaling="none", factor=1.0, trained=Non
     return f.to(device), scale
 
 
-def _heads3(x, name):
-    if x.dim() != 3 or x.dtype not in _TYPES:
-        raise ValueError(f"{name} must be [tokens][heads][head_dim], fp32, fp16 or bf16")
-    # the stride of an axis of one entry has no meaning, and may be anything
-    if x.shape[2] > 1 and x.stride(2) != 1:
-        raise ValueError(f"{name}: the values of a head must be contiguous")
-    return (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+def _raise_bad(checks):
+    """The first check that fails, as a ValueError."""
+    for ok, text in checks:
+        if not ok:
+            raise ValueError(text)
+    raise ValueError("unusable arguments")
 
 
-def _of(x, dtype, name, shape=None, device=None):
-    if x.dtype != dtype or not x.is_contiguous() or (shape is not None and x.shape != shape):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor"
-                         + (f" of shape {tuple(shape)}" if shape is not None else ""))
-    return x
+def _rows_ok(x, T, D, dtype):
+    """[T][heads][D] on the device with contiguous heads."""
+    return x.dim() == 3 and x.is_cuda and x.dtype is dtype and x.shape[0] == T and \
+        x.shape[2] == D and (D < 2 or x.stride(2) == 1)
 
 
-def _rope_desc(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
-               out_dtype):
-    _cuda(q, k, v, positions, inv_freq, q_norm, k_norm)
-    d = ffi.RopeDesc()
+def _vec_ok(x, n, dtype):
+    return x.dtype is dtype and x.numel() == n and x.is_contiguous() and x.is_cuda
+
+
+def _strides(x):
+    """Token and head strides; that of an axis of one entry has no meaning."""
+    (a, b, _), (m, n, _) = x.stride(), x.shape
+    return a if m > 1 else 0, b if n > 1 else 0
+
+
+def _rope_pack(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale, q_out,
+               k_out, out_dtype):
     x = q if q is not None else k
     if x is None:
         raise ValueError("neither queries nor keys")
-    T, _, D = x.shape if x.dim() == 3 else (0, 0, 0)
-    d.tokens, d.head_dim = T, D
-    d.type, d.out_type = _TYPES.get(x.dtype, -1), _TYPES.get(out_dtype, -1)
+    if x.dim() != 3 or x.dtype not in _TYPES:
+        raise ValueError("queries and keys must be [tokens][heads][head_dim], fp32, fp16 or bf16")
+    T, _, D = x.shape
+    dt = x.dtype
+    if not ((q is None or _rows_ok(q, T, D, dt)) and (k is None or _rows_ok(k, T, D, dt)) and
+            (v is None or (_rows_ok(v, T, D, dt) and v.shape[1] == k.shape[1])) and
+            (inv_freq is None or (inv_freq.dtype is torch.float64 and inv_freq.is_cuda and
+                                  inv_freq.is_contiguous() and positions is not None and
+                                  _vec_ok(positions, T, torch.int32))) and
+            (q_norm is None or _vec_ok(q_norm, D, torch.float32)) and
+            (k_norm is None or _vec_ok(k_norm, D, torch.float32))):
+        _cuda(q, k, v, positions, inv_freq, q_norm, k_norm)
+        rows = "must be [tokens][heads][head_dim] with contiguous heads, of one dtype"
+        _raise_bad([
+            (q is None or _rows_ok(q, T, D, dt), "q " + rows),
+            (k is None or _rows_ok(k, T, D, dt), "k " + rows + ", as q's"),
+            (v is None or (_rows_ok(v, T, D, dt) and v.shape[1] == k.shape[1]),
+             "v " + rows + ", as k's"),
+            (inv_freq is None or (inv_freq.dtype is torch.float64 and inv_freq.is_contiguous()),
+             "inv_freq must be contiguous float64"),
+            (inv_freq is None or (positions is not None and _vec_ok(positions, T, torch.int32)),
+             "positions must be contiguous int32 [tokens]"),
+            (q_norm is None or _vec_ok(q_norm, D, torch.float32),
+             "q_norm must be contiguous float32 [head_dim]"),
+            (k_norm is None or _vec_ok(k_norm, D, torch.float32),
+             "k_norm must be contiguous float32 [head_dim]")])
+    qt = qh = kt = kh = vt = vh = nq = nk = qp = kp = vp = 0
     if q is not None:
-        d.q_token, d.q_head = _heads3(q, "q")
-        d.q, d.q_heads = q.data_ptr(), q.shape[1]
+        (qt, qh), nq, qp = _strides(q), q.shape[1], q.data_ptr()
     if k is not None:
-        d.k_token, d.k_head = _heads3(k, "k")
-        d.k, d.kv_heads = k.data_ptr(), k.shape[1]
-        if k.shape[0] != T or k.shape[2] != D or k.dtype != x.dtype:
-            raise ValueError("k must have q's tokens, head_dim and dtype")
+        (kt, kh), nk, kp = _strides(k), k.shape[1], k.data_ptr()
     if v is not None:
-        d.v_token, d.v_head = _heads3(v, "v")
-        d.v = v.data_ptr()
-        if k is None or v.shape != k.shape or v.dtype != k.dtype:
-            raise ValueError("v must have k's shape and dtype")
-    if inv_freq is not None:
-        _of(inv_freq, torch.float64, "inv_freq")
-        _of(positions, torch.int32, "positions", (T,))
-        d.inv_freq, d.positions = inv_freq.data_ptr(), positions.data_ptr()
-        d.rot_dim = 2 * inv_freq.numel()
-    if q_norm is not None:
-        d.q_norm = _of(q_norm, torch.float32, "q_norm", (D,)).data_ptr()
-    if k_norm is not None:
-        d.k_norm = _of(k_norm, torch.float32, "k_norm", (D,)).data_ptr()
-    d.eps, d.interleaved, d.rot_scale = eps, int(interleaved), rot_scale
-    return d
+        (vt, vh), vp = _strides(v), v.data_ptr()
+    rot = positions is not None and inv_freq is not None
+    return ffi.ROPE_DESC.pack(
+        T, nq, nk, D, _TYPES[dt], _TYPES.get(out_dtype, -1), qp, kp, vp, qt, qh, kt, kh, vt, vh,
+        q_out.data_ptr() if q_out is not None else 0, k_out.data_ptr() if k_out is not None else 0,
+        q_norm.data_ptr() if q_norm is not None else 0,
+        k_norm.data_ptr() if k_norm is not None else 0, eps, inv_freq.data_ptr() if rot else 0,
+        2 * inv_freq.numel() if rot else 0, interleaved, rot_scale,
+        positions.data_ptr() if rot else 0)
+
+
+def _dense(x, dtype):
+    """A new contiguous tensor of x's shape."""
+    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6,
@@ -278,36 +304,30 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6,
     inv_freq fp64 [R/2] rotates the first R dimensions (rope_inv_freq; None:
     no rotation).  Returns contiguous (q_out, k_out) in out_dtype: the inputs'
     own, or any for fp32 inputs."""
-    x = q if q is not None else k
-    out_dtype = out_dtype or (x.dtype if x is not None else None)
-    d = _rope_desc(q, k, None, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
-                   out_dtype)
-    q_out = k_out = None
-    if q is not None:
-        q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-        d.q_out = q_out.data_ptr()
-    if k is not None:
-        k_out = torch.empty(k.shape, dtype=out_dtype, device=k.device)
-        d.k_out = k_out.data_ptr()
-    ffi.check(ffi.load().warp_qk_norm_rope(ctypes.byref(d), _stream()))
+    if out_dtype is None and (q is not None or k is not None):
+        out_dtype = (q if q is not None else k).dtype
+    q_out = None if q is None else _dense(q, out_dtype)
+    k_out = None if k is None else _dense(k, out_dtype)
+    d = _rope_pack(q, k, None, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
+                   q_out, k_out, out_dtype)
+    ffi.check(ffi.load().warp_qk_norm_rope(d, _stream()))
     return q_out, k_out
 
 
-def _pages(k_pages, v_pages):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+def _pages_pack(k_pages, v_pages):
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or \
+            not k_pages.is_cuda or not v_pages.is_cuda or \
+            (shape[3] > 1 and (ks[3] != 1 or vs[3] != 1)):
+        _cuda(k_pages, v_pages)
         raise ValueError("k_pages and v_pages must be [pages][page_size][kv_heads][head_dim] "
-                         "of one shape and dtype")
-    n, size, heads, dim = k_pages.shape
-    if dim > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
-        raise ValueError("the values of a head must be contiguous in the pages")
-    c = ffi.KVPages()
-    c.k, c.v, c.type = k_pages.data_ptr(), v_pages.data_ptr(), _TYPES.get(k_pages.dtype, -1)
-    c.pages, c.page_size, c.kv_heads, c.head_dim = n, size, heads, dim
-    one = [s if e > 1 else 0 for s, e in zip(k_pages.stride(), k_pages.shape)]
-    c.k_page, c.k_slot, c.k_head = one[:3]
-    one = [s if e > 1 else 0 for s, e in zip(v_pages.stride(), v_pages.shape)]
-    c.v_page, c.v_slot, c.v_head = one[:3]
-    return c
+                         "of one shape and dtype with contiguous heads")
+    n, size, heads, dim = shape
+    if n == 1 or size == 1 or heads == 1:   # the stride of an axis of one entry has no meaning
+        ks, vs = ([s if e > 1 else 0 for s, e in zip(x, shape)] for x in (ks, vs))
+    return ffi.KV_PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(),
+                             _TYPES.get(k_pages.dtype, -1), size, heads, dim, n, ks[0], ks[1],
+                             ks[2], vs[0], vs[1], vs[2])
 
 
 def kv_append(q, k, v, k_pages, v_pages, slots, positions, inv_freq, q_norm=None, k_norm=None,
@@ -320,18 +340,15 @@ def kv_append(q, k, v, k_pages, v_pages, slots, positions, inv_freq, q_norm=None
     contiguous heads (a transposed [pages][Hk][page_size][D], say); slots int64
     [T]: token t's slot (page * page_size + offset; negative: not stored), as
     kv_slots makes them."""
-    _cuda(k_pages, v_pages, slots)
-    c = _pages(k_pages, v_pages)
     if k is None or v is None:
         raise ValueError("kv_append needs keys and values")
-    d = _rope_desc(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
-                   k_pages.dtype)
-    _of(slots, torch.int64, "slots", (d.tokens,))
-    q_out = None
-    if q is not None:
-        q_out = torch.empty(q.shape, dtype=k_pages.dtype, device=q.device)
-        d.q_out = q_out.data_ptr()
-    ffi.check(ffi.load().warp_kv_append(ctypes.byref(d), ctypes.byref(c), _p(slots), _stream()))
+    c = _pages_pack(k_pages, v_pages)
+    q_out = None if q is None else _dense(q, k_pages.dtype)
+    d = _rope_pack(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
+                   q_out, None, k_pages.dtype)
+    if not _vec_ok(slots, k.shape[0], torch.int64):
+        raise ValueError("slots must be contiguous int64 [tokens] on the device")
+    ffi.check(ffi.load().warp_kv_append(d, c, slots.data_ptr(), _stream()))
     return q_out
 
 
@@ -339,23 +356,27 @@ def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
     """(positions int32 [T], slots int64 [T]) of a step's tokens for kv_append
     (warp_kv_slots): q_start int32 [B+1], kv_len int32 [B] own keys with the
     new ones counted, pages int32 [B][n]; base: the shared prefix's length."""
-    _cuda(q_start, kv_len, pages)
-    B = kv_len.numel()
-    _of(kv_len, torch.int32, "kv_len", (B,))
-    _of(q_start, torch.int32, "q_start", (B + 1,))
-    row, wide = _page_table(pages, B)
+    row, wide = _batch(q_start, kv_len, pages)
     positions = torch.empty(tokens, dtype=torch.int32, device=q_start.device)
     slots = torch.empty(tokens, dtype=torch.int64, device=q_start.device)
-    ffi.check(ffi.load().warp_kv_slots(_p(q_start), _p(kv_len), B, tokens, _p(pages), row, wide,
-                                       page_size, base, _p(positions), _p(slots), _stream()))
+    ffi.check(ffi.load().warp_kv_slots(
+        q_start.data_ptr(), kv_len.data_ptr(), kv_len.numel(), tokens, pages.data_ptr(), row, wide,
+        page_size, base, positions.data_ptr(), slots.data_ptr(), _stream()))
     return positions, slots
 
 
-def _page_table(pages, batch):
-    if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != batch or \
-            (pages.shape[1] > 1 and pages.stride(1) != 1):
-        raise ValueError("pages must be int32 [batch][pages a request], rows contiguous")
-    return (pages.stride(0) if batch > 1 else 0), pages.shape[1]
+def _batch(q_start, kv_len, pages):
+    """Checks a batch's device tensors; the page table's row stride and width."""
+    B = kv_len.numel()
+    if not (_vec_ok(kv_len, B, torch.int32) and _vec_ok(q_start, B + 1, torch.int32) and
+            pages.dim() == 2 and pages.is_cuda and pages.dtype is torch.int32 and
+            pages.shape[0] == B and (pages.shape[1] < 2 or pages.stride(1) == 1)):
+        _cuda(q_start, kv_len, pages)
+        _raise_bad([
+            (_vec_ok(kv_len, B, torch.int32), "kv_len must be contiguous int32 [batch]"),
+            (_vec_ok(q_start, B + 1, torch.int32), "q_start must be contiguous int32 [batch + 1]"),
+            (False, "pages must be int32 [batch][pages a request], rows contiguous")])
+    return (pages.stride(0) if B > 1 else 0), pages.shape[1]
 
 
 def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale=None,
@@ -369,40 +390,40 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
     the device); max_q and max_kv bound both on the host.  causal: the queries
     are the request's last positions; False: every query sees every key.  With
     prefix_len, all queries also see the first prefix_len keys of prefix_pages
-    (int32 [n]), before their own.  A query that sees nothing gets zeros.
-    scale: 1/sqrt(D) by default.  Returns [T][Hq][D] in q's dtype."""
-    _cuda(q, k_pages, v_pages, pages, kv_len, q_start, prefix_pages)
-    c = _pages(k_pages, v_pages)
-    d = ffi.AttnDesc()
-    d.q_token, d.q_head = _heads3(q, "q")
+    (int32 [n]), before their own.  A query that sees nothing gets zeros; a
+    token of no request is not written.  scale: 1/sqrt(D) by default.  Returns
+    [T][Hq][D] in q's dtype."""
+    c = _pages_pack(k_pages, v_pages)
+    row, wide = _batch(q_start, kv_len, pages)
+    if q.dim() != 3 or not _rows_ok(q, q.shape[0], q.shape[2], q.dtype) or q.dtype not in _TYPES:
+        _cuda(q)
+        raise ValueError("q must be [tokens][heads][head_dim], fp16 or bf16, with contiguous heads")
     T, Hq, D = q.shape
-    B = kv_len.numel()
+    qt, qh = _strides(q)
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        out = _dense(q, q.dtype)
+    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or \
+            not out.is_cuda:
         raise ValueError("out must be contiguous, of q's shape and dtype")
-    _of(kv_len, torch.int32, "kv_len", (B,))
-    _of(q_start, torch.int32, "q_start", (B + 1,))
-    d.pages_row, d.pages_per_row = _page_table(pages, B)
-    d.batch, d.tokens, d.q_heads, d.kv_heads, d.head_dim = B, T, Hq, c.kv_heads, D
-    d.type = _TYPES[q.dtype]
-    d.q, d.out, d.pages = q.data_ptr(), out.data_ptr(), pages.data_ptr()
-    d.q_start, d.kv_len = q_start.data_ptr(), kv_len.data_ptr()
-    d.max_q, d.max_kv, d.causal = max_q, max_kv, int(causal)
-    d.scale = 1.0 / math.sqrt(D) if scale is None else scale
+    pp = 0
     if prefix_len:
-        if prefix_pages is None or prefix_len > prefix_pages.numel() * c.page_size:
+        if prefix_pages is None or prefix_len > prefix_pages.numel() * k_pages.shape[1]:
             raise ValueError("prefix_pages hold fewer than prefix_len keys")
-        d.prefix_pages = _of(prefix_pages, torch.int32, "prefix_pages").data_ptr()
-        d.prefix_len = prefix_len
+        if not _vec_ok(prefix_pages, prefix_pages.numel(), torch.int32):
+            raise ValueError("prefix_pages must be contiguous int32 [n] on the device")
+        pp = prefix_pages.data_ptr()
+    d = ffi.ATTN_DESC.pack(
+        kv_len.numel(), T, Hq, k_pages.shape[2], D, _TYPES[q.dtype], q.data_ptr(), qt, qh,
+        out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), row, wide, max_q,
+        max_kv, causal, (D or 1) ** -0.5 if scale is None else scale, pp, prefix_len)
     lib = ffi.load()
-    need = lib.warp_attn_scratch(ctypes.byref(d), ctypes.byref(c))
+    need = lib.warp_attn_scratch(d, c)
     if need < 0:
         ffi.check(need)
     # from torch's allocator: ordered by the stream, and private to a graph
     # where one is being captured
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    ffi.check(lib.warp_paged_attention(ctypes.byref(d), ctypes.byref(c), _p(scratch), _stream()))
+    ffi.check(lib.warp_paged_attention(d, c, scratch.data_ptr() if need else None, _stream()))
     return out
 
 
