@@ -532,6 +532,7 @@ static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
              "%s: negative size", who);
     WARP_ARG(d->q_heads >= 1 && d->kv_heads >= 1 && d->q_heads % d->kv_heads == 0,
              "%s: %d query heads over %d kv heads", who, d->q_heads, d->kv_heads);
+    WARP_ARG(d->q_heads <= 65536, "%s: %d query heads", who, d->q_heads);
     WARP_ARG(d->head_dim == 64 || d->head_dim == 128, "%s: head_dim %d is not 64 or 128", who,
              d->head_dim);
     WARP_ARG(c->kv_heads == d->kv_heads && c->head_dim == d->head_dim && c->type == d->type,

@@ -16,12 +16,18 @@
 // factor.
 //
 // What bounds it: per pair of 128 x 128 tiles the products take
-// 2 * 2 * 128 * 128 * D / 8192 FMA a clock = 1024 cycles at D = 128, and
-// 2 * 128 * 128 exponentials at 16 a clock 2048. So a share of them is
-// computed on the FMA pipe instead (ex2_poly).
+// 2 * 2 * 128 * 128 * D / 4096 FMA a clock = 2048 cycles at D = 128 (half at
+// 64), and so do 2 * 128 * 128 exponentials at 16 a clock. A tile's next
+// scores wait for its weights, so what counts is that one tile's softmax fits
+// into the time of the other's products: a share of the exponentials is
+// computed on the FMA pipe (ex2_poly), sums and scalings go two at a time
+// (f32x2), and the first half of a tile's weights is handed over while the
+// second is computed.
 //
-// Warps: 0-3 rows of tile 0, 4-7 rows of tile 1, 8 issues the products, 9
-// loads keys and values by TMA, a box a page, into a ring of tiles.
+// Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each of
+// them with half the keys of a tile (a warp alone on its scheduler spends two
+// thirds of its time on the latency of its own instructions); 16 issues the
+// products; 17 loads keys and values by TMA, a box a page, into a ring of tiles.
 #include "attn.cuh"
 #include "umma.cuh"
 
@@ -32,7 +38,8 @@ namespace {
 
 constexpr int kRows = 128;                  // rows a tile
 constexpr int kKeys = kAttnWide;            // keys a tile
-constexpr int kThreads = 320;
+constexpr int kHalf = kKeys / 2;              // keys of a row that one thread weighs
+constexpr int kThreads = 18 * 32;
 
 template <int D> struct Lay {
     static constexpr int q_tile = kRows * D * 2;
@@ -40,8 +47,9 @@ template <int D> struct Lay {
     static constexpr int half = kKeys * 128;            // 64 columns of a tile
     static constexpr int stages = D == 128 ? 5 : 8;
     static constexpr int ring = 2 * q_tile;
-    static constexpr int bars = ring + stages * kv_tile;
-    static constexpr int bytes = bars + 256 + 1024;     // 1024: alignment of the base
+    static constexpr int swap = ring + stages * kv_tile;  // [tile][half][row] fp32
+    static constexpr int bars = swap + 4 * kRows * 4;
+    static constexpr int bytes = bars + 256;
     // tensor memory columns
     static constexpr int s(int t) { return t * 128; }
     static constexpr int o(int t) { return 256 + t * D; }
@@ -62,15 +70,44 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc(int N, bool b
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 }
 
+// The products and commits are issued by one lane, by predicate rather than by
+// branch: in uniform control flow the descriptors stay in uniform registers,
+// where the instruction wants them.
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b,
+                                       uint32_t id, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"((uint32_t)accumulate), "r"(leader)
+        : "memory");
+}
 // A from tensor memory.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
-                                       bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b,
+                                       uint32_t id, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"((uint32_t)accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
+        ::"r"(bar), "r"(leader) : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t e;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"((uint32_t)accumulate)
-        : "memory");
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+    return e;
 }
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int slot,
@@ -90,14 +127,94 @@ __device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes) {
                  ::"r"(bar), "r"(bytes) : "memory");
 }
 
+// Two fp32 at a time.
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Largest of three; a NaN wins.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x on the FMA pipe: x = n + f with n the nearest integer (by adding and
+// taking off 1.5 * 2^23, whose low bits then hold n) and 2^f on [-1/2, 1/2] by
+// the cubic of least relative error, 2^-13.7: an eighth of the last place of
+// fp16, which the result is rounded to at the least.  Below -125 it stays at
+// 2^-125, so it is not for masked scores, which have to give 0.
+__device__ __forceinline__ float2 ex2_poly(uint64_t x2) {
+    float2 x = both(x2);
+    x.x = fmaxf(x.x, -125.f);
+    x.y = fmaxf(x.y, -125.f);
+    x2 = pair2(x.x, x.y);
+    const uint64_t big = pair2(12582912.f, 12582912.f), less = pair2(-12582912.f, -12582912.f);
+    const uint64_t r = add2(x2, big);
+    const uint64_t f = fma2(add2(r, less), pair2(-1.f, -1.f), x2);
+    uint64_t p = fma2(pair2(0.055171669f, 0.055171669f), f, pair2(0.24261113f, 0.24261113f));
+    p = fma2(p, f, pair2(0.69326097f, 0.69326097f));
+    p = fma2(p, f, pair2(0.99992806f, 0.99992806f));
+    const float2 n = both(r), v = both(p);
+    return make_float2(
+        __uint_as_float(__float_as_uint(v.x) + (__float_as_uint(n.x) << 23)),
+        __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// x / g for x below 2^20: the quotient of x + 1/2 stays 1/(2g) away from the
+// integers, further than its rounding.
+__device__ __forceinline__ int small_div(int x, float inv_g) {
+    return (int)(((float)x + 0.5f) * inv_g);
+}
+
+// Barriers of the two warps that share 32 rows, and of a tile's eight warps.
+__device__ __forceinline__ void pair_sync(int t, int quad) {
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory");
+}
+__device__ __forceinline__ void tile_sync(int t) {
+    asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory");
+}
+
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done;
+}
+
 // A bounded wait.  Once one has given up, `fail` ends all others at once.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *fail) {
-    for (int i = 0; i < 1 << 10; i++) {
-        if (umma::mbar_wait(bar, parity, umma::kWaitLimit >> 10)) return true;
-        if (*fail) return false;
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int *fail) {
+    for (uint32_t i = 0; i < umma::kWaitLimit; i++) {
+        if (try_wait(bar, parity)) return true;
+        if (i % 4096 == 4095 && *fail) return false;
     }
     *fail = 1;
     return false;
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *fail) {
+#pragma unroll 1
+    for (int i = 0; i < 64; i++)
+        if (try_wait(bar, parity)) return true;
+    return wait_long(bar, parity, fail);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float *v) {
@@ -130,6 +247,40 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
         : "memory");
 }
 
+// Of every 16 pairs of exponentials, those computed by ex2_poly.
+constexpr int kPoly = 6;
+
+// p = 2^(c s - c m) of half a row's scores into the place of the first of them,
+// and their sum.
+template <typename T, int POLY>
+__device__ __forceinline__ void weights(const float (&s)[kHalf], uint64_t c2, uint64_t mc2,
+                                        uint64_t &sum, uint32_t st) {
+    uint64_t l1 = pair2(0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < kHalf; x += 32) {
+        uint32_t p[16];
+#pragma unroll
+        for (int y = 0; y < 16; y++) {
+            const uint64_t v = fma2(pair2(s[x + 2 * y], s[x + 2 * y + 1]), c2, mc2);
+            float2 e;
+            // spread evenly over the 16
+            if ((y + 1) * POLY / 16 > y * POLY / 16) {
+                e = ex2_poly(v);
+            } else {
+                e = both(v);
+                e.x = ex2(e.x);
+                e.y = ex2(e.y);
+            }
+            if (y & 1) l1 = add2(l1, pair2(e.x, e.y));
+            else sum = add2(sum, pair2(e.x, e.y));
+            p[y] = pack2<T>(e.x, e.y);
+        }
+        tmem_st16(st + x / 2, p);
+    }
+    tmem_st_wait();
+    sum = add2(sum, l1);
+}
+
 }  // namespace
 
 // PACKED: rows are those of all the batch's tokens, keys the shared prefix.
@@ -139,7 +290,7 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap vmap) {
     using L = Lay<D>;
     constexpr int NS = L::stages;
-    extern __shared__ uint8_t smem_raw[];
+    extern __shared__ __align__(1024) uint8_t basep[];
     const int kvh = blockIdx.y;
     const AttnReq rq = PACKED ? AttnReq{0, a.tokens, 0} : attn_req(a, blockIdx.z);
     const int rows = rq.n * a.group;
@@ -174,11 +325,10 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
     const int cnt0 = count_of(seen_t0), cnt = count_of(own_seen);
     const int see_first = PACKED ? 0 : causal ? rq.len - rq.n + row0 / a.group + 1 : rq.len;
 
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t *const basep = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t base = smem_u32(basep);
     const uint32_t bars = base + L::bars;
     const uint32_t kv_full = bars, kv_empty = bars + NS * 8, q_full = kv_empty + NS * 8,
-                   s_full = q_full + 16, p_full = s_full + 16, o_done = p_full + 16,
+                   s_full = q_full + 16, p_full = s_full + 16, o_done = p_full + 32,
                    drain = o_done + 16, tmem_slot = drain + 8;
     volatile int *const fail = (volatile int *)(basep + L::bars + (tmem_slot - bars) + 4);
     volatile int *const dirty = fail + 1;
@@ -190,9 +340,10 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
             umma::mbar_init(kv_empty + 8 * i, 1);
         }
         for (int t = 0; t < 2; t++) {
-            umma::mbar_init(q_full + 8 * t, kRows);
+            umma::mbar_init(q_full + 8 * t, 2 * kRows);
             umma::mbar_init(s_full + 8 * t, 1);
-            umma::mbar_init(p_full + 8 * t, kRows);
+            umma::mbar_init(p_full + 16 * t, kRows);
+            umma::mbar_init(p_full + 16 * t + 8, kRows);
             umma::mbar_init(o_done + 8 * t, 1);
         }
         umma::mbar_init(drain, 1);
@@ -200,13 +351,13 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
         *dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) umma::tmem_alloc(tmem_slot, 512);
+    if (warp == 16) umma::tmem_alloc(tmem_slot, 512);
     umma::fence_before();
     __syncthreads();
     umma::fence_after();
     const uint32_t tmem = *(volatile uint32_t *)(basep + (tmem_slot - base));
 
-    if (warp == 9) {
+    if (warp == 17) {
         // ---- keys and values: K of tile j in ring tile 2j, V in 2j + 1 --------------
         const int32_t *own_pages = PACKED ? nullptr : a.pages + (int64_t)blockIdx.z * a.pages_row;
         const int box = min(kKeys, 1 << a.page_shift);  // keys a box
@@ -246,91 +397,119 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
         if (!ok)                            // let the copies in flight land
             for (int i = max(0, issued - NS); i < issued; i++)
                 umma::mbar_wait(kv_full + 8 * (i % NS), (i / NS) & 1, umma::kWaitLimit);
-    } else if (warp == 8) {
-        // ---- the products, issued by one thread ------------------------------------
-        if (lane == 0 && cnt > 0) {
+    } else if (warp == 16) {
+        // ---- the products ------------------------------------------------------------
+        if (cnt > 0) {
+            const uint32_t leader = elect();
+            // descriptors of tile 0 and ring tile 0; the address field counts 16 bytes
+            const uint64_t q_desc = desc128(base, 16, 1024),
+                           k_desc = desc128(base + L::ring, 16, 1024),
+                           v_desc = desc128(base + L::ring, L::half, 1024);
             auto qk = [&](int t, int st) {
-                const uint32_t q = base + t * L::q_tile, k = base + L::ring + st * L::kv_tile;
+                const uint64_t q = q_desc + t * (L::q_tile >> 4),
+                               k = k_desc + st * (L::kv_tile >> 4);
 #pragma unroll
                 for (int x = 0; x < D / 16; x++) {
-                    const uint32_t off = (x / 4) * L::half + (x % 4) * 32;
-                    umma::mma_f16(tmem + L::s(t), desc128(q + off, 16, 1024),
-                                  desc128(k + off, 16, 1024), idesc<T>(kKeys, false), x > 0);
+                    const int off = ((x / 4) * L::half + (x % 4) * 32) >> 4;
+                    mma_ss(leader, tmem + L::s(t), q + off, k + off, idesc<T>(kKeys, false), x > 0);
                 }
-                umma::commit(s_full + 8 * t);
+                commit(leader, s_full + 8 * t);
             };
-            auto pv = [&](int t, int st, bool acc) {
-                const uint32_t v = base + L::ring + st * L::kv_tile;
+            // half the keys of a tile
+            auto pv = [&](int t, int st, int h, bool acc) {
+                const uint64_t v = v_desc + st * (L::kv_tile >> 4);
 #pragma unroll
-                for (int x = 0; x < kKeys / 16; x++)
-                    mma_ts(tmem + L::o(t), tmem + L::s(t) + x * 8,
-                           desc128(v + x * 2048, L::half, 1024), idesc<T>(D, true), acc || x > 0);
-                umma::commit(o_done + 8 * t);
+                for (int y = 0; y < kKeys / 32; y++) {
+                    const int x = h * (kKeys / 32) + y;
+                    mma_ts(leader, tmem + L::o(t), tmem + L::s(t) + h * kHalf + y * 8,
+                           v + x * (2048 >> 4), idesc<T>(D, true), acc || y > 0);
+                }
             };
             bool ok = wait(q_full, 0, fail);
-            if (ok && tiles_rows == 2) ok = wait(q_full + 8, 0, fail);
-            if (ok) ok = wait(kv_full, 0, fail);
+            if (tiles_rows == 2) ok = ok && wait(q_full + 8, 0, fail);
+            ok = ok && wait(kv_full, 0, fail);
+            ok = __all_sync(~0u, ok);
             umma::fence_after();
             if (ok) {
                 if (cnt0 > 0) qk(0, 0);
                 if (tiles_rows == 2) qk(1, 0);
-                if (NS < 2 * cnt) umma::commit(kv_empty);
+                if (NS < 2 * cnt) commit(leader, kv_empty);
             }
+            int sv = 1, sk = 2, fv = 0, fk = 0; // ring tiles of V j and K j + 1, their parities
             for (int j = 0; j < cnt && ok; j++) {
-                const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % NS, sk = ik % NS;
-                ok = wait(kv_full + 8 * sv, (iv / NS) & 1, fail);
-                bool k_here = false;
+                ok = wait(kv_full + 8 * sv, fv, fail);
+                if (j + 1 < cnt) ok = ok && wait(kv_full + 8 * sk, fk, fail);
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     const int mine = t == 0 ? cnt0 : tiles_rows == 2 ? cnt : 0;
-                    if (ok && j < mine) {
-                        ok = wait(p_full + 8 * t, j & 1, fail);
-                        umma::fence_after();
-                        if (ok) pv(t, sv, j > 0);
-                    }
-                    if (ok && j + 1 < mine) {
-                        if (!k_here) ok = wait(kv_full + 8 * sk, (ik / NS) & 1, fail);
-                        k_here = true;
-                        if (ok) qk(t, sk);
-                    }
+                    if (j >= mine) continue;
+                    ok = ok && wait(p_full + 16 * t, j & 1, fail);
+                    ok = ok && wait(p_full + 16 * t + 8, j & 1, fail);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    umma::fence_after();
+                    pv(t, sv, 0, j > 0);
+                    pv(t, sv, 1, true);
+                    commit(leader, o_done + 8 * t);
+                    if (j + 1 < mine) qk(t, sk);
                 }
                 if (!ok) break;
                 // only what the loader will wait for
-                if (iv + NS < 2 * cnt) umma::commit(kv_empty + 8 * sv);
-                if (ik + NS < 2 * cnt) umma::commit(kv_empty + 8 * sk);
+                if (2 * j + 1 + NS < 2 * cnt) commit(leader, kv_empty + 8 * sv);
+                if (2 * j + 2 + NS < 2 * cnt) commit(leader, kv_empty + 8 * sk);
+                sv += 2, sk += 2;
+                if (sv >= NS) sv -= NS, fv ^= 1;
+                if (sk >= NS) sk -= NS, fk ^= 1;
             }
             if (!ok) {                      // let the products in flight end
-                umma::commit(drain);
+                commit(leader, drain);
                 umma::mbar_wait(drain, 0, umma::kWaitLimit);
             }
         }
         __syncwarp();
     } else {
         // ---- the rows ----------------------------------------------------------------
-        const int t = warp / 4, r = threadIdx.x % kRows;
+        const int t = warp / 8, h = warp / 4 % 2, quad = warp % 4, r = threadIdx.x % kRows;
+        const int tid = threadIdx.x % (2 * kRows);      // in the tile
         const int row = row0 + t * kRows + r;
+        // row0's token and its head in the group; row0 + x is then token
+        // tok0 + (rem0 + x) / group
+        const int tok0 = row0 / a.group, rem0 = row0 - tok0 * a.group;
+        const float inv_group = 1.f / (float)a.group;
         const int mine = t == 0 ? cnt0 : tiles_rows == 2 ? cnt : 0;
         if (t < tiles_rows) {
-            // Q into its swizzled place, a row by D / 8 neighbouring threads
-            constexpr int CH = D / 8;
-            for (int i = r; i < kRows * CH; i += kRows) {
-                const int qr = i / CH, c = i % CH, x = row0 + t * kRows + qr;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (x < rows)
-                    v = *(const uint4 *)((const T *)a.q + (int64_t)(rq.t0 + x / a.group) * a.q_token +
-                                         (int64_t)(kvh * a.group + x % a.group) * a.q_head + c * 8);
+            // Q into its swizzled place, a row by D / 8 neighbouring threads, all of a
+            // thread's loads in flight
+            constexpr int CH = D / 8, RP = 2 * kRows / CH, N = kRows / RP;
+            const T *q = (const T *)a.q + (int64_t)(rq.t0 + tok0) * a.q_token +
+                         (int64_t)kvh * a.group * a.q_head + (tid % CH) * 8;
+            uint4 v[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int x = t * kRows + i * RP + tid / CH;
+                const int y = rem0 + x, tok = small_div(y, inv_group);
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (row0 + x < rows)
+                    v[i] = *(const uint4 *)(q + tok * a.q_token + (y - tok * a.group) * a.q_head);
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int qr = i * RP + tid / CH, c = tid % CH;
                 *(uint4 *)(basep + t * L::q_tile + (c / 8) * L::half + qr * 128 +
-                           (((c % 8) ^ (qr & 7)) << 4)) = v;
+                           (((c % 8) ^ (qr & 7)) << 4)) = v[i];
             }
             umma::fence_smem_async();
             arrive(q_full + 8 * t);
         }
-        const uint32_t lanes = (uint32_t)(warp % 4) * 32 << 16;
-        const uint32_t st = tmem + L::s(t) + lanes, ot = tmem + L::o(t) + lanes;
-        const bool warp_live = row0 + t * kRows + (warp % 4) * 32 < rows;
+        // this thread's half of the scores, later of the weights, and of the results
+        const uint32_t lanes = (uint32_t)quad * 32 << 16;
+        const uint32_t st = tmem + L::s(t) + h * kHalf + lanes, ot = tmem + L::o(t) + lanes;
+        float *const swap = (float *)(basep + L::swap) + t * 2 * kRows;
+        const bool warp_live = row0 + t * kRows + quad * 32 < rows;
         const int see = PACKED ? 0 : row < rows ? sees(row) : 0;
         const float c = a.scale_log2;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY;
+        float2 l = make_float2(0.f, 0.f);    // two halves of the sum
         bool ok = true;
         for (int j = 0; j < mine; j++) {
             const bool pre = first + j < pre_tiles;
@@ -343,13 +522,18 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
             if (held < kKeys || cut) {
                 const int i = 2 * j + 1;
                 ok = ok && wait(kv_full + 8 * (i % NS), (i / NS) & 1, fail);
-                uint8_t *v = basep + L::ring + (i % NS) * L::kv_tile + r * 128;
-                bool wipe = r >= held;
-                if (cut && !wipe && k0 + r >= see_first) {
+                // two threads a key of this half
+                const int key = h * kHalf + r % kHalf, part_bytes = D;
+                uint8_t *v = basep + L::ring + (i % NS) * L::kv_tile + key * 128;
+                const int x0 = r / kHalf * part_bytes, x1 = x0 + part_bytes;
+                auto at = [&](int x) { return v + (x / 128) * L::half + x % 128; };
+                if (key >= held) {
+                    for (int x = x0; x < x1; x += 16) *(uint4 *)at(x) = make_uint4(0, 0, 0, 0);
+                } else if (cut && k0 + key >= see_first) {
                     constexpr uint32_t E = fmt16<T>() ? 0x7f80u : 0x7c00u;
                     bool bad = false;
-                    for (int x = 0; x < D / 8; x++) {
-                        const uint4 q = *(const uint4 *)(v + (x / 8) * L::half + (x % 8) * 16);
+                    for (int x = x0; x < x1; x += 16) {
+                        const uint4 q = *(const uint4 *)at(x);
                         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                         for (int y = 0; y < 4; y++)
@@ -358,52 +542,54 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                     if (bad) {
                         *dirty = 1;
                         __threadfence_block();
-                        for (int x = 0; x < D / 2; x++) {
-                            uint32_t *q = (uint32_t *)(v + (x / 32) * L::half + (x % 32) * 4);
-                            uint32_t w = *q;
+                        for (int x = x0; x < x1; x += 4) {
+                            uint32_t *q = (uint32_t *)at(x), w = *q;
                             if ((w & E) == E) w &= 0xffff0000u;
                             if ((w >> 16 & E) == E) w &= 0xffffu;
                             *q = w;
                         }
                     }
                 }
-                if (wipe)
-                    for (int x = 0; x < D / 8; x++)
-                        *(uint4 *)(v + (x / 8) * L::half + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
                 umma::fence_smem_async();
             }
             ok = ok && wait(s_full + 8 * t, j & 1, fail);
-            if (!__all_sync(~0u, ok)) break;
+            // A wait that gave up leaves the results unusable, but every warp still
+            // takes every step, as its partner waits for it.
+            ok = __all_sync(~0u, ok);
             umma::fence_after();
             if (warp_live) {
-                float s[kKeys];
+                float s[kHalf];
 #pragma unroll
-                for (int x = 0; x < kKeys; x += 32) tmem_ld32(st + x, s + x);
+                for (int x = 0; x < kHalf; x += 32) tmem_ld32(st + x, s + x);
                 tmem_ld_wait();
-                const int lim = pre ? held : min(held, see - k0);
+                const int lim = (pre ? held : min(held, see - k0)) - h * kHalf;
                 if (held < kKeys || cut) {
 #pragma unroll
-                    for (int x = 0; x < kKeys; x++) s[x] = x < lim ? s[x] : -INFINITY;
+                    for (int x = 0; x < kHalf; x++) s[x] = x < lim ? s[x] : -INFINITY;
                 }
-                float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+                float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int x = 4; x < kKeys; x += 4) {
-                    mx0 = fmaxf(mx0, s[x]);
-                    mx1 = fmaxf(mx1, s[x + 1]);
-                    mx2 = fmaxf(mx2, s[x + 2]);
-                    mx3 = fmaxf(mx3, s[x + 3]);
-                }
-                const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-                const bool grow = (mx - m) * c > 8.f;
+                for (int x = 4; x + 8 <= kHalf; x += 8)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) mx[y] = max3(mx[y], s[x + y], s[x + y + 4]);
+                mx[0] = max3(mx[0], s[kHalf - 4], s[kHalf - 3]);
+                mx[1] = max3(mx[1], s[kHalf - 2], s[kHalf - 1]);
+                float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+                // the other half's; it is read before this row's weights are handed
+                // over, so before either half's next scores
+                swap[h * kRows + r] = top;
+                pair_sync(t, quad);
+                top = max3(top, swap[(h ^ 1) * kRows + r], top);
+                const bool grow = !((top - m) * c <= 8.f);
                 if (__any_sync(~0u, grow)) {
-                    const float to = grow ? mx : m;
-                    const float w = grow ? ex2(m * c - to * c) : 1.f;
+                    const float to = grow ? top : m;
+                    const float w = !grow || to == -INFINITY ? 1.f : ex2(m * c - to * c);
                     if (j > 0) {
-                        ok = wait(o_done + 8 * t, (j - 1) & 1, fail);
-                        if (!__all_sync(~0u, ok)) break;
+                        ok = ok && wait(o_done + 8 * t, (j - 1) & 1, fail);
+                        ok = __all_sync(~0u, ok);
                         umma::fence_after();
-#pragma unroll
-                        for (int x = 0; x < D; x += 16) {
+#pragma unroll 1
+                        for (int x = h * (D / 2); x < (h + 1) * (D / 2); x += 16) {
                             float o[16];
                             umma::tmem_ld16(ot + x, o);
                             uint32_t u[16];
@@ -412,93 +598,113 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                             tmem_st16(ot + x, u);
                         }
                     }
-                    l *= w;
+                    l.x *= w;
+                    l.y *= w;
                     m = to;
                 }
-                const float mc = m == -INFINITY ? 0.f : m * c;
-                float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                for (int x = 0; x < kKeys; x += 32) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int y = 0; y < 16; y++) {
-                        const float p0 = ex2(fmaf(s[x + 2 * y], c, -mc));
-                        const float p1 = ex2(fmaf(s[x + 2 * y + 1], c, -mc));
-                        l0 += p0;
-                        l1 += p1;
-                        p[y] = pack2<T>(p0, p1);
-                    }
-                    tmem_st16(st + x / 2, p);
-                }
-                l += l0 + l1;
-                tmem_st_wait();
+                // a row with an infinite or NaN score is NaN altogether
+                const float mc = m == -INFINITY ? 0.f : m < INFINITY ? m * c : NAN;
+                const uint64_t c2 = pair2(c, c), mc2 = pair2(-mc, -mc);
+                uint64_t l2 = pair2(l.x, l.y);
+                if (held < kKeys || cut) weights<T, 0>(s, c2, mc2, l2, st);
+                else weights<T, kPoly>(s, c2, mc2, l2, st);
+                l = both(l2);
             }
             umma::fence_before();
-            arrive(p_full + 8 * t);
+            arrive(p_full + 16 * t + 8 * h);
         }
         if (mine > 0 && ok) ok = wait(o_done + 8 * t, (mine - 1) & 1, fail);
         umma::fence_after();
         ok = __all_sync(~0u, ok);
-        if (t < tiles_rows && warp_live && ok) {
+        if (t < tiles_rows) {
+            // The results go through the tile's place of Q, which is done with, so
+            // that rows are written by neighbouring threads.
             const bool direct = !PACKED && !a.packed && parts == 1;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int64_t orow = (int64_t)(rq.t0 + row / a.group) * a.q_heads + kvh * a.group +
-                                 row % a.group;
-            const int64_t slot = (int64_t)(PACKED ? part : a.prefix_parts + part) * a.tokens *
-                                     a.q_heads + orow;
+            const int y = rem0 + t * kRows + r, tok = small_div(y, inv_group);
+            const int64_t part_row = (int64_t)(PACKED ? part : a.prefix_parts + part) * a.tokens *
+                                     a.q_heads;
+            const int64_t out_row = (int64_t)(rq.t0 + tok0) * a.q_heads + kvh * a.group;
             __threadfence_block();
             const bool mend = *dirty && causal;
+            uint8_t *const stage = basep + t * L::q_tile;
+            swap[h * kRows + r] = l.x + l.y;
+            tile_sync(t);
+            const float sum = swap[r] + swap[kRows + r];
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            // columns at a time, half of them by each of a row's threads: all of 16
+            // bits, or half of 32
+            const int wide = direct ? D : D / 2;
+            for (int x0 = 0; x0 < D; x0 += wide) {
 #pragma unroll 1
-            for (int x = 0; x < D; x += 32) {
-                __syncwarp();
-                float o[32];
-                if (mine > 0) {
-                    tmem_ld32(ot + x, o);
-                    tmem_ld_wait();
-                } else {
+                for (int x = x0 + h * (wide / 2); x < x0 + (h + 1) * (wide / 2); x += 16) {
+                    __syncwarp();
+                    float o[16];
+                    if (mine > 0 && warp_live && ok) {
+                        umma::tmem_ld16(ot + x, o);
+                    } else {
 #pragma unroll
-                    for (int y = 0; y < 32; y++) o[y] = 0.f;
-                }
-                if (row >= rows) continue;
-                if (mend) {
-                    // what was wiped and is in sight of this row
-                    const int end = min(see, max(0, first + each - pre_tiles) * kKeys);
-                    for (int k = max(max(see_first, 0), (first - pre_tiles) * kKeys); k < end; k++) {
-                        const int page = attn_page(a, a.pages + (int64_t)blockIdx.z * a.pages_row, k);
-                        const T *v = (const T *)a.vp + (int64_t)page * a.v_page +
-                                     (int64_t)(k & ((1 << a.page_shift) - 1)) * a.v_slot +
-                                     (int64_t)kvh * a.v_head + x;
+                        for (int i = 0; i < 16; i++) o[i] = 0.f;
+                    }
+                    if (mend && row < rows) {
+                        // what was wiped and is in sight of this row
+                        const int end = min(see, max(0, first + each - pre_tiles) * kKeys);
+                        for (int k = max(max(see_first, 0), (first - pre_tiles) * kKeys); k < end;
+                             k++) {
+                            const int page =
+                                attn_page(a, a.pages + (int64_t)blockIdx.z * a.pages_row, k);
+                            const T *v = (const T *)a.vp + (int64_t)page * a.v_page +
+                                         (int64_t)(k & ((1 << a.page_shift) - 1)) * a.v_slot +
+                                         (int64_t)kvh * a.v_head + x;
 #pragma unroll
-                        for (int y = 0; y < 32; y++) {
-                            const float f = AttnType<T>::up(v[y]);
-                            if (!isfinite(f)) o[y] += f;
+                            for (int i = 0; i < 16; i++) {
+                                const float f = AttnType<T>::up(v[i]);
+                                if (!isfinite(f)) o[i] += f;
+                            }
                         }
                     }
-                }
-                if (direct) {
+                    // 16-byte pieces, their places in the row turned by the row
+                    uint8_t *const at = stage + r * (D * 2);
+                    constexpr int turn = D / 8 - 1;
+                    if (direct) {
 #pragma unroll
-                    for (int y = 0; y < 32; y += 8) {
-                        uint4 w;
-                        w.x = pack2<T>(o[y] * inv, o[y + 1] * inv);
-                        w.y = pack2<T>(o[y + 2] * inv, o[y + 3] * inv);
-                        w.z = pack2<T>(o[y + 4] * inv, o[y + 5] * inv);
-                        w.w = pack2<T>(o[y + 6] * inv, o[y + 7] * inv);
-                        *(uint4 *)((T *)a.out + orow * D + x + y) = w;
+                        for (int i = 0; i < 16; i += 8)
+                            *(uint4 *)(at + ((((x + i) / 8) ^ (r & turn)) << 4)) =
+                                make_uint4(pack2<T>(o[i] * inv, o[i + 1] * inv),
+                                           pack2<T>(o[i + 2] * inv, o[i + 3] * inv),
+                                           pack2<T>(o[i + 4] * inv, o[i + 5] * inv),
+                                           pack2<T>(o[i + 6] * inv, o[i + 7] * inv));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *(float4 *)(at + ((((x - x0 + i) / 4) ^ (r & turn)) << 4)) =
+                                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
-                } else {
-#pragma unroll
-                    for (int y = 0; y < 32; y += 4)
-                        *(float4 *)(a.part_o + slot * D + x + y) =
-                            make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
                 }
+                tile_sync(t);
+                constexpr int CH = D / 8;               // pieces a row, either way
+#pragma unroll 4
+                for (int i = 0; i < CH / 2; i++) {
+                    const int or_ = i * (2 * kRows / CH) + tid / CH, c = tid % CH,
+                              yy = rem0 + t * kRows + or_;
+                    if (row0 + t * kRows + or_ >= rows) break;
+                    const int tk = small_div(yy, inv_group);
+                    const int64_t o_row = out_row + (int64_t)tk * a.q_heads + (yy - tk * a.group);
+                    const uint4 v =
+                        *(const uint4 *)(stage + or_ * (D * 2) + ((c ^ (or_ & (CH - 1))) << 4));
+                    if (direct) *(uint4 *)((T *)a.out + o_row * D + c * 8) = v;
+                    else *(uint4 *)(a.part_o + (part_row + o_row) * D + x0 + c * 4) = v;
+                }
+                tile_sync(t);
             }
-            if (!direct && row < rows) a.part_ml[slot] = make_float2(m * c, l);
+            if (!direct && h == 0 && row < rows)
+                a.part_ml[part_row + out_row + (int64_t)tok * a.q_heads + (y - tok * a.group)] =
+                    make_float2(m * c, sum);
         }
     }
     umma::fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *fail) atomicOr(a.err, kAttnTimeout);
-    if (warp == 8) {
+    if (warp == 16) {
         umma::fence_after();
         umma::tmem_free(tmem, 512);
     }
