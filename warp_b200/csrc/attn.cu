@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     const AttnReq rq = attn_req(a, b);
     if (t >= rq.t0 + rq.n) return;
     const bool wide = rq.n * a.group > a.rows_small;
-    const int tile = wide ? kAttnWide : kAttnTile;
+    const int tile = wide ? attn_wide(D) : kAttnTile;
     const int own = (a.packed ? 0 : (a.prefix_len + tile - 1) / tile) + (rq.len + tile - 1) / tile;
     int parts = max(1, attn_parts(own, wide ? a.wide_each : a.split_tiles));
     if (!a.packed && parts == 1) return;
@@ -486,6 +486,7 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     const int64_t held = (int64_t)d->pages_per_row * c->page_size;
     p.max_kv = d->max_kv < held ? d->max_kv : (int)held;
     const int64_t group = d->q_heads / d->kv_heads;
+    const int keys = attn_wide(d->head_dim);
     // The prefix apart, for all rows at once, where a request's rows alone
     // would leave a row tile mostly empty.
     p.packed = d->prefix_len > 0 && d->batch > 1 && d->tokens * group <= (int64_t)128 * d->batch;
@@ -496,7 +497,7 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     if (rows > p.rows_small) {
         const int64_t pairs = up(rows, 256) * d->batch, by_tokens = up(d->tokens * group, 256);
         const int64_t ctas = pairs < by_tokens + d->batch - 1 ? pairs : by_tokens + d->batch - 1;
-        const int64_t tiles = up(p.max_kv, kAttnWide) + up(pre, kAttnWide);
+        const int64_t tiles = up(p.max_kv, keys) + up(pre, keys);
         p.wide_each = pick_wide(tiles, ctas * d->kv_heads);
         p.wide_parts = tiles ? (int)up(tiles, p.wide_each) : 1;
     }
@@ -509,7 +510,7 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     if (p.packed) {
         const int64_t all = d->tokens * group;
         p.packed_wide = all > kADRows;
-        const int64_t tiles = up(d->prefix_len, p.packed_wide ? kAttnWide : kAttnTile);
+        const int64_t tiles = up(d->prefix_len, p.packed_wide ? keys : kAttnTile);
         p.prefix_each = p.packed_wide ? pick_wide(tiles, up(all, 256) * d->kv_heads)
                                       : pick_split(tiles, up(all, kADRows) * d->kv_heads);
         p.prefix_parts = (int)up(tiles, p.prefix_each);

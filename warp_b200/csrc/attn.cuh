@@ -51,7 +51,7 @@ struct AttnArgs {
     float2 *part_ml;
     int packed, prefix_parts;
     // Requests with more rows a kv head than rows_small go to attn_umma_kernel,
-    // which counts keys in tiles of kAttnWide; the others to attn_rows_kernel.
+    // which counts keys in tiles of attn_wide; the others to attn_rows_kernel.
     int rows_small;
     int split_tiles;                        // key tiles of a request's part
     int prefix_split_tiles;                 // and of a part of the prefix
@@ -87,7 +87,8 @@ __device__ __forceinline__ int attn_page(const AttnArgs &a, const int32_t *table
 // Keys come in tiles of kAttnTile; the prefix's last tile and a request's last
 // one may be partly filled, and a tile never mixes the two.
 constexpr int kAttnTile = 16;
-constexpr int kAttnWide = 128;
+// Keys a tile of attn_umma_kernel.
+__host__ __device__ constexpr int attn_wide(int) { return 128; }
 
 // How many parts a range of `tiles` key tiles is split into, `each` tiles a part.
 __device__ __forceinline__ int attn_parts(int tiles, int each) {

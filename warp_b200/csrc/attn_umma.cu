@@ -2,13 +2,13 @@
 // key head: prompts, chunks and the rows of a batch behind a shared prefix.
 //
 // A CTA holds 256 rows (token, head of the group) of one kv head as two tiles
-// of 128 and walks the keys in tiles of 128. Per tile, on the tensor cores
-// with the accumulators in tensor memory:
+// of 128 and walks the keys a tile of 128 a step. Per step and row tile, on the
+// tensor cores with the accumulators in tensor memory:
 //     S = Q K^T      (both from shared memory, 128B-swizzled, K-major)
 //     O += P V       (P from tensor memory, V as it lies: N-major)
-// and between them, one thread a row: the running maximum m, p = 2^(c s - c m)
-// and the sum l. P takes the place of S. While one tile's exponentials are
-// computed the other's products run, so neither pipe waits for the other.
+// and between them, two threads a row: the running maximum m, p = 2^(c s - c m)
+// and the sum l. P takes the place of S. While one row tile's exponentials are
+// computed the other's products run.
 //
 // The maximum that p is measured from moves only when a row outgrows it by
 // 2^8, so the accumulated O is rescaled rarely; p then stays below 2^8, which
@@ -17,17 +17,14 @@
 //
 // What bounds it: per pair of 128 x 128 tiles the products take
 // 2 * 2 * 128 * 128 * D / 4096 FMA a clock = 2048 cycles at D = 128 (half at
-// 64), and so do 2 * 128 * 128 exponentials at 16 a clock. A tile's next
-// scores wait for its weights, so what counts is that one tile's softmax fits
-// into the time of the other's products: a share of the exponentials is
-// computed on the FMA pipe (ex2_poly), sums and scalings go two at a time
-// (f32x2), and the first half of a tile's weights is handed over while the
-// second is computed.
+// 64), and so do 2 * 128 * 128 exponentials at 16 a clock. A share of the
+// exponentials is computed on the FMA pipe (ex2_poly), and sums and scalings go
+// two at a time (f32x2).
 //
-// Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each of
-// them with half the keys of a tile (a warp alone on its scheduler spends two
-// thirds of its time on the latency of its own instructions); 16 issues the
-// products; 17 loads keys and values by TMA, a box a page, into a ring of tiles.
+// Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each with
+// half the keys of a step (one warp a 32 rows leaves two to a scheduler, which
+// do not hide each other's latency); 16 issues the products, 17 loads keys and
+// values by TMA, boxes of 16 keys, into a ring of tiles.
 #include "attn.cuh"
 #include "umma.cuh"
 
@@ -37,22 +34,32 @@ namespace warp {
 namespace {
 
 constexpr int kRows = 128;                  // rows a tile
-constexpr int kKeys = kAttnWide;            // keys a tile
-constexpr int kHalf = kKeys / 2;              // keys of a row that one thread weighs
+constexpr int kBox = 16;                    // keys a TMA box: no page is smaller
 constexpr int kThreads = 18 * 32;
 
 template <int D> struct Lay {
+    static constexpr int keys = attn_wide(D);           // keys a tile
     static constexpr int q_tile = kRows * D * 2;
-    static constexpr int kv_tile = kKeys * D * 2;
-    static constexpr int half = kKeys * 128;            // 64 columns of a tile
+    static constexpr int q_half = kRows * 128;          // 64 columns of a tile
+    static constexpr int kv_tile = keys * D * 2;
+    static constexpr int kv_half = keys * 128;
     static constexpr int stages = D == 128 ? 5 : 8;
     static constexpr int ring = 2 * q_tile;
     static constexpr int swap = ring + stages * kv_tile;  // [tile][half][row] fp32
     static constexpr int bars = swap + 4 * kRows * 4;
-    static constexpr int bytes = bars + 256;
+    static constexpr int cols = keys / 2;               // keys of a row and thread
+    // offsets in the barrier section
+    static constexpr int kv_full = 0, kv_empty = kv_full + stages * 8,
+                         q_full = kv_empty + stages * 8, s_full = q_full + 16,
+                         p_full = s_full + 16, o_end = p_full + 16, drain = o_end + 16,
+                         tmem = drain + 8, fail = tmem + 4, dirty = fail + 4;
+    static constexpr int bytes = bars + dirty + 8;
+    static_assert(bytes <= 227 * 1024, "shared memory of a block");
+    static_assert(cols % 8 == 0 && kv_half % 1024 == 0 && keys % kBox == 0, "swizzle atoms of 8 rows, whole boxes");
     // tensor memory columns
-    static constexpr int s(int t) { return t * 128; }
-    static constexpr int o(int t) { return 256 + t * D; }
+    static constexpr int o(int t) { return t * D; }
+    static constexpr int s(int t) { return 2 * D + t * keys; }
+    static_assert(2 * D + 2 * keys <= 512, "tensor memory");
 };
 
 // Shared-memory matrix descriptor, 128-byte swizzle (layout type 2).
@@ -191,45 +198,37 @@ __device__ __forceinline__ void tile_sync(int t) {
     asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory");
 }
 
-__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    return done;
-}
+// Polls before a wait gives up (each may itself wait a while in hardware):
+// seconds, far longer than any tile takes.
+constexpr uint32_t kPolls = 1u << 19;
 
-// A bounded wait.  Once one has given up, `fail` ends all others at once.
-__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int *fail) {
-    for (uint32_t i = 0; i < umma::kWaitLimit; i++) {
-        if (try_wait(bar, parity)) return true;
-        if (i % 4096 == 4095 && *fail) return false;
-    }
-    *fail = 1;
-    return false;
-}
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *fail) {
-#pragma unroll 1
-    for (int i = 0; i < 64; i++)
-        if (try_wait(bar, parity)) return true;
-    return wait_long(bar, parity, fail);
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float *v) {
-    uint32_t *r = (uint32_t *)v;
+// A bounded wait, in as few instructions as a wait that is over already can do
+// with: it has no result, and every role goes on step by step either way. One
+// that gives up sets `fail` (a word of shared memory), which ends all others at
+// once; results are then unusable, and the launch says so.
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, uint32_t fail) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-          "=r"(r[31])
-        : "r"(addr));
+        "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+        "@p bra DONE;\n\t"
+        "mov.u32 n, 0;\n\t"
+        "POLL:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+        "@p bra DONE;\n\t"
+        "ld.volatile.shared.u32 f, [%2];\n\t"
+        "setp.ne.u32 p, f, 0;\n\t"
+        "@p bra DONE;\n\t"
+        "add.u32 n, n, 1;\n\t"
+        "setp.lt.u32 p, n, %3;\n\t"
+        "@p bra POLL;\n\t"
+        "st.volatile.shared.u32 [%2], 1;\n\t"
+        "DONE:\n\t}\n"
+        ::"r"(bar), "r"(parity), "r"(fail), "n"(kPolls) : "memory");
+    __syncwarp();
+}
+// The same that ends with `fail` set or not, for copies and products in flight.
+__device__ __forceinline__ void wait_over(uint32_t bar, uint32_t parity) {
+    umma::mbar_wait(bar, parity, kPolls);
 }
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -237,48 +236,55 @@ __device__ __forceinline__ void tmem_ld_wait() {
 __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, float *v) {
+    uint32_t *r = (uint32_t *)v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t *r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
         ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-          "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-          "r"(r[14]), "r"(r[15])
+          "r"(r[7])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 
-// Of every 16 pairs of exponentials, those computed by ex2_poly.
-constexpr int kPoly = 6;
+// Of every 4 pairs of exponentials, those computed by ex2_poly: at D = 64, where
+// the products are half as long, one (4096 keys: 668 TFLOP/s against 636 for
+// none and 624 for two); at 128 none (1208 against 1136 and 1047).
+constexpr int poly_pairs(int D) { return D == 64 ? 1 : 0; }
 
-// p = 2^(c s - c m) of half a row's scores into the place of the first of them,
+// p = 2^(c s - c m) of a thread's scores of one step into their place,
 // and their sum.
-template <typename T, int POLY>
-__device__ __forceinline__ void weights(const float (&s)[kHalf], uint64_t c2, uint64_t mc2,
+template <typename T, int POLY, int N>
+__device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64_t mc2,
                                         uint64_t &sum, uint32_t st) {
-    uint64_t l1 = pair2(0.f, 0.f);
 #pragma unroll
-    for (int x = 0; x < kHalf; x += 32) {
-        uint32_t p[16];
+    for (int x = 0; x < N; x += 8) {
+        uint32_t p[4];
 #pragma unroll
-        for (int y = 0; y < 16; y++) {
+        for (int y = 0; y < 4; y++) {
             const uint64_t v = fma2(pair2(s[x + 2 * y], s[x + 2 * y + 1]), c2, mc2);
             float2 e;
-            // spread evenly over the 16
-            if ((y + 1) * POLY / 16 > y * POLY / 16) {
+            if (y < POLY) {
                 e = ex2_poly(v);
             } else {
                 e = both(v);
                 e.x = ex2(e.x);
                 e.y = ex2(e.y);
             }
-            if (y & 1) l1 = add2(l1, pair2(e.x, e.y));
-            else sum = add2(sum, pair2(e.x, e.y));
+            sum = add2(sum, pair2(e.x, e.y));
             p[y] = pack2<T>(e.x, e.y);
         }
-        tmem_st16(st + x / 2, p);
+        tmem_st4(st + x / 2, p);
     }
     tmem_st_wait();
-    sum = add2(sum, l1);
 }
 
 }  // namespace
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap vmap) {
     using L = Lay<D>;
-    constexpr int NS = L::stages;
+    constexpr int NS = L::stages, KEYS = L::keys;
     extern __shared__ __align__(1024) uint8_t basep[];
     const int kvh = blockIdx.y;
     const AttnReq rq = PACKED ? AttnReq{0, a.tokens, 0} : attn_req(a, blockIdx.z);
@@ -304,8 +310,8 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
     const int row0 = pair * 2 * kRows;
 
     const int n_pre = PACKED || !a.packed ? a.prefix_len : 0;
-    const int pre_tiles = (n_pre + kKeys - 1) / kKeys;
-    const int all_tiles = pre_tiles + (PACKED ? 0 : (rq.len + kKeys - 1) / kKeys);
+    const int pre_tiles = (n_pre + KEYS - 1) / KEYS;
+    const int all_tiles = pre_tiles + (PACKED ? 0 : (rq.len + KEYS - 1) / KEYS);
     const int each = PACKED ? a.prefix_wide_each : a.wide_each;
     const int parts = max(1, attn_parts(all_tiles, each));
     if (part >= parts) return;
@@ -320,18 +326,20 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
     const int seen_t0 = PACKED ? 0 : sees(min(rows, row0 + kRows) - 1);
     const int first = part * each;
     auto count_of = [&](int seen) {
-        return max(0, min(first + each, pre_tiles + (seen + kKeys - 1) / kKeys) - first);
+        return max(0, min(first + each, pre_tiles + (seen + KEYS - 1) / KEYS) - first);
     };
     const int cnt0 = count_of(seen_t0), cnt = count_of(own_seen);
     const int see_first = PACKED ? 0 : causal ? rq.len - rq.n + row0 / a.group + 1 : rq.len;
 
     const uint32_t base = smem_u32(basep);
     const uint32_t bars = base + L::bars;
-    const uint32_t kv_full = bars, kv_empty = bars + NS * 8, q_full = kv_empty + NS * 8,
-                   s_full = q_full + 16, p_full = s_full + 16, o_done = p_full + 32,
-                   drain = o_done + 16, tmem_slot = drain + 8;
-    volatile int *const fail = (volatile int *)(basep + L::bars + (tmem_slot - bars) + 4);
-    volatile int *const dirty = fail + 1;
+    const uint32_t kv_full = bars + L::kv_full, kv_empty = bars + L::kv_empty,
+                   q_full = bars + L::q_full, s_full = bars + L::s_full,
+                   p_full = bars + L::p_full, o_end = bars + L::o_end, drain = bars + L::drain,
+                   tmem_slot = bars + L::tmem;
+    const uint32_t fail = bars + L::fail;
+    volatile int *const failed = (volatile int *)(basep + L::bars + L::fail);
+    volatile int *const dirty = (volatile int *)(basep + L::bars + L::dirty);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
@@ -342,12 +350,11 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
         for (int t = 0; t < 2; t++) {
             umma::mbar_init(q_full + 8 * t, 2 * kRows);
             umma::mbar_init(s_full + 8 * t, 1);
-            umma::mbar_init(p_full + 16 * t, kRows);
-            umma::mbar_init(p_full + 16 * t + 8, kRows);
-            umma::mbar_init(o_done + 8 * t, 1);
+            umma::mbar_init(p_full + 8 * t, 8);
+            umma::mbar_init(o_end + 8 * t, 1);
         }
         umma::mbar_init(drain, 1);
-        *fail = 0;
+        *failed = 0;
         *dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -355,37 +362,35 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
     umma::fence_before();
     __syncthreads();
     umma::fence_after();
-    const uint32_t tmem = *(volatile uint32_t *)(basep + (tmem_slot - base));
+    const uint32_t tmem = *(volatile uint32_t *)(basep + L::bars + L::tmem);
 
     if (warp == 17) {
         // ---- keys and values: K of tile j in ring tile 2j, V in 2j + 1 --------------
         const int32_t *own_pages = PACKED ? nullptr : a.pages + (int64_t)blockIdx.z * a.pages_row;
-        const int box = min(kKeys, 1 << a.page_shift);  // keys a box
-        const int boxes = kKeys / box;
+        constexpr int boxes = KEYS / kBox;
         const int bi = lane % boxes, bh = lane / boxes;  // this lane's box and column half
         auto page_of = [&](int j, int &key, bool &want) {
             const bool pre = first + j < pre_tiles;
-            key = (first + j - (pre ? 0 : pre_tiles)) * kKeys + bi * box;
+            key = (first + j - (pre ? 0 : pre_tiles)) * KEYS + bi * kBox;
             want = j < cnt && bh < D / 64 && key < (pre ? n_pre : own_seen);
             return want ? attn_page(a, pre ? a.prefix_pages : own_pages, key) : 0;
         };
         int key, next_key;
         bool want, next_want;
         int page = page_of(0, key, want), issued = 0;
-        bool ok = true;
-        for (int j = 0; j < cnt && ok; j++) {
+        for (int j = 0; j < cnt; j++) {
+            if (__any_sync(~0u, *failed)) break;
             const int next_page = page_of(j + 1, next_key, next_want);
-            const uint32_t bytes = __popc(__ballot_sync(~0u, want)) * box * 128;
+            const uint32_t bytes = __popc(__ballot_sync(~0u, want)) * kBox * 128;
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 const int i = 2 * j + w, st = i % NS;
-                if (i >= NS && !wait(kv_empty + 8 * st, (i / NS - 1) & 1, fail)) ok = false;
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
+                if (i >= NS) wait(kv_empty + 8 * st, (i / NS - 1) & 1, fail);
+                if (__any_sync(~0u, *failed)) break;
                 if (lane == 0) arrive_tx(kv_full + 8 * st, bytes);
                 __syncwarp();
                 if (want)
-                    tma_box(base + L::ring + st * L::kv_tile + bh * L::half + bi * box * 128,
+                    tma_box(base + L::ring + st * L::kv_tile + bh * L::kv_half + bi * kBox * 128,
                             w ? &vmap : &kmap, bh * 64, key & ((1 << a.page_shift) - 1), kvh, page,
                             kv_full + 8 * st);
                 issued++;
@@ -394,9 +399,9 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
             key = next_key;
             want = next_want;
         }
-        if (!ok)                            // let the copies in flight land
+        if (*failed)                        // let the copies in flight land
             for (int i = max(0, issued - NS); i < issued; i++)
-                umma::mbar_wait(kv_full + 8 * (i % NS), (i / NS) & 1, umma::kWaitLimit);
+                wait_over(kv_full + 8 * (i % NS), (i / NS) & 1);
     } else if (warp == 16) {
         // ---- the products ------------------------------------------------------------
         if (cnt > 0) {
@@ -404,56 +409,50 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
             // descriptors of tile 0 and ring tile 0; the address field counts 16 bytes
             const uint64_t q_desc = desc128(base, 16, 1024),
                            k_desc = desc128(base + L::ring, 16, 1024),
-                           v_desc = desc128(base + L::ring, L::half, 1024);
+                           v_desc = desc128(base + L::ring, L::kv_half, 1024);
             auto qk = [&](int t, int st) {
                 const uint64_t q = q_desc + t * (L::q_tile >> 4),
                                k = k_desc + st * (L::kv_tile >> 4);
 #pragma unroll
-                for (int x = 0; x < D / 16; x++) {
-                    const int off = ((x / 4) * L::half + (x % 4) * 32) >> 4;
-                    mma_ss(leader, tmem + L::s(t), q + off, k + off, idesc<T>(kKeys, false), x > 0);
-                }
+                for (int x = 0; x < D / 16; x++)
+                    mma_ss(leader, tmem + L::s(t), q + (((x / 4) * L::q_half + (x % 4) * 32) >> 4),
+                           k + (((x / 4) * L::kv_half + (x % 4) * 32) >> 4), idesc<T>(KEYS, false),
+                           x > 0);
                 commit(leader, s_full + 8 * t);
             };
-            // half the keys of a tile
-            auto pv = [&](int t, int st, int h, bool acc) {
+            auto pv = [&](int t, int st, bool acc) {
                 const uint64_t v = v_desc + st * (L::kv_tile >> 4);
 #pragma unroll
-                for (int y = 0; y < kKeys / 32; y++) {
-                    const int x = h * (kKeys / 32) + y;
-                    mma_ts(leader, tmem + L::o(t), tmem + L::s(t) + h * kHalf + y * 8,
-                           v + x * (2048 >> 4), idesc<T>(D, true), acc || y > 0);
-                }
+                for (int x = 0; x < KEYS / 16; x++)
+                    // the weights of each half of the keys lie where its scores did
+                    mma_ts(leader, tmem + L::o(t),
+                           tmem + L::s(t) + x / (L::cols / 16) * L::cols + x % (L::cols / 16) * 8,
+                           v + x * (2048 >> 4), idesc<T>(D, true), acc || x > 0);
             };
-            bool ok = wait(q_full, 0, fail);
-            if (tiles_rows == 2) ok = ok && wait(q_full + 8, 0, fail);
-            ok = ok && wait(kv_full, 0, fail);
-            ok = __all_sync(~0u, ok);
+            const int cnt1 = tiles_rows == 2 ? cnt : 0;
+            wait(q_full, 0, fail);
+            if (tiles_rows == 2) wait(q_full + 8, 0, fail);
+            wait(kv_full, 0, fail);
             umma::fence_after();
-            if (ok) {
-                if (cnt0 > 0) qk(0, 0);
-                if (tiles_rows == 2) qk(1, 0);
-                if (NS < 2 * cnt) commit(leader, kv_empty);
-            }
+            if (cnt0 > 0) qk(0, 0);
+            if (cnt1 > 0) qk(1, 0);
+            if (NS < 2 * cnt) commit(leader, kv_empty);
             int sv = 1, sk = 2, fv = 0, fk = 0; // ring tiles of V j and K j + 1, their parities
-            for (int j = 0; j < cnt && ok; j++) {
-                ok = wait(kv_full + 8 * sv, fv, fail);
-                if (j + 1 < cnt) ok = ok && wait(kv_full + 8 * sk, fk, fail);
+            for (int j = 0; j < cnt; j++) {
+                if (__any_sync(~0u, *failed)) break;
+                wait(kv_full + 8 * sv, fv, fail);
+                if (j + 1 < cnt) wait(kv_full + 8 * sk, fk, fail);
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const int mine = t == 0 ? cnt0 : tiles_rows == 2 ? cnt : 0;
+                    const int mine = t == 0 ? cnt0 : cnt1;
                     if (j >= mine) continue;
-                    ok = ok && wait(p_full + 16 * t, j & 1, fail);
-                    ok = ok && wait(p_full + 16 * t + 8, j & 1, fail);
-                    ok = __all_sync(~0u, ok);
-                    if (!ok) break;
+                    wait(p_full + 8 * t, j & 1, fail);
                     umma::fence_after();
-                    pv(t, sv, 0, j > 0);
-                    pv(t, sv, 1, true);
-                    commit(leader, o_done + 8 * t);
+                    pv(t, sv, j > 0);
+                    // in order behind it: the next scores take the weights' place
                     if (j + 1 < mine) qk(t, sk);
+                    else commit(leader, o_end + 8 * t);
                 }
-                if (!ok) break;
                 // only what the loader will wait for
                 if (2 * j + 1 + NS < 2 * cnt) commit(leader, kv_empty + 8 * sv);
                 if (2 * j + 2 + NS < 2 * cnt) commit(leader, kv_empty + 8 * sk);
@@ -461,12 +460,11 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                 if (sv >= NS) sv -= NS, fv ^= 1;
                 if (sk >= NS) sk -= NS, fk ^= 1;
             }
-            if (!ok) {                      // let the products in flight end
+            if (*failed) {                  // let the products in flight end
                 commit(leader, drain);
-                umma::mbar_wait(drain, 0, umma::kWaitLimit);
+                wait_over(drain, 0);
             }
         }
-        __syncwarp();
     } else {
         // ---- the rows ----------------------------------------------------------------
         const int t = warp / 8, h = warp / 4 % 2, quad = warp % 4, r = threadIdx.x % kRows;
@@ -495,41 +493,44 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int qr = i * RP + tid / CH, c = tid % CH;
-                *(uint4 *)(basep + t * L::q_tile + (c / 8) * L::half + qr * 128 +
+                *(uint4 *)(basep + t * L::q_tile + (c / 8) * L::q_half + qr * 128 +
                            (((c % 8) ^ (qr & 7)) << 4)) = v[i];
             }
             umma::fence_smem_async();
             arrive(q_full + 8 * t);
         }
-        // this thread's half of the scores, later of the weights, and of the results
         const uint32_t lanes = (uint32_t)quad * 32 << 16;
-        const uint32_t st = tmem + L::s(t) + h * kHalf + lanes, ot = tmem + L::o(t) + lanes;
+        // this thread's half of the scores and of the weights
+        const uint32_t ot = tmem + L::o(t) + lanes, st = tmem + L::s(t) + h * L::cols + lanes;
         float *const swap = (float *)(basep + L::swap) + t * 2 * kRows;
         const bool warp_live = row0 + t * kRows + quad * 32 < rows;
         const int see = PACKED ? 0 : row < rows ? sees(row) : 0;
         const float c = a.scale_log2;
         float m = -INFINITY;
         float2 l = make_float2(0.f, 0.f);    // two halves of the sum
-        bool ok = true;
+        // Steps that are not full, and those with keys that only some rows see: what
+        // lies behind the keys may be anything, and a weight of zero does not hide a
+        // NaN.  They are the last ones, and the prefix's last.
+        const int whole = min(causal ? max(see_first, 0) : own_seen, own_seen) / KEYS;
+        const int masked_from = pre_tiles + whole - first;
+        const int masked_pre = n_pre % KEYS ? pre_tiles - 1 - first : -1;
         for (int j = 0; j < mine; j++) {
-            const bool pre = first + j < pre_tiles;
-            const int k0 = (first + j - (pre ? 0 : pre_tiles)) * kKeys;
-            const int held = (pre ? n_pre : own_seen) - k0;     // keys in the tile
-            // A tile that is not full: what lies behind its keys may be anything,
-            // and a weight of zero does not hide a NaN.  The same for keys that
-            // only some rows see, unless they are finite.
-            const bool cut = causal && !pre && min(own_seen, k0 + kKeys) > see_first;
-            if (held < kKeys || cut) {
-                const int i = 2 * j + 1;
-                ok = ok && wait(kv_full + 8 * (i % NS), (i / NS) & 1, fail);
-                // two threads a key of this half
-                const int key = h * kHalf + r % kHalf, part_bytes = D;
-                uint8_t *v = basep + L::ring + (i % NS) * L::kv_tile + key * 128;
-                const int x0 = r / kHalf * part_bytes, x1 = x0 + part_bytes;
-                auto at = [&](int x) { return v + (x / 128) * L::half + x % 128; };
+            const bool masked = j >= masked_from || j == masked_pre;
+            int lim = 0;                    // keys of the step that this row sees
+            if (__builtin_expect(masked, 0)) {
+                const bool pre = first + j < pre_tiles;
+                const int k0 = (first + j - (pre ? 0 : pre_tiles)) * KEYS;
+                const int held = (pre ? n_pre : own_seen) - k0;
+                lim = pre ? held : min(held, see - k0);
+                const int n = 2 * j + 1;        // the n-th tile in the ring
+                wait(kv_full + 8 * (n % NS), (n / NS) & 1, fail);
+                // two threads a key
+                const int key = r, x0 = r < KEYS ? h * D : 0, x1 = r < KEYS ? x0 + D : 0;
+                uint8_t *v = basep + L::ring + (n % NS) * L::kv_tile + key * 128;
+                auto at = [&](int x) { return v + (x / 128) * L::kv_half + x % 128; };
                 if (key >= held) {
                     for (int x = x0; x < x1; x += 16) *(uint4 *)at(x) = make_uint4(0, 0, 0, 0);
-                } else if (cut && k0 + key >= see_first) {
+                } else if (causal && !pre && k0 + key >= see_first) {
                     constexpr uint32_t E = fmt16<T>() ? 0x7f80u : 0x7c00u;
                     bool bad = false;
                     for (int x = x0; x < x1; x += 16) {
@@ -552,42 +553,36 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                 }
                 umma::fence_smem_async();
             }
-            ok = ok && wait(s_full + 8 * t, j & 1, fail);
-            // A wait that gave up leaves the results unusable, but every warp still
-            // takes every step, as its partner waits for it.
-            ok = __all_sync(~0u, ok);
+            wait(s_full + 8 * t, j & 1, fail);
             umma::fence_after();
             if (warp_live) {
-                float s[kHalf];
+                float s[L::cols];
 #pragma unroll
-                for (int x = 0; x < kHalf; x += 32) tmem_ld32(st + x, s + x);
+                for (int x = 0; x < L::cols; x += 8) tmem_ld8(st + x, s + x);
                 tmem_ld_wait();
-                const int lim = (pre ? held : min(held, see - k0)) - h * kHalf;
-                if (held < kKeys || cut) {
+                if (__builtin_expect(masked, 0)) {
+                    lim -= h * L::cols;
 #pragma unroll
-                    for (int x = 0; x < kHalf; x++) s[x] = x < lim ? s[x] : -INFINITY;
+                    for (int x = 0; x < L::cols; x++) s[x] = x < lim ? s[x] : -INFINITY;
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int x = 4; x + 8 <= kHalf; x += 8)
+                for (int x = 4; x + 8 <= L::cols; x += 8)
 #pragma unroll
                     for (int y = 0; y < 4; y++) mx[y] = max3(mx[y], s[x + y], s[x + y + 4]);
-                mx[0] = max3(mx[0], s[kHalf - 4], s[kHalf - 3]);
-                mx[1] = max3(mx[1], s[kHalf - 2], s[kHalf - 1]);
+                mx[0] = max3(mx[0], s[L::cols - 4], s[L::cols - 3]);
+                mx[1] = max3(mx[1], s[L::cols - 2], s[L::cols - 1]);
                 float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                // the other half's; it is read before this row's weights are handed
-                // over, so before either half's next scores
+                // (the scores are there, so the product of the step before is done, and
+                // with it the other half's reading of that step's maximum)
                 swap[h * kRows + r] = top;
                 pair_sync(t, quad);
                 top = max3(top, swap[(h ^ 1) * kRows + r], top);
                 const bool grow = !((top - m) * c <= 8.f);
-                if (__any_sync(~0u, grow)) {
+                if (__builtin_expect(__any_sync(~0u, grow), 0)) {
                     const float to = grow ? top : m;
                     const float w = !grow || to == -INFINITY ? 1.f : ex2(m * c - to * c);
                     if (j > 0) {
-                        ok = ok && wait(o_done + 8 * t, (j - 1) & 1, fail);
-                        ok = __all_sync(~0u, ok);
-                        umma::fence_after();
 #pragma unroll 1
                         for (int x = h * (D / 2); x < (h + 1) * (D / 2); x += 16) {
                             float o[16];
@@ -595,7 +590,8 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                             uint32_t u[16];
 #pragma unroll
                             for (int y = 0; y < 16; y++) u[y] = __float_as_uint(o[y] * w);
-                            tmem_st16(ot + x, u);
+                            tmem_st8(ot + x, u);
+                            tmem_st8(ot + x + 8, u + 8);
                         }
                     }
                     l.x *= w;
@@ -606,16 +602,16 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                 const float mc = m == -INFINITY ? 0.f : m < INFINITY ? m * c : NAN;
                 const uint64_t c2 = pair2(c, c), mc2 = pair2(-mc, -mc);
                 uint64_t l2 = pair2(l.x, l.y);
-                if (held < kKeys || cut) weights<T, 0>(s, c2, mc2, l2, st);
-                else weights<T, kPoly>(s, c2, mc2, l2, st);
+                if (__builtin_expect(masked, 0)) weights<T, 0>(s, c2, mc2, l2, st);
+                else weights<T, poly_pairs(D)>(s, c2, mc2, l2, st);
                 l = both(l2);
             }
             umma::fence_before();
-            arrive(p_full + 16 * t + 8 * h);
+            __syncwarp();
+            if (lane == 0) arrive(p_full + 8 * t);
         }
-        if (mine > 0 && ok) ok = wait(o_done + 8 * t, (mine - 1) & 1, fail);
+        if (mine > 0) wait(o_end + 8 * t, 0, fail);
         umma::fence_after();
-        ok = __all_sync(~0u, ok);
         if (t < tiles_rows) {
             // The results go through the tile's place of Q, which is done with, so
             // that rows are written by neighbouring threads.
@@ -627,6 +623,7 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
             __threadfence_block();
             const bool mend = *dirty && causal;
             uint8_t *const stage = basep + t * L::q_tile;
+            tile_sync(t);                   // the last maxima are read
             swap[h * kRows + r] = l.x + l.y;
             tile_sync(t);
             const float sum = swap[r] + swap[kRows + r];
@@ -639,7 +636,7 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                 for (int x = x0 + h * (wide / 2); x < x0 + (h + 1) * (wide / 2); x += 16) {
                     __syncwarp();
                     float o[16];
-                    if (mine > 0 && warp_live && ok) {
+                    if (mine > 0 && warp_live) {
                         umma::tmem_ld16(ot + x, o);
                     } else {
 #pragma unroll
@@ -647,8 +644,8 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                     }
                     if (mend && row < rows) {
                         // what was wiped and is in sight of this row
-                        const int end = min(see, max(0, first + each - pre_tiles) * kKeys);
-                        for (int k = max(max(see_first, 0), (first - pre_tiles) * kKeys); k < end;
+                        const int end = min(see, max(0, first + each - pre_tiles) * KEYS);
+                        for (int k = max(max(see_first, 0), (first - pre_tiles) * KEYS); k < end;
                              k++) {
                             const int page =
                                 attn_page(a, a.pages + (int64_t)blockIdx.z * a.pages_row, k);
@@ -703,7 +700,7 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
     }
     umma::fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && *fail) atomicOr(a.err, kAttnTimeout);
+    if (threadIdx.x == 0 && *failed) atomicOr(a.err, kAttnTimeout);
     if (warp == 16) {
         umma::fence_after();
         umma::tmem_free(tmem, 512);
@@ -730,8 +727,7 @@ static CUresult (*encode_fn())(CUtensorMap *, CUtensorMapDataType, cuuint32_t, v
     return fn;
 }
 
-// The pages as a tensor (dim, slot, head, page), boxes of 64 columns by the
-// keys of a page (128 at most).
+// The pages as a tensor (dim, slot, head, page), boxes of 64 columns by 16 keys.
 static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t page, int64_t slot,
                     int64_t head) {
     const auto fn = encode_fn();
@@ -746,7 +742,7 @@ static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t p
     const cuuint64_t strides[3] = {slot ? (cuuint64_t)slot * 2 : row,
                                    head ? (cuuint64_t)head * 2 : row,
                                    page ? (cuuint64_t)page * 2 : row};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(c->page_size < kKeys ? c->page_size : kKeys), 1, 1};
+    const cuuint32_t box[4] = {64, kBox, 1, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     const CUresult r = fn(m, c->type == WARP_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
