@@ -58,84 +58,114 @@ struct RopeArgs {
     float eps, rot_scale;
     int tokens, q_heads, kv_heads, D, rot, interleaved, page_shift;
     int rows;                               // rows a token: q, then k, then v (append)
-    int rows_per_cta;
+    int shares, rows_per_share;             // of a token's rows, one share a warp
 };
 
 template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) RopeVec {
     T x[N];
 };
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeWarps = 4;
+constexpr int kRopeCtas = 8;                // an SM: occupancy is what hides the latency here
 constexpr int kRopeMaxPairs = 128;          // head_dim up to 256
+
+template <int VEC> __device__ __forceinline__ void rope_f32(float (&x)[VEC], const float *p) {
+    const RopeVec<float, VEC> v = *(const RopeVec<float, VEC> *)p;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) x[i] = v.x[i];
+}
 
 // L lanes a row, UPL units a lane.
 template <typename TI, typename TO, int VEC, int L, int UPL>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
-    __shared__ float2 cs[kRopeMaxPairs];
-    const int t = blockIdx.x;
-    const int row0 = blockIdx.y * a.rows_per_cta;
-    const int row1 = min(a.rows, row0 + a.rows_per_cta);
+__global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const RopeArgs a) {
+    __shared__ alignas(16) float turns_of[kRopeWarps][2 * kRopeMaxPairs];
+    constexpr int RPW = 32 / L;             // rows of a warp at a time
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % L;
+    const int64_t id = (int64_t)blockIdx.x * kRopeWarps + warp;
+    const int t = (int)(id / a.shares);
+    if (t >= a.tokens) return;
+    const int row0 = (int)(id - (int64_t)t * a.shares) * a.rows_per_share + threadIdx.x % 32 / L;
+    const int row1 = min(a.rows, row0 - threadIdx.x % 32 / L + a.rows_per_share);
     const int half = a.rot / 2;
+    const int units = a.D / (2 * VEC), rot_units = a.rot / (2 * VEC);
+    const int k0 = a.q_heads, v0 = a.q_heads + a.kv_heads;      // first rows of k and v
+
+    // Where unit n's two vectors start.  Half layout: the rotated units first,
+    // behind them the rest of the row in two halves; interleaved: the whole row in
+    // two halves, as pairs lie within a vector (but for single values).
+    // Neighbouring lanes' vectors are neighbours either way.
+    int at0[UPL], at1[UPL];
+#pragma unroll
+    for (int n = 0; n < UPL; n++) {
+        const int u = lane + n * L;
+        if (a.interleaved) {
+            at0[n] = VEC > 1 ? u * VEC : 2 * u;
+            at1[n] = VEC > 1 ? (units + u) * VEC : 2 * u + 1;
+        } else {
+            const bool turned = u < rot_units;
+            at0[n] = turned ? u * VEC : a.rot + (u - rot_units) * VEC;
+            at1[n] = turned ? half + u * VEC : at0[n] + (units - rot_units) * VEC;
+        }
+    }
+    const TI *const q = (const TI *)a.q + t * a.q_token;
+    const TI *const k = (const TI *)a.k + t * a.k_token - k0 * a.k_head;
+    const TI *const v = (const TI *)a.v + t * a.v_token - v0 * a.v_head;
+
     // The angle in turns, reduced in 64 bits: what is left is a fraction of a
     // turn that fp32 holds to 2^-25, whatever the position.
-    if ((int)threadIdx.x < half) {
-        double turns = (double)a.positions[t] * a.inv_freq[threadIdx.x] * 0.15915494309189533577;
-        turns -= rint(turns);
-        float s, c;
-        sincospif(2.0f * (float)turns, &s, &c);
-        cs[threadIdx.x] = make_float2(c * a.rot_scale, s * a.rot_scale);
+    float *const cosines = turns_of[warp], *const sines = cosines + kRopeMaxPairs;
+    if (half) {
+        const double pos = (double)a.positions[t];
+        for (int i = threadIdx.x % 32; i < half; i += 32) {
+            double turns = pos * a.inv_freq[i] * 0.15915494309189533577;
+            turns -= rint(turns);
+            float si, co;
+            sincospif(2.0f * (float)turns, &si, &co);
+            cosines[i] = co * a.rot_scale;
+            sines[i] = si * a.rot_scale;
+        }
+        __syncwarp();
     }
-    int64_t slot = -1;
+    int64_t slot = -1, page = 0, off = 0;
     if (a.slots) {
         slot = a.slots[t];
         if (slot >= a.n_slots) {
-            if (threadIdx.x == 0) atomicOr(a.err, kAttnBadSlot);
+            if (threadIdx.x % 32 == 0) atomicOr(a.err, kAttnBadSlot);
             slot = -1;
         }
+        page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
     }
-    __syncthreads();
+    TO *const qd = (TO *)a.q_out + (int64_t)t * a.q_heads * a.D;
+    TO *kd = (TO *)a.k_out + ((int64_t)t * a.kv_heads - k0) * a.D, *vd = nullptr;
+    int64_t kd_head = a.D;
+    if (a.slots) {
+        kd = (TO *)a.kp + page * a.k_page + off * a.k_slot - k0 * a.k_ph;
+        vd = (TO *)a.vp + page * a.v_page + off * a.v_slot - v0 * a.v_ph;
+        kd_head = a.k_ph;
+    }
+    const float inv_d = 1.0f / (float)a.D;
+    const bool norms = a.q_norm || a.k_norm;
 
-    constexpr int RPP = kRopeThreads / L;   // rows in flight
-    const int lane = threadIdx.x % L;
-    const int units = a.D / (2 * VEC), rot_units = a.rot / (2 * VEC);
-    for (int base = row0; base < row1; base += RPP) {
-        const int r = base + (int)threadIdx.x / L;
+    // Every lane takes every step, for the sums across lanes.
+    for (int r = row0; r - (int)(threadIdx.x % 32) / L < row1; r += RPW) {
         const bool live = r < row1;
-        // whose row: 0 q, 1 k, 2 v
-        const int rr = live ? r : row0;
-        const int who = rr < a.q_heads ? 0 : rr < a.q_heads + a.kv_heads ? 1 : 2;
-        const int h = who == 0 ? rr : who == 1 ? rr - a.q_heads : rr - a.q_heads - a.kv_heads;
-        const TI *src = who == 0 ? (const TI *)a.q + t * a.q_token + h * a.q_head
-                      : who == 1 ? (const TI *)a.k + t * a.k_token + h * a.k_head
-                                 : (const TI *)a.v + t * a.v_token + h * a.v_head;
         float x0[UPL][VEC], x1[UPL][VEC];
-        int at0[UPL], at1[UPL];             // where the unit's two vectors start
+        const TI *const src = r < k0 ? q + r * a.q_head : r < v0 ? k + r * a.k_head
+                                                                 : v + r * a.v_head;
 #pragma unroll
         for (int n = 0; n < UPL; n++) {
-            const int u = lane + n * L;
-            // rotated units first; behind them the rest of the row, two vectors a unit
-            if (u < rot_units && !a.interleaved) {
-                at0[n] = u * VEC;
-                at1[n] = half + u * VEC;
-            } else {
-                at0[n] = u * 2 * VEC;
-                at1[n] = at0[n] + VEC;
+            RopeVec<TI, VEC> a0 = {}, a1 = {};
+            if (live && lane + n * L < units) {
+                a0 = *(const RopeVec<TI, VEC> *)(src + at0[n]);
+                a1 = *(const RopeVec<TI, VEC> *)(src + at1[n]);
             }
-            if (live && u < units) {
-                const RopeVec<TI, VEC> v0 = *(const RopeVec<TI, VEC> *)(src + at0[n]);
-                const RopeVec<TI, VEC> v1 = *(const RopeVec<TI, VEC> *)(src + at1[n]);
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    x0[n][i] = AttnType<TI>::up(v0.x[i]);
-                    x1[n][i] = AttnType<TI>::up(v1.x[i]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) x0[n][i] = x1[n][i] = 0.f;
+            for (int i = 0; i < VEC; i++) {
+                x0[n][i] = AttnType<TI>::up(a0.x[i]);
+                x1[n][i] = AttnType<TI>::up(a1.x[i]);
             }
         }
-        const float *w = who == 0 ? a.q_norm : who == 1 ? a.k_norm : nullptr;
-        if (a.q_norm || a.k_norm) {         // the same branch for the whole warp
+        if (norms) {
             float ss = 0.f;
 #pragma unroll
             for (int n = 0; n < UPL; n++)
@@ -143,78 +173,84 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
                 for (int i = 0; i < VEC; i++) ss += x0[n][i] * x0[n][i] + x1[n][i] * x1[n][i];
 #pragma unroll
             for (int o = L / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+            const float *w = r < k0 ? a.q_norm : r < v0 ? a.k_norm : nullptr;
             if (w) {
-                const float inv = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+                const float inv = rsqrtf(ss * inv_d + a.eps);
 #pragma unroll
                 for (int n = 0; n < UPL; n++) {
                     if (lane + n * L >= units) continue;
+                    float w0[VEC], w1[VEC];
+                    rope_f32<VEC>(w0, w + at0[n]);
+                    rope_f32<VEC>(w1, w + at1[n]);
 #pragma unroll
                     for (int i = 0; i < VEC; i++) {
-                        x0[n][i] *= inv * __ldg(w + at0[n] + i);
-                        x1[n][i] *= inv * __ldg(w + at1[n] + i);
+                        x0[n][i] *= inv * w0[i];
+                        x1[n][i] *= inv * w1[i];
                     }
                 }
             }
         }
-        if (!live) continue;
-        TO *dst;
-        if (who == 0) {
-            dst = (TO *)a.q_out + ((int64_t)t * a.q_heads + h) * a.D;
-        } else if (a.slots) {
-            if (slot < 0) continue;
-            const int64_t page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
-            dst = who == 1 ? (TO *)a.kp + page * a.k_page + off * a.k_slot + h * a.k_ph
-                           : (TO *)a.vp + page * a.v_page + off * a.v_slot + h * a.v_ph;
-        } else {
-            dst = (TO *)a.k_out + ((int64_t)t * a.kv_heads + h) * a.D;
-        }
+        if (!live || (r >= k0 && a.slots && slot < 0)) continue;
+        TO *const dst = r < k0 ? qd + r * a.D : r < v0 ? kd + r * kd_head : vd + r * a.v_ph;
 #pragma unroll
         for (int n = 0; n < UPL; n++) {
-            const int u = lane + n * L;
-            if (u >= units) continue;
-            if (u < rot_units && who != 2) {
-                if (a.interleaved) {
-                    // pairs are neighbours: (x0[0], x0[1]) ..., then x1's
+            if (lane + n * L >= units) continue;
+            auto turn = [](float &x, float &y, float c, float s) {
+                const float r0 = x * c - y * s, r1 = x * s + y * c;
+                x = r0;
+                y = r1;
+            };
+            if (r >= v0 || !half) {
+                // passes through
+            } else if (VEC > 1 && a.interleaved) {
+                constexpr int P = (VEC + 1) / 2;
+                float c[P], s[P];
+                if (at0[n] < a.rot) {
+                    rope_f32<P>(c, cosines + at0[n] / 2);
+                    rope_f32<P>(s, sines + at0[n] / 2);
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        // value i of the unit's 2*VEC, pair u*VEC + i
-                        float &p = 2 * i < VEC ? x0[n][(2 * i) % VEC] : x1[n][(2 * i) % VEC];
-                        float &q = 2 * i + 1 < VEC ? x0[n][(2 * i + 1) % VEC]
-                                                   : x1[n][(2 * i + 1) % VEC];
-                        const float2 c = cs[u * VEC + i];
-                        const float y0 = p * c.x - q * c.y, y1 = p * c.y + q * c.x;
-                        p = y0;
-                        q = y1;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        const float2 c = cs[u * VEC + i];
-                        const float y0 = x0[n][i] * c.x - x1[n][i] * c.y;
-                        const float y1 = x0[n][i] * c.y + x1[n][i] * c.x;
-                        x0[n][i] = y0;
-                        x1[n][i] = y1;
-                    }
+                    for (int i = 0; i < P; i++)
+                        turn(x0[n][2 * i % VEC], x0[n][(2 * i + 1) % VEC], c[i], s[i]);
                 }
+                if (at1[n] < a.rot) {
+                    rope_f32<P>(c, cosines + at1[n] / 2);
+                    rope_f32<P>(s, sines + at1[n] / 2);
+#pragma unroll
+                    for (int i = 0; i < P; i++)
+                        turn(x1[n][2 * i % VEC], x1[n][(2 * i + 1) % VEC], c[i], s[i]);
+                }
+            } else if (lane + n * L < rot_units) {
+                float c[VEC], s[VEC];
+                rope_f32<VEC>(c, cosines + (lane + n * L) * VEC);
+                rope_f32<VEC>(s, sines + (lane + n * L) * VEC);
+#pragma unroll
+                for (int i = 0; i < VEC; i++) turn(x0[n][i], x1[n][i], c[i], s[i]);
             }
-            RopeVec<TO, VEC> v0, v1;
+            RopeVec<TO, VEC> o0, o1;
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                v0.x[i] = AttnType<TO>::down(x0[n][i]);
-                v1.x[i] = AttnType<TO>::down(x1[n][i]);
+                o0.x[i] = AttnType<TO>::down(x0[n][i]);
+                o1.x[i] = AttnType<TO>::down(x1[n][i]);
             }
-            *(RopeVec<TO, VEC> *)(dst + at0[n]) = v0;
-            *(RopeVec<TO, VEC> *)(dst + at1[n]) = v1;
+            *(RopeVec<TO, VEC> *)(dst + at0[n]) = o0;
+            *(RopeVec<TO, VEC> *)(dst + at1[n]) = o1;
         }
     }
 }
 
 template <typename TI, typename TO, int VEC, int L, int UPL>
 static int rope_launch(RopeArgs &a, cudaStream_t st) {
-    constexpr int RPP = kRopeThreads / L;
-    a.rows_per_cta = RPP;
+    constexpr int RPW = 32 / L;
+    // A token's rows are shared out among warps while there are fewer than
+    // 32 an SM, down to one step of a warp each.
+    const int64_t steps = (a.rows + RPW - 1) / RPW, want = (int64_t)32 * 148;
+    int64_t shares = a.tokens < want ? want / a.tokens : 1;
+    shares = shares < 1 ? 1 : shares > steps ? steps : shares;
+    const int64_t each = (steps + shares - 1) / shares;
+    a.rows_per_share = (int)(each * RPW);
+    a.shares = (int)((steps + each - 1) / each);
     rope_kernel<TI, TO, VEC, L, UPL>
-        <<<dim3(a.tokens, cdiv(a.rows, a.rows_per_cta)), kRopeThreads, 0, st>>>(a);
+        <<<cdiv((size_t)a.tokens * a.shares, kRopeWarps), kRopeWarps * 32, 0, st>>>(a);
     WARP_CHECK_LAUNCH("rope_kernel");
     return WARP_OK;
 }
@@ -227,6 +263,8 @@ static int rope_vec(RopeArgs &a, cudaStream_t st) {
         const uintptr_t ob = vec * sizeof(TO) < 16 ? vec * sizeof(TO) : 16;
         if (a.rot % (2 * vec) || a.D % (2 * vec)) return false;
         uintptr_t in = 0, out = (uintptr_t)a.q_out | (uintptr_t)a.k_out;
+        const uintptr_t wb = vec * sizeof(float) < 16 ? vec * sizeof(float) : 16;
+        if (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) % wb) return false;
         auto add = [&](const void *p, int64_t s0, int64_t s1) {
             if (p) in |= (uintptr_t)p | (uintptr_t)(s0 * sizeof(TI)) | (uintptr_t)(s1 * sizeof(TI));
         };
