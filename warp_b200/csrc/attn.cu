@@ -117,9 +117,8 @@ template <int D> struct ADLay {
 // (one "request" for the batch).  Otherwise rows and keys of one request, with
 // the prefix's keys in front where there is one that is not computed apart.
 template <typename T, int D, bool PACKED>
-__global__ void __launch_bounds__(kADWarps * 32, 2) attn_rows_kernel(const AttnArgs a) {
+__device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
     using Lay = ADLay<D>;
-    extern __shared__ __align__(128) uint8_t smem[];
     const int kvh = blockIdx.y;
     AttnReq rq;
     int part, row0, pre_tiles, own_tiles;
@@ -381,37 +380,57 @@ __global__ void __launch_bounds__(kADWarps * 32, 2) attn_rows_kernel(const AttnA
     }
 }
 
+// The kernels of one call are launched so that each may start while the one
+// before it runs (they read the same inputs and write different parts), and
+// each waits for that one at its end, so that the last one's end is the end of all.
+template <typename T, int D, bool PACKED>
+__global__ void __launch_bounds__(kADWarps * 32, 2)
+attn_rows_kernel(const __grid_constant__ AttnArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    pdl_trigger();
+    attn_rows<T, D, PACKED>(a, smem);
+    pdl_wait();
+}
+
 // Joins the parts of each row: a warp a (token, head).  Rows whose request has
-// one part were written by their CTA.
+// one part were written by their CTA.  Each lane has D / 32 values of a row and,
+// for the weights, the maximum and sum of one part in 32.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
     const int lane = threadIdx.x % 32;
     const int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
     const int64_t rows = (int64_t)a.tokens * a.q_heads;
-    if (row >= rows) return;
-    const int t = (int)(row / a.q_heads);
-    // the token's request: the last one that starts at or before it
-    int b = -1;
-    for (int i0 = 0; i0 < a.batch; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned hit = __ballot_sync(~0u, i < a.batch && a.q_start[i] <= t);
-        if (hit) b = i0 + 31 - __clz(hit);
-        if (hit != ~0u) break;
+    int parts = 0;
+    if (row < rows) {
+        const int t = (int)(row / a.q_heads);
+        // the token's request: the last one that starts at or before it
+        int b = -1;
+        for (int i0 = 0; i0 < a.batch; i0 += 32) {
+            const int i = i0 + lane;
+            const unsigned hit = __ballot_sync(~0u, i < a.batch && a.q_start[i] <= t);
+            if (hit) b = i0 + 31 - __clz(hit);
+            if (hit != ~0u) break;
+        }
+        if (b >= 0) {
+            const AttnReq rq = attn_req(a, b);
+            const bool wide = rq.n * a.group > a.rows_small;
+            const int tile = wide ? attn_wide(D) : kAttnTile;
+            const int own = (a.packed ? 0 : (a.prefix_len + tile - 1) / tile) +
+                            (rq.len + tile - 1) / tile;
+            parts = max(1, attn_parts(own, wide ? a.wide_each : a.split_tiles));
+            if ((!a.packed && parts == 1) || t >= rq.t0 + rq.n) parts = 0;
+            else parts += a.prefix_parts;
+        }
     }
-    if (b < 0) return;
-    const AttnReq rq = attn_req(a, b);
-    if (t >= rq.t0 + rq.n) return;
-    const bool wide = rq.n * a.group > a.rows_small;
-    const int tile = wide ? attn_wide(D) : kAttnTile;
-    const int own = (a.packed ? 0 : (a.prefix_len + tile - 1) / tile) + (rq.len + tile - 1) / tile;
-    int parts = max(1, attn_parts(own, wide ? a.wide_each : a.split_tiles));
-    if (!a.packed && parts == 1) return;
-    parts += a.prefix_parts;
+    pdl_wait();
+    if (!parts) return;
     constexpr int V = D / 32;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0.f;
     float M = -INFINITY, l = 0.f;
+    const float *src = a.part_o + row * D + lane * V;
+    const int64_t stride = rows * D;
     for (int p0 = 0; p0 < parts; p0 += 32) {
         const int p = p0 + lane;
         const float2 ml = p < parts ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f);
@@ -425,19 +444,33 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
         for (int i = 0; i < V; i++) acc[i] *= keep;
         M = m;
         const int here = min(32, parts - p0);
-        for (int k = 0; k < here; k++) {
-            const float f = __shfl_sync(~0u, w, k);
-            const float *src = a.part_o + ((p0 + k) * rows + row) * D + lane * V;
+        // in order, eight parts' loads in flight
+        for (int k0 = 0; k0 < here; k0 += 8) {
+            float v[8][V];
 #pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += f * src[i];
+            for (int k = 0; k < 8; k++)
+                if (k0 + k < here) {
+                    if (V == 4) *(float4 *)v[k] = *(const float4 *)(src + (p0 + k0 + k) * stride);
+                    else *(float2 *)v[k] = *(const float2 *)(src + (p0 + k0 + k) * stride);
+                }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = __shfl_sync(~0u, w, k0 + k);
+                if (k0 + k < here)
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[i] += f * v[k][i];
+            }
         }
     }
 #pragma unroll
     for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T *dst = (T *)a.out + row * D + lane * V;
+    uint32_t o[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; i += 2) *(uint32_t *)(dst + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+    for (int i = 0; i < V; i += 2) o[i / 2] = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+    T *dst = (T *)a.out + row * D + lane * V;
+    if (V == 4) *(uint2 *)dst = *(uint2 *)o;
+    else *(uint32_t *)dst = o[0];
 }
 
 // ------------------------------------------------------------ host side --
@@ -455,29 +488,44 @@ struct AttnPlan {
 
 static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Key tiles a part of attn_rows_kernel: CTAs enough to fill the card twice
-// over where there are keys enough, no fewer than 16 tiles (4 a warp).
-static int pick_split(int64_t tiles, int64_t ctas) {
-    const int64_t want = 2 * 2 * 148;
+// Key tiles a part, for `ctas` CTAs of `tiles` tiles each: the split that takes
+// the fewest microseconds by the measured time of a tile, of a CTA around its
+// tiles and, if there are parts, of the join (its launch, and `rows` rows of
+// fp32 parts written and read again).
+static int pick_split(int64_t tiles, int64_t ctas, int64_t slots, double tile_us, double cta_us,
+                      int64_t least, double rows, int D) {
     ctas = ctas < 1 ? 1 : ctas;
-    int64_t parts = up(want, ctas);
-    parts = parts > 256 ? 256 : parts;
-    const int64_t each = up(tiles, parts);
-    return (int)(each < 16 ? 16 : each);
-}
-
-// Key tiles a part of attn_umma_kernel, one CTA an SM: the split with the
-// fewest tiles in a row on the busiest SM, counting a part's start, end and
-// join as the like of three tiles.
-static int pick_wide(int64_t tiles, int64_t ctas) {
-    ctas = ctas < 1 ? 1 : ctas;
-    int64_t best = tiles < 1 ? 1 : tiles, cost = up(ctas, 148) * (tiles + 3);
-    for (int64_t parts = 2; parts <= 64 && parts * 2 <= tiles; parts++) {
-        const int64_t each = up(tiles, parts);
-        const int64_t now = up(ctas * up(tiles, each), 148) * (each + 3) + 3;
-        if (now < cost) best = each, cost = now;
+    int64_t best = tiles < 1 ? 1 : tiles;
+    double least_us = 1e30;
+    for (int64_t parts = 1; parts <= 128; parts++) {
+        const int64_t each = up(tiles < 1 ? 1 : tiles, parts);
+        if (parts > 1 && each < least) break;
+        const int64_t n = up(tiles < 1 ? 1 : tiles, each);
+        const double x = (double)ctas * n / slots;
+        // Lengths are known on the device alone.  If they are all the same: whole
+        // waves while there are few of them (many even out).  If they spread
+        // from a fifth of the largest up: their mean's work evened out, and half
+        // a CTA's time until the last one is done, but no less than the longest.
+        const double one = each * tile_us, waves = x < 4 ? (double)up(ctas * n, slots) : x + 0.5;
+        const double same = waves * (one + cta_us);
+        const double mixed = 0.6 * x * one + 0.5 * one;
+        double us = 0.5 * same + 0.5 * ((mixed > one ? mixed : one) + (x < 1 ? 1 : x) * cta_us);
+        if (n > 1) us += 3 + rows * n * D * 8 / 4e6;
+        if (us < least_us * 0.98) best = each, least_us = us;
     }
     return (int)best;
+}
+
+// attn_rows_kernel: two CTAs an SM; 16 keys of K and V of one head at an even
+// share of the memory's rate, or at least what a CTA's own latency allows.
+static int split_rows(int64_t tiles, int64_t ctas, double rows, int D) {
+    const double tile_us = D == 128 ? 0.36 : 0.20;
+    return pick_split(tiles, ctas, 2 * 148, tile_us, 3.0, 4, rows, D);
+}
+
+// attn_umma_kernel: one CTA an SM.
+static int split_wide(int64_t tiles, int64_t ctas, double rows, int D) {
+    return pick_split(tiles, ctas, 148, D == 128 ? 1.75 : 1.6, 6.0, 2, rows, D);
 }
 
 static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
@@ -487,6 +535,7 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     p.max_kv = d->max_kv < held ? d->max_kv : (int)held;
     const int64_t group = d->q_heads / d->kv_heads;
     const int keys = attn_wide(d->head_dim);
+    const int64_t out = (int64_t)d->tokens * d->q_heads;        // rows of the result
     // The prefix apart, for all rows at once, where a request's rows alone
     // would leave a row tile mostly empty.
     p.packed = d->prefix_len > 0 && d->batch > 1 && d->tokens * group <= (int64_t)128 * d->batch;
@@ -498,26 +547,28 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
         const int64_t pairs = up(rows, 256) * d->batch, by_tokens = up(d->tokens * group, 256);
         const int64_t ctas = pairs < by_tokens + d->batch - 1 ? pairs : by_tokens + d->batch - 1;
         const int64_t tiles = up(p.max_kv, keys) + up(pre, keys);
-        p.wide_each = pick_wide(tiles, ctas * d->kv_heads);
+        p.wide_each = split_wide(tiles, ctas * d->kv_heads, out, d->head_dim);
         p.wide_parts = tiles ? (int)up(tiles, p.wide_each) : 1;
     }
     if (p.rows_small) {
         const int64_t tiles = up(p.max_kv, kAttnTile) + up(pre, kAttnTile);
         p.small_tiles = (int)up(rows < p.rows_small ? rows : p.rows_small, kADRows);
-        p.each = pick_split(tiles, (int64_t)d->batch * d->kv_heads * p.small_tiles);
+        p.each = split_rows(tiles, (int64_t)d->batch * d->kv_heads * p.small_tiles, out,
+                            d->head_dim);
         p.parts = tiles ? (int)up(tiles, p.each) : 1;
     }
     if (p.packed) {
         const int64_t all = d->tokens * group;
         p.packed_wide = all > kADRows;
         const int64_t tiles = up(d->prefix_len, p.packed_wide ? keys : kAttnTile);
-        p.prefix_each = p.packed_wide ? pick_wide(tiles, up(all, 256) * d->kv_heads)
-                                      : pick_split(tiles, up(all, kADRows) * d->kv_heads);
+        p.prefix_each =
+            p.packed_wide ? split_wide(tiles, up(all, 256) * d->kv_heads, out, d->head_dim)
+                          : split_rows(tiles, up(all, kADRows) * d->kv_heads, out, d->head_dim);
         p.prefix_parts = (int)up(tiles, p.prefix_each);
     }
     const int own = p.parts > p.wide_parts ? p.parts : p.wide_parts;
     p.join = p.packed || own > 1;
-    const int64_t all = p.join ? p.prefix_parts + own : 0, out = (int64_t)d->tokens * d->q_heads;
+    const int64_t all = p.join ? p.prefix_parts + own : 0;
     p.o_bytes = up(all * out * d->head_dim * 4, 256) * 256;
     p.ml_bytes = up(all * out * 8, 256) * 256;
     return p;
@@ -549,7 +600,7 @@ static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
 }
 
 template <typename T, int D>
-static int attn_launch(const AttnArgs &a, const AttnPlan &p, cudaStream_t st) {
+static int attn_launch(const AttnArgs &a, const AttnPlan &p, bool first, cudaStream_t st) {
     using Lay = ADLay<D>;
     static bool attr_done = false;                      // per instantiation, per process
     if (!attr_done) {
@@ -562,22 +613,28 @@ static int attn_launch(const AttnArgs &a, const AttnPlan &p, cudaStream_t st) {
         if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
         attr_done = true;
     }
+    cudaError_t e;
     if (p.packed && !p.packed_wide) {
-        attn_rows_kernel<T, D, true>
-            <<<dim3((unsigned)(up((int64_t)a.tokens * a.group, kADRows) * p.prefix_parts),
-                    a.kv_heads, 1), kADWarps * 32, Lay::bytes, st>>>(a);
-        WARP_CHECK_LAUNCH("attn_rows_kernel (prefix)");
+        e = attn_start(attn_rows_kernel<T, D, true>,
+                       dim3((unsigned)(up((int64_t)a.tokens * a.group, kADRows) * p.prefix_parts),
+                            a.kv_heads, 1), kADWarps * 32, Lay::bytes, st, first, a);
+        if (e != cudaSuccess) return cuda_fail(e, "attn_rows_kernel (prefix)");
+        count_launch();
+        first = false;
     }
     if (p.small_tiles) {
-        attn_rows_kernel<T, D, false>
-            <<<dim3(p.small_tiles * p.parts, a.kv_heads, a.batch), kADWarps * 32, Lay::bytes,
-               st>>>(a);
-        WARP_CHECK_LAUNCH("attn_rows_kernel");
+        e = attn_start(attn_rows_kernel<T, D, false>,
+                       dim3(p.small_tiles * p.parts, a.kv_heads, a.batch), kADWarps * 32,
+                       Lay::bytes, st, first, a);
+        if (e != cudaSuccess) return cuda_fail(e, "attn_rows_kernel");
+        count_launch();
+        first = false;
     }
     if (p.join) {
-        attn_join_kernel<T, D>
-            <<<cdiv((size_t)a.tokens * a.q_heads, 8), 256, 0, st>>>(a);
-        WARP_CHECK_LAUNCH("attn_join_kernel");
+        e = attn_start(attn_join_kernel<T, D>, dim3(cdiv((size_t)a.tokens * a.q_heads, 8)), 256, 0,
+                       st, first, a);
+        if (e != cudaSuccess) return cuda_fail(e, "attn_join_kernel");
+        count_launch();
     }
     return WARP_OK;
 }
@@ -629,12 +686,13 @@ extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages
     rc = warp::attn_err_word(&a.err);
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    if (p.packed_wide) rc = warp::attn_umma(a, c, true, st);
-    if (!rc && p.wide_parts) rc = warp::attn_umma(a, c, false, st);
+    bool first = true;
+    if (p.packed_wide) rc = warp::attn_umma(a, c, true, first, st), first = false;
+    if (!rc && p.wide_parts) rc = warp::attn_umma(a, c, false, first, st), first = false;
     if (rc) return rc;
     if (d->type == WARP_T_F16)
-        return d->head_dim == 64 ? warp::attn_launch<__half, 64>(a, p, st)
-                                 : warp::attn_launch<__half, 128>(a, p, st);
-    return d->head_dim == 64 ? warp::attn_launch<__nv_bfloat16, 64>(a, p, st)
-                             : warp::attn_launch<__nv_bfloat16, 128>(a, p, st);
+        return d->head_dim == 64 ? warp::attn_launch<__half, 64>(a, p, first, st)
+                                 : warp::attn_launch<__half, 128>(a, p, first, st);
+    return d->head_dim == 64 ? warp::attn_launch<__nv_bfloat16, 64>(a, p, first, st)
+                             : warp::attn_launch<__nv_bfloat16, 128>(a, p, first, st);
 }

@@ -113,6 +113,21 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 
 // The tensor-core kernel: the requests with many rows, or (packed) the shared
 // prefix for all rows of the batch.
-int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, cudaStream_t st);
+int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,
+              cudaStream_t st);
+
+// Launches a call's first kernel behind everything before it on the stream, and
+// each further one so that it may start early.
+template <typename... KArgs, typename... Args>
+inline cudaError_t attn_start(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem,
+                              cudaStream_t st, bool first, const Args &...args) {
+    if (!first) return launch_pdl(kernel, grid, dim3(threads), smem, st, args...);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 }  // namespace warp

@@ -291,12 +291,10 @@ __device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64
 
 // PACKED: rows are those of all the batch's tokens, keys the shared prefix.
 template <typename T, int D, bool PACKED>
-__global__ void __launch_bounds__(kThreads, 1)
-attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
-                 const __grid_constant__ CUtensorMap vmap) {
+__device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensorMap &kmap,
+                                               const CUtensorMap &vmap, uint8_t *basep) {
     using L = Lay<D>;
     constexpr int NS = L::stages, KEYS = L::keys;
-    extern __shared__ __align__(1024) uint8_t basep[];
     const int kvh = blockIdx.y;
     const AttnReq rq = PACKED ? AttnReq{0, a.tokens, 0} : attn_req(a, blockIdx.z);
     const int rows = rq.n * a.group;
@@ -341,6 +339,29 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
     volatile int *const failed = (volatile int *)(basep + L::bars + L::fail);
     volatile int *const dirty = (volatile int *)(basep + L::bars + L::dirty);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    // The rows' warps: row tile, half of the keys, quarter of the rows, row.
+    const int t = warp / 8, h = warp / 4 % 2, quad = warp % 4, r = threadIdx.x % kRows;
+    const int tid = threadIdx.x % (2 * kRows);          // in the tile
+    // row0's token and its head in the group; row0 + x is then token
+    // tok0 + (rem0 + x) / group
+    const int tok0 = row0 / a.group, rem0 = row0 - tok0 * a.group;
+    const float inv_group = 1.f / (float)a.group;
+    // Q is asked for first of all, a row by D / 8 neighbouring threads.
+    constexpr int CH = D / 8, RP = 2 * kRows / CH, N = kRows / RP;
+    uint4 qv[N];
+    if (t < tiles_rows) {
+        const T *q = (const T *)a.q + (int64_t)(rq.t0 + tok0) * a.q_token +
+                     (int64_t)kvh * a.group * a.q_head + (tid % CH) * 8;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int x = t * kRows + i * RP + tid / CH;
+            const int y = rem0 + x, tok = small_div(y, inv_group);
+            qv[i] = make_uint4(0, 0, 0, 0);
+            if (row0 + x < rows)
+                qv[i] = *(const uint4 *)(q + tok * a.q_token + (y - tok * a.group) * a.q_head);
+        }
+    }
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; i++) {
@@ -467,34 +488,15 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
         }
     } else {
         // ---- the rows ----------------------------------------------------------------
-        const int t = warp / 8, h = warp / 4 % 2, quad = warp % 4, r = threadIdx.x % kRows;
-        const int tid = threadIdx.x % (2 * kRows);      // in the tile
         const int row = row0 + t * kRows + r;
-        // row0's token and its head in the group; row0 + x is then token
-        // tok0 + (rem0 + x) / group
-        const int tok0 = row0 / a.group, rem0 = row0 - tok0 * a.group;
-        const float inv_group = 1.f / (float)a.group;
         const int mine = t == 0 ? cnt0 : tiles_rows == 2 ? cnt : 0;
         if (t < tiles_rows) {
-            // Q into its swizzled place, a row by D / 8 neighbouring threads, all of a
-            // thread's loads in flight
-            constexpr int CH = D / 8, RP = 2 * kRows / CH, N = kRows / RP;
-            const T *q = (const T *)a.q + (int64_t)(rq.t0 + tok0) * a.q_token +
-                         (int64_t)kvh * a.group * a.q_head + (tid % CH) * 8;
-            uint4 v[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int x = t * kRows + i * RP + tid / CH;
-                const int y = rem0 + x, tok = small_div(y, inv_group);
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (row0 + x < rows)
-                    v[i] = *(const uint4 *)(q + tok * a.q_token + (y - tok * a.group) * a.q_head);
-            }
+            // into its swizzled place
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int qr = i * RP + tid / CH, c = tid % CH;
                 *(uint4 *)(basep + t * L::q_tile + (c / 8) * L::q_half + qr * 128 +
-                           (((c % 8) ^ (qr & 7)) << 4)) = v[i];
+                           (((c % 8) ^ (qr & 7)) << 4)) = qv[i];
             }
             umma::fence_smem_async();
             arrive(q_full + 8 * t);
@@ -678,7 +680,7 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                     }
                 }
                 tile_sync(t);
-                constexpr int CH = D / 8;               // pieces a row, either way
+                // CH pieces a row, either way
 #pragma unroll 4
                 for (int i = 0; i < CH / 2; i++) {
                     const int or_ = i * (2 * kRows / CH) + tid / CH, c = tid % CH,
@@ -705,6 +707,17 @@ attn_umma_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
         umma::fence_after();
         umma::tmem_free(tmem, 512);
     }
+}
+
+// See attn_rows_kernel.
+template <typename T, int D, bool PACKED>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_umma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ __align__(1024) uint8_t shared[];
+    pdl_trigger();
+    attn_wide_rows<T, D, PACKED>(a, kmap, vmap, shared);
+    pdl_wait();
 }
 
 // ------------------------------------------------------------ host side --
@@ -758,7 +771,7 @@ static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t p
 
 template <typename T, int D, bool PACKED>
 static int umma_launch(const AttnArgs &a, const CUtensorMap &km, const CUtensorMap &vm, int pairs,
-                       int parts, cudaStream_t st) {
+                       int parts, bool first, cudaStream_t st) {
     static bool attr_done = false;                      // per instantiation, per process
     if (!attr_done) {
         const cudaError_t e =
@@ -767,14 +780,17 @@ static int umma_launch(const AttnArgs &a, const CUtensorMap &km, const CUtensorM
         if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
         attr_done = true;
     }
-    attn_umma_kernel<T, D, PACKED>
-        <<<dim3((unsigned)pairs * parts, a.kv_heads, PACKED ? 1 : a.batch), kThreads,
-           Lay<D>::bytes, st>>>(a, km, vm);
-    WARP_CHECK_LAUNCH("attn_umma_kernel");
+    const cudaError_t e = attn_start(attn_umma_kernel<T, D, PACKED>,
+                                     dim3((unsigned)pairs * parts, a.kv_heads,
+                                          PACKED ? 1 : a.batch),
+                                     kThreads, Lay<D>::bytes, st, first, a, km, vm);
+    if (e != cudaSuccess) return cuda_fail(e, "attn_umma_kernel");
+    count_launch();
     return WARP_OK;
 }
 
-int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, cudaStream_t st) {
+int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,
+              cudaStream_t st) {
     CUtensorMap km, vm;
     int rc = page_map(&km, c, c->k, c->k_page, c->k_slot, c->k_head);
     if (!rc) rc = page_map(&vm, c, c->v, c->v_page, c->v_slot, c->v_head);
@@ -784,14 +800,14 @@ int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, cudaStream
     const int parts = packed ? a.prefix_parts : a.wide_parts;
     const bool h = c->type == WARP_T_F16, d64 = c->head_dim == 64;
     if (packed)
-        return h ? d64 ? umma_launch<__half, 64, true>(a, km, vm, pairs, parts, st)
-                       : umma_launch<__half, 128, true>(a, km, vm, pairs, parts, st)
-                 : d64 ? umma_launch<__nv_bfloat16, 64, true>(a, km, vm, pairs, parts, st)
-                       : umma_launch<__nv_bfloat16, 128, true>(a, km, vm, pairs, parts, st);
-    return h ? d64 ? umma_launch<__half, 64, false>(a, km, vm, pairs, parts, st)
-                   : umma_launch<__half, 128, false>(a, km, vm, pairs, parts, st)
-             : d64 ? umma_launch<__nv_bfloat16, 64, false>(a, km, vm, pairs, parts, st)
-                   : umma_launch<__nv_bfloat16, 128, false>(a, km, vm, pairs, parts, st);
+        return h ? d64 ? umma_launch<__half, 64, true>(a, km, vm, pairs, parts, first, st)
+                       : umma_launch<__half, 128, true>(a, km, vm, pairs, parts, first, st)
+                 : d64 ? umma_launch<__nv_bfloat16, 64, true>(a, km, vm, pairs, parts, first, st)
+                       : umma_launch<__nv_bfloat16, 128, true>(a, km, vm, pairs, parts, first, st);
+    return h ? d64 ? umma_launch<__half, 64, false>(a, km, vm, pairs, parts, first, st)
+                   : umma_launch<__half, 128, false>(a, km, vm, pairs, parts, first, st)
+             : d64 ? umma_launch<__nv_bfloat16, 64, false>(a, km, vm, pairs, parts, first, st)
+                   : umma_launch<__nv_bfloat16, 128, false>(a, km, vm, pairs, parts, first, st);
 }
 
 }  // namespace warp
