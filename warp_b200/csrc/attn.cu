@@ -392,48 +392,23 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a) {
     pdl_wait();
 }
 
-// Joins the parts of each row: a warp a (token, head).  Rows whose request has
-// one part were written by their CTA.  Each lane has D / 32 values of a row and,
-// for the weights, the maximum and sum of one part in 32.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
-    const int lane = threadIdx.x % 32;
-    const int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-    const int64_t rows = (int64_t)a.tokens * a.q_heads;
-    int parts = 0;
-    if (row < rows) {
-        const int t = (int)(row / a.q_heads);
-        // the token's request: the last one that starts at or before it
-        int b = -1;
-        for (int i0 = 0; i0 < a.batch; i0 += 32) {
-            const int i = i0 + lane;
-            const unsigned hit = __ballot_sync(~0u, i < a.batch && a.q_start[i] <= t);
-            if (hit) b = i0 + 31 - __clz(hit);
-            if (hit != ~0u) break;
-        }
-        if (b >= 0) {
-            const AttnReq rq = attn_req(a, b);
-            const bool wide = rq.n * a.group > a.rows_small;
-            const int tile = wide ? attn_wide(D) : kAttnTile;
-            const int own = (a.packed ? 0 : (a.prefix_len + tile - 1) / tile) +
-                            (rq.len + tile - 1) / tile;
-            parts = max(1, attn_parts(own, wide ? a.wide_each : a.split_tiles));
-            if ((!a.packed && parts == 1) || t >= rq.t0 + rq.n) parts = 0;
-            else parts += a.prefix_parts;
-        }
-    }
-    pdl_wait();
-    if (!parts) return;
+// Parts p0..p1-1 of one row, in order: the largest maximum M, the sum l and the
+// lane's D / 32 values of o, both measured from M.  Each lane keeps the weight of
+// one part in 32.
+template <int D>
+__device__ __forceinline__ void join_parts(const AttnArgs &a, int64_t row, int p0, int p1, float &M,
+                                           float &l, float (&acc)[D / 32]) {
     constexpr int V = D / 32;
-    float acc[V];
+    const int lane = threadIdx.x % 32;
+    const int64_t rows = (int64_t)a.tokens * a.q_heads, stride = rows * D;
+    const float *const src = a.part_o + row * D + lane * V;
+    M = -INFINITY;
+    l = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0.f;
-    float M = -INFINITY, l = 0.f;
-    const float *src = a.part_o + row * D + lane * V;
-    const int64_t stride = rows * D;
-    for (int p0 = 0; p0 < parts; p0 += 32) {
-        const int p = p0 + lane;
-        const float2 ml = p < parts ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f);
+    for (; p0 < p1; p0 += 32) {
+        const int p = p0 + lane, here = min(32, p1 - p0);
+        const float2 ml = p < p1 ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f);
         float m = fmaxf(M, ml.x);
 #pragma unroll
         for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
@@ -443,8 +418,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] *= keep;
         M = m;
-        const int here = min(32, parts - p0);
-        // in order, eight parts' loads in flight
+        // eight parts' loads in flight
         for (int k0 = 0; k0 < here; k0 += 8) {
             float v[8][V];
 #pragma unroll
@@ -464,13 +438,82 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     }
 #pragma unroll
     for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void join_store(const AttnArgs &a, int64_t row, float l,
+                                           const float (&acc)[D / 32]) {
+    constexpr int V = D / 32;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t o[V / 2];
 #pragma unroll
     for (int i = 0; i < V; i += 2) o[i / 2] = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
-    T *dst = (T *)a.out + row * D + lane * V;
+    T *const dst = (T *)a.out + row * D + threadIdx.x % 32 * V;
     if (V == 4) *(uint2 *)dst = *(uint2 *)o;
     else *(uint32_t *)dst = o[0];
+}
+
+// Joins the parts of each row.  Rows whose request has one part were written by
+// their CTA.  A block has a token, or a share of its heads, and a warp of it a
+// row; with SPREAD, where rows are few, a block has one row and its warps a share
+// of the parts each (37 parts of 64 rows: 8 us against 13).
+template <typename T, int D, bool SPREAD>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int V = D / 32;
+    __shared__ float2 ml_of[8];
+    __shared__ float o_of[8][D];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, t = blockIdx.x;
+    int parts = 0;
+    // the token's request: the last one that starts at or before it
+    int b = -1;
+    for (int i0 = 0; i0 < a.batch; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned hit = __ballot_sync(~0u, i < a.batch && a.q_start[i] <= t);
+        if (hit) b = i0 + 31 - __clz(hit);
+        if (hit != ~0u) break;
+    }
+    if (b >= 0) {
+        const AttnReq rq = attn_req(a, b);
+        const bool wide = rq.n * a.group > a.rows_small;
+        const int tile = wide ? attn_wide(D) : kAttnTile;
+        const int own = (a.packed ? 0 : (a.prefix_len + tile - 1) / tile) +
+                        (rq.len + tile - 1) / tile;
+        parts = max(1, attn_parts(own, wide ? a.wide_each : a.split_tiles));
+        if ((!a.packed && parts == 1) || t >= rq.t0 + rq.n) parts = 0;
+        else parts += a.prefix_parts;
+    }
+    pdl_wait();
+    if (!parts) return;
+    float M, l, acc[V];
+    if (!SPREAD) {
+        for (int head = blockIdx.y * 8 + warp; head < a.q_heads; head += gridDim.y * 8) {
+            const int64_t row = (int64_t)t * a.q_heads + head;
+            join_parts<D>(a, row, 0, parts, M, l, acc);
+            join_store<T, D>(a, row, l, acc);
+        }
+        return;
+    }
+    const int64_t row = (int64_t)t * a.q_heads + blockIdx.y;
+    const int each = (parts + 7) / 8;
+    join_parts<D>(a, row, min(parts, warp * each), min(parts, (warp + 1) * each), M, l, acc);
+    if (lane == 0) ml_of[warp] = make_float2(M, l);
+#pragma unroll
+    for (int i = 0; i < V; i++) o_of[warp][lane * V + i] = acc[i];
+    __syncthreads();
+    if (warp) return;
+    M = -INFINITY;
+    for (int w = 0; w < 8; w++) M = fmaxf(M, ml_of[w].x);
+    const float z = M == -INFINITY ? 0.f : M;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = 0.f;
+    for (int w = 0; w < 8; w++) {
+        const float f = ex2(ml_of[w].x - z);
+        l += f * ml_of[w].y;
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] += f * o_of[w][lane * V + i];
+    }
+    join_store<T, D>(a, row, l, acc);
 }
 
 // ------------------------------------------------------------ host side --
@@ -631,8 +674,15 @@ static int attn_launch(const AttnArgs &a, const AttnPlan &p, bool first, cudaStr
         first = false;
     }
     if (p.join) {
-        e = attn_start(attn_join_kernel<T, D>, dim3(cdiv((size_t)a.tokens * a.q_heads, 8)), 256, 0,
-                       st, first, a);
+        // a token's heads in one block, or shared out while the card has room, down
+        // to a block a row
+        const unsigned most = cdiv(a.q_heads, 8), room = cdiv(8 * 148, a.tokens);
+        const bool spread = p.prefix_parts + (p.parts > p.wide_parts ? p.parts : p.wide_parts) > 8 &&
+                            (int64_t)a.tokens * a.q_heads <= 8 * 148;
+        e = spread ? attn_start(attn_join_kernel<T, D, true>, dim3(a.tokens, a.q_heads), 256, 0, st,
+                                first, a)
+                   : attn_start(attn_join_kernel<T, D, false>,
+                                dim3(a.tokens, most < room ? most : room), 256, 0, st, first, a);
         if (e != cudaSuccess) return cuda_fail(e, "attn_join_kernel");
         count_launch();
     }

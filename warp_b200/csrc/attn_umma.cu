@@ -55,7 +55,7 @@ template <int D> struct Lay {
                          tmem = drain + 8, fail = tmem + 4, dirty = fail + 4;
     static constexpr int bytes = bars + dirty + 8;
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
-    static_assert(cols % 8 == 0 && kv_half % 1024 == 0 && keys % kBox == 0, "swizzle atoms of 8 rows, whole boxes");
+    static_assert(cols % 32 == 0 && kv_half % 1024 == 0 && keys % kBox == 0, "swizzle atoms of 8 rows, whole boxes");
     // tensor memory columns
     static constexpr int o(int t) { return t * D; }
     static constexpr int s(int t) { return 2 * D + t * keys; }
@@ -236,25 +236,29 @@ __device__ __forceinline__ void tmem_ld_wait() {
 __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, float *v) {
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float *v) {
     uint32_t *r = (uint32_t *)v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-                   "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr));
-}
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t *r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-          "r"(r[7])
+          "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+          "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
-                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-}
-
 // Of every 4 pairs of exponentials, those computed by ex2_poly: at D = 64, where
 // the products are half as long, one (4096 keys: 668 TFLOP/s against 636 for
 // none and 624 for two); at 128 none (1208 against 1136 and 1047).
@@ -266,13 +270,13 @@ template <typename T, int POLY, int N>
 __device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64_t mc2,
                                         uint64_t &sum, uint32_t st) {
 #pragma unroll
-    for (int x = 0; x < N; x += 8) {
-        uint32_t p[4];
+    for (int x = 0; x < N; x += 32) {
+        uint32_t p[16];
 #pragma unroll
-        for (int y = 0; y < 4; y++) {
+        for (int y = 0; y < 16; y++) {
             const uint64_t v = fma2(pair2(s[x + 2 * y], s[x + 2 * y + 1]), c2, mc2);
             float2 e;
-            if (y < POLY) {
+            if (y % 4 < POLY) {
                 e = ex2_poly(v);
             } else {
                 e = both(v);
@@ -282,7 +286,7 @@ __device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64
             sum = add2(sum, pair2(e.x, e.y));
             p[y] = pack2<T>(e.x, e.y);
         }
-        tmem_st4(st + x / 2, p);
+        tmem_st16(st + x / 2, p);
     }
     tmem_st_wait();
 }
@@ -338,7 +342,8 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     const uint32_t fail = bars + L::fail;
     volatile int *const failed = (volatile int *)(basep + L::bars + L::fail);
     volatile int *const dirty = (volatile int *)(basep + L::bars + L::dirty);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // the warp's number from one lane, so that it counts as uniform
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
 
     // The rows' warps: row tile, half of the keys, quarter of the rows, row.
     const int t = warp / 8, h = warp / 4 % 2, quad = warp % 4, r = threadIdx.x % kRows;
@@ -363,27 +368,34 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         }
     }
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; i++) {
-            umma::mbar_init(kv_full + 8 * i, 1);
-            umma::mbar_init(kv_empty + 8 * i, 1);
+    // The loading warp makes the barriers and goes on at once; the others meet
+    // behind it.
+    if (warp == 17) {
+        if (lane == 0) {
+            for (int i = 0; i < NS; i++) {
+                umma::mbar_init(kv_full + 8 * i, 1);
+                umma::mbar_init(kv_empty + 8 * i, 1);
+            }
+            for (int x = 0; x < 2; x++) {
+                umma::mbar_init(q_full + 8 * x, 2 * kRows);
+                umma::mbar_init(s_full + 8 * x, 1);
+                umma::mbar_init(p_full + 8 * x, 8);
+                umma::mbar_init(o_end + 8 * x, 1);
+            }
+            umma::mbar_init(drain, 1);
+            *failed = 0;
+            *dirty = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        for (int t = 0; t < 2; t++) {
-            umma::mbar_init(q_full + 8 * t, 2 * kRows);
-            umma::mbar_init(s_full + 8 * t, 1);
-            umma::mbar_init(p_full + 8 * t, 8);
-            umma::mbar_init(o_end + 8 * t, 1);
-        }
-        umma::mbar_init(drain, 1);
-        *failed = 0;
-        *dirty = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
+        asm volatile("bar.arrive 11, %0;" ::"n"(kThreads) : "memory");
+    } else {
+        if (warp == 16) umma::tmem_alloc(tmem_slot, 512);
+        umma::fence_before();
+        asm volatile("bar.sync 11, %0;" ::"n"(kThreads) : "memory");
+        umma::fence_after();
     }
-    if (warp == 16) umma::tmem_alloc(tmem_slot, 512);
-    umma::fence_before();
-    __syncthreads();
-    umma::fence_after();
-    const uint32_t tmem = *(volatile uint32_t *)(basep + L::bars + L::tmem);
+    const uint32_t tmem = warp == 17 ? 0 : *(volatile uint32_t *)(basep + L::bars + L::tmem);
 
     if (warp == 17) {
         // ---- keys and values: K of tile j in ring tile 2j, V in 2j + 1 --------------
@@ -560,7 +572,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             if (warp_live) {
                 float s[L::cols];
 #pragma unroll
-                for (int x = 0; x < L::cols; x += 8) tmem_ld8(st + x, s + x);
+                for (int x = 0; x < L::cols; x += 32) tmem_ld32(st + x, s + x);
                 tmem_ld_wait();
                 if (__builtin_expect(masked, 0)) {
                     lim -= h * L::cols;
@@ -592,8 +604,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                             uint32_t u[16];
 #pragma unroll
                             for (int y = 0; y < 16; y++) u[y] = __float_as_uint(o[y] * w);
-                            tmem_st8(ot + x, u);
-                            tmem_st8(ot + x + 8, u + 8);
+                            tmem_st16(ot + x, u);
                         }
                     }
                     l.x *= w;
