@@ -645,18 +645,10 @@ static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
 template <typename T, int D>
 static int attn_launch(const AttnArgs &a, const AttnPlan &p, bool first, cudaStream_t st) {
     using Lay = ADLay<D>;
-    static bool attr_done = false;                      // per instantiation, per process
-    if (!attr_done) {
-        cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<T, D, false>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Lay::bytes);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_rows_kernel<T, D, true>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::bytes);
-        if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
-        attr_done = true;
-    }
-    cudaError_t e;
+    static std::atomic<uint64_t> done[2];
+    cudaError_t e = attn_smem(attn_rows_kernel<T, D, false>, Lay::bytes, done[0]);
+    if (e == cudaSuccess) e = attn_smem(attn_rows_kernel<T, D, true>, Lay::bytes, done[1]);
+    if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
     if (p.packed && !p.packed_wide) {
         e = attn_start(attn_rows_kernel<T, D, true>,
                        dim3((unsigned)(up((int64_t)a.tokens * a.group, kADRows) * p.prefix_parts),

@@ -3,6 +3,8 @@
 #pragma once
 #include "common.cuh"
 
+#include <atomic>
+
 namespace warp {
 
 // Bits of the error word.
@@ -115,6 +117,19 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 // prefix for all rows of the batch.
 int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,
               cudaStream_t st);
+
+// Allows `kernel` its dynamic shared memory, once for each device; `done` is the
+// kernel's own, a bit a device.
+template <typename K>
+inline cudaError_t attn_smem(K *kernel, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (e != cudaSuccess || (done.load() & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
+}
 
 // Launches a call's first kernel behind everything before it on the stream, and
 // each further one so that it may start early.

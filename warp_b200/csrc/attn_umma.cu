@@ -783,18 +783,12 @@ static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t p
 template <typename T, int D, bool PACKED>
 static int umma_launch(const AttnArgs &a, const CUtensorMap &km, const CUtensorMap &vm, int pairs,
                        int parts, bool first, cudaStream_t st) {
-    static bool attr_done = false;                      // per instantiation, per process
-    if (!attr_done) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(attn_umma_kernel<T, D, PACKED>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::bytes);
-        if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
-        attr_done = true;
-    }
-    const cudaError_t e = attn_start(attn_umma_kernel<T, D, PACKED>,
-                                     dim3((unsigned)pairs * parts, a.kv_heads,
-                                          PACKED ? 1 : a.batch),
-                                     kThreads, Lay<D>::bytes, st, first, a, km, vm);
+    static std::atomic<uint64_t> done;
+    cudaError_t e = attn_smem(attn_umma_kernel<T, D, PACKED>, Lay<D>::bytes, done);
+    if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
+    e = attn_start(attn_umma_kernel<T, D, PACKED>,
+                   dim3((unsigned)pairs * parts, a.kv_heads, PACKED ? 1 : a.batch), kThreads,
+                   Lay<D>::bytes, st, first, a, km, vm);
     if (e != cudaSuccess) return cuda_fail(e, "attn_umma_kernel");
     count_launch();
     return WARP_OK;

@@ -15,13 +15,23 @@
 // row's units sit on neighbouring lanes, and the norm's sum is a butterfly over them.
 #include "attn.cuh"
 
+#include <atomic>
+
 namespace warp {
 
 __device__ unsigned g_attn_err;
 
+// The word's address is fixed once its device is in use: looked up once for each.
 int attn_err_word(unsigned **out) {
-    const cudaError_t e = cudaGetSymbolAddress((void **)out, g_attn_err);
-    return e == cudaSuccess ? WARP_OK : cuda_fail(e, "attention error word");
+    constexpr int kDevices = 64;
+    static std::atomic<unsigned *> known[kDevices];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev < kDevices && (*out = known[dev].load())) return WARP_OK;
+    if (e == cudaSuccess) e = cudaGetSymbolAddress((void **)out, g_attn_err);
+    if (e != cudaSuccess) return cuda_fail(e, "attention error word");
+    if (dev < kDevices) known[dev].store(*out);
+    return WARP_OK;
 }
 
 int kv_pages_check(const warp_kv_pages *c, const char *who) {

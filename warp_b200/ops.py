@@ -217,76 +217,66 @@ def rope_inv_freq(rot_dim, base=10000.0, scaling="none", factor=1.0, trained=Non
     return f.to(device), scale
 
 
-def _raise_bad(checks):
-    """The first check that fails, as a ValueError."""
-    for ok, text in checks:
-        if not ok:
-            raise ValueError(text)
-    raise ValueError("unusable arguments")
-
-
-def _rows_ok(x, T, D, dtype):
-    """[T][heads][D] on the device with contiguous heads."""
-    return x.dim() == 3 and x.is_cuda and x.dtype is dtype and x.shape[0] == T and \
-        x.shape[2] == D and (D < 2 or x.stride(2) == 1)
-
-
 def _vec_ok(x, n, dtype):
     return x.dtype is dtype and x.numel() == n and x.is_contiguous() and x.is_cuda
 
 
-def _strides(x):
-    """Token and head strides; that of an axis of one entry has no meaning."""
-    (a, b, _), (m, n, _) = x.stride(), x.shape
-    return a if m > 1 else 0, b if n > 1 else 0
+def _rows(x, name, T, D, dtype):
+    """(heads, token stride, head stride, address) of [T][heads][D] on the
+    device with contiguous heads; the stride of an axis of one entry is 0, as
+    it has no meaning."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != T or shape[2] != D or x.dtype is not dtype or \
+            not x.is_cuda or (strides[2] != 1 and D > 1):
+        _cuda(x)
+        raise ValueError(f"{name} must be [tokens][heads][head_dim] with contiguous heads, all "
+                         "of one dtype, token count and head_dim")
+    heads = shape[1]
+    return heads, strides[0] if T > 1 else 0, strides[1] if heads > 1 else 0, x.data_ptr()
 
 
 def _rope_pack(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale, q_out,
                k_out, out_dtype):
-    x = q if q is not None else k
+    x = k if q is None else q
     if x is None:
         raise ValueError("neither queries nor keys")
-    if x.dim() != 3 or x.dtype not in _TYPES:
-        raise ValueError("queries and keys must be [tokens][heads][head_dim], fp32, fp16 or bf16")
-    T, _, D = x.shape
     dt = x.dtype
-    if not ((q is None or _rows_ok(q, T, D, dt)) and (k is None or _rows_ok(k, T, D, dt)) and
-            (v is None or (_rows_ok(v, T, D, dt) and v.shape[1] == k.shape[1])) and
-            (inv_freq is None or (inv_freq.dtype is torch.float64 and inv_freq.is_cuda and
-                                  inv_freq.is_contiguous() and positions is not None and
-                                  _vec_ok(positions, T, torch.int32))) and
-            (q_norm is None or _vec_ok(q_norm, D, torch.float32)) and
-            (k_norm is None or _vec_ok(k_norm, D, torch.float32))):
-        _cuda(q, k, v, positions, inv_freq, q_norm, k_norm)
-        rows = "must be [tokens][heads][head_dim] with contiguous heads, of one dtype"
-        _raise_bad([
-            (q is None or _rows_ok(q, T, D, dt), "q " + rows),
-            (k is None or _rows_ok(k, T, D, dt), "k " + rows + ", as q's"),
-            (v is None or (_rows_ok(v, T, D, dt) and v.shape[1] == k.shape[1]),
-             "v " + rows + ", as k's"),
-            (inv_freq is None or (inv_freq.dtype is torch.float64 and inv_freq.is_contiguous()),
-             "inv_freq must be contiguous float64"),
-            (inv_freq is None or (positions is not None and _vec_ok(positions, T, torch.int32)),
-             "positions must be contiguous int32 [tokens]"),
-            (q_norm is None or _vec_ok(q_norm, D, torch.float32),
-             "q_norm must be contiguous float32 [head_dim]"),
-            (k_norm is None or _vec_ok(k_norm, D, torch.float32),
-             "k_norm must be contiguous float32 [head_dim]")])
-    qt = qh = kt = kh = vt = vh = nq = nk = qp = kp = vp = 0
+    if x.dim() != 3 or dt not in _TYPES:
+        raise ValueError("queries and keys must be [tokens][heads][head_dim], fp32, fp16 or bf16")
+    T, nk, D = x.shape
+    nq = qt = qh = qp = kt = kh = kp = vt = vh = vp = qn = kn = f = p = rot = 0
     if q is not None:
-        (qt, qh), nq, qp = _strides(q), q.shape[1], q.data_ptr()
+        nq, qt, qh, qp = _rows(q, "q", T, D, dt)
+        nk = 0
     if k is not None:
-        (kt, kh), nk, kp = _strides(k), k.shape[1], k.data_ptr()
+        nk, kt, kh, kp = _rows(k, "k", T, D, dt)
     if v is not None:
-        (vt, vh), vp = _strides(v), v.data_ptr()
-    rot = positions is not None and inv_freq is not None
+        nv, vt, vh, vp = _rows(v, "v", T, D, dt)
+        if nv != nk:
+            raise ValueError("v must have k's heads")
+    if inv_freq is not None:
+        rot = 2 * inv_freq.numel()
+        if not _vec_ok(inv_freq, rot // 2, torch.float64):
+            _cuda(inv_freq)
+            raise ValueError("inv_freq must be contiguous float64")
+        if positions is None or not _vec_ok(positions, T, torch.int32):
+            _cuda(positions)
+            raise ValueError("positions must be contiguous int32 [tokens]")
+        f, p = inv_freq.data_ptr(), positions.data_ptr()
+    if q_norm is not None:
+        if not _vec_ok(q_norm, D, torch.float32):
+            _cuda(q_norm)
+            raise ValueError("q_norm must be contiguous float32 [head_dim]")
+        qn = q_norm.data_ptr()
+    if k_norm is not None:
+        if not _vec_ok(k_norm, D, torch.float32):
+            _cuda(k_norm)
+            raise ValueError("k_norm must be contiguous float32 [head_dim]")
+        kn = k_norm.data_ptr()
     return ffi.ROPE_DESC.pack(
         T, nq, nk, D, _TYPES[dt], _TYPES.get(out_dtype, -1), qp, kp, vp, qt, qh, kt, kh, vt, vh,
-        q_out.data_ptr() if q_out is not None else 0, k_out.data_ptr() if k_out is not None else 0,
-        q_norm.data_ptr() if q_norm is not None else 0,
-        k_norm.data_ptr() if k_norm is not None else 0, eps, inv_freq.data_ptr() if rot else 0,
-        2 * inv_freq.numel() if rot else 0, interleaved, rot_scale,
-        positions.data_ptr() if rot else 0)
+        0 if q_out is None else q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
+        qn, kn, eps, f, rot, interleaved, rot_scale, p)
 
 
 def _dense(x, dtype):
@@ -356,27 +346,30 @@ def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
     """(positions int32 [T], slots int64 [T]) of a step's tokens for kv_append
     (warp_kv_slots): q_start int32 [B+1], kv_len int32 [B] own keys with the
     new ones counted, pages int32 [B][n]; base: the shared prefix's length."""
-    row, wide = _batch(q_start, kv_len, pages)
+    B, row, wide = _batch(q_start, kv_len, pages)
     positions = torch.empty(tokens, dtype=torch.int32, device=q_start.device)
     slots = torch.empty(tokens, dtype=torch.int64, device=q_start.device)
     ffi.check(ffi.load().warp_kv_slots(
-        q_start.data_ptr(), kv_len.data_ptr(), kv_len.numel(), tokens, pages.data_ptr(), row, wide,
+        q_start.data_ptr(), kv_len.data_ptr(), B, tokens, pages.data_ptr(), row, wide,
         page_size, base, positions.data_ptr(), slots.data_ptr(), _stream()))
     return positions, slots
 
 
 def _batch(q_start, kv_len, pages):
-    """Checks a batch's device tensors; the page table's row stride and width."""
+    """(requests, row stride and width of the page table)."""
     B = kv_len.numel()
-    if not (_vec_ok(kv_len, B, torch.int32) and _vec_ok(q_start, B + 1, torch.int32) and
-            pages.dim() == 2 and pages.is_cuda and pages.dtype is torch.int32 and
-            pages.shape[0] == B and (pages.shape[1] < 2 or pages.stride(1) == 1)):
-        _cuda(q_start, kv_len, pages)
-        _raise_bad([
-            (_vec_ok(kv_len, B, torch.int32), "kv_len must be contiguous int32 [batch]"),
-            (_vec_ok(q_start, B + 1, torch.int32), "q_start must be contiguous int32 [batch + 1]"),
-            (False, "pages must be int32 [batch][pages a request], rows contiguous")])
-    return (pages.stride(0) if B > 1 else 0), pages.shape[1]
+    if not _vec_ok(kv_len, B, torch.int32):
+        _cuda(kv_len)
+        raise ValueError("kv_len must be contiguous int32 [batch]")
+    if not _vec_ok(q_start, B + 1, torch.int32):
+        _cuda(q_start)
+        raise ValueError("q_start must be contiguous int32 [batch + 1]")
+    shape, strides = pages.shape, pages.stride()
+    if len(shape) != 2 or shape[0] != B or pages.dtype is not torch.int32 or \
+            not pages.is_cuda or (strides[1] != 1 and shape[1] > 1):
+        _cuda(pages)
+        raise ValueError("pages must be int32 [batch][pages a request], rows contiguous")
+    return B, strides[0] if B > 1 else 0, shape[1]
 
 
 def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale=None,
@@ -394,15 +387,15 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
     token of no request is not written.  scale: 1/sqrt(D) by default.  Returns
     [T][Hq][D] in q's dtype."""
     c = _pages_pack(k_pages, v_pages)
-    row, wide = _batch(q_start, kv_len, pages)
-    if q.dim() != 3 or not _rows_ok(q, q.shape[0], q.shape[2], q.dtype) or q.dtype not in _TYPES:
-        _cuda(q)
-        raise ValueError("q must be [tokens][heads][head_dim], fp16 or bf16, with contiguous heads")
-    T, Hq, D = q.shape
-    qt, qh = _strides(q)
+    B, row, wide = _batch(q_start, kv_len, pages)
+    dt = q.dtype
+    if q.dim() != 3 or dt not in _TYPES:
+        raise ValueError("q must be [tokens][heads][head_dim], fp16 or bf16")
+    T, _, D = q.shape
+    Hq, qt, qh, qp = _rows(q, "q", T, D, dt)
     if out is None:
-        out = _dense(q, q.dtype)
-    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or \
+        out = _dense(q, dt)
+    elif out.shape != q.shape or out.dtype is not dt or not out.is_contiguous() or \
             not out.is_cuda:
         raise ValueError("out must be contiguous, of q's shape and dtype")
     pp = 0
@@ -413,7 +406,7 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
             raise ValueError("prefix_pages must be contiguous int32 [n] on the device")
         pp = prefix_pages.data_ptr()
     d = ffi.ATTN_DESC.pack(
-        kv_len.numel(), T, Hq, k_pages.shape[2], D, _TYPES[q.dtype], q.data_ptr(), qt, qh,
+        B, T, Hq, k_pages.shape[2], D, _TYPES[dt], qp, qt, qh,
         out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), row, wide, max_q,
         max_kv, causal, (D or 1) ** -0.5 if scale is None else scale, pp, prefix_len)
     lib = ffi.load()
