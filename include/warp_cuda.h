@@ -303,7 +303,8 @@ WARP_API int warp_qk_norm_rope(const warp_rope_desc *d, void *stream);
  * token t's go to slot slots[t] (int64, device; a negative one stores
  * nothing).  out_type is the pages' type; k_out is not used; q may be NULL
  * with q_heads 0.  A slot past the pages is not written and is reported by
- * warp_attn_status.  Two tokens with the same slot: one of them is stored. */
+ * warp_attn_status.  Slots of one call are distinct (what two tokens leave in
+ * one slot is not defined). */
 WARP_API int warp_kv_append(const warp_rope_desc *d, const warp_kv_pages *c,
                             const int64_t *slots, void *stream);
 
@@ -338,8 +339,9 @@ WARP_API int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int ba
  * queries and own keys; what exceeds them, or a page number outside the pages,
  * is left out and reported by warp_attn_status.
  * scratch: warp_attn_scratch(d, c) bytes of device memory, 256-byte aligned,
- * free again when the stream has passed the call.  No host synchronisation;
- * capturable. */
+ * free again when the stream has passed the call.  A token of no request is not
+ * written.  No host synchronisation; capturable, once a call of the same type,
+ * head_dim and kind of batch has been made outside (it sets the kernels up). */
 typedef struct {
     int batch, tokens, q_heads, kv_heads, head_dim, type;
     const void *q;

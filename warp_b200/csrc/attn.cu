@@ -383,11 +383,13 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
 // The kernels of one call are launched so that each may start while the one
 // before it runs (they read the same inputs and write different parts), and
 // each waits for that one at its end, so that the last one's end is the end of all.
+// That one lets nothing start early: what follows the call may count on its
+// results as soon as it runs.
 template <typename T, int D, bool PACKED>
 __global__ void __launch_bounds__(kADWarps * 32, 2)
 attn_rows_kernel(const __grid_constant__ AttnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
-    pdl_trigger();
+    if (a.more) pdl_trigger();
     attn_rows<T, D, PACKED>(a, smem);
     pdl_wait();
 }
@@ -643,13 +645,14 @@ static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
 }
 
 template <typename T, int D>
-static int attn_launch(const AttnArgs &a, const AttnPlan &p, bool first, cudaStream_t st) {
+static int attn_launch(AttnArgs a, const AttnPlan &p, bool first, cudaStream_t st) {
     using Lay = ADLay<D>;
     static std::atomic<uint64_t> done[2];
     cudaError_t e = attn_smem(attn_rows_kernel<T, D, false>, Lay::bytes, done[0]);
     if (e == cudaSuccess) e = attn_smem(attn_rows_kernel<T, D, true>, Lay::bytes, done[1]);
     if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
     if (p.packed && !p.packed_wide) {
+        a.more = 1;
         e = attn_start(attn_rows_kernel<T, D, true>,
                        dim3((unsigned)(up((int64_t)a.tokens * a.group, kADRows) * p.prefix_parts),
                             a.kv_heads, 1), kADWarps * 32, Lay::bytes, st, first, a);
@@ -658,6 +661,7 @@ static int attn_launch(const AttnArgs &a, const AttnPlan &p, bool first, cudaStr
         first = false;
     }
     if (p.small_tiles) {
+        a.more = p.join;
         e = attn_start(attn_rows_kernel<T, D, false>,
                        dim3(p.small_tiles * p.parts, a.kv_heads, a.batch), kADWarps * 32,
                        Lay::bytes, st, first, a);
@@ -729,8 +733,14 @@ extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     bool first = true;
-    if (p.packed_wide) rc = warp::attn_umma(a, c, true, first, st), first = false;
-    if (!rc && p.wide_parts) rc = warp::attn_umma(a, c, false, first, st), first = false;
+    if (p.packed_wide) {
+        a.more = 1;
+        rc = warp::attn_umma(a, c, true, first, st), first = false;
+    }
+    if (!rc && p.wide_parts) {
+        a.more = p.small_tiles || p.join;
+        rc = warp::attn_umma(a, c, false, first, st), first = false;
+    }
     if (rc) return rc;
     if (d->type == WARP_T_F16)
         return d->head_dim == 64 ? warp::attn_launch<__half, 64>(a, p, first, st)

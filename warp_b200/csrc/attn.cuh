@@ -52,6 +52,7 @@ struct AttnArgs {
     float *part_o;
     float2 *part_ml;
     int packed, prefix_parts;
+    int more;                               // another kernel of the call follows
     // Requests with more rows a kv head than rows_small go to attn_umma_kernel,
     // which counts keys in tiles of attn_wide; the others to attn_rows_kernel.
     int rows_small;

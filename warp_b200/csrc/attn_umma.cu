@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attn_umma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ __align__(1024) uint8_t shared[];
-    pdl_trigger();
+    if (a.more) pdl_trigger();
     attn_wide_rows<T, D, PACKED>(a, kmap, vmap, shared);
     pdl_wait();
 }

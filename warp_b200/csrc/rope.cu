@@ -76,7 +76,7 @@ template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N :
 };
 
 constexpr int kRopeWarps = 4;
-constexpr int kRopeCtas = 8;                // an SM: occupancy is what hides the latency here
+constexpr int kRopeCtas = 7;                // an SM: occupancy is what hides the latency here
 constexpr int kRopeMaxPairs = 128;          // head_dim up to 256
 
 template <int VEC> __device__ __forceinline__ void rope_f32(float (&x)[VEC], const float *p) {
