@@ -51,7 +51,7 @@ template <int D> struct Lay {
     // offsets in the barrier section
     static constexpr int kv_full = 0, kv_empty = kv_full + stages * 8,
                          q_full = kv_empty + stages * 8, s_full = q_full + 16,
-                         p_full = s_full + 16, o_end = p_full + 16, drain = o_end + 16,
+                         p_full = s_full + 16, o_end = p_full + 32, drain = o_end + 16,
                          tmem = drain + 8, fail = tmem + 4, dirty = fail + 4;
     static constexpr int bytes = bars + dirty + 8;
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
@@ -194,6 +194,17 @@ __device__ __forceinline__ int small_div(int x, float inv_g) {
 __device__ __forceinline__ void pair_sync(int t, int quad) {
     asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory");
 }
+// The same barrier of the two warps, and whether any of their threads says so.
+__device__ __forceinline__ bool pair_any(int t, int quad, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "bar.red.or.pred q, %1, 64, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(r) : "r"(1 + t * 4 + quad), "r"((uint32_t)x) : "memory");
+    return r;
+}
 __device__ __forceinline__ void tile_sync(int t) {
     asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory");
 }
@@ -264,11 +275,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
 // none and 624 for two); at 128 none (1208 against 1136 and 1047).
 constexpr int poly_pairs(int D) { return D == 64 ? 1 : 0; }
 
+// A warp's weights, in tensor memory by now, to the issuing warp.
+__device__ __forceinline__ void hand_over(uint32_t ready) {
+    umma::fence_before();
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) arrive(ready);
+}
+
 // p = 2^(c s - c m) of a thread's scores of one step into their place,
-// and their sum.
+// handed over by halves, and their sum.
 template <typename T, int POLY, int N>
 __device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64_t mc2,
-                                        uint64_t &sum, uint32_t st) {
+                                        uint64_t &sum, uint32_t st, uint32_t ready) {
 #pragma unroll
     for (int x = 0; x < N; x += 32) {
         uint32_t p[16];
@@ -287,8 +305,9 @@ __device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64
             p[y] = pack2<T>(e.x, e.y);
         }
         tmem_st16(st + x / 2, p);
+        tmem_st_wait();
+        hand_over(ready + (x ? 8 : 0));
     }
-    tmem_st_wait();
 }
 
 }  // namespace
@@ -379,7 +398,8 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             for (int x = 0; x < 2; x++) {
                 umma::mbar_init(q_full + 8 * x, 2 * kRows);
                 umma::mbar_init(s_full + 8 * x, 1);
-                umma::mbar_init(p_full + 8 * x, 8);
+                umma::mbar_init(p_full + 16 * x, 8);
+                umma::mbar_init(p_full + 16 * x + 8, 8);
                 umma::mbar_init(o_end + 8 * x, 1);
             }
             umma::mbar_init(drain, 1);
@@ -453,14 +473,17 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                            x > 0);
                 commit(leader, s_full + 8 * t);
             };
-            auto pv = [&](int t, int st, bool acc) {
+            // The weights of each half of the keys lie where its scores did, and come
+            // in two parts: part w is keys w * cols/2 on of both halves.
+            auto pv = [&](int t, int st, int w, bool acc) {
                 const uint64_t v = v_desc + st * (L::kv_tile >> 4);
+                constexpr int H = L::cols / 16, Q = H / 2;
 #pragma unroll
-                for (int x = 0; x < KEYS / 16; x++)
-                    // the weights of each half of the keys lie where its scores did
-                    mma_ts(leader, tmem + L::o(t),
-                           tmem + L::s(t) + x / (L::cols / 16) * L::cols + x % (L::cols / 16) * 8,
-                           v + x * (2048 >> 4), idesc<T>(D, true), acc || x > 0);
+                for (int i = 0; i < H; i++) {
+                    const int x = i / Q * H + w * Q + i % Q;
+                    mma_ts(leader, tmem + L::o(t), tmem + L::s(t) + x / H * L::cols + x % H * 8,
+                           v + x * (2048 >> 4), idesc<T>(D, true), acc || i > 0);
+                }
             };
             const int cnt1 = tiles_rows == 2 ? cnt : 0;
             wait(q_full, 0, fail);
@@ -479,9 +502,12 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 for (int t = 0; t < 2; t++) {
                     const int mine = t == 0 ? cnt0 : cnt1;
                     if (j >= mine) continue;
-                    wait(p_full + 8 * t, j & 1, fail);
+                    wait(p_full + 16 * t, j & 1, fail);
                     umma::fence_after();
-                    pv(t, sv, j > 0);
+                    pv(t, sv, 0, j > 0);
+                    wait(p_full + 16 * t + 8, j & 1, fail);
+                    umma::fence_after();
+                    pv(t, sv, 1, true);
                     // in order behind it: the next scores take the weights' place
                     if (j + 1 < mine) qk(t, sk);
                     else commit(leader, o_end + 8 * t);
@@ -587,13 +613,12 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 mx[0] = max3(mx[0], s[L::cols - 4], s[L::cols - 3]);
                 mx[1] = max3(mx[1], s[L::cols - 2], s[L::cols - 1]);
                 float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                // (the scores are there, so the product of the step before is done, and
-                // with it the other half's reading of that step's maximum)
-                swap[h * kRows + r] = top;
-                pair_sync(t, quad);
-                top = max3(top, swap[(h ^ 1) * kRows + r], top);
-                const bool grow = !((top - m) * c <= 8.f);
-                if (__builtin_expect(__any_sync(~0u, grow), 0)) {
+                // the halves' maxima are exchanged only if one outgrows the old one
+                if (__builtin_expect(pair_any(t, quad, !((top - m) * c <= 8.f)), 0)) {
+                    swap[h * kRows + r] = top;
+                    pair_sync(t, quad);
+                    top = max3(top, swap[(h ^ 1) * kRows + r], top);
+                    const bool grow = !((top - m) * c <= 8.f);
                     const float to = grow ? top : m;
                     const float w = !grow || to == -INFINITY ? 1.f : ex2(m * c - to * c);
                     if (j > 0) {
@@ -615,13 +640,13 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 const float mc = m == -INFINITY ? 0.f : m < INFINITY ? m * c : NAN;
                 const uint64_t c2 = pair2(c, c), mc2 = pair2(-mc, -mc);
                 uint64_t l2 = pair2(l.x, l.y);
-                if (__builtin_expect(masked, 0)) weights<T, 0>(s, c2, mc2, l2, st);
-                else weights<T, poly_pairs(D)>(s, c2, mc2, l2, st);
+                if (__builtin_expect(masked, 0)) weights<T, 0>(s, c2, mc2, l2, st, p_full + 16 * t);
+                else weights<T, poly_pairs(D)>(s, c2, mc2, l2, st, p_full + 16 * t);
                 l = both(l2);
+            } else {
+                hand_over(p_full + 16 * t);
+                hand_over(p_full + 16 * t + 8);
             }
-            umma::fence_before();
-            __syncwarp();
-            if (lane == 0) arrive(p_full + 8 * t);
         }
         if (mine > 0) wait(o_end + 8 * t, 0, fail);
         umma::fence_after();
