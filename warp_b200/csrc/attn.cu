@@ -382,7 +382,8 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
 
 // The kernels of one call are launched so that each may start while the one
 // before it runs (they read the same inputs and write different parts), and
-// each waits for that one at its end, so that the last one's end is the end of all.
+// the last block of each waits for that one before it ends, so that the last
+// one's end is the end of all.
 // That one lets nothing start early: what follows the call may count on its
 // results as soon as it runs.
 template <typename T, int D, bool PACKED>
@@ -391,7 +392,7 @@ attn_rows_kernel(const __grid_constant__ AttnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     if (a.more) pdl_trigger();
     attn_rows<T, D, PACKED>(a, smem);
-    pdl_wait();
+    attn_wait_last();
 }
 
 // Parts p0..p1-1 of one row, in order: the largest maximum M, the sum l and the
@@ -568,9 +569,30 @@ static int split_rows(int64_t tiles, int64_t ctas, double rows, int D) {
     return pick_split(tiles, ctas, 2 * 148, tile_us, 3.0, 4, rows, D);
 }
 
-// attn_umma_kernel: one CTA an SM.
+// attn_umma_kernel: one CTA an SM; 128 keys for 256 rows, and a CTA around them.
+static double wide_tile_us(int D) { return D == 128 ? 1.7 : 1.4; }
+constexpr double kWideCtaUs = 7.0;
+
 static int split_wide(int64_t tiles, int64_t ctas, double rows, int D) {
-    return pick_split(tiles, ctas, 148, D == 128 ? 1.75 : 1.6, 6.0, 2, rows, D);
+    return pick_split(tiles, ctas, 148, wide_tile_us(D), kWideCtaUs, 2, rows, D);
+}
+
+// The same for a prefix, whose CTAs share the card with the requests' own keys
+// (`bytes` of them, at the memory's rate if they had it alone): no SM idles, so
+// what counts is the work in all, or one CTA's time where that is longer. More
+// parts shorten the one and add to the other (64 streams behind 16001 keys: 66 us
+// with 5 parts, 79 with 9, 107 with 32).
+static int split_prefix(int64_t tiles, int64_t ctas, double bytes, double rows, int D) {
+    const double tile_us = wide_tile_us(D), own = 148 * (bytes / 6.2e6 + 3.0);
+    int64_t best = tiles;
+    double least_us = 1e30;
+    for (int64_t parts = 1; parts <= 128 && (parts == 1 || up(tiles, parts) >= 2); parts++) {
+        const int64_t each = up(tiles, parts), n = up(tiles, each);
+        const double one = each * tile_us + kWideCtaUs + 2.0, all = (ctas * n * one + own) / 148;
+        const double us = (one > all ? one : all) + rows * n * D * 8 / 4e6;
+        if (us < least_us * 0.98) best = each, least_us = us;
+    }
+    return (int)best;
 }
 
 static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
@@ -607,7 +629,9 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
         p.packed_wide = all > kADRows;
         const int64_t tiles = up(d->prefix_len, p.packed_wide ? keys : kAttnTile);
         p.prefix_each =
-            p.packed_wide ? split_wide(tiles, up(all, 256) * d->kv_heads, out, d->head_dim)
+            p.packed_wide ? split_prefix(tiles, up(all, 256) * d->kv_heads,
+                                         0.6 * d->batch * p.max_kv * d->kv_heads * d->head_dim * 4,
+                                         out, d->head_dim)
                           : split_rows(tiles, up(all, kADRows) * d->kv_heads, out, d->head_dim);
         p.prefix_parts = (int)up(tiles, p.prefix_each);
     }

@@ -119,6 +119,13 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,
               cudaStream_t st);
 
+// The wait for the kernel before this one, by one block, the last to start: a
+// grid is not complete before it, and the others leave their places at once.
+__device__ __forceinline__ void attn_wait_last() {
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+        pdl_wait();
+}
+
 // Allows `kernel` its dynamic shared memory, once for each device; `done` is the
 // kernel's own, a bit a device.
 template <typename K>

@@ -753,7 +753,7 @@ attn_umma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     extern __shared__ __align__(1024) uint8_t shared[];
     if (a.more) pdl_trigger();
     attn_wide_rows<T, D, PACKED>(a, kmap, vmap, shared);
-    pdl_wait();
+    attn_wait_last();
 }
 
 // ------------------------------------------------------------ host side --
