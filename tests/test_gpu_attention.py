@@ -558,3 +558,24 @@ def test_wrapper_refusals(cuda):
         ops.kv_append(None, q[:, :2], q[:, :2], k, v, pos, pos, f)
     with pytest.raises(ffi.WarpError, match="heads"):
         ops.kv_append(None, q, q, k, v, pos.long(), pos, f)
+
+
+def test_scores_of_minus_infinity(cuda):
+    """Keys that score -inf weigh nothing, and a row with no other score gives zeros."""
+    for n, L in ((1, 300), (150, 300)):
+        c = Case([n], [L], 4, 2, 64, 16, torch.float16, seed=27)
+        c.q[..., 0] = 1.0
+        want_all = c.k.clone()
+        j = torch.arange(L)
+        at = c.pages[0][j // 16].long(), j % 16
+        c.k[at[0], at[1], 0, 0] = -math.inf         # kv head 0: every key
+        c.k[at[0][1::2], at[1][1::2], 1, 0] = -math.inf     # kv head 1: every other
+        got = c.run(causal=False)
+        assert not got[:, :2].any()
+        c.k = want_all
+        keep = c.k[at][0::2], c.v[at][0::2]
+        for h in (2, 3):
+            p = (c.q[:, h].double() @ keep[0][:, 1].double().T / 8).softmax(-1)
+            o, mag = p @ keep[1][:, 1].double(), p @ keep[1][:, 1].double().abs()
+            tol = 2 * (2.0 ** -11 * o.abs() + (2.0 ** -11 + 2.0 ** -14) * mag)
+            assert ((got[:, h].double() - o).abs() <= tol).all()

@@ -7,8 +7,9 @@
 //     S = Q K^T      (both from shared memory, 128B-swizzled, K-major)
 //     O += P V       (P from tensor memory, V as it lies: N-major)
 // and between them, two threads a row: the running maximum m, p = 2^(c s - c m)
-// and the sum l. P takes the place of S. While one row tile's exponentials are
-// computed the other's products run.
+// and the sum l. P takes the place of S, half of each thread's share at a time,
+// so that O += P V starts on the first while the second is computed. While one
+// row tile's exponentials are computed the other's products run.
 //
 // The maximum that p is measured from moves only when a row outgrows it by
 // 2^8, so the accumulated O is rescaled rarely; p then stays below 2^8, which
@@ -17,14 +18,18 @@
 //
 // What bounds it: per pair of 128 x 128 tiles the products take
 // 2 * 2 * 128 * 128 * D / 4096 FMA a clock = 2048 cycles at D = 128 (half at
-// 64), and so do 2 * 128 * 128 exponentials at 16 a clock. A share of the
-// exponentials is computed on the FMA pipe (ex2_poly), and sums and scalings go
-// two at a time (f32x2).
+// 64), and so do 2 * 128 * 128 exponentials at 16 a clock; a row tile's step is
+// its softmax and then its products, and two row tiles in turn do not quite hide
+// the one behind the other. Measured with 256 rows on each of 148 SMs and 4096
+// keys in pages of 128: 63.7 us, 1247 TFLOP/s at D = 128, 53.6 us, 742 TFLOP/s
+// at 64 (pages of 16: 1208 and 743). Tried and slower: two places of S for 64
+// keys each (966), P apart from S with 80 keys a step (904 to 1031), one warp a
+// 32 rows (843).
 //
 // Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each with
-// half the keys of a step (one warp a 32 rows leaves two to a scheduler, which
-// do not hide each other's latency); 16 issues the products, 17 loads keys and
-// values by TMA, boxes of 16 keys, into a ring of tiles.
+// half the keys of a step (with one, a scheduler has two warps, which do not hide
+// each other's latency); 16 issues the products, 17 loads keys and values by TMA,
+// boxes of 16 keys, into a ring of tiles.
 #include "attn.cuh"
 #include "umma.cuh"
 
@@ -55,7 +60,8 @@ template <int D> struct Lay {
                          tmem = drain + 8, fail = tmem + 4, dirty = fail + 4;
     static constexpr int bytes = bars + dirty + 8;
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
-    static_assert(cols % 32 == 0 && kv_half % 1024 == 0 && keys % kBox == 0, "swizzle atoms of 8 rows, whole boxes");
+    static_assert(cols % 32 == 0 && kv_half % 1024 == 0 && keys % kBox == 0,
+                  "swizzle atoms of 8 rows, whole boxes");
     // tensor memory columns
     static constexpr int o(int t) { return t * D; }
     static constexpr int s(int t) { return 2 * D + t * keys; }
@@ -134,7 +140,8 @@ __device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes) {
                  ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Two fp32 at a time.
+// Two fp32 at a time: half the instructions, though each takes the pipe as long
+// as two.
 __device__ __forceinline__ uint64_t pair2(float x, float y) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
@@ -166,7 +173,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // taking off 1.5 * 2^23, whose low bits then hold n) and 2^f on [-1/2, 1/2] by
 // the cubic of least relative error, 2^-13.7: an eighth of the last place of
 // fp16, which the result is rounded to at the least.  Below -125 it stays at
-// 2^-125, so it is not for masked scores, which have to give 0.
+// 2^-125, so it is not for steps with masked scores, which have to give 0.
 __device__ __forceinline__ float2 ex2_poly(uint64_t x2) {
     float2 x = both(x2);
     x.x = fmaxf(x.x, -125.f);
@@ -241,6 +248,7 @@ __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, uint32_t fai
 __device__ __forceinline__ void wait_over(uint32_t bar, uint32_t parity) {
     umma::mbar_wait(bar, parity, kPolls);
 }
+
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -270,9 +278,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
           "r"(r[14]), "r"(r[15])
         : "memory");
 }
+
 // Of every 4 pairs of exponentials, those computed by ex2_poly: at D = 64, where
-// the products are half as long, one (4096 keys: 668 TFLOP/s against 636 for
-// none and 624 for two); at 128 none (1208 against 1136 and 1047).
+// the products are half as long, one (4096 keys in pages of 128: 742 TFLOP/s
+// against 667 for none); at 128 none (1247 against 1172 for one).
 constexpr int poly_pairs(int D) { return D == 64 ? 1 : 0; }
 
 // A warp's weights, in tensor memory by now, to the issuing warp.
@@ -664,7 +673,8 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             tile_sync(t);                   // the last maxima are read
             swap[h * kRows + r] = l.x + l.y;
             tile_sync(t);
-            const float sum = swap[r] + swap[kRows + r];
+            // (a row without a finite score has what ex2_poly makes of -inf: nothing)
+            const float sum = m == -INFINITY ? 0.f : swap[r] + swap[kRows + r];
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             // columns at a time, half of them by each of a row's threads: all of 16
             // bits, or half of 32
