@@ -271,7 +271,9 @@ static int rope_vec(RopeArgs &a, cudaStream_t st) {
     auto fits = [&](int vec) {
         const uintptr_t ib = vec * sizeof(TI) < 16 ? vec * sizeof(TI) : 16;
         const uintptr_t ob = vec * sizeof(TO) < 16 ? vec * sizeof(TO) : 16;
-        if (a.rot % (2 * vec) || a.D % (2 * vec)) return false;
+        // half layout: whole vectors on both sides of a row's three boundaries;
+        // interleaved: a vector is turned whole or not at all
+        if (a.rot % (a.interleaved ? vec : 2 * vec) || a.D % (2 * vec)) return false;
         uintptr_t in = 0, out = (uintptr_t)a.q_out | (uintptr_t)a.k_out;
         const uintptr_t wb = vec * sizeof(float) < 16 ? vec * sizeof(float) : 16;
         if (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) % wb) return false;
@@ -283,13 +285,23 @@ static int rope_vec(RopeArgs &a, cudaStream_t st) {
         if (a.slots) add(a.v, a.v_token, a.v_head);
         return in % ib == 0 && out % ob == 0;
     };
-    const int units = a.D / 16;
+    // and the fewest lanes that hold a row (4922 tokens, 20 heads of 64, 52 of it
+    // turned in halves: 28 us with 32 lanes and vectors of two, 10 with 16)
     if (fits(8)) {
-        if (units <= 4) return rope_launch<TI, TO, 8, 4, 1>(a, st);
-        if (units <= 8) return rope_launch<TI, TO, 8, 8, 1>(a, st);
+        if (a.D <= 64) return rope_launch<TI, TO, 8, 4, 1>(a, st);
+        if (a.D <= 128) return rope_launch<TI, TO, 8, 8, 1>(a, st);
         return rope_launch<TI, TO, 8, 16, 1>(a, st);
     }
-    if (fits(2)) return rope_launch<TI, TO, 2, 32, 2>(a, st);
+    if (fits(4)) {
+        if (a.D <= 64) return rope_launch<TI, TO, 4, 8, 1>(a, st);
+        if (a.D <= 128) return rope_launch<TI, TO, 4, 16, 1>(a, st);
+        return rope_launch<TI, TO, 4, 32, 1>(a, st);
+    }
+    if (fits(2)) {
+        if (a.D <= 64) return rope_launch<TI, TO, 2, 16, 1>(a, st);
+        if (a.D <= 128) return rope_launch<TI, TO, 2, 32, 1>(a, st);
+        return rope_launch<TI, TO, 2, 32, 2>(a, st);
+    }
     return rope_launch<TI, TO, 1, 32, 4>(a, st);
 }
 
