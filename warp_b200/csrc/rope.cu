@@ -16,6 +16,7 @@
 #include "attn.cuh"
 
 #include <atomic>
+#include <climits>
 
 namespace warp {
 
@@ -117,10 +118,6 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
             at1[n] = turned ? half + u * VEC : at0[n] + (units - rot_units) * VEC;
         }
     }
-    const TI *const q = (const TI *)a.q + t * a.q_token;
-    const TI *const k = (const TI *)a.k + t * a.k_token - k0 * a.k_head;
-    const TI *const v = (const TI *)a.v + t * a.v_token - v0 * a.v_head;
-
     // The angle in turns, reduced in 64 bits: what is left is a fraction of a
     // turn that fp32 holds to 2^-25, whatever the position.
     float *const cosines = turns_of[warp], *const sines = cosines + kRopeMaxPairs;
@@ -145,23 +142,51 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
         }
         page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
     }
-    TO *const qd = (TO *)a.q_out + (int64_t)t * a.q_heads * a.D;
-    TO *kd = (TO *)a.k_out + ((int64_t)t * a.kv_heads - k0) * a.D, *vd = nullptr;
-    int64_t kd_head = a.D;
-    if (a.slots) {
-        kd = (TO *)a.kp + page * a.k_page + off * a.k_slot - k0 * a.k_ph;
-        vd = (TO *)a.vp + page * a.v_page + off * a.v_slot - v0 * a.v_ph;
-        kd_head = a.k_ph;
-    }
     const float inv_d = 1.0f / (float)a.D;
     const bool norms = a.q_norm || a.k_norm;
+
+    // Where the lane's row is read and written, and how far on its next one is, for
+    // as long as it stays among q's, k's or v's rows (up to row `until`).
+    const TI *src = nullptr;
+    TO *dst = nullptr;
+    const float *w = nullptr;
+    int64_t src_step = 0, dst_step = 0;
+    int until = 0;
+    bool turned = false;
+    auto enter = [&](int r) {
+        if (r < k0) {
+            src = (const TI *)a.q + t * a.q_token + r * a.q_head;
+            src_step = RPW * a.q_head;
+            dst = (TO *)a.q_out + ((int64_t)t * a.q_heads + r) * a.D;
+            dst_step = RPW * a.D;
+            w = a.q_norm;
+            until = k0;
+        } else if (r < v0) {
+            const int h = r - k0;
+            src = (const TI *)a.k + t * a.k_token + h * a.k_head;
+            src_step = RPW * a.k_head;
+            dst = a.slots ? (TO *)a.kp + page * a.k_page + off * a.k_slot + h * a.k_ph
+                          : (TO *)a.k_out + ((int64_t)t * a.kv_heads + h) * a.D;
+            dst_step = RPW * (a.slots ? a.k_ph : a.D);
+            w = a.k_norm;
+            until = v0;
+        } else {
+            const int h = r - v0;
+            src = (const TI *)a.v + t * a.v_token + h * a.v_head;
+            src_step = RPW * a.v_head;
+            dst = (TO *)a.vp + page * a.v_page + off * a.v_slot + h * a.v_ph;
+            dst_step = RPW * a.v_ph;
+            w = nullptr;
+            until = INT_MAX;
+        }
+        turned = half && r < v0;
+    };
 
     // Every lane takes every step, for the sums across lanes.
     for (int r = row0; r - (int)(threadIdx.x % 32) / L < row1; r += RPW) {
         const bool live = r < row1;
         float x0[UPL][VEC], x1[UPL][VEC];
-        const TI *const src = r < k0 ? q + r * a.q_head : r < v0 ? k + r * a.k_head
-                                                                 : v + r * a.v_head;
+        if (r >= until && live) enter(r);
 #pragma unroll
         for (int n = 0; n < UPL; n++) {
             RopeVec<TI, VEC> a0 = {}, a1 = {};
@@ -183,7 +208,6 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
                 for (int i = 0; i < VEC; i++) ss += x0[n][i] * x0[n][i] + x1[n][i] * x1[n][i];
 #pragma unroll
             for (int o = L / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-            const float *w = r < k0 ? a.q_norm : r < v0 ? a.k_norm : nullptr;
             if (w) {
                 const float inv = rsqrtf(ss * inv_d + a.eps);
 #pragma unroll
@@ -200,8 +224,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
                 }
             }
         }
-        if (!live || (r >= k0 && a.slots && slot < 0)) continue;
-        TO *const dst = r < k0 ? qd + r * a.D : r < v0 ? kd + r * kd_head : vd + r * a.v_ph;
+        TO *const to = dst;
+        src += src_step;
+        dst += dst_step;
+        if (!live || (slot < 0 && a.slots && r >= k0)) continue;
 #pragma unroll
         for (int n = 0; n < UPL; n++) {
             if (lane + n * L >= units) continue;
@@ -210,7 +236,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
                 x = r0;
                 y = r1;
             };
-            if (r >= v0 || !half) {
+            if (!turned) {
                 // passes through
             } else if (VEC > 1 && a.interleaved) {
                 constexpr int P = (VEC + 1) / 2;
@@ -242,8 +268,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
                 o0.x[i] = AttnType<TO>::down(x0[n][i]);
                 o1.x[i] = AttnType<TO>::down(x1[n][i]);
             }
-            *(RopeVec<TO, VEC> *)(dst + at0[n]) = o0;
-            *(RopeVec<TO, VEC> *)(dst + at1[n]) = o1;
+            *(RopeVec<TO, VEC> *)(to + at0[n]) = o0;
+            *(RopeVec<TO, VEC> *)(to + at1[n]) = o1;
         }
     }
 }
@@ -286,7 +312,7 @@ static int rope_vec(RopeArgs &a, cudaStream_t st) {
         return in % ib == 0 && out % ob == 0;
     };
     // and the fewest lanes that hold a row (4922 tokens, 20 heads of 64, 52 of it
-    // turned in halves: 28 us with 32 lanes and vectors of two, 10 with 16)
+    // turned in halves: 28 us with 32 lanes and vectors of two, 8.4 with 16)
     if (fits(8)) {
         if (a.D <= 64) return rope_launch<TI, TO, 8, 4, 1>(a, st);
         if (a.D <= 128) return rope_launch<TI, TO, 8, 8, 1>(a, st);
