@@ -29,7 +29,7 @@
 // Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each with
 // half the keys of a step (with one, a scheduler has two warps, which do not hide
 // each other's latency); 16 issues the products, 17 loads keys and values by TMA,
-// boxes of 16 keys, into a ring of tiles.
+// a box a page (its issue takes some 70 cycles), into a ring of tiles.
 #include "attn.cuh"
 #include "umma.cuh"
 
@@ -39,7 +39,6 @@ namespace warp {
 namespace {
 
 constexpr int kRows = 128;                  // rows a tile
-constexpr int kBox = 16;                    // keys a TMA box: no page is smaller
 constexpr int kThreads = 18 * 32;
 
 template <int D> struct Lay {
@@ -60,8 +59,7 @@ template <int D> struct Lay {
                          tmem = drain + 8, fail = tmem + 4, dirty = fail + 4;
     static constexpr int bytes = bars + dirty + 8;
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
-    static_assert(cols % 32 == 0 && kv_half % 1024 == 0 && keys % kBox == 0,
-                  "swizzle atoms of 8 rows, whole boxes");
+    static_assert(cols % 32 == 0 && keys == 128, "whole boxes, swizzle atoms of 8 rows");
     // tensor memory columns
     static constexpr int o(int t) { return t * D; }
     static constexpr int s(int t) { return 2 * D + t * keys; }
@@ -429,11 +427,13 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     if (warp == 17) {
         // ---- keys and values: K of tile j in ring tile 2j, V in 2j + 1 --------------
         const int32_t *own_pages = PACKED ? nullptr : a.pages + (int64_t)blockIdx.z * a.pages_row;
-        constexpr int boxes = KEYS / kBox;
-        const int bi = lane % boxes, bh = lane / boxes;  // this lane's box and column half
+        // a box is a page, or a tile's part of one
+        const int box_shift = min(7, a.page_shift), box = 1 << box_shift;
+        const int bi = lane & ((KEYS >> box_shift) - 1);        // this lane's box
+        const int bh = lane >> (7 - box_shift);                 // and column half
         auto page_of = [&](int j, int &key, bool &want) {
             const bool pre = first + j < pre_tiles;
-            key = (first + j - (pre ? 0 : pre_tiles)) * KEYS + bi * kBox;
+            key = (first + j - (pre ? 0 : pre_tiles)) * KEYS + (bi << box_shift);
             want = j < cnt && bh < D / 64 && key < (pre ? n_pre : own_seen);
             return want ? attn_page(a, pre ? a.prefix_pages : own_pages, key) : 0;
         };
@@ -443,7 +443,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         for (int j = 0; j < cnt; j++) {
             if (__any_sync(~0u, *failed)) break;
             const int next_page = page_of(j + 1, next_key, next_want);
-            const uint32_t bytes = __popc(__ballot_sync(~0u, want)) * kBox * 128;
+            const uint32_t bytes = __popc(__ballot_sync(~0u, want)) * box * 128;
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 const int i = 2 * j + w, st = i % NS;
@@ -452,7 +452,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 if (lane == 0) arrive_tx(kv_full + 8 * st, bytes);
                 __syncwarp();
                 if (want)
-                    tma_box(base + L::ring + st * L::kv_tile + bh * L::kv_half + bi * kBox * 128,
+                    tma_box(base + L::ring + st * L::kv_tile + bh * L::kv_half + bi * box * 128,
                             w ? &vmap : &kmap, bh * 64, key & ((1 << a.page_shift) - 1), kvh, page,
                             kv_full + 8 * st);
                 issued++;
@@ -786,7 +786,8 @@ static CUresult (*encode_fn())(CUtensorMap *, CUtensorMapDataType, cuuint32_t, v
     return fn;
 }
 
-// The pages as a tensor (dim, slot, head, page), boxes of 64 columns by 16 keys.
+// The pages as a tensor (dim, slot, head, page), boxes of 64 columns by a page's
+// keys (a tile's at most).
 static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t page, int64_t slot,
                     int64_t head) {
     const auto fn = encode_fn();
@@ -801,7 +802,8 @@ static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t p
     const cuuint64_t strides[3] = {slot ? (cuuint64_t)slot * 2 : row,
                                    head ? (cuuint64_t)head * 2 : row,
                                    page ? (cuuint64_t)page * 2 : row};
-    const cuuint32_t box[4] = {64, kBox, 1, 1};
+    const int keys = attn_wide(c->head_dim);
+    const cuuint32_t box[4] = {64, (cuuint32_t)(c->page_size < keys ? c->page_size : keys), 1, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
     const CUresult r = fn(m, c->type == WARP_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
