@@ -21,14 +21,15 @@
 // 64), and so do 2 * 128 * 128 exponentials at 16 a clock; a row tile's step is
 // its softmax and then its products, and two row tiles in turn do not quite hide
 // the one behind the other. Measured with 256 rows on each of 148 SMs and 4096
-// keys in pages of 128: 63.7 us, 1247 TFLOP/s at D = 128, 53.6 us, 742 TFLOP/s
-// at 64 (pages of 16: 1208 and 743). Tried and slower: two places of S for 64
+// keys: 59.6 us, 1333 TFLOP/s at D = 128, 49.8 us, 797 TFLOP/s at 64, whatever
+// the page size. Tried and slower: two places of S for 64
 // keys each (966), P apart from S with 80 keys a step (904 to 1031), one warp a
-// 32 rows (843).
+// 32 rows (843), one loading warp for both (1207 with pages of 16, whose boxes it
+// issues one after another).
 //
 // Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each with
 // half the keys of a step (with one, a scheduler has two warps, which do not hide
-// each other's latency); 16 issues the products, 17 loads keys and values by TMA,
+// each other's latency); 16 issues the products, 17 loads keys and 18 values by TMA,
 // a box a page (its issue takes some 70 cycles), into a ring of tiles.
 #include "attn.cuh"
 #include "umma.cuh"
@@ -39,7 +40,7 @@ namespace warp {
 namespace {
 
 constexpr int kRows = 128;                  // rows a tile
-constexpr int kThreads = 18 * 32;
+constexpr int kThreads = 19 * 32;
 
 template <int D> struct Lay {
     static constexpr int keys = attn_wide(D);           // keys a tile
@@ -278,8 +279,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
 }
 
 // Of every 4 pairs of exponentials, those computed by ex2_poly: at D = 64, where
-// the products are half as long, one (4096 keys in pages of 128: 742 TFLOP/s
-// against 667 for none); at 128 none (1247 against 1172 for one).
+// the products are half as long, one (4096 keys: 742 TFLOP/s against 667 for
+// none, at the time); at 128 none (1247 against 1172 for one).
 constexpr int poly_pairs(int D) { return D == 64 ? 1 : 0; }
 
 // A warp's weights, in tensor memory by now, to the issuing warp.
@@ -422,10 +423,12 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         asm volatile("bar.sync 11, %0;" ::"n"(kThreads) : "memory");
         umma::fence_after();
     }
-    const uint32_t tmem = warp == 17 ? 0 : *(volatile uint32_t *)(basep + L::bars + L::tmem);
+    const uint32_t tmem = warp >= 17 ? 0 : *(volatile uint32_t *)(basep + L::bars + L::tmem);
 
-    if (warp == 17) {
-        // ---- keys and values: K of tile j in ring tile 2j, V in 2j + 1 --------------
+    if (warp >= 17) {
+        // ---- keys (warp 17) and values (18): K of tile j in ring tile 2j, V in 2j + 1 --
+        const int w = warp - 17;
+        const CUtensorMap *const map = w ? &vmap : &kmap;
         const int32_t *own_pages = PACKED ? nullptr : a.pages + (int64_t)blockIdx.z * a.pages_row;
         // a box is a page, or a tile's part of one
         const int box_shift = min(7, a.page_shift), box = 1 << box_shift;
@@ -444,26 +447,22 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             if (__any_sync(~0u, *failed)) break;
             const int next_page = page_of(j + 1, next_key, next_want);
             const uint32_t bytes = __popc(__ballot_sync(~0u, want)) * box * 128;
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const int i = 2 * j + w, st = i % NS;
-                if (i >= NS) wait(kv_empty + 8 * st, (i / NS - 1) & 1, fail);
-                if (__any_sync(~0u, *failed)) break;
-                if (lane == 0) arrive_tx(kv_full + 8 * st, bytes);
-                __syncwarp();
-                if (want)
-                    tma_box(base + L::ring + st * L::kv_tile + bh * L::kv_half + bi * box * 128,
-                            w ? &vmap : &kmap, bh * 64, key & ((1 << a.page_shift) - 1), kvh, page,
-                            kv_full + 8 * st);
-                issued++;
-            }
+            const int i = 2 * j + w, st = i % NS;
+            if (i >= NS) wait(kv_empty + 8 * st, (i / NS - 1) & 1, fail);
+            if (__any_sync(~0u, *failed)) break;
+            if (lane == 0) arrive_tx(kv_full + 8 * st, bytes);
+            __syncwarp();
+            if (want)
+                tma_box(base + L::ring + st * L::kv_tile + bh * L::kv_half + bi * box * 128, map,
+                        bh * 64, key & ((1 << a.page_shift) - 1), kvh, page, kv_full + 8 * st);
+            issued++;
             page = next_page;
             key = next_key;
             want = next_want;
         }
         if (*failed)                        // let the copies in flight land
-            for (int i = max(0, issued - NS); i < issued; i++)
-                wait_over(kv_full + 8 * (i % NS), (i / NS) & 1);
+            for (int j = max(0, issued - NS); j < issued; j++)
+                wait_over(kv_full + 8 * ((2 * j + w) % NS), ((2 * j + w) / NS) & 1);
     } else if (warp == 16) {
         // ---- the products ------------------------------------------------------------
         if (cnt > 0) {
