@@ -574,7 +574,7 @@ static int split_rows(int64_t tiles, int64_t ctas, double rows, int D) {
 }
 
 // attn_umma_kernel: one CTA an SM; 128 keys for 256 rows, and a CTA around them.
-static double wide_tile_us(int D) { return D == 128 ? 1.7 : 1.4; }
+static double wide_tile_us(int D) { return D == 128 ? 1.55 : 1.25; }
 constexpr double kWideCtaUs = 7.0;
 
 static int split_wide(int64_t tiles, int64_t ctas, double rows, int D) {
