@@ -757,6 +757,10 @@ extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages
     a.rows_small = p.rows_small;
     a.split_tiles = p.each, a.wide_each = p.wide_each, a.wide_parts = p.wide_parts;
     a.prefix_split_tiles = a.prefix_wide_each = p.prefix_each;
+    a.by_group = warp::attn_div(a.group);
+    a.by_wide_parts = warp::attn_div(p.wide_parts), a.by_wide_each = warp::attn_div(p.wide_each);
+    a.by_prefix_parts = warp::attn_div(p.prefix_parts);
+    a.by_prefix_each = warp::attn_div(p.prefix_each);
     rc = warp::attn_err_word(&a.err);
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;

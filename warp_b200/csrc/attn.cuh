@@ -32,6 +32,19 @@ template <> struct AttnType<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
 };
 
+// x / d for x below 2^31 by the reciprocal that the host gives with d, and a step
+// of correction: a quarter of a division's time, and several stand at the start of
+// a block one behind another.
+struct AttnDiv { uint32_t d, mul; };
+inline AttnDiv attn_div(int d) {
+    const uint32_t u = d < 1 ? 1 : (uint32_t)d;
+    return {u, u == 1 ? 0xffffffffu : (uint32_t)(((uint64_t)1 << 32) / u)};
+}
+__device__ __forceinline__ int operator/(int x, const AttnDiv &v) {
+    const uint32_t q = __umulhi((uint32_t)x, v.mul);
+    return (int)(q + ((uint32_t)x - q * v.d >= v.d));
+}
+
 // One attention call as its kernels see it.
 struct AttnArgs {
     const void *q, *kp, *vp;
@@ -60,6 +73,8 @@ struct AttnArgs {
     int prefix_split_tiles;                 // and of a part of the prefix
     int wide_each, wide_parts;              // the same for attn_umma_kernel: wide tiles
     int prefix_wide_each;                   // of a part, and parts at most
+    // divisions of attn_umma_kernel: by group, by parts, by tiles of a part
+    AttnDiv by_group, by_wide_parts, by_prefix_parts, by_wide_each, by_prefix_each;
 };
 
 // Request b as the host's bounds leave it: its first token, its queries and

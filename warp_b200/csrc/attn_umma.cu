@@ -330,11 +330,11 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     const AttnReq rq = PACKED ? AttnReq{0, a.tokens, 0} : attn_req(a, blockIdx.z);
     const int rows = rq.n * a.group;
     if (!PACKED && rows <= a.rows_small) return;
-    const int parts_max = PACKED ? a.prefix_parts : a.wide_parts;
-    const int part = blockIdx.x % parts_max;
+    const int bx = (int)blockIdx.x / (PACKED ? a.by_prefix_parts : a.by_wide_parts);
+    const int part = (int)blockIdx.x - bx * (PACKED ? a.prefix_parts : a.wide_parts);
     const int pairs = (rows + 2 * kRows - 1) / (2 * kRows);
     // the rows that see the most keys first
-    const int pair = pairs - 1 - (int)(blockIdx.x / parts_max);
+    const int pair = pairs - 1 - bx;
     if (pair < 0) return;
     const int row0 = pair * 2 * kRows;
 
@@ -342,12 +342,13 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     const int pre_tiles = (n_pre + KEYS - 1) / KEYS;
     const int all_tiles = pre_tiles + (PACKED ? 0 : (rq.len + KEYS - 1) / KEYS);
     const int each = PACKED ? a.prefix_wide_each : a.wide_each;
-    const int parts = max(1, attn_parts(all_tiles, each));
+    const int parts =
+        max(1, (all_tiles + each - 1) / (PACKED ? a.by_prefix_each : a.by_wide_each));
     if (part >= parts) return;
     // own keys that row r sees
     const bool causal = !PACKED && a.causal;
     auto sees = [&](int r) {
-        return causal ? max(0, min(rq.len, rq.len - rq.n + r / a.group + 1)) : rq.len;
+        return causal ? max(0, min(rq.len, rq.len - rq.n + r / a.by_group + 1)) : rq.len;
     };
     const int tiles_rows = rows - row0 > kRows ? 2 : 1;
     // keys in sight of each tile's last row, and the key tiles that hold them
@@ -358,7 +359,10 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         return max(0, min(first + each, pre_tiles + (seen + KEYS - 1) / KEYS) - first);
     };
     const int cnt0 = count_of(seen_t0), cnt = count_of(own_seen);
-    const int see_first = PACKED ? 0 : causal ? rq.len - rq.n + row0 / a.group + 1 : rq.len;
+    // row0's token and its head in the group; row0 + x is then token
+    // tok0 + (rem0 + x) / group
+    const int tok0 = row0 / a.by_group, rem0 = row0 - tok0 * a.group;
+    const int see_first = PACKED ? 0 : causal ? rq.len - rq.n + tok0 + 1 : rq.len;
 
     const uint32_t base = smem_u32(basep);
     const uint32_t bars = base + L::bars;
@@ -375,9 +379,6 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     // The rows' warps: row tile, half of the keys, quarter of the rows, row.
     const int t = warp / 8, h = warp / 4 % 2, quad = warp % 4, r = threadIdx.x % kRows;
     const int tid = threadIdx.x % (2 * kRows);          // in the tile
-    // row0's token and its head in the group; row0 + x is then token
-    // tok0 + (rem0 + x) / group
-    const int tok0 = row0 / a.group, rem0 = row0 - tok0 * a.group;
     const float inv_group = 1.f / (float)a.group;
     // Q is asked for first of all, a row by D / 8 neighbouring threads.
     constexpr int CH = D / 8, RP = 2 * kRows / CH, N = kRows / RP;
