@@ -257,8 +257,8 @@ typedef enum { WARP_T_F32 = 0, WARP_T_F16 = 1, WARP_T_BF16 = 2 } warp_type;
  * k + page*k_page + slot*k_slot + head*k_head + d, and v alike, so pages may
  * be laid out [slot][head] or [head][slot].  page_size is a power of two from
  * 16 to 4096; type is WARP_T_F16 or WARP_T_BF16; base addresses and strides are
- * multiples of 16 bytes.  Slot number n is slot n % page_size of page
- * n / page_size. */
+ * multiples of 16 bytes, strides positive (0 on an axis of one entry).  Slot
+ * number n is slot n % page_size of page n / page_size. */
 typedef struct {
     void *k, *v;
     int type, page_size, kv_heads, head_dim;

@@ -106,6 +106,21 @@ def test_append_refusals(lib, kw, ckw, text):
     assert lib.warp_kv_append(ctypes.byref(rope_desc()), None, None, None) == -1
 
 
+@pytest.mark.parametrize("ckw", [dict(k_slot=0), dict(v_page=0), dict(kv_heads=2, k_head=0),
+                                 dict(kv_heads=2, v_head=0)])
+def test_broadcast_pages_are_refused(lib, ckw):
+    """A stride of 0 has a meaning only where there is one entry."""
+    heads = ckw.get("kv_heads", 1)
+    c = kv_pages(**ckw)
+    assert lib.warp_kv_append(ctypes.byref(rope_desc(kv_heads=heads)), ctypes.byref(c),
+                              ctypes.c_void_p(256), None) == -1
+    assert b"strides" in lib.warp_last_error()
+    d = attn_desc(kv_heads=heads, max_q=100, tokens=100)
+    assert lib.warp_attn_scratch(ctypes.byref(d), ctypes.byref(c)) == -1
+    one = kv_pages(k_head=0, v_head=0, pages=1, k_page=0, v_page=0)
+    assert lib.warp_attn_scratch(ctypes.byref(attn_desc()), ctypes.byref(one)) >= 0
+
+
 @pytest.mark.parametrize("kw, ckw, text", [
     (dict(tokens=-1), {}, b"negative"), (dict(q_heads=3, kv_heads=2), dict(kv_heads=2), b"over"),
     (dict(q_heads=0), {}, b"over"), (dict(head_dim=96), dict(head_dim=96), b"head_dim"),

@@ -333,6 +333,25 @@ def test_prefix_shapes(cuda, q, kv, prefix, causal):
     Case(q, kv, 8, 2, 128, 32, torch.bfloat16, prefix=prefix, seed=len(q)).check(causal=causal)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B, Hq, Hk", [(2, 4, 4), (3, 10, 2), (16, 2, 2), (17, 2, 2)])
+@pytest.mark.parametrize("prefix", [5, 333, 2600])
+def test_prefix_few_rows(cuda, dtype, D, B, Hq, Hk, prefix):
+    """All the batch's rows of a kv head in one tile of 16, and one more."""
+    Case([1] * B, [i * 7 % 40 for i in range(B)], Hq, Hk, D, 16, dtype, prefix=prefix,
+         seed=B + prefix).check()
+
+
+def test_one_page_and_one_head(cuda):
+    """Axes of one entry, whose strides mean nothing."""
+    for n in (1, 40):
+        c = Case([n], [60], 2, 1, 64, 64, torch.float16, seed=28)
+        at = c.pages[0, :1].long()
+        c.k, c.v, c.pages = c.k[at], c.v[at], torch.zeros(1, 1, dtype=torch.int32)
+        c.check()
+
+
 def test_prefix_is_the_same_as_its_own_copy(cuda):
     """A shared prefix gives what the same keys at the head of each request's own pages give."""
     P, own = 96, [5, 33]

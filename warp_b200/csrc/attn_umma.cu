@@ -21,10 +21,10 @@
 // 64), and so do 2 * 128 * 128 exponentials at 16 a clock; a row tile's step is
 // its softmax and then its products, and two row tiles in turn do not quite hide
 // the one behind the other. Measured with 256 rows on each of 148 SMs and 4096
-// keys: 59.6 us, 1333 TFLOP/s at D = 128, 49.8 us, 797 TFLOP/s at 64, whatever
-// the page size. Tried and slower: two places of S for 64
-// keys each (966), P apart from S with 80 keys a step (904 to 1031), one warp a
-// 32 rows (843), one loading warp for both (1207 with pages of 16, whose boxes it
+// keys: 59.6 us, 1333 TFLOP/s at D = 128; 774 to 797 TFLOP/s at 64, 49.8 us at
+// best; whatever the page size. Tried and slower: two places of S for 64 keys
+// each (966), P apart from S with 80 keys a step (904 to 1031), one warp a 32
+// rows (843), one loading warp for both (1207 with pages of 16, whose boxes it
 // issues one after another).
 //
 // Warps: 0-7 rows of tile 0, 8-15 rows of tile 1, two warps a 32 rows, each with

@@ -48,9 +48,11 @@ int kv_pages_check(const warp_kv_pages *c, const char *who) {
     WARP_ARG((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, "%s: pages must be 16-byte aligned",
              who);
     const int64_t st[6] = {c->k_page, c->k_slot, c->k_head, c->v_page, c->v_slot, c->v_head};
+    const int64_t extent[3] = {c->pages, c->page_size, c->kv_heads};
     for (int i = 0; i < 6; i++)
-        WARP_ARG(st[i] >= 0 && (st[i] & 7) == 0,
-                 "%s: page strides must be non-negative multiples of 16 bytes", who);
+        WARP_ARG(st[i] >= (extent[i % 3] > 1) && (st[i] & 7) == 0,
+                 "%s: page strides must be positive multiples of 16 bytes (0 only on an axis of "
+                 "one entry)", who);
     return WARP_OK;
 }
 

@@ -221,6 +221,12 @@ def _vec_ok(x, n, dtype):
     return x.dtype is dtype and x.numel() == n and x.is_contiguous() and x.is_cuda
 
 
+def _here(x):
+    """Calls run on torch's current device and its stream."""
+    if x.is_cuda and x.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on {x.device}, which is not the current device")
+
+
 def _rows(x, name, T, D, dtype):
     """(heads, token stride, head stride, address) of [T][heads][D] on the
     device with contiguous heads; the stride of an axis of one entry is 0, as
@@ -243,6 +249,7 @@ def _rope_pack(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, r
     dt = x.dtype
     if x.dim() != 3 or dt not in _TYPES:
         raise ValueError("queries and keys must be [tokens][heads][head_dim], fp32, fp16 or bf16")
+    _here(x)
     T, nk, D = x.shape
     nq = qt = qh = qp = kt = kh = kp = vt = vh = vp = qn = kn = f = p = rot = 0
     if q is not None:
@@ -358,6 +365,7 @@ def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
 def _batch(q_start, kv_len, pages):
     """(requests, row stride and width of the page table)."""
     B = kv_len.numel()
+    _here(kv_len)
     if not _vec_ok(kv_len, B, torch.int32):
         _cuda(kv_len)
         raise ValueError("kv_len must be contiguous int32 [batch]")
@@ -391,6 +399,7 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
     dt = q.dtype
     if q.dim() != 3 or dt not in _TYPES:
         raise ValueError("q must be [tokens][heads][head_dim], fp16 or bf16")
+    _here(q)
     T, _, D = q.shape
     Hq, qt, qh, qp = _rows(q, "q", T, D, dt)
     if out is None:
