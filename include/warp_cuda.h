@@ -335,7 +335,8 @@ WARP_API int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int ba
  * type is that of q, out and the pages (WARP_T_F16 or WARP_T_BF16); head_dim
  * is 64 or 128.  The products take their operands in that type and accumulate
  * in fp32; softmax statistics are fp32, and its weights are rounded to `type`
- * for the second product.  max_q and max_kv are host bounds on the requests'
+ * for the second product (fp16: relatively down to 2^-25 of the row's largest
+ * weight, by at most 2^-36 of it below that).  max_q and max_kv are host bounds on the requests'
  * queries and own keys; what exceeds them, or a page number outside the pages,
  * is left out and reported by warp_attn_status.
  * scratch: warp_attn_scratch(d, c) bytes of device memory, 256-byte aligned,

@@ -228,6 +228,8 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    // the running maxima, lowered
+    constexpr float lift = attn_lift<T>(0.f);
     float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
 
     int n = 0;
@@ -251,7 +253,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
         const int j0 = (pre ? i : i - pre_tiles) * kAttnTile;
         const int lim_lo = pre ? n_pre - j0 : min(see_lo, own_seen) - j0;
         const int lim_hi = pre ? n_pre - j0 : min(see_hi, own_seen) - j0;
-        float mx_lo = m_lo, mx_hi = m_hi;
+        float mx_lo = -INFINITY, mx_hi = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -267,6 +269,8 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
             mx_lo = fmaxf(mx_lo, __shfl_xor_sync(~0u, mx_lo, x));
             mx_hi = fmaxf(mx_hi, __shfl_xor_sync(~0u, mx_hi, x));
         }
+        mx_lo = fmaxf(m_lo, mx_lo - lift);
+        mx_hi = fmaxf(m_hi, mx_hi - lift);
         if (__any_sync(~0u, mx_lo > m_lo || mx_hi > m_hi)) {
             const float w_lo = mx_lo == -INFINITY ? 1.f : ex2(m_lo - mx_lo);
             const float w_hi = mx_hi == -INFINITY ? 1.f : ex2(m_hi - mx_hi);

@@ -129,6 +129,20 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
     return *(const uint32_t *)&h;
 }
 
+// The softmax's weights are rounded to the pages' type for the second product, as
+// the matrix instructions take both operands in one type; their sum is taken
+// before.  bf16 has fp32's exponents.  fp16 rounds what is below 2^-14 ever more
+// coarsely and below 2^-25 to nothing, though a long row's many small weights may
+// count: so weights are measured from a maximum lowered by 2^lift, up to 2^15 of
+// fp16's 2^16, and what is recorded as the maximum is the lowered one.  A weight
+// is then rounded relatively down to 2^-(14 + lift) of the row's largest, and the
+// error of each below is 2^-(25 + lift) at most.  `slack`: how far a row may
+// outgrow its maximum (as a power of two) before that is moved.
+template <typename T> __host__ __device__ constexpr float attn_lift(float) { return 0.f; }
+template <> __host__ __device__ constexpr float attn_lift<__half>(float slack) {
+    return 15.f - slack;
+}
+
 // The tensor-core kernel: the requests with many rows, or (packed) the shared
 // prefix for all rows of the batch.
 int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,

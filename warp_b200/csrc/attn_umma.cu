@@ -12,9 +12,9 @@
 // row tile's exponentials are computed the other's products run.
 //
 // The maximum that p is measured from moves only when a row outgrows it by
-// 2^8, so the accumulated O is rescaled rarely; p then stays below 2^8, which
-// both 16-bit types hold, and the result is the same as O and l carry the same
-// factor.
+// 2^8 (fp16: 2^4), so the accumulated O is rescaled rarely; p then stays below 2^8
+// (fp16, whose weights attn_lift raises: 2^15), which the type holds, and the result
+// is the same as O and l carry the same factor.
 //
 // What bounds it: per pair of 128 x 128 tiles the products take
 // 2 * 2 * 128 * 128 * D / 4096 FMA a clock = 2048 cycles at D = 128 (half at
@@ -282,6 +282,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
 // the products are half as long, one (4096 keys: 742 TFLOP/s against 667 for
 // none, at the time); at 128 none (1247 against 1172 for one).
 constexpr int poly_pairs(int D) { return D == 64 ? 1 : 0; }
+
+// How far a row outgrows its maximum before that is moved, see attn_lift.  fp16 with
+// 4 and a lift of 11 in place of 8 and 7 rounds weights 16 times finer; 4096 causal
+// tokens, 32 heads of 64 over 8: 119 us either way with scores of deviation 1, 143
+// against 133 with scores of deviation 4, which move it more often.
+template <typename T> __device__ constexpr float slack() { return 8.f; }
+template <> __device__ constexpr float slack<__half>() { return 4.f; }
 
 // A warp's weights, in tensor memory by now, to the issuing warp.
 __device__ __forceinline__ void hand_over(uint32_t ready) {
@@ -555,6 +562,8 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         const bool warp_live = row0 + t * kRows + quad * 32 < rows;
         const int see = PACKED ? 0 : row < rows ? sees(row) : 0;
         const float c = a.scale_log2;
+        // what p is measured from, in the log2 domain
+        auto lowered = [&](float m) { return __fmaf_rn(m, c, -attn_lift<T>(slack<T>())); };
         float m = -INFINITY;
         float2 l = make_float2(0.f, 0.f);    // two halves of the sum
         // Steps that are not full, and those with keys that only some rows see: what
@@ -623,11 +632,11 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 mx[1] = max3(mx[1], s[L::cols - 2], s[L::cols - 1]);
                 float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 // the halves' maxima are exchanged only if one outgrows the old one
-                if (__builtin_expect(pair_any(t, quad, !((top - m) * c <= 8.f)), 0)) {
+                if (__builtin_expect(pair_any(t, quad, !((top - m) * c <= slack<T>())), 0)) {
                     swap[h * kRows + r] = top;
                     pair_sync(t, quad);
                     top = max3(top, swap[(h ^ 1) * kRows + r], top);
-                    const bool grow = !((top - m) * c <= 8.f);
+                    const bool grow = !((top - m) * c <= slack<T>());
                     const float to = grow ? top : m;
                     const float w = !grow || to == -INFINITY ? 1.f : ex2(m * c - to * c);
                     if (j > 0) {
@@ -646,7 +655,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                     m = to;
                 }
                 // a row with an infinite or NaN score is NaN altogether
-                const float mc = m == -INFINITY ? 0.f : m < INFINITY ? m * c : NAN;
+                const float mc = m == -INFINITY ? 0.f : m < INFINITY ? lowered(m) : NAN;
                 const uint64_t c2 = pair2(c, c), mc2 = pair2(-mc, -mc);
                 uint64_t l2 = pair2(l.x, l.y);
                 if (__builtin_expect(masked, 0)) weights<T, 0>(s, c2, mc2, l2, st, p_full + 16 * t);
@@ -743,7 +752,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             }
             if (!direct && h == 0 && row < rows)
                 a.part_ml[part_row + out_row + (int64_t)tok * a.q_heads + (y - tok * a.group)] =
-                    make_float2(m * c, sum);
+                    make_float2(lowered(m), sum);
         }
     }
     umma::fence_before();
