@@ -22,6 +22,9 @@ namespace warp {
 
 __device__ unsigned g_attn_err;
 
+// Takes off the bits that have been reported, and no other.
+__global__ void attn_err_clear_kernel(unsigned bits) { atomicAnd(&g_attn_err, ~bits); }
+
 // The word's address is fixed once its device is in use: looked up once for each.
 int attn_err_word(unsigned **out) {
     constexpr int kDevices = 64;
@@ -453,11 +456,14 @@ extern "C" int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int 
 
 extern "C" int warp_attn_status(int clear) {
     unsigned v = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&v, warp::g_attn_err, sizeof(v));
+    // a copy by itself does not wait for streams that do not block the default one
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, warp::g_attn_err, sizeof(v));
     if (e != cudaSuccess) return warp::cuda_fail(e, "warp_attn_status");
     if (clear && v) {
-        const unsigned z = 0;
-        e = cudaMemcpyToSymbol(warp::g_attn_err, &z, sizeof(z));
+        warp::attn_err_clear_kernel<<<1, 1>>>(v);
+        WARP_CHECK_LAUNCH("attn_err_clear_kernel");
+        e = cudaDeviceSynchronize();        // before anything that may report anew
         if (e != cudaSuccess) return warp::cuda_fail(e, "warp_attn_status");
     }
     if (v & warp::kAttnTimeout) {
