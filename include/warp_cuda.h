@@ -314,8 +314,9 @@ WARP_API int warp_kv_append(const warp_rope_desc *d, const warp_kv_pages *c,
  * slot j % page_size of page pages[b*pages_row + j / page_size].  Writes for
  * token t positions[t] = base + j and slots[t]; base is the length of a prefix
  * that the requests share (warp_paged_attention), else 0.  A token whose j is
- * negative or past the row's pages_per_row pages gets slot -1, and so does one
- * of no request. */
+ * negative gets slot -1, and so does one of no request.  So do a j past the
+ * row's pages_per_row pages and one in a page with a negative number, but these
+ * are reported by warp_attn_status, as their keys would be lost. */
 WARP_API int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int batch, int tokens,
                            const int32_t *pages, int64_t pages_row, int pages_per_row,
                            int page_size, int base, int32_t *positions, int64_t *slots,
@@ -364,7 +365,8 @@ WARP_API int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *
                                   void *stream);
 
 /* What the kernels above left out since the last clear: WARP_OK, WARP_E_ARG
- * (a slot or page number outside the pages, a length over its bound) or
+ * (a slot or page number outside the pages, a length over its bound or past
+ * its row of pages) or
  * WARP_E_TIMEOUT (a bounded wait gave up; that launch's output is
  * incomplete).  Synchronises the device; clear = 1 resets. */
 WARP_API int warp_attn_status(int clear);

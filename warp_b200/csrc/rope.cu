@@ -416,9 +416,14 @@ __global__ void kv_slots_kernel(const int32_t *__restrict__ q_start,
     if (t >= first && t < end) {
         const int64_t j = (int64_t)kv_len[lo] - end + t;
         pos = (int32_t)(base + j);
-        if (j >= 0 && (j >> page_shift) < pages_per_row)
-            slot = ((int64_t)pages[lo * pages_row + (j >> page_shift)] << page_shift) +
-                   (j & ((1 << page_shift) - 1));
+        if ((j >> page_shift) >= pages_per_row) {
+            atomicOr(&g_attn_err, kAttnBadLen);
+        } else if (j >= 0) {
+            const int page = pages[lo * pages_row + (j >> page_shift)];
+            // a negative slot would pass for a token that is not to be stored
+            if (page < 0) atomicOr(&g_attn_err, kAttnBadPage);
+            else slot = ((int64_t)page << page_shift) + (j & ((1 << page_shift) - 1));
+        }
     }
     positions[t] = pos;
     slots[t] = slot;

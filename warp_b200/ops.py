@@ -352,7 +352,9 @@ def kv_append(q, k, v, k_pages, v_pages, slots, positions, inv_freq, q_norm=None
 def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
     """(positions int32 [T], slots int64 [T]) of a step's tokens for kv_append
     (warp_kv_slots): q_start int32 [B+1], kv_len int32 [B] own keys with the
-    new ones counted, pages int32 [B][n]; base: the shared prefix's length."""
+    new ones counted, pages int32 [B][n]; base: the shared prefix's length.
+    Keys past a row's pages or in a page of negative number have no slot, and
+    attn_status raises."""
     B, row, wide = _batch(q_start, kv_len, pages)
     positions = torch.empty(tokens, dtype=torch.int32, device=q_start.device)
     slots = torch.empty(tokens, dtype=torch.int64, device=q_start.device)
