@@ -217,24 +217,35 @@ def rope_inv_freq(rot_dim, base=10000.0, scaling="none", factor=1.0, trained=Non
     return f.to(device), scale
 
 
-def _vec_ok(x, n, dtype):
-    return x.dtype is dtype and x.numel() == n and x.is_contiguous() and x.is_cuda
+def _device(x):
+    """The number of torch's current device, on whose current stream calls run, for
+    a call with tensor x."""
+    if not x.is_cuda:           # without a device there is no current one to ask for
+        _cuda(x)
+    return torch._C._cuda_getDevice()
 
 
-def _here(x):
-    """Calls run on torch's current device and its stream."""
-    if x.is_cuda and x.get_device() != torch._C._cuda_getDevice():
-        raise ValueError(f"the tensors are on {x.device}, which is not the current device")
+def _elsewhere(x):
+    """Refuses a tensor whose device is not the current one."""
+    _cuda(x)
+    raise ValueError(f"a tensor is on {x.device}, which is not the current device")
 
 
-def _rows(x, name, T, D, dtype):
+def _vec_ok(x, n, dtype, dev):
+    if x.get_device() != dev:
+        _elsewhere(x)
+    return x.dtype is dtype and x.numel() == n and x.is_contiguous()
+
+
+def _rows(x, name, T, D, dtype, dev):
     """(heads, token stride, head stride, address) of [T][heads][D] on the
     device with contiguous heads; the stride of an axis of one entry is 0, as
     it has no meaning."""
+    if x.get_device() != dev:
+        _elsewhere(x)
     shape, strides = x.shape, x.stride()
     if len(shape) != 3 or shape[0] != T or shape[2] != D or x.dtype is not dtype or \
-            not x.is_cuda or (strides[2] != 1 and D > 1):
-        _cuda(x)
+            (strides[2] != 1 and D > 1):
         raise ValueError(f"{name} must be [tokens][heads][head_dim] with contiguous heads, all "
                          "of one dtype, token count and head_dim")
     heads = shape[1]
@@ -249,35 +260,31 @@ def _rope_pack(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, r
     dt = x.dtype
     if x.dim() != 3 or dt not in _TYPES:
         raise ValueError("queries and keys must be [tokens][heads][head_dim], fp32, fp16 or bf16")
-    _here(x)
+    dev = _device(x)
     T, nk, D = x.shape
     nq = qt = qh = qp = kt = kh = kp = vt = vh = vp = qn = kn = f = p = rot = 0
     if q is not None:
-        nq, qt, qh, qp = _rows(q, "q", T, D, dt)
+        nq, qt, qh, qp = _rows(q, "q", T, D, dt, dev)
         nk = 0
     if k is not None:
-        nk, kt, kh, kp = _rows(k, "k", T, D, dt)
+        nk, kt, kh, kp = _rows(k, "k", T, D, dt, dev)
     if v is not None:
-        nv, vt, vh, vp = _rows(v, "v", T, D, dt)
+        nv, vt, vh, vp = _rows(v, "v", T, D, dt, dev)
         if nv != nk:
             raise ValueError("v must have k's heads")
     if inv_freq is not None:
         rot = 2 * inv_freq.numel()
-        if not _vec_ok(inv_freq, rot // 2, torch.float64):
-            _cuda(inv_freq)
+        if not _vec_ok(inv_freq, rot // 2, torch.float64, dev):
             raise ValueError("inv_freq must be contiguous float64")
-        if positions is None or not _vec_ok(positions, T, torch.int32):
-            _cuda(positions)
+        if positions is None or not _vec_ok(positions, T, torch.int32, dev):
             raise ValueError("positions must be contiguous int32 [tokens]")
         f, p = inv_freq.data_ptr(), positions.data_ptr()
     if q_norm is not None:
-        if not _vec_ok(q_norm, D, torch.float32):
-            _cuda(q_norm)
+        if not _vec_ok(q_norm, D, torch.float32, dev):
             raise ValueError("q_norm must be contiguous float32 [head_dim]")
         qn = q_norm.data_ptr()
     if k_norm is not None:
-        if not _vec_ok(k_norm, D, torch.float32):
-            _cuda(k_norm)
+        if not _vec_ok(k_norm, D, torch.float32, dev):
             raise ValueError("k_norm must be contiguous float32 [head_dim]")
         kn = k_norm.data_ptr()
     return ffi.ROPE_DESC.pack(
@@ -311,12 +318,12 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6,
     return q_out, k_out
 
 
-def _pages_pack(k_pages, v_pages):
+def _pages_pack(k_pages, v_pages, dev):
+    if k_pages.get_device() != dev or v_pages.get_device() != dev:
+        _elsewhere(k_pages if k_pages.get_device() != dev else v_pages)
     shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
     if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or \
-            not k_pages.is_cuda or not v_pages.is_cuda or \
             (shape[3] > 1 and (ks[3] != 1 or vs[3] != 1)):
-        _cuda(k_pages, v_pages)
         raise ValueError("k_pages and v_pages must be [pages][page_size][kv_heads][head_dim] "
                          "of one shape and dtype with contiguous heads")
     n, size, heads, dim = shape
@@ -339,12 +346,13 @@ def kv_append(q, k, v, k_pages, v_pages, slots, positions, inv_freq, q_norm=None
     kv_slots makes them."""
     if k is None or v is None:
         raise ValueError("kv_append needs keys and values")
-    c = _pages_pack(k_pages, v_pages)
+    dev = _device(k)
+    c = _pages_pack(k_pages, v_pages, dev)
     q_out = None if q is None else _dense(q, k_pages.dtype)
     d = _rope_pack(q, k, v, positions, inv_freq, q_norm, k_norm, eps, interleaved, rot_scale,
                    q_out, None, k_pages.dtype)
-    if not _vec_ok(slots, k.shape[0], torch.int64):
-        raise ValueError("slots must be contiguous int64 [tokens] on the device")
+    if not _vec_ok(slots, k.shape[0], torch.int64, dev):
+        raise ValueError("slots must be contiguous int64 [tokens]")
     ffi.check(ffi.load().warp_kv_append(d, c, slots.data_ptr(), _stream()))
     return q_out
 
@@ -355,7 +363,7 @@ def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
     new ones counted, pages int32 [B][n]; base: the shared prefix's length.
     Keys past a row's pages or in a page of negative number have no slot, and
     attn_status raises."""
-    B, row, wide = _batch(q_start, kv_len, pages)
+    B, row, wide = _batch(q_start, kv_len, pages, _device(kv_len))
     positions = torch.empty(tokens, dtype=torch.int32, device=q_start.device)
     slots = torch.empty(tokens, dtype=torch.int64, device=q_start.device)
     ffi.check(ffi.load().warp_kv_slots(
@@ -364,20 +372,18 @@ def kv_slots(q_start, kv_len, pages, page_size, tokens, base=0):
     return positions, slots
 
 
-def _batch(q_start, kv_len, pages):
+def _batch(q_start, kv_len, pages, dev):
     """(requests, row stride and width of the page table)."""
     B = kv_len.numel()
-    _here(kv_len)
-    if not _vec_ok(kv_len, B, torch.int32):
-        _cuda(kv_len)
+    if not _vec_ok(kv_len, B, torch.int32, dev):
         raise ValueError("kv_len must be contiguous int32 [batch]")
-    if not _vec_ok(q_start, B + 1, torch.int32):
-        _cuda(q_start)
+    if not _vec_ok(q_start, B + 1, torch.int32, dev):
         raise ValueError("q_start must be contiguous int32 [batch + 1]")
+    if pages.get_device() != dev:
+        _elsewhere(pages)
     shape, strides = pages.shape, pages.stride()
     if len(shape) != 2 or shape[0] != B or pages.dtype is not torch.int32 or \
-            not pages.is_cuda or (strides[1] != 1 and shape[1] > 1):
-        _cuda(pages)
+            (strides[1] != 1 and shape[1] > 1):
         raise ValueError("pages must be int32 [batch][pages a request], rows contiguous")
     return B, strides[0] if B > 1 else 0, shape[1]
 
@@ -396,25 +402,27 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
     (int32 [n]), before their own.  A query that sees nothing gets zeros; a
     token of no request is not written.  scale: 1/sqrt(D) by default.  Returns
     [T][Hq][D] in q's dtype."""
-    c = _pages_pack(k_pages, v_pages)
-    B, row, wide = _batch(q_start, kv_len, pages)
+    dev = _device(q)
+    c = _pages_pack(k_pages, v_pages, dev)
+    B, row, wide = _batch(q_start, kv_len, pages, dev)
     dt = q.dtype
     if q.dim() != 3 or dt not in _TYPES:
         raise ValueError("q must be [tokens][heads][head_dim], fp16 or bf16")
-    _here(q)
     T, _, D = q.shape
-    Hq, qt, qh, qp = _rows(q, "q", T, D, dt)
+    Hq, qt, qh, qp = _rows(q, "q", T, D, dt, dev)
     if out is None:
         out = _dense(q, dt)
-    elif out.shape != q.shape or out.dtype is not dt or not out.is_contiguous() or \
-            not out.is_cuda:
-        raise ValueError("out must be contiguous, of q's shape and dtype")
+    else:
+        if out.get_device() != dev:
+            _elsewhere(out)
+        if out.shape != q.shape or out.dtype is not dt or not out.is_contiguous():
+            raise ValueError("out must be contiguous, of q's shape and dtype")
     pp = 0
     if prefix_len:
         if prefix_pages is None or prefix_len > prefix_pages.numel() * k_pages.shape[1]:
             raise ValueError("prefix_pages hold fewer than prefix_len keys")
-        if not _vec_ok(prefix_pages, prefix_pages.numel(), torch.int32):
-            raise ValueError("prefix_pages must be contiguous int32 [n] on the device")
+        if not _vec_ok(prefix_pages, prefix_pages.numel(), torch.int32, dev):
+            raise ValueError("prefix_pages must be contiguous int32 [n]")
         pp = prefix_pages.data_ptr()
     d = ffi.ATTN_DESC.pack(
         B, T, Hq, k_pages.shape[2], D, _TYPES[dt], qp, qt, qh,
