@@ -56,9 +56,20 @@ class Step:
 
     @classmethod
     def plan(cls, q_lens, kv_lens, pages, page_size, prefix_pages=None, prefix_len=0):
-        """q_lens and kv_lens are lists; pages int32 [batch][n] on the device."""
+        """q_lens and kv_lens are lists; pages int32 [batch][n] on the device.  What
+        the page numbers themselves leave out is for ops.attn_status to say."""
         if len(q_lens) != len(kv_lens) or not q_lens:
             raise ValueError("q_lens and kv_lens must name the same requests, one at least")
+        if pages.dim() != 2 or pages.shape[0] != len(q_lens):
+            raise ValueError("pages must have a row for each request")
+        held = pages.shape[1] * page_size
+        for b, (n, kv) in enumerate(zip(q_lens, kv_lens)):
+            if not 0 <= n <= kv <= held:
+                raise ValueError(f"request {b}: {n} tokens, the last of {kv} keys, in pages for "
+                                 f"{held}")
+        front = 0 if prefix_pages is None else prefix_pages.numel() * page_size
+        if not 0 <= prefix_len <= front:
+            raise ValueError(f"a prefix of {prefix_len} keys in pages for {front}")
         starts = [0]
         for n in q_lens:
             starts.append(starts[-1] + n)
