@@ -274,7 +274,7 @@ typedef struct {
  *     positions[t] * inv_freq[i] (inv_freq fp64 [rot_dim/2], radians a
  *     position), where pair i is (i, i + rot_dim/2), or (2i, 2i+1) with
  *     interleaved set; cos and sin are multiplied by rot_scale.  The angle is
- *     reduced in 64 bits, so far positions lose nothing;
+ *     good to 2^-26 of a turn at every position;
  *   - the rest passes through.
  * type is that of q, k and v, out_type that of the results: the same type, or
  * any type when type is WARP_T_F32.  Arithmetic is fp32, rounded once.

@@ -123,14 +123,18 @@ __global__ void __launch_bounds__(kRopeWarps * 32, kRopeCtas) rope_kernel(const 
             at1[n] = turned ? half + u * VEC : at0[n] + (units - rot_units) * VEC;
         }
     }
-    // The angle in turns, reduced in 64 bits: what is left is a fraction of a
-    // turn that fp32 holds to 2^-25, whatever the position.
+    // The angle in turns, its two products with their rounding errors kept and
+    // 1 / (2 pi) in two words, so that the fraction of a turn that is left is as
+    // exact at position 2^31 (some 2^28 turns, of which one product alone would lose
+    // 2^-25) as at 1: fp32 holds it to 2^-26.
     float *const cosines = turns_of[warp], *const sines = cosines + kRopeMaxPairs;
     if (half) {
         const double pos = (double)a.positions[t];
         for (int i = threadIdx.x % 32; i < half; i += 32) {
-            double turns = pos * a.inv_freq[i] * 0.15915494309189533577;
-            turns -= rint(turns);
+            constexpr double hi = 0.15915494309189533577, lo = -9.839338337591243e-18;
+            const double f = a.inv_freq[i], x = pos * f, x_low = fma(pos, f, -x);
+            const double whole = x * hi, low = fma(x, hi, -whole) + fma(x, lo, x_low * hi);
+            const double turns = (whole - rint(whole)) + low;
             float si, co;
             sincospif(2.0f * (float)turns, &si, &co);
             cosines[i] = co * a.rot_scale;
