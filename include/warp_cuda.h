@@ -342,8 +342,10 @@ WARP_API int warp_kv_slots(const int32_t *q_start, const int32_t *kv_len, int ba
  * is left out and reported by warp_attn_status.
  * scratch: warp_attn_scratch(d, c) bytes of device memory, 256-byte aligned,
  * free again when the stream has passed the call.  A token of no request is not
- * written.  No host synchronisation; capturable, once a call of the same type,
- * head_dim and kind of batch has been made outside (it sets the kernels up). */
+ * written.  q and out are 16-byte aligned, q's strides multiples of 16 bytes;
+ * tokens, batch or max_q 0 is no work.  No host synchronisation; capturable,
+ * once a call of the same type, head_dim and kind of batch has been made outside
+ * (it sets the kernels up). */
 typedef struct {
     int batch, tokens, q_heads, kv_heads, head_dim, type;
     const void *q;
@@ -366,9 +368,9 @@ WARP_API int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *
 
 /* What the kernels above left out since the last clear: WARP_OK, WARP_E_ARG
  * (a slot or page number outside the pages, a length over its bound or past
- * its row of pages) or
- * WARP_E_TIMEOUT (a bounded wait gave up; that launch's output is
- * incomplete).  Synchronises the device; clear = 1 resets. */
+ * its row of pages) or WARP_E_TIMEOUT (a bounded wait gave up; that launch's
+ * output is incomplete).  Synchronises the device, every stream of it; clear = 1 takes off
+ * what is reported. */
 WARP_API int warp_attn_status(int clear);
 
 /* ---- resident MoE layer ---------------------------------------------------------- */
