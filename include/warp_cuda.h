@@ -366,10 +366,136 @@ WARP_API int64_t warp_attn_scratch(const warp_attn_desc *d, const warp_kv_pages 
 WARP_API int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *c, void *scratch,
                                   void *stream);
 
+/* ---- drafted tokens: a step that checks several continuations at once ------------------
+ *
+ * A request's queries of one step are the nodes of a tree of drafted tokens.
+ * Node 0 is the last token that is certain; every other node continues its
+ * parent, which comes before it; it sees its ancestors and itself, and all keys
+ * before the tree.  The masks are rows of 64-bit words: bit m % 64 of word m / 64
+ * of a node's row says that it sees node m of its request.  A step is
+ *   warp_step_plan        pages for the new keys, slots, positions, masks
+ *   (per layer)           warp_kv_append, warp_tree_attention, the MoE layer
+ *   warp_pick_tokens      the token that follows each node
+ *   warp_tree_accept      the longest path of drafted tokens that were picked,
+ *                         and its keys moved to stand behind the certain ones */
+
+/* A step's plan from the requests' lengths, on the device.  With a pool (and
+ * held) it first sees to the rows of the page table: request b has held[b]
+ * pages there and needs ceil(kv_len[b] / page_size), pages_per_row at most.
+ * Surplus pages go back to the pool and their entries become -1; then missing
+ * ones are taken from it, in order of the requests.  What is given back last comes off
+ * first, so that requests that shrink and grow again get their pages back.
+ * A pool that runs empty leaves entries as they are and held[b] short, and
+ * warp_attn_status says so.
+ *   pool   int32 [1 + pool_pages]: how many pages are free, then their numbers
+ *          (the last of them comes off first)
+ * Then, for each of `tokens` tokens, positions and slots as warp_kv_slots makes
+ * them.  With parents (int32 [tokens]: the number of a node's parent among
+ * its request's, negative for none) the request's tokens are a tree's nodes:
+ * node i's position is base + kv_len[b] - n + its depth, and its row of masks is
+ * written to seen [tokens][ceil(max_q / 64)].  max_q bounds the nodes of a
+ * request; nodes past it, and a parent that does not come before its node (taken as
+ * none), are reported by warp_attn_status.
+ * pages, held and pool are read and written in place: order the calls of one pool.
+ * tokens 0 is no work but the pages'. */
+typedef struct {
+    int batch, tokens;
+    const int32_t *q_start, *kv_len;        /* [batch + 1], [batch] */
+    int32_t *pages;
+    int64_t pages_row;
+    int pages_per_row, page_size, base;
+    int32_t *held, *pool;                   /* both, or both NULL */
+    int64_t pool_pages;
+    const int32_t *parents;
+    uint64_t *seen;
+    int max_q;
+    int32_t *positions;
+    int64_t *slots;
+} warp_plan_desc;
+
+WARP_API int warp_step_plan(const warp_plan_desc *d, void *stream);
+
+/* warp_paged_attention where a request's queries are the nodes of a tree: the
+ * request's own keys before its last n (n its queries) are seen by all, and of
+ * the last n node i sees those of its row of masks, seen[t * seen_words ..].
+ * seen_words is at least ceil(max_q / 64).  d->causal is not used. */
+WARP_API int warp_tree_attention(const warp_attn_desc *d, const warp_kv_pages *c,
+                                 const uint64_t *seen, int64_t seen_words, void *scratch,
+                                 void *stream);
+
+/* Logits [tokens][vocab] adjusted, and the largest of each row.  Row t belongs to
+ * request b, q_start[b] <= t < q_start[b+1] (q_start NULL: to request t).  With c the
+ * number of times that token v is in the row's context,
+ *   x = logits[t][v];
+ *   where c > 0:  x = x > 0 ? x / repetition[b] : x * repetition[b];
+ *                 x = x - frequency[b] * c;  x = x - presence[b]
+ *   x = x + bias[v];  where the row's mask does not allow v: x = -inf
+ * each an fp32 operation rounded by itself; NULL leaves one out (1, 0, 0, 0, all
+ * allowed).  The context: the first history_len[b] tokens of history[b], and with
+ * seen the drafted tokens of the nodes that the row sees (as above; numbers
+ * outside the vocabulary count for nothing).  Masks: bit v % 32 of word v / 32 of
+ * the row's words.  picked[t]: the lowest v of the largest x; -1 where nothing is
+ * above -inf (a NaN never is).  out (NULL for none; may be logits) takes x,
+ * rounded to `type`.  max_q bounds the rows of a request; rows past it are left
+ * out and reported by warp_attn_status, rows of no request are not written. */
+typedef struct {
+    int tokens, batch, vocab, type, max_q;
+    const void *logits;
+    int64_t row;                            /* elements from row to row */
+    void *out;
+    int64_t out_row;
+    int32_t *picked;                        /* [tokens] */
+    const int32_t *q_start;
+    const int32_t *history, *history_len;
+    int64_t history_row;
+    int history_wide;                       /* places of a row, a bound on its length */
+    const float *repetition, *frequency, *presence;     /* [batch] each */
+    const float *bias;
+    int64_t bias_row;                       /* 0: one for all */
+    const uint32_t *allowed;
+    int64_t allowed_row;                    /* words from row to row; 0: one for all */
+    const int32_t *drafted;                 /* [tokens] */
+    const uint64_t *seen;
+    int64_t seen_words;
+} warp_pick_desc;
+
+WARP_API int warp_pick_tokens(const warp_pick_desc *d, void *stream);
+
+/* The drafted tokens checked.  Node i of a request agrees if it is node 0, or if
+ * drafted[i] is picked[p] of its parent p (the last node before it that it sees)
+ * and not negative.  Of the nodes whose whole path from node 0 agrees, the
+ * deepest (the first of equals) ends the accepted path.  Written for
+ * each request:
+ *   count   nodes of the path (0 for a request without nodes)
+ *   path    [max_q] their numbers, ascending, then -1
+ *   chosen  [max_q] what was picked behind each of them (the step's new
+ *           tokens), then -1
+ *   kv_after  kv_len - n + count
+ * and in each of n_caches caches (one a layer) the path's keys and values move to the
+ * places behind the request's keys before the tree, so that the first
+ * kv_after keys are the accepted ones.  The caches share the layout of c, whose own
+ * k and v are not used; theirs are k[i] and v[i] (host arrays).  kv_after is not
+ * kv_len. */
+typedef struct {
+    int batch, tokens, max_q;
+    const int32_t *drafted, *picked;        /* [tokens] */
+    const uint64_t *seen;
+    int64_t seen_words;
+    const int32_t *q_start, *kv_len;
+    const int32_t *pages;
+    int64_t pages_row;
+    int pages_per_row;
+    int32_t *count, *path, *chosen, *kv_after;
+} warp_accept_desc;
+
+WARP_API int warp_tree_accept(const warp_accept_desc *d, const warp_kv_pages *c, int n_caches,
+                              void *const *k, void *const *v, void *stream);
+
 /* What the kernels above left out since the last clear: WARP_OK, WARP_E_ARG
  * (a slot or page number outside the pages, a length over its bound or past
- * its row of pages) or WARP_E_TIMEOUT (a bounded wait gave up; that launch's
- * output is incomplete).  Synchronises the device, every stream of it; clear = 1 takes off
+ * its row of pages, a pool without a page left, a tree's node before its parent) or
+ * WARP_E_TIMEOUT (a bounded wait gave up; that launch's output is incomplete).
+ * Synchronises the device, every stream of it; clear = 1 takes off
  * what is reported. */
 WARP_API int warp_attn_status(int clear);
 

@@ -117,12 +117,13 @@ template <int D> struct ADLay {
     static constexpr int bytes = ring > join ? ring : join;
 };
 
-// PACKED: rows are those of all the batch's tokens, keys the shared prefix
+// kAttnPacked: rows are those of all the batch's tokens, keys the shared prefix
 // (one "request" for the batch).  Otherwise rows and keys of one request, with
 // the prefix's keys in front where there is one that is not computed apart.
-template <typename T, int D, bool PACKED>
+template <typename T, int D, AttnKind KIND>
 __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
     using Lay = ADLay<D>;
+    constexpr bool PACKED = KIND == kAttnPacked, TREE = KIND == kAttnTree;
     const int kvh = blockIdx.y;
     AttnReq rq;
     int part, row0, pre_tiles, own_tiles;
@@ -145,7 +146,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
     // own keys that the tile's last row sees
     const int last_row = min(rows, row0 + kADRows) - 1;
     int own_seen = rq.len;
-    if (!PACKED && a.causal)
+    if (KIND == kAttnOwn && a.causal)
         own_seen = max(0, min(rq.len, rq.len - rq.n + last_row / a.group + 1));
     own_tiles = PACKED ? 0 : (own_seen + kAttnTile - 1) / kAttnTile;
     // parts are counted by the request's keys, whatever a tile's rows see, so
@@ -219,7 +220,14 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
     }
     // own keys that the thread's two rows and the tile's first row see
     int see_lo = own_seen, see_hi = own_seen, see_first = own_seen;
-    if (!PACKED && a.causal) {
+    // a tree's masks for the two rows, and the key of its first node
+    const uint64_t *tree_lo = nullptr, *tree_hi = nullptr;
+    const int tree0 = rq.len - rq.n;
+    if (TREE) {
+        see_first = max(0, tree0);
+        tree_lo = a.seen + (rq.t0 + min(rlo, rows - 1) / a.group) * a.seen_words;
+        tree_hi = a.seen + (rq.t0 + min(rhi, rows - 1) / a.group) * a.seen_words;
+    } else if (!PACKED && a.causal) {
         see_first = rq.len - rq.n + row0 / a.group + 1;
         see_lo = rq.len - rq.n + rlo / a.group + 1;
         see_hi = rq.len - rq.n + rhi / a.group + 1;
@@ -253,14 +261,26 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
         const int j0 = (pre ? i : i - pre_tiles) * kAttnTile;
         const int lim_lo = pre ? n_pre - j0 : min(see_lo, own_seen) - j0;
         const int lim_hi = pre ? n_pre - j0 : min(see_hi, own_seen) - j0;
+        // a tile that some of the rows see only in part
+        const bool cut = !PACKED && !pre && min(own_seen, j0 + kAttnTile) > see_first;
+        // the tile's keys that the two rows see, where that is not all up to a limit
+        uint32_t bits_lo = 0, bits_hi = 0;
+        if (TREE && cut) {
+            const uint64_t held = low_bits(min(own_seen - j0, kAttnTile));
+            bits_lo = (uint32_t)(tree_sight(tree_lo, a.seen_words, j0 - tree0) & held);
+            bits_hi = (uint32_t)(tree_sight(tree_hi, a.seen_words, j0 - tree0) & held);
+        }
+        auto shown = [&](int j, int lim, uint32_t bits) {
+            return TREE && cut ? (bool)(bits >> j & 1) : j < lim;
+        };
         float mx_lo = -INFINITY, mx_hi = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const int j = t * 8 + (lane % 4) * 2 + e;
-                s[t][e] = j < lim_lo ? s[t][e] * a.scale_log2 : -INFINITY;
-                s[t][2 + e] = j < lim_hi ? s[t][2 + e] * a.scale_log2 : -INFINITY;
+                s[t][e] = shown(j, lim_lo, bits_lo) ? s[t][e] * a.scale_log2 : -INFINITY;
+                s[t][2 + e] = shown(j, lim_hi, bits_hi) ? s[t][2 + e] * a.scale_log2 : -INFINITY;
                 mx_lo = fmaxf(mx_lo, s[t][e]);
                 mx_hi = fmaxf(mx_hi, s[t][2 + e]);
             }
@@ -298,15 +318,16 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
             }
         uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]),
                          pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
-        // a tile that some of the rows see only in part
-        const bool cut = !PACKED && !pre && min(own_seen, j0 + kAttnTile) > see_first;
         uint32_t seen[4];
         if (cut) {
             const int c = (lane % 4) * 2;
-            seen[0] = pack2<T>(c < lim_lo, c + 1 < lim_lo);
-            seen[1] = pack2<T>(c < lim_hi, c + 1 < lim_hi);
-            seen[2] = pack2<T>(c + 8 < lim_lo, c + 9 < lim_lo);
-            seen[3] = pack2<T>(c + 8 < lim_hi, c + 9 < lim_hi);
+            auto two = [&](int j, int lim, uint32_t bits) {
+                return pack2<T>(shown(j, lim, bits), shown(j + 1, lim, bits));
+            };
+            seen[0] = two(c, lim_lo, bits_lo);
+            seen[1] = two(c, lim_hi, bits_hi);
+            seen[2] = two(c + 8, lim_lo, bits_lo);
+            seen[3] = two(c + 8, lim_hi, bits_hi);
         }
 #pragma unroll
         for (int d = 0; d < D / 16; d++) {
@@ -394,12 +415,12 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &a, uint8_t *smem) {
 // one's end is the end of all.
 // That one lets nothing start early: what follows the call may count on its
 // results as soon as it runs.
-template <typename T, int D, bool PACKED>
+template <typename T, int D, AttnKind KIND>
 __global__ void __launch_bounds__(kADWarps * 32, 2)
 attn_rows_kernel(const __grid_constant__ AttnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     if (a.more) pdl_trigger();
-    attn_rows<T, D, PACKED>(a, smem);
+    attn_rows<T, D, KIND>(a, smem);
     attn_wait_last();
 }
 
@@ -651,8 +672,8 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     return p;
 }
 
-static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
-    const char *who = "warp_paged_attention";
+static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c,
+                      const char *who = "warp_paged_attention") {
     WARP_ARG(d, "%s: NULL description", who);
     const int rc = kv_pages_check(c, who);
     if (rc) return rc;
@@ -679,13 +700,15 @@ static int attn_check(const warp_attn_desc *d, const warp_kv_pages *c) {
 template <typename T, int D>
 static int attn_launch(AttnArgs a, const AttnPlan &p, bool first, cudaStream_t st) {
     using Lay = ADLay<D>;
-    static std::atomic<uint64_t> done[2];
-    cudaError_t e = attn_smem(attn_rows_kernel<T, D, false>, Lay::bytes, done[0]);
-    if (e == cudaSuccess) e = attn_smem(attn_rows_kernel<T, D, true>, Lay::bytes, done[1]);
+    static std::atomic<uint64_t> done[3];
+    const bool tree = a.seen;
+    cudaError_t e = tree ? attn_smem(attn_rows_kernel<T, D, kAttnTree>, Lay::bytes, done[2])
+                         : attn_smem(attn_rows_kernel<T, D, kAttnOwn>, Lay::bytes, done[0]);
+    if (e == cudaSuccess) e = attn_smem(attn_rows_kernel<T, D, kAttnPacked>, Lay::bytes, done[1]);
     if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
     if (p.packed && !p.packed_wide) {
         a.more = 1;
-        e = attn_start(attn_rows_kernel<T, D, true>,
+        e = attn_start(attn_rows_kernel<T, D, kAttnPacked>,
                        dim3((unsigned)(up((int64_t)a.tokens * a.group, kADRows) * p.prefix_parts),
                             a.kv_heads, 1), kADWarps * 32, Lay::bytes, st, first, a);
         if (e != cudaSuccess) return cuda_fail(e, "attn_rows_kernel (prefix)");
@@ -694,9 +717,11 @@ static int attn_launch(AttnArgs a, const AttnPlan &p, bool first, cudaStream_t s
     }
     if (p.small_tiles) {
         a.more = p.join;
-        e = attn_start(attn_rows_kernel<T, D, false>,
-                       dim3(p.small_tiles * p.parts, a.kv_heads, a.batch), kADWarps * 32,
-                       Lay::bytes, st, first, a);
+        const dim3 grid(p.small_tiles * p.parts, a.kv_heads, a.batch);
+        e = tree ? attn_start(attn_rows_kernel<T, D, kAttnTree>, grid, kADWarps * 32, Lay::bytes,
+                              st, first, a)
+                 : attn_start(attn_rows_kernel<T, D, kAttnOwn>, grid, kADWarps * 32, Lay::bytes,
+                              st, first, a);
         if (e != cudaSuccess) return cuda_fail(e, "attn_rows_kernel");
         count_launch();
         first = false;
@@ -726,22 +751,22 @@ extern "C" int64_t warp_attn_scratch(const warp_attn_desc *d, const warp_kv_page
     return p.o_bytes + p.ml_bytes;
 }
 
-extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *c, void *scratch,
-                                    void *stream) {
-    int rc = warp::attn_check(d, c);
-    if (rc) return rc;
-    if (d->tokens == 0 || d->batch == 0 || d->max_q == 0) return WARP_OK;
-    const char *who = "warp_paged_attention";
+namespace warp {
+
+// `seen`: the masks of a tree of drafted tokens (NULL for none).
+static int attn_run(const warp_attn_desc *d, const warp_kv_pages *c, const uint64_t *seen,
+                    int64_t seen_words, void *scratch, const char *who, cudaStream_t st) {
+    int rc;
     WARP_ARG(d->q && d->out && d->q_start && d->kv_len, "%s: NULL pointer", who);
     WARP_ARG(d->pages || d->pages_per_row == 0, "%s: NULL page table", who);
     WARP_ARG(d->prefix_pages || d->prefix_len == 0, "%s: NULL prefix page table", who);
     WARP_ARG(((uintptr_t)d->q & 15) == 0 && ((uintptr_t)d->out & 15) == 0 && d->q_token % 8 == 0 &&
                  d->q_head % 8 == 0,
              "%s: queries and results must be 16-byte aligned, strides multiples of 16 bytes", who);
-    const warp::AttnPlan p = warp::attn_plan(d, c);
+    const AttnPlan p = attn_plan(d, c);
     WARP_ARG(p.o_bytes + p.ml_bytes == 0 || (scratch && ((uintptr_t)scratch & 255) == 0),
              "%s: scratch must be 256-byte aligned", who);
-    warp::AttnArgs a = {};
+    AttnArgs a = {};
     a.q = d->q, a.kp = c->k, a.vp = c->v, a.out = d->out;
     a.q_token = d->q_token, a.q_head = d->q_head;
     a.k_page = c->k_page, a.k_slot = c->k_slot, a.k_head = c->k_head;
@@ -761,26 +786,51 @@ extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages
     a.rows_small = p.rows_small;
     a.split_tiles = p.each, a.wide_each = p.wide_each, a.wide_parts = p.wide_parts;
     a.prefix_split_tiles = a.prefix_wide_each = p.prefix_each;
-    a.by_group = warp::attn_div(a.group);
-    a.by_wide_parts = warp::attn_div(p.wide_parts), a.by_wide_each = warp::attn_div(p.wide_each);
-    a.by_prefix_parts = warp::attn_div(p.prefix_parts);
-    a.by_prefix_each = warp::attn_div(p.prefix_each);
-    rc = warp::attn_err_word(&a.err);
+    a.by_group = attn_div(a.group);
+    a.by_wide_parts = attn_div(p.wide_parts), a.by_wide_each = attn_div(p.wide_each);
+    a.by_prefix_parts = attn_div(p.prefix_parts);
+    a.by_prefix_each = attn_div(p.prefix_each);
+    a.seen = seen, a.seen_words = seen_words;
+    rc = attn_err_word(&a.err);
     if (rc) return rc;
-    cudaStream_t st = (cudaStream_t)stream;
     bool first = true;
     if (p.packed_wide) {
         a.more = 1;
-        rc = warp::attn_umma(a, c, true, first, st), first = false;
+        rc = attn_umma(a, c, kAttnPacked, first, st), first = false;
     }
     if (!rc && p.wide_parts) {
         a.more = p.small_tiles || p.join;
-        rc = warp::attn_umma(a, c, false, first, st), first = false;
+        rc = attn_umma(a, c, seen ? kAttnTree : kAttnOwn, first, st), first = false;
     }
     if (rc) return rc;
     if (d->type == WARP_T_F16)
-        return d->head_dim == 64 ? warp::attn_launch<__half, 64>(a, p, first, st)
-                                 : warp::attn_launch<__half, 128>(a, p, first, st);
-    return d->head_dim == 64 ? warp::attn_launch<__nv_bfloat16, 64>(a, p, first, st)
-                             : warp::attn_launch<__nv_bfloat16, 128>(a, p, first, st);
+        return d->head_dim == 64 ? attn_launch<__half, 64>(a, p, first, st)
+                                 : attn_launch<__half, 128>(a, p, first, st);
+    return d->head_dim == 64 ? attn_launch<__nv_bfloat16, 64>(a, p, first, st)
+                             : attn_launch<__nv_bfloat16, 128>(a, p, first, st);
+}
+
+}  // namespace warp
+
+extern "C" int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *c, void *scratch,
+                                    void *stream) {
+    const int rc = warp::attn_check(d, c);
+    if (rc) return rc;
+    if (d->tokens == 0 || d->batch == 0 || d->max_q == 0) return WARP_OK;
+    return warp::attn_run(d, c, nullptr, 0, scratch, "warp_paged_attention", (cudaStream_t)stream);
+}
+
+extern "C" int warp_tree_attention(const warp_attn_desc *d, const warp_kv_pages *c,
+                                   const uint64_t *seen, int64_t seen_words, void *scratch,
+                                   void *stream) {
+    const char *who = "warp_tree_attention";
+    const int rc = warp::attn_check(d, c, who);
+    if (rc) return rc;
+    if (d->tokens == 0 || d->batch == 0 || d->max_q == 0) return WARP_OK;
+    WARP_ARG(seen && ((uintptr_t)seen & 7) == 0, "%s: the masks are NULL or not 8-byte aligned", who);
+    const int nodes = d->max_q < d->tokens ? d->max_q : d->tokens;
+    WARP_ARG(seen_words >= (nodes + 63) / 64 && seen_words < (1 << 24),
+             "%s: %lld words of 64 bits for masks of up to %d nodes", who, (long long)seen_words,
+             nodes);
+    return warp::attn_run(d, c, seen, seen_words, scratch, who, (cudaStream_t)stream);
 }

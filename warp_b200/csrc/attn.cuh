@@ -12,6 +12,8 @@ constexpr unsigned kAttnBadSlot = 1u;     // a slot outside the pages
 constexpr unsigned kAttnBadPage = 2u;     // a page number outside the pages
 constexpr unsigned kAttnBadLen = 4u;      // a length over its host bound
 constexpr unsigned kAttnTimeout = 8u;     // a bounded wait gave up
+constexpr unsigned kAttnNoPage = 16u;     // the pool of pages is empty
+constexpr unsigned kAttnBadTree = 32u;    // a parent that does not come before its node
 
 // Device address of the error word (one per device).
 int attn_err_word(unsigned **out);
@@ -75,7 +77,15 @@ struct AttnArgs {
     int prefix_wide_each;                   // of a part, and parts at most
     // divisions of attn_umma_kernel: by group, by parts, by tiles of a part
     AttnDiv by_group, by_wide_parts, by_prefix_parts, by_wide_each, by_prefix_each;
+    // Trees: the nodes that token t sees, bit m of seen[t * seen_words + m / 64] for node m.
+    const uint64_t *seen;
+    int64_t seen_words;
 };
+
+// What a kernel's rows and keys are: those of one request (causal or not), all the
+// batch's rows and the shared prefix, or those of one request whose queries are the
+// nodes of a tree.
+enum AttnKind { kAttnOwn, kAttnPacked, kAttnTree };
 
 // Request b as the host's bounds leave it: its first token, its queries and
 // its own keys.
@@ -100,6 +110,22 @@ __device__ __forceinline__ int attn_page(const AttnArgs &a, const int32_t *table
     if ((unsigned)p < (unsigned)a.n_pages) return p;
     atomicOr(a.err, kAttnBadPage);
     return 0;
+}
+
+// The keys from node number `from` on that a node sees, one a bit: keys before the
+// tree (negative numbers) are seen by all.  `words` is the node's row of the masks.
+__device__ __forceinline__ uint64_t tree_sight(const uint64_t *words, int64_t n, int from) {
+    if (from <= -64) return ~0ull;
+    const int w = max(from, 0) >> 6;
+    const uint64_t lo = w < n ? words[w] : 0;
+    if (from < 0) return lo << -from | ((1ull << -from) - 1);
+    const int s = from & 63;
+    if (!s) return lo;
+    return lo >> s | (w + 1 < n ? words[w + 1] << (64 - s) : 0);
+}
+// The first `n` bits.
+__device__ __forceinline__ uint64_t low_bits(int n) {
+    return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 
 // Keys come in tiles of kAttnTile; the prefix's last tile and a request's last
@@ -143,9 +169,9 @@ template <> __host__ __device__ constexpr float attn_lift<__half>(float slack) {
     return 15.f - slack;
 }
 
-// The tensor-core kernel: the requests with many rows, or (packed) the shared
+// The tensor-core kernel: the requests with many rows, or (kAttnPacked) the shared
 // prefix for all rows of the batch.
-int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,
+int attn_umma(const AttnArgs &a, const warp_kv_pages *c, AttnKind kind, bool first,
               cudaStream_t st);
 
 // The wait for the kernel before this one, by one block, the last to start: a

@@ -327,11 +327,12 @@ __device__ __forceinline__ void weights(const float (&s)[N], uint64_t c2, uint64
 
 }  // namespace
 
-// PACKED: rows are those of all the batch's tokens, keys the shared prefix.
-template <typename T, int D, bool PACKED>
+// kAttnPacked: rows are those of all the batch's tokens, keys the shared prefix.
+template <typename T, int D, AttnKind KIND>
 __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensorMap &kmap,
                                                const CUtensorMap &vmap, uint8_t *basep) {
     using L = Lay<D>;
+    constexpr bool PACKED = KIND == kAttnPacked, TREE = KIND == kAttnTree;
     constexpr int NS = L::stages, KEYS = L::keys;
     const int kvh = blockIdx.y;
     const AttnReq rq = PACKED ? AttnReq{0, a.tokens, 0} : attn_req(a, blockIdx.z);
@@ -353,7 +354,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         max(1, (all_tiles + each - 1) / (PACKED ? a.by_prefix_each : a.by_wide_each));
     if (part >= parts) return;
     // own keys that row r sees
-    const bool causal = !PACKED && a.causal;
+    const bool causal = KIND == kAttnOwn && a.causal;
     auto sees = [&](int r) {
         return causal ? max(0, min(rq.len, rq.len - rq.n + r / a.by_group + 1)) : rq.len;
     };
@@ -369,7 +370,10 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     // row0's token and its head in the group; row0 + x is then token
     // tok0 + (rem0 + x) / group
     const int tok0 = row0 / a.by_group, rem0 = row0 - tok0 * a.group;
-    const int see_first = PACKED ? 0 : causal ? rq.len - rq.n + tok0 + 1 : rq.len;
+    // the first key that only some rows see
+    const int tree0 = rq.len - rq.n;                    // key of a tree's first node
+    const bool some = causal || TREE;
+    const int see_first = PACKED ? 0 : TREE ? tree0 : causal ? tree0 + tok0 + 1 : rq.len;
 
     const uint32_t base = smem_u32(basep);
     const uint32_t bars = base + L::bars;
@@ -569,17 +573,26 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         // Steps that are not full, and those with keys that only some rows see: what
         // lies behind the keys may be anything, and a weight of zero does not hide a
         // NaN.  They are the last ones, and the prefix's last.
-        const int whole = min(causal ? max(see_first, 0) : own_seen, own_seen) / KEYS;
+        const int whole = min(some ? max(see_first, 0) : own_seen, own_seen) / KEYS;
         const int masked_from = pre_tiles + whole - first;
         const int masked_pre = n_pre % KEYS ? pre_tiles - 1 - first : -1;
+        // the nodes that this row's sees, where it is one of a tree's
+        const uint64_t *const sight =
+            TREE ? a.seen + (int64_t)(rq.t0 + min(row, rows - 1) / a.by_group) * a.seen_words
+                 : nullptr;
         for (int j = 0; j < mine; j++) {
             const bool masked = j >= masked_from || j == masked_pre;
             int lim = 0;                    // keys of the step that this row sees
+            uint64_t bits = 0;              // and of this thread's half, one a bit
             if (__builtin_expect(masked, 0)) {
                 const bool pre = first + j < pre_tiles;
                 const int k0 = (first + j - (pre ? 0 : pre_tiles)) * KEYS;
                 const int held = (pre ? n_pre : own_seen) - k0;
                 lim = pre ? held : min(held, see - k0);
+                if (TREE) {
+                    bits = low_bits(held - h * L::cols);
+                    if (!pre) bits &= tree_sight(sight, a.seen_words, k0 + h * L::cols - tree0);
+                }
                 const int n = 2 * j + 1;        // the n-th tile in the ring
                 wait(kv_full + 8 * (n % NS), (n / NS) & 1, fail);
                 // two threads a key
@@ -588,7 +601,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 auto at = [&](int x) { return v + (x / 128) * L::kv_half + x % 128; };
                 if (key >= held) {
                     for (int x = x0; x < x1; x += 16) *(uint4 *)at(x) = make_uint4(0, 0, 0, 0);
-                } else if (causal && !pre && k0 + key >= see_first) {
+                } else if (some && !pre && k0 + key >= see_first) {
                     constexpr uint32_t E = fmt16<T>() ? 0x7f80u : 0x7c00u;
                     bool bad = false;
                     for (int x = x0; x < x1; x += 16) {
@@ -621,7 +634,8 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 if (__builtin_expect(masked, 0)) {
                     lim -= h * L::cols;
 #pragma unroll
-                    for (int x = 0; x < L::cols; x++) s[x] = x < lim ? s[x] : -INFINITY;
+                    for (int x = 0; x < L::cols; x++)
+                        s[x] = (TREE ? (bool)(bits >> x & 1) : x < lim) ? s[x] : -INFINITY;
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -677,7 +691,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                                      a.q_heads;
             const int64_t out_row = (int64_t)(rq.t0 + tok0) * a.q_heads + kvh * a.group;
             __threadfence_block();
-            const bool mend = *dirty && causal;
+            const bool mend = *dirty && some;
             uint8_t *const stage = basep + t * L::q_tile;
             tile_sync(t);                   // the last maxima are read
             swap[h * kRows + r] = l.x + l.y;
@@ -704,6 +718,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                         const int end = min(see, max(0, first + each - pre_tiles) * KEYS);
                         for (int k = max(max(see_first, 0), (first - pre_tiles) * KEYS); k < end;
                              k++) {
+                            if (TREE && !(tree_sight(sight, a.seen_words, k - tree0) & 1)) continue;
                             const int page =
                                 attn_page(a, a.pages + (int64_t)blockIdx.z * a.pages_row, k);
                             const T *v = (const T *)a.vp + (int64_t)page * a.v_page +
@@ -765,13 +780,13 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
 }
 
 // See attn_rows_kernel.
-template <typename T, int D, bool PACKED>
+template <typename T, int D, AttnKind KIND>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_umma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                  const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ __align__(1024) uint8_t shared[];
     if (a.more) pdl_trigger();
-    attn_wide_rows<T, D, PACKED>(a, kmap, vmap, shared);
+    attn_wide_rows<T, D, KIND>(a, kmap, vmap, shared);
     attn_wait_last();
 }
 
@@ -826,39 +841,43 @@ static int page_map(CUtensorMap *m, const warp_kv_pages *c, void *ptr, int64_t p
     return WARP_OK;
 }
 
-template <typename T, int D, bool PACKED>
+template <typename T, int D, AttnKind KIND>
 static int umma_launch(const AttnArgs &a, const CUtensorMap &km, const CUtensorMap &vm, int pairs,
                        int parts, bool first, cudaStream_t st) {
     static std::atomic<uint64_t> done;
-    cudaError_t e = attn_smem(attn_umma_kernel<T, D, PACKED>, Lay<D>::bytes, done);
+    cudaError_t e = attn_smem(attn_umma_kernel<T, D, KIND>, Lay<D>::bytes, done);
     if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
-    e = attn_start(attn_umma_kernel<T, D, PACKED>,
-                   dim3((unsigned)pairs * parts, a.kv_heads, PACKED ? 1 : a.batch), kThreads,
-                   Lay<D>::bytes, st, first, a, km, vm);
+    e = attn_start(attn_umma_kernel<T, D, KIND>,
+                   dim3((unsigned)pairs * parts, a.kv_heads, KIND == kAttnPacked ? 1 : a.batch),
+                   kThreads, Lay<D>::bytes, st, first, a, km, vm);
     if (e != cudaSuccess) return cuda_fail(e, "attn_umma_kernel");
     count_launch();
     return WARP_OK;
 }
 
-int attn_umma(const AttnArgs &a, const warp_kv_pages *c, bool packed, bool first,
+template <AttnKind KIND>
+static int umma_typed(const AttnArgs &a, const warp_kv_pages *c, const CUtensorMap &km,
+                      const CUtensorMap &vm, int pairs, int parts, bool first, cudaStream_t st) {
+    const bool h = c->type == WARP_T_F16, d64 = c->head_dim == 64;
+    return h ? d64 ? umma_launch<__half, 64, KIND>(a, km, vm, pairs, parts, first, st)
+                   : umma_launch<__half, 128, KIND>(a, km, vm, pairs, parts, first, st)
+             : d64 ? umma_launch<__nv_bfloat16, 64, KIND>(a, km, vm, pairs, parts, first, st)
+                   : umma_launch<__nv_bfloat16, 128, KIND>(a, km, vm, pairs, parts, first, st);
+}
+
+int attn_umma(const AttnArgs &a, const warp_kv_pages *c, AttnKind kind, bool first,
               cudaStream_t st) {
     CUtensorMap km, vm;
     int rc = page_map(&km, c, c->k, c->k_page, c->k_slot, c->k_head);
     if (!rc) rc = page_map(&vm, c, c->v, c->v_page, c->v_slot, c->v_head);
     if (rc) return rc;
+    const bool packed = kind == kAttnPacked;
     const int64_t rows = (int64_t)(packed ? a.tokens : a.max_q) * a.group;
     const int pairs = (int)((rows + 2 * kRows - 1) / (2 * kRows));
     const int parts = packed ? a.prefix_parts : a.wide_parts;
-    const bool h = c->type == WARP_T_F16, d64 = c->head_dim == 64;
-    if (packed)
-        return h ? d64 ? umma_launch<__half, 64, true>(a, km, vm, pairs, parts, first, st)
-                       : umma_launch<__half, 128, true>(a, km, vm, pairs, parts, first, st)
-                 : d64 ? umma_launch<__nv_bfloat16, 64, true>(a, km, vm, pairs, parts, first, st)
-                       : umma_launch<__nv_bfloat16, 128, true>(a, km, vm, pairs, parts, first, st);
-    return h ? d64 ? umma_launch<__half, 64, false>(a, km, vm, pairs, parts, first, st)
-                   : umma_launch<__half, 128, false>(a, km, vm, pairs, parts, first, st)
-             : d64 ? umma_launch<__nv_bfloat16, 64, false>(a, km, vm, pairs, parts, first, st)
-                   : umma_launch<__nv_bfloat16, 128, false>(a, km, vm, pairs, parts, first, st);
+    return packed              ? umma_typed<kAttnPacked>(a, c, km, vm, pairs, parts, first, st)
+           : kind == kAttnTree ? umma_typed<kAttnTree>(a, c, km, vm, pairs, parts, first, st)
+                               : umma_typed<kAttnOwn>(a, c, km, vm, pairs, parts, first, st);
 }
 
 }  // namespace warp

@@ -480,9 +480,11 @@ extern "C" int warp_attn_status(int clear) {
         return WARP_E_TIMEOUT;
     }
     if (v) {
-        warp::set_error("attention:%s%s%s",
+        warp::set_error("attention:%s%s%s%s%s",
                         v & warp::kAttnBadSlot ? " a slot outside the pages;" : "",
                         v & warp::kAttnBadPage ? " a page number outside the pages;" : "",
+                        v & warp::kAttnNoPage ? " no page left in the pool;" : "",
+                        v & warp::kAttnBadTree ? " a parent behind its node;" : "",
                         v & warp::kAttnBadLen ? " a length over its bound" : "");
         return WARP_E_ARG;
     }

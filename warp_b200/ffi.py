@@ -50,6 +50,10 @@ SIGNATURES = {
     "warp_kv_slots": (I, [P, P, I, I, P, I64, I, I, I, P, P, P]),
     "warp_attn_scratch": (I64, [P, P]),
     "warp_paged_attention": (I, [P, P, P, P]),
+    "warp_step_plan": (I, [P, P]),
+    "warp_tree_attention": (I, [P, P, P, I64, P, P]),
+    "warp_pick_tokens": (I, [P, P]),
+    "warp_tree_accept": (I, [P, P, I, P, P, P]),
     "warp_attn_status": (I, [I]),
     "warp_moe_layer_create": (I, [P, I, P]),
     "warp_moe_layer_destroy": (None, [P]),
@@ -130,12 +134,46 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
-# The three descriptions above as struct formats (native alignment), for
+class PlanDesc(ctypes.Structure):
+    """warp_plan_desc (include/warp_cuda.h)."""
+    _fields_ = [
+        ("batch", I), ("tokens", I), ("q_start", P), ("kv_len", P), ("pages", P),
+        ("pages_row", I64), ("pages_per_row", I), ("page_size", I), ("base", I),
+        ("held", P), ("pool", P), ("pool_pages", I64), ("parents", P), ("seen", P),
+        ("max_q", I), ("positions", P), ("slots", P),
+    ]
+
+
+class PickDesc(ctypes.Structure):
+    """warp_pick_desc (include/warp_cuda.h)."""
+    _fields_ = [
+        ("tokens", I), ("batch", I), ("vocab", I), ("type", I), ("max_q", I),
+        ("logits", P), ("row", I64), ("out", P), ("out_row", I64), ("picked", P),
+        ("q_start", P), ("history", P), ("history_len", P), ("history_row", I64),
+        ("history_wide", I), ("repetition", P), ("frequency", P), ("presence", P),
+        ("bias", P), ("bias_row", I64), ("allowed", P), ("allowed_row", I64),
+        ("drafted", P), ("seen", P), ("seen_words", I64),
+    ]
+
+
+class AcceptDesc(ctypes.Structure):
+    """warp_accept_desc (include/warp_cuda.h)."""
+    _fields_ = [
+        ("batch", I), ("tokens", I), ("max_q", I), ("drafted", P), ("picked", P), ("seen", P),
+        ("seen_words", I64), ("q_start", P), ("kv_len", P), ("pages", P), ("pages_row", I64),
+        ("pages_per_row", I), ("count", P), ("path", P), ("chosen", P), ("kv_after", P),
+    ]
+
+
+# The descriptions above as struct formats (native alignment), for
 # callers that fill one per call: packing is several times cheaper than setting
 # a Structure's fields one by one.
 KV_PAGES = struct.Struct("@PP4iq6q")
 ROPE_DESC = struct.Struct("@6iPPP6qPPPPfPiifP")
 ATTN_DESC = struct.Struct("@6iPqqPPPPqiiiifPi0P")
+PLAN_DESC = struct.Struct("@2iPPPq3iPPqPPiPP")
+PICK_DESC = struct.Struct("@5iPqPqPPPPqiPPPPqPqPPq")
+ACCEPT_DESC = struct.Struct("@3iPPPqPPPqiPPPP")
 
 
 _lib = None

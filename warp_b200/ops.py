@@ -21,11 +21,20 @@ family on the CPU, is served by operators of its own shape:
     kv_append       qk_norm_rope with keys and values written to the pages
     paged_attention attention over the pages, with or without a shared prefix
 
+and a step that checks drafted tokens, several continuations of a request at once:
+
+    page_pool       the pages that are free, for step_plan
+    step_plan       pages, slots, positions and tree masks of a step, on the device
+    tree_attention  paged_attention where a request's queries are the nodes of a tree
+    pick_tokens     penalties, biases and masks on logits, and the largest of each row
+    tree_accept     the path of drafted tokens that were picked, its keys put in order
+
 Every tensor argument must already be on the CUDA device; calls are
 asynchronous on torch's current stream.  A failure raises ffi.WarpError.
 """
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -402,6 +411,12 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
     (int32 [n]), before their own.  A query that sees nothing gets zeros; a
     token of no request is not written.  scale: 1/sqrt(D) by default.  Returns
     [T][Hq][D] in q's dtype."""
+    return _attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale, causal,
+                      prefix_pages, prefix_len, out)
+
+
+def _attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale, causal,
+               prefix_pages, prefix_len, out, seen=None):
     dev = _device(q)
     c = _pages_pack(k_pages, v_pages, dev)
     B, row, wide = _batch(q_start, kv_len, pages, dev)
@@ -424,6 +439,8 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
         if not _vec_ok(prefix_pages, prefix_pages.numel(), torch.int32, dev):
             raise ValueError("prefix_pages must be contiguous int32 [n]")
         pp = prefix_pages.data_ptr()
+    if seen is not None:
+        words = _seen_ok(seen, T, max_q, dev)
     d = ffi.ATTN_DESC.pack(
         B, T, Hq, k_pages.shape[2], D, _TYPES[dt], qp, qt, qh,
         out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), row, wide, max_q,
@@ -435,8 +452,244 @@ def paged_attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, 
     # from torch's allocator: ordered by the stream, and private to a graph
     # where one is being captured
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    ffi.check(lib.warp_paged_attention(d, c, scratch.data_ptr() if need else None, _stream()))
+    at = scratch.data_ptr() if need else None
+    if seen is None:
+        ffi.check(lib.warp_paged_attention(d, c, at, _stream()))
+    else:
+        ffi.check(lib.warp_tree_attention(d, c, seen.data_ptr(), words, at, _stream()))
     return out
+
+
+def page_pool(pages, device="cuda"):
+    """A pool with all of `pages` pages free, for step_plan: int32 [1 + pages], how
+    many are free and their numbers, of which page 0 comes off first."""
+    pool = torch.arange(pages, -1, -1, dtype=torch.int32, device=device)
+    pool[1:] = pool[1:].clone()
+    return pool
+
+
+def step_plan(q_start, kv_len, pages, page_size, tokens, base=0, held=None, pool=None,
+              parents=None, max_q=0):
+    """A step's plan from its requests' lengths, on the device (warp_step_plan):
+    (positions int32 [T], slots int64 [T]) of its tokens, as kv_slots makes them.
+
+    q_start int32 [B+1], kv_len int32 [B] own keys with the new ones counted,
+    pages int32 [B][n].  With held (int32 [B], pages that each row has) and pool
+    (page_pool) the rows first give back the pages that kv_len does not need and
+    take those that it does, in place; a length of 0 gives all back.  A pool that
+    runs empty leaves held short and the keys without a slot, and attn_status raises.
+
+    With parents (int32 [T]: a node's parent among its request's tokens, -1 for
+    the first) each request's tokens are the nodes of a tree, max_q at most: their
+    positions go by depth, and a third result, seen int64 [T][ceil(max_q / 64)], has
+    bit m of a node's words set for each node m that it sees: its ancestors
+    and itself."""
+    dev = _device(kv_len)
+    B, row, wide = _batch(q_start, kv_len, pages, dev)
+    hp = pp = np = up = sp = 0
+    if held is not None or pool is not None:
+        if held is None or pool is None:
+            raise ValueError("held and pool go together")
+        if not _vec_ok(held, B, torch.int32, dev):
+            raise ValueError("held must be contiguous int32 [batch]")
+        np = pool.numel() - 1
+        if not _vec_ok(pool, np + 1, torch.int32, dev) or np < 0:
+            raise ValueError("pool must be contiguous int32 [1 + pages]")
+        hp, pp = held.data_ptr(), pool.data_ptr()
+    seen = None
+    if parents is not None:
+        if not _vec_ok(parents, tokens, torch.int32, dev):
+            raise ValueError("parents must be contiguous int32 [tokens]")
+        if max_q < 1:
+            raise ValueError("a tree's nodes need their bound max_q")
+        seen = torch.empty(tokens, (max_q + 63) // 64, dtype=torch.int64, device=kv_len.device)
+        up, sp = parents.data_ptr(), seen.data_ptr()
+    positions = torch.empty(tokens, dtype=torch.int32, device=kv_len.device)
+    slots = torch.empty(tokens, dtype=torch.int64, device=kv_len.device)
+    d = ffi.PLAN_DESC.pack(B, tokens, q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), row,
+                           wide, page_size, base, hp, pp, np, up, sp, max_q, positions.data_ptr(),
+                           slots.data_ptr())
+    ffi.check(ffi.load().warp_step_plan(d, _stream()))
+    return (positions, slots) if parents is None else (positions, slots, seen)
+
+
+def _seen_ok(seen, T, max_q, dev):
+    """Words of a row of masks [T][words]."""
+    if seen.get_device() != dev:
+        _elsewhere(seen)
+    if seen.dim() != 2 or seen.shape[0] != T or seen.dtype is not torch.int64 or \
+            not seen.is_contiguous() or seen.shape[1] * 64 < min(max_q, T):
+        raise ValueError("seen must be contiguous int64 [tokens][words] with a bit for each of "
+                         "max_q nodes")
+    return seen.shape[1]
+
+
+def tree_attention(q, k_pages, v_pages, pages, kv_len, q_start, seen, max_q, max_kv, scale=None,
+                   prefix_pages=None, prefix_len=0, out=None):
+    """paged_attention where a request's queries are the nodes of a tree
+    (warp_tree_attention): its own keys before its last n, one a query, are
+    seen by all its queries, and of the last n query i sees those whose bits
+    are set in its row of seen (step_plan's).  A query that sees nothing gets
+    zeros."""
+    if seen is None:
+        raise ValueError("a tree needs its masks")
+    return _attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale, False,
+                      prefix_pages, prefix_len, out, seen)
+
+
+def _table(x, name, rows, wide, dtype, dev):
+    """Row stride of [rows][wide], or of [wide] for all rows: 0."""
+    if x.get_device() != dev:
+        _elsewhere(x)
+    shape, strides = x.shape, x.stride()
+    if len(shape) not in (1, 2) or x.dtype is not dtype or shape[-1] < wide or \
+            (len(shape) == 2 and shape[0] != rows) or (strides[-1] != 1 and shape[-1] > 1):
+        raise ValueError(f"{name} must be {dtype} [rows][{wide}] or [{wide}], rows contiguous")
+    return strides[0] if len(shape) == 2 and rows > 1 else 0
+
+
+def pick_tokens(logits, q_start=None, max_q=1, history=None, history_len=None, repetition=None,
+                frequency=None, presence=None, bias=None, allowed=None, drafted=None, seen=None,
+                out=None):
+    """The token of the largest adjusted logit of each row, int32 [T]; -1 where
+    none is above -inf (warp_pick_tokens).
+
+    logits [T][V] fp32, fp16 or bf16, rows contiguous; row t belongs to request t,
+    or to the one with q_start[b] <= t < q_start[b+1] (int32 [B+1]; max_q rows a
+    request at most).  With c the number of times that a token is in the row's
+    context,
+
+        x > 0 ? x / repetition : x * repetition, then less frequency * c and
+        presence, where c > 0 (float32 [B] each); plus bias (float32 [V] or
+        [B][V]); -inf where allowed (int32 [T][ceil(V / 32)] or [ceil(V / 32)],
+        a bit a token, the lowest first) has no bit.
+
+    The context: the first history_len[b] (int32 [B]) tokens of history[b] (int32
+    [B][H]), and with drafted (int32 [T]) and seen (step_plan's) the drafted
+    tokens of the nodes that the row's node sees.  out, of logits' shape and
+    dtype, takes the adjusted logits; it may be logits itself.  A row of no
+    request is not written."""
+    dev = _device(logits)
+    if logits.get_device() != dev:
+        _elsewhere(logits)
+    dt = logits.dtype
+    if logits.dim() != 2 or dt not in _TYPES or logits.shape[1] < 1 or \
+            (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [rows][vocabulary], fp32, fp16 or bf16, rows contiguous")
+    T, V = logits.shape
+    row = logits.stride(0) if T > 1 else 0
+    B = T
+    qp = op = orow = hp = lp = hrow = wide = bp = brow = ap = arow = dp = sp = words = 0
+    if q_start is not None:
+        B = q_start.numel() - 1
+        if B < 0 or not _vec_ok(q_start, B + 1, torch.int32, dev):
+            raise ValueError("q_start must be contiguous int32 [batch + 1]")
+        qp = q_start.data_ptr()
+    if out is not None:
+        if out.get_device() != dev:
+            _elsewhere(out)
+        if out.shape != logits.shape or out.dtype is not dt or (out.stride(1) != 1 and V > 1):
+            raise ValueError("out must be of logits' shape and dtype, rows contiguous")
+        op, orow = out.data_ptr(), out.stride(0) if T > 1 else 0
+        if T > 1 and orow < V:
+            raise ValueError("rows of out overlap")
+    if history is not None or history_len is not None:
+        if history is None or history_len is None:
+            raise ValueError("history and history_len go together")
+        if not _vec_ok(history_len, B, torch.int32, dev):
+            raise ValueError("history_len must be contiguous int32 [batch]")
+        if history.dim() != 2:
+            raise ValueError("history must be int32 [batch][places]")
+        hrow = _table(history, "history", B, 0, torch.int32, dev)
+        hp, lp, wide = history.data_ptr(), history_len.data_ptr(), history.shape[1]
+    if drafted is not None or seen is not None:
+        if drafted is None or seen is None or q_start is None:
+            raise ValueError("drafted, seen and q_start go together")
+        if not _vec_ok(drafted, T, torch.int32, dev):
+            raise ValueError("drafted must be contiguous int32 [rows]")
+        words = _seen_ok(seen, T, max_q, dev)
+        dp, sp = drafted.data_ptr(), seen.data_ptr()
+    scalars = []
+    for x in (repetition, frequency, presence):
+        if x is not None and not _vec_ok(x, B, torch.float32, dev):
+            raise ValueError("repetition, frequency and presence must be contiguous float32 [batch]")
+        scalars.append(0 if x is None else x.data_ptr())
+    if bias is not None:
+        brow = _table(bias, "bias", B, V, torch.float32, dev)
+        bp = bias.data_ptr()
+    if allowed is not None:
+        arow = _table(allowed, "allowed", T, (V + 31) // 32, torch.int32, dev)
+        ap = allowed.data_ptr()
+    picked = torch.empty(T, dtype=torch.int32, device=logits.device)
+    d = ffi.PICK_DESC.pack(T, B, V, _TYPES[dt], max_q, logits.data_ptr(), row, op, orow,
+                           picked.data_ptr(), qp, hp, lp, hrow, wide, *scalars, bp, brow, ap, arow,
+                           dp, sp, words)
+    ffi.check(ffi.load().warp_pick_tokens(d, _stream()))
+    return picked
+
+
+def tree_accept(drafted, picked, seen, q_start, kv_len, max_q, caches=(), pages=None):
+    """The drafted tokens checked against what was picked, and the caches put in
+    order (warp_tree_accept): (count int32 [B], path int32 [B][max_q], chosen int32
+    [B][max_q], kv_after int32 [B]).
+
+    drafted and picked int32 [T] of the nodes (a negative drafted token is never
+    accepted); seen and max_q as for step_plan; kv_len int32 [B] with the nodes
+    counted.  path holds the `count` nodes of the longest path from node 0 on which
+    each drafted token is what was picked behind its parent, chosen what was picked behind
+    them (the step's new tokens), both -1 from there on; kv_after = kv_len - nodes
+    + count.
+
+    caches: (k_pages, v_pages) of all layers, [layers][pages][page_size][Hk][D], or
+    a list of each layer's pair, all of one layout; their keys and values of the
+    path move behind the keys before the tree, pages int32 [B][n] being the page table."""
+    dev = _device(kv_len)
+    T, B = drafted.numel(), kv_len.numel()
+    words = _seen_ok(seen, T, max_q, dev)
+    if not _vec_ok(drafted, T, torch.int32, dev) or not _vec_ok(picked, T, torch.int32, dev):
+        raise ValueError("drafted and picked must be contiguous int32 [tokens]")
+    if not _vec_ok(kv_len, B, torch.int32, dev):
+        raise ValueError("kv_len must be contiguous int32 [batch]")
+    if not _vec_ok(q_start, B + 1, torch.int32, dev):
+        raise ValueError("q_start must be contiguous int32 [batch + 1]")
+    n = row = wide = tp = 0
+    c = ks = vs = None
+    if len(caches):
+        if pages is None:
+            raise ValueError("caches need the page table")
+        _, row, wide = _batch(q_start, kv_len, pages, dev)
+        tp = pages.data_ptr()
+        n, c, ks, vs = _caches_pack(caches, dev)
+    count = torch.empty(2, B, dtype=torch.int32, device=kv_len.device)
+    path = torch.empty(2, B, max_q, dtype=torch.int32, device=kv_len.device)
+    count, after = count.unbind()
+    path, chosen = path.unbind()
+    d = ffi.ACCEPT_DESC.pack(B, T, max_q, drafted.data_ptr(), picked.data_ptr(), seen.data_ptr(),
+                             words, q_start.data_ptr(), kv_len.data_ptr(), tp, row, wide,
+                             count.data_ptr(), path.data_ptr(), chosen.data_ptr(),
+                             after.data_ptr())
+    ffi.check(ffi.load().warp_tree_accept(d, c, n, ks, vs, _stream()))
+    return count, path, chosen, after
+
+
+def _caches_pack(caches, dev):
+    """(layers, their layout, addresses of their keys and of their values)."""
+    if isinstance(caches[0], torch.Tensor):
+        k, v = caches
+        if k.dim() != 5 or v.dim() != 5 or k.shape[0] != v.shape[0]:
+            raise ValueError("caches must be a pair [layers][pages][page_size][kv_heads][head_dim]")
+        n = k.shape[0]
+        if not n:
+            return 0, None, None, None
+        c = _pages_pack(k[0], v[0], dev)
+        at = [struct.pack(f"@{n}P", *(x.data_ptr() + i * x.stride(0) * x.element_size()
+                                      for i in range(n))) for x in (k, v)]
+        return n, c, *at
+    packed = [_pages_pack(k, v, dev) for k, v in caches]
+    if any(x[16:] != packed[0][16:] for x in packed):
+        raise ValueError("caches must have one shape, dtype and layout")
+    at = [struct.pack(f"@{len(caches)}P", *(x.data_ptr() for x in side)) for side in zip(*caches)]
+    return len(caches), packed[0], *at
 
 
 def attn_status(clear=True):
