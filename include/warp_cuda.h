@@ -437,7 +437,9 @@ WARP_API int warp_tree_attention(const warp_attn_desc *d, const warp_kv_pages *c
  * the row's words.  picked[t]: the lowest v of the largest x; -1 where nothing is
  * above -inf (a NaN never is).  out (NULL for none; may be logits) takes x,
  * rounded to `type`.  max_q bounds the rows of a request; rows past it are left
- * out and reported by warp_attn_status, rows of no request are not written. */
+ * out and reported by warp_attn_status, rows of no request are not written.
+ * scratch: warp_pick_scratch(d) bytes of device memory, 256-byte aligned, free
+ * again when the stream has passed the call. */
 typedef struct {
     int tokens, batch, vocab, type, max_q;
     const void *logits;
@@ -459,7 +461,8 @@ typedef struct {
     int64_t seen_words;
 } warp_pick_desc;
 
-WARP_API int warp_pick_tokens(const warp_pick_desc *d, void *stream);
+WARP_API int64_t warp_pick_scratch(const warp_pick_desc *d);
+WARP_API int warp_pick_tokens(const warp_pick_desc *d, void *scratch, void *stream);
 
 /* The drafted tokens checked.  Node i of a request agrees if it is node 0, or if
  * drafted[i] is picked[p] of its parent p (the last node before it that it sees)

@@ -73,9 +73,11 @@ def test_nothing_to_do(lib):
     assert lib.warp_step_plan(None, None) == -1
     assert lib.warp_step_plan(ctypes.byref(plan_desc(batch=0, tokens=0)), None) == 0
     assert lib.warp_step_plan(ctypes.byref(plan_desc(tokens=0, held=None, pool=None)), None) == 0
-    assert lib.warp_pick_tokens(None, None) == -1
+    assert lib.warp_pick_tokens(None, None, None) == -1
+    assert lib.warp_pick_scratch(None) == -1
     for kw in (dict(tokens=0), dict(batch=0), dict(max_q=0)):
-        assert lib.warp_pick_tokens(ctypes.byref(pick_desc(**kw)), None) == 0
+        assert lib.warp_pick_scratch(ctypes.byref(pick_desc(**kw))) >= 0
+        assert lib.warp_pick_tokens(ctypes.byref(pick_desc(**kw)), None, None) == 0
     assert lib.warp_tree_accept(None, None, 0, None, None, None) == -1
     assert lib.warp_tree_accept(ctypes.byref(accept_desc(batch=0)), None, 0, None, None, None) == 0
     for kw in (dict(tokens=0), dict(batch=0), dict(max_q=0)):
@@ -107,8 +109,14 @@ def test_tree_refusals(lib, kw, seen, words, text):
     (dict(out=257, type=1), b"aligned"), (dict(out=256, out_row=104), b"layout"),
     (dict(q_start=None, batch=2), b"together")])
 def test_pick_refusals(lib, kw, text):
-    assert lib.warp_pick_tokens(ctypes.byref(pick_desc(**kw)), None) == -1
+    assert lib.warp_pick_tokens(ctypes.byref(pick_desc(**kw)), ctypes.c_void_p(256), None) == -1
     assert text in lib.warp_last_error()
+
+
+def test_pick_refuses_bad_scratch(lib):
+    for at in (None, 264):
+        assert lib.warp_pick_tokens(ctypes.byref(pick_desc()), at, None) == -1
+        assert b"scratch" in lib.warp_last_error()
 
 
 @pytest.mark.parametrize("kw, ckw, text", [

@@ -1,12 +1,19 @@
 // logits.cu — penalties for repeated tokens, biases and masks on logits, and the
 // largest of each row.
 //
-// One read of the logits (and, where they are kept, one write): bound by memory.
-// A cluster of blocks shares the vocabulary of a few rows of one request, so that
-// the blocks' choices are joined in the cluster and nothing is left to a second
-// launch.  A block counts its part of the context once, in shared memory: a bit
-// for each token that occurs, which a thread looks at for a whole vector of logits,
-// and the numbers, which are read only where a bit is set.
+// The logits are read once (and, where they are kept, written once), which is what
+// bounds it.  Two kernels: the first counts each request's history, a block to a slice of
+// the vocabulary, and leaves a bit for each token that occurs, and the numbers where
+// there are such bits.  The second streams over the rows, in equal runs, and joins
+// a row's parts by an atomic maximum of (logit, token) in one number, which any order
+// leaves the same.
+//
+// Division: x / r for a row's many x and one r is q = x y with y = 1 / r rounded,
+// corrected twice by the remainder: q += y (x - q r), each step one fused
+// operation (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990: the last step rounds as a division does if y is rounded to nearest
+// and q is off by one place at most, which the first step sees to).  Where a quotient or
+// remainder could leave the normal numbers it divides.
 #include "attn.cuh"
 
 namespace warp {
@@ -21,16 +28,105 @@ struct PickArgs {
     const uint64_t *seen;
     int64_t row, out_row, history_row, bias_row, allowed_row, seen_words;
     unsigned *err;
-    int tokens, batch, vocab, history_wide;
-    int max_q, rows, groups;                // rows a cluster, clusters a request
-    int part;                               // tokens of the vocabulary a block and pass
-    int passes;
+    int tokens, batch, vocab, history_wide, max_q;
+    // the first kernel's results: [batch][words], and [batch][32 * words]
+    uint32_t *bits;
+    void *counts;
+    int words;                              // of 32 tokens in the vocabulary
+    int slice, slices;                      // words a block of the first, blocks a request
+    unsigned long long *best;               // [tokens]; and how many pieces are done
+    unsigned *done;
+    int pieces;                             // of a row, for the second
 };
 
-constexpr int kPickThreads = 256;
-constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kPickRows = 16;               // rows a cluster, at most
-constexpr int kPickPart = 32768;            // tokens a block and pass, at most
+// ------------------------------------------------------------- the history --
+
+// A block reads all of the history and counts the tokens of its slice, whose counts
+// take most of an SM's shared memory: with slices of an eighth of that the histories' reads
+// from the L2 were what took the time (64 of up to 30000 tokens, 131072 in the
+// vocabulary: 14 us for the reads alone).
+constexpr int kPickCounters = 1024;         // threads
+constexpr int kPickSlice = 2048;            // words of 16-bit counts a block, at most
+
+template <typename C>
+__global__ void __launch_bounds__(kPickCounters)
+pick_history_kernel(const __grid_constant__ PickArgs a) {
+    extern __shared__ __align__(16) uint32_t counts[];  // [slice * 32] of C
+    constexpr int PER = 4 / sizeof(C), U = 4;
+    pdl_trigger();
+    const int tid = threadIdx.x;
+    for (int t = blockIdx.x * kPickCounters + tid; t < a.tokens; t += gridDim.x * kPickCounters) {
+        a.best[t] = 0;
+        a.done[t] = 0;
+    }
+    if (!a.history) return;
+    const int b = blockIdx.x / a.slices, w0 = (blockIdx.x - b * a.slices) * a.slice;
+    const int n = min(a.slice, a.words - w0), v0 = w0 * 32;
+    const int end = min(n * 32, a.vocab - v0);          // tokens of the slice
+    const int said = a.history_len[b], len = min(max(said, 0), a.history_wide);
+    if (tid == 0 && said != len) atomicOr(a.err, kAttnBadLen);
+    const int32_t *const past = a.history + b * a.history_row;
+    const int lead = min((int)(-((uintptr_t)past / 4) % 4), len), fours = (len - lead) / 4;
+    int4 v[U];
+    auto read = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            v[u] = make_int4(-1, -1, -1, -1);
+            if (i + u * kPickCounters < fours)
+                v[u] = __ldg((const int4 *)(past + lead) + i + u * kPickCounters);
+        }
+    };
+    read(tid);
+    for (int x = 4 * tid; x < n * (32 / PER); x += 4 * kPickCounters)
+        *(uint4 *)(counts + x) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    auto add = [&](int token) {
+        const int at = token - v0;
+        if (token >= v0 && at < end)
+            atomicAdd(counts + at / PER, 1u << at % PER * (8 * (int)sizeof(C)));
+    };
+    if (tid < lead) add(past[tid]);
+    if (tid < len - lead - 4 * fours) add(past[lead + 4 * fours + tid]);
+    for (int i = tid; i < fours; i += U * kPickCounters) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            add(v[u].x);
+            add(v[u].y);
+            add(v[u].z);
+            add(v[u].w);
+        }
+        read(i + U * kPickCounters);
+    }
+    __syncthreads();
+    // a word of bits from 32 counts, which are written where there is one
+    for (int w = tid; w < n; w += kPickCounters) {
+        uint32_t bits = 0;
+        uint4 z[8 / PER];
+#pragma unroll
+        for (int q = 0; q < 8 / PER; q++) {
+            z[q] = *(const uint4 *)(counts + w * (32 / PER) + 4 * q);
+            const uint32_t y[4] = {z[q].x, z[q].y, z[q].z, z[q].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int at = (4 * q + k) * PER;
+                if (PER == 1) {
+                    bits |= (uint32_t)(y[k] != 0) << at;
+                } else {
+                    bits |= (uint32_t)((y[k] & 0xffffu) != 0) << at;
+                    bits |= (uint32_t)(y[k] >> 16 != 0) << (at + 1);
+                }
+            }
+        }
+        const int64_t word = b * (int64_t)a.words + w0 + w;
+        a.bits[word] = bits;
+        uint4 *const to = (uint4 *)((C *)a.counts + word * 32);
+        if (bits)
+#pragma unroll
+            for (int q = 0; q < 8 / PER; q++) to[q] = z[q];
+    }
+}
+
+// ---------------------------------------------------------------- the rows --
 
 // A choice as one number that the larger of two is the better of: larger logit,
 // then lower token.  0 is no choice.
@@ -40,27 +136,11 @@ __device__ __forceinline__ unsigned long long pick_key(float x, int v) {
     return (unsigned long long)up << 32 | (uint32_t)~v;
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-// A word of block `rank`'s shared memory, at the address that it has in this one's.
-__device__ __forceinline__ unsigned long long cluster_ld64(uint32_t addr, uint32_t rank) {
-    unsigned long long v;
-    asm volatile(
-        "{\n\t.reg .u32 a;\n\t"
-        "mapa.shared::cluster.u32 a, %1, %2;\n\t"
-        "ld.shared::cluster.u64 %0, [a];\n\t}\n" : "=l"(v) : "r"(addr), "r"(rank) : "memory");
-    return v;
+// The warp's largest value.
+__device__ __forceinline__ float warp_max(float x) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+    return m;
 }
 
 // 16 bytes of a row's values.
@@ -69,157 +149,453 @@ template <typename T> struct alignas(16) PickVec {
     T x[n];
 };
 
-// The context's part of the penalties of one request.
-struct PickLess { float repetition, frequency, presence; };
+// The penalties of one request.
+struct PickLess {
+    float repetition, frequency, presence;
+    float inverse;                          // of the first, rounded; 0 where it is divided by
+};
 
-__device__ __forceinline__ float pick_less(float x, int count, const PickLess &p) {
-    x = x > 0.f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
-    x = __fsub_rn(x, __fmul_rn(p.frequency, (float)count));
+__device__ __forceinline__ float pick_less(float x, float count, const PickLess &p, bool divide) {
+    float q;
+    if (divide) {
+        q = __fdiv_rn(x, p.repetition);
+    } else {
+        q = __fmul_rn(x, p.inverse);
+        q = __fmaf_rn(__fmaf_rn(-q, p.repetition, x), p.inverse, q);
+        q = __fmaf_rn(__fmaf_rn(-q, p.repetition, x), p.inverse, q);
+    }
+    x = x > 0.f ? q : __fmul_rn(x, p.repetition);
+    x = __fsub_rn(x, __fmul_rn(p.frequency, count));
     return __fsub_rn(x, p.presence);
 }
+// Whether x is so far from the normal numbers' ends that the products above are exact
+// where they have to be; 2^-80 .. 2^80.
+__device__ __forceinline__ bool pick_tame(float x) {
+    constexpr uint32_t lo = (127u - 80u) << 24, hi = (127u + 80u) << 24;
+    return (__float_as_uint(x) << 1) - lo < hi - lo;
+}
+// A count as a number: 16 bits below the last place of 2^23, and 2^23 taken off.
+__device__ __forceinline__ float pick_float(uint16_t c) {
+    return __fsub_rn(__uint_as_float(0x4b000000u | c), 8388608.f);
+}
+__device__ __forceinline__ float pick_float(uint32_t c) { return (float)c; }
 
-// Shared memory: counts [part], bits [part / 32], bits of each row's own nodes
-// [rows][part / 32].
-template <typename T>
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const __grid_constant__ PickArgs a) {
-    extern __shared__ __align__(16) uint32_t smem[];
-    __shared__ unsigned long long best[kPickRows][kPickWarps];
-    constexpr int N = PickVec<T>::n;
-    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    const int rank = (int)cluster_rank(), size = (int)cluster_size();
-    const int cluster = blockIdx.x / size;
-    const int b = cluster / a.groups, group = cluster - b * a.groups;
-    int t0 = b, n = 1;
-    if (a.q_start) {
-        const int s = a.q_start[b], e = a.q_start[b + 1];
-        t0 = min(max(s, 0), a.tokens);
-        n = min(min(max(e - s, 0), a.max_q), a.tokens - t0);
-        if (tid == 0 && (t0 != s || n != e - s)) atomicOr(a.err, kAttnBadLen);
-    }
-    const int r0 = group * a.rows, rows = min(a.rows, n - r0);
-    if (rows <= 0) return;                  // all blocks of the cluster
-    const int words = a.part / 32;
-    int *const counts = (int *)smem;
-    uint32_t *const occurs = smem + a.part, *const own = occurs + words;
-    const bool context = a.history || a.seen;
-    PickLess less = {1.f, 0.f, 0.f};
-    if (a.repetition) less.repetition = a.repetition[b];
-    if (a.frequency) less.frequency = a.frequency[b];
-    if (a.presence) less.presence = a.presence[b];
-    for (int x = tid; x < kPickRows * kPickWarps; x += kPickThreads) (&best[0][0])[x] = 0;
+// What a kernel does besides the penalties: asked for each value, this would cost
+// more than the rest of the stream.
+constexpr int kPickBias = 1, kPickAllowed = 2, kPickKeep = 4;
+constexpr int kPickThreads = 256;
+constexpr int kPickWarps = kPickThreads / 32;
+constexpr int kPickOwn = 256;               // nodes' tokens that a block keeps
+constexpr int kPickPart = 65536;            // tokens of a row at once, at most
+constexpr int kPickPiece = 2048;            // tokens of a row that one block takes, at least
 
-    for (int pass = 0; pass < a.passes; pass++) {
-        const int64_t from = ((int64_t)pass * size + rank) * a.part;
-        const int v0 = (int)min(from, (int64_t)a.vocab);
-        const int v1 = (int)min(from + a.part, (int64_t)a.vocab);
-        __syncthreads();
-        if (context) {
-            for (int x = tid; x < a.part + words + rows * words; x += kPickThreads) smem[x] = 0;
-            __syncthreads();
-            if (a.history) {
-                const int said = a.history_len[b], len = min(max(said, 0), a.history_wide);
-                if (tid == 0 && said != len) atomicOr(a.err, kAttnBadLen);
-                const int32_t *const past = a.history + b * a.history_row;
-                for (int i = tid; i < len; i += kPickThreads) {
-                    const int v = past[i];
-                    if (v < v0 || v >= v1) continue;
-                    atomicAdd(counts + (v - v0), 1);
-                    atomicOr(occurs + (v - v0) / 32, 1u << (v - v0) % 32);
-                }
-            }
-            if (a.seen)
-                for (int x = tid; x < rows * n; x += kPickThreads) {
-                    const int r = x / n, m = x - r * n;
-                    const int v = a.drafted[t0 + m];
-                    if (v < v0 || v >= v1 || m >= a.seen_words * 64) continue;
-                    const uint64_t *const row = a.seen + (t0 + r0 + r) * a.seen_words;
-                    if (row[m >> 6] >> (m & 63) & 1)
-                        atomicOr(own + r * words + (v - v0) / 32, 1u << (v - v0) % 32);
-                }
-            __syncthreads();
-        }
-        for (int r = 0; r < rows; r++) {
-            const int t = t0 + r0 + r;
-            const T *const x = (const T *)a.logits + t * a.row;
-            T *const y = a.out ? (T *)a.out + t * a.out_row : nullptr;
-            const float *const bias = a.bias ? a.bias + b * a.bias_row : nullptr;
-            const uint32_t *const allowed = a.allowed ? a.allowed + t * a.allowed_row : nullptr;
-            float top = -INFINITY;
-            int at = -1;
-            auto adjust = [&](float f, int v) {
-                if (context) {
-                    const int w = (v - v0) / 32, bit = (v - v0) % 32;
-                    const bool mine = own[r * words + w] >> bit & 1;
-                    if (mine || (occurs[w] >> bit & 1)) {
-                        int count = counts[v - v0];
-                        if (mine) {
-                            const uint64_t *const row = a.seen + t * a.seen_words;
-                            for (int m = 0; m < n && m < a.seen_words * 64; m++)
-                                if (row[m >> 6] >> (m & 63) & 1) count += a.drafted[t0 + m] == v;
-                        }
-                        f = pick_less(f, count, less);
-                    }
-                }
-                if (bias) f = __fadd_rn(f, bias[v]);
-                if (allowed && !(allowed[v >> 5] >> (v & 31) & 1)) f = -INFINITY;
-                if (f > top) {
-                    top = f;
-                    at = v;
-                }
-                return f;
-            };
-            for (int v = v0 + tid; v < v1; v += kPickThreads) {
-                const float f = adjust(AttnType<T>::up(x[v]), v);
-                if (y) y[v] = AttnType<T>::down(f);
-            }
-            unsigned long long key = at < 0 ? 0 : pick_key(top, at);
-#pragma unroll
-            for (int d = 16; d; d >>= 1) key = max(key, __shfl_xor_sync(~0u, key, d));
-            if (lane == 0) best[r][warp] = max(best[r][warp], key);
-        }
-    }
-    cluster_sync();
-    for (int r = rank * kPickWarps + warp; r < rows; r += size * kPickWarps) {
-        unsigned long long key = 0;
-        for (int x = lane; x < size * kPickWarps; x += 32)
-            key = max(key, cluster_ld64(smem_u32(&best[r][x % kPickWarps]), x / kPickWarps));
-#pragma unroll
-        for (int d = 16; d; d >>= 1) key = max(key, __shfl_xor_sync(~0u, key, d));
-        if (lane == 0) a.picked[t0 + r0 + r] = key ? (int)~(uint32_t)key : -1;
-    }
-    cluster_sync();                         // no block leaves while its words are read
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
+                 : "memory");
 }
 
-template <typename T>
-static int pick_launch(const PickArgs &a, int size, cudaStream_t st) {
+// A thread's place in the ring, for each vector under way: the values, the biases of a
+// kernel that adds some, and the counts, of which there are twice as many where
+// vectors are not aligned to their words.
+template <typename T, typename C, int OPT> struct PickSlot {
+    static constexpr int n = PickVec<T>::n;
+    static constexpr int bias = 16;
+    static constexpr int window = n * sizeof(C);        // bytes of a vector's counts
+    static constexpr int counts = bias + (OPT & kPickBias ? n * 4 : 0);
+    static constexpr int bytes = counts + 2 * window;
+    static constexpr int ahead = bytes <= 48 ? 8 : bytes <= 80 ? 6 : 4;  // vectors under way
+    static constexpr int ring = ahead * bytes * kPickThreads;
+};
+
+// The rows lie one behind another in pieces of kPickPiece tokens, and the blocks take
+// equal runs of them; a row's part in a run is gone through at once.
+//
+// A thread's vectors of 16 bytes come through a ring of its own in shared memory: the
+// loads that are under way take no registers, and no thread waits for another.  With a
+// vector come its biases and, if one of its tokens occurs, its counts.  That is
+// known ahead: a warp's bits of G vectors are one register a lane (N words a vector, and one
+// more where they are not aligned), asked for G vectors before they are needed.
+template <typename T, typename C, int OPT>
+__global__ void __launch_bounds__(kPickThreads)
+pick_rows_kernel(const __grid_constant__ PickArgs a) {
+    using Slot = PickSlot<T, C, OPT>;
+    constexpr int N = Slot::n, STEP = kPickThreads * N, R = Slot::ahead;
+    constexpr int G = 32 / (N + 1);
+    constexpr bool BIAS = OPT & kPickBias, ALLOWED = OPT & kPickAllowed, KEEP = OPT & kPickKeep;
+    __shared__ uint32_t drafts[kPickPart / 32 + 1];     // the row's nodes' tokens, a bit each
+    __shared__ int own[kPickOwn];                       // and themselves
+    __shared__ int n_own;
+    __shared__ unsigned long long best[kPickWarps];
+    extern __shared__ __align__(16) uint8_t ring[];     // [vector][part of a slot][thread]
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const int64_t all = (int64_t)a.tokens * a.pieces, blocks = gridDim.x;
+    const int64_t last = (blockIdx.x + 1) * all / blocks;
+    bool waited = false;
+    for (int64_t piece = blockIdx.x * all / blocks, next; piece < last; piece = next) {
+        const int t = (int)(piece / a.pieces), first = (int)(piece - (int64_t)t * a.pieces);
+        next = min(min(last, piece - first + a.pieces), piece + kPickPart / kPickPiece);
+        const int v0 = first * kPickPiece;
+        const int v1 = (int)min((int64_t)a.vocab, v0 + (next - piece) * kPickPiece);
+        const T *const x = (const T *)a.logits + t * a.row;
+        T *const y = KEEP ? (T *)a.out + t * a.out_row : nullptr;
+        // the request: the last one that starts at or before the row
+        int b = t, i = 0, n = 1;
+        if (a.q_start) {
+            b = -1;
+            for (int i0 = 0; i0 < a.batch; i0 += 32) {
+                const unsigned hit = __ballot_sync(~0u, i0 + lane < a.batch &&
+                                                            a.q_start[i0 + lane] <= t);
+                if (hit) b = i0 + 31 - __clz(hit);
+                if (hit != ~0u) break;
+            }
+            const int s = b < 0 ? 0 : a.q_start[b], e = b < 0 ? 0 : a.q_start[b + 1];
+            i = t - s;
+            n = min(e - s, a.max_q);
+            if (t < e && (s < 0 || e > a.tokens || i >= n) && tid == 0)
+                atomicOr(a.err, kAttnBadLen);
+            if (t >= e || s < 0 || i >= n) continue;
+            n = min(n, a.tokens - s);
+        }
+        const int t0 = t - i;
+        const uint64_t *const sees = a.seen ? a.seen + t * a.seen_words : nullptr;
+        const float *const bias = BIAS ? a.bias + b * a.bias_row : nullptr;
+        const uint32_t *const allowed = ALLOWED ? a.allowed + t * a.allowed_row : nullptr;
+        const uint32_t *const occurs = a.history ? a.bits + b * (int64_t)a.words : nullptr;
+        const C *const counts = (const C *)a.counts + b * (int64_t)a.words * 32;
+        // Vectors are aligned in memory, from value a0 on; what is left over at the
+        // part's ends goes one by one.
+        const int a0 = min(v1, v0 + (int)(-((uintptr_t)(x + v0) / sizeof(T)) % N));
+        const int vectors = (v1 - a0) / N, end = a0 + vectors * N;
+        const int rounds = (vectors + kPickThreads - 1) / kPickThreads;
+        const int v_tid = a0 + tid * N, skew = a0 % N;
+        const bool y_vec = ((uintptr_t)(y + a0) & 15) == 0;
+        const bool bias_vec = ((uintptr_t)(bias + a0) & 15) == 0;
+        PickLess less = {1.f, 0.f, 0.f, 0.f};
+        if (a.repetition) less.repetition = a.repetition[b];
+        if (a.frequency) less.frequency = a.frequency[b];
+        if (a.presence) less.presence = a.presence[b];
+        if (less.repetition >= 0x1p-20f && less.repetition <= 0x1p20f)
+            less.inverse = __frcp_rn(less.repetition);
+        if (sees) {
+            __syncthreads();                // the last part's are read
+            for (int w = tid; w < (v1 - v0 + 31) / 32 + 1; w += kPickThreads) drafts[w] = 0;
+            if (tid == 0) n_own = 0;
+            __syncthreads();
+            for (int m = tid; m < n && m < a.seen_words * 64; m += kPickThreads) {
+                const int v = a.drafted[t0 + m];
+                if (!(sees[m >> 6] >> (m & 63) & 1) || v < v0 || v >= v1) continue;
+                const int k = atomicAdd(&n_own, 1);
+                if (k < kPickOwn) own[k] = v;
+                atomicOr(drafts + (v - v0) / 32, 1u << (v - v0) % 32);
+            }
+            __syncthreads();
+        }
+        float top = -INFINITY;
+        int at = -1;
+
+        // how many of the nodes that the row sees have token v
+        auto nodes_with = [&](int v) {
+            int count = 0;
+            if (n_own <= kPickOwn)
+                for (int k = 0; k < n_own; k++) count += own[k] == v;
+            else
+                for (int m = 0; m < n && m < a.seen_words * 64; m++)
+                    if (sees[m >> 6] >> (m & 63) & 1) count += a.drafted[t0 + m] == v;
+            return count;
+        };
+        // the value of token v less what its context takes off, the long way
+        auto adjusted = [&](float f, int v) {
+            uint32_t count = 0;
+            if (occurs && (occurs[v >> 5] >> (v & 31) & 1)) count = (uint32_t)counts[v];
+            if (sees && (drafts[(v - v0) >> 5] >> (v & 31) & 1)) count += nodes_with(v);
+            return count ? pick_less(f, (float)count, less, true) : f;
+        };
+        auto single = [&](int v) {
+            float f = adjusted(AttnType<T>::up(x[v]), v);
+            if (BIAS) f = __fadd_rn(f, __ldg(bias + v));
+            if (ALLOWED && !(__ldg(allowed + (v >> 5)) >> (v & 31) & 1)) f = -INFINITY;
+            if (f > top || (f == top && v < at)) {
+                top = f;
+                at = v;
+            }
+            if (KEEP) y[v] = AttnType<T>::down(f);
+        };
+        const int lane_g = lane / (N + 1), lane_w = lane % (N + 1);
+        const int word0 = ((a0 + lane_g * STEP + warp * 32 * N) >> 5) + lane_w;
+        // a lane's word of the bits of G vectors from round k on
+        auto hits_of = [&](int k) {
+            const int w = word0 + k * (STEP / 32);
+            if (lane_g >= G || w >= a.words || k >= rounds) return 0u;
+            uint32_t bits = occurs ? occurs[w] : 0;
+            if (sees && w <= (v1 - v0 + 31) / 32 + (v0 >> 5)) bits |= drafts[w - (v0 >> 5)];
+            return bits;
+        };
+        auto may_of = [&](int k) {
+            const int w = word0 + k * (STEP / 32);
+            return ALLOWED && lane_g < G && w < a.words && k < rounds ? __ldg(allowed + w) : 0u;
+        };
+        const int shift = (a0 + lane * N) & 31, in_vector = ((a0 & 31) + lane * N) >> 5;
+        auto bits_of = [&](uint32_t word, int g) {
+            const uint32_t lo = __shfl_sync(~0u, word, g * (N + 1) + in_vector);
+            const uint32_t hi = __shfl_sync(~0u, word, g * (N + 1) + min(in_vector + 1, N));
+            return __funnelshift_r(lo, hi, shift) & ((1u << N) - 1);
+        };
+        if (!waited) pdl_wait();
+        waited = true;
+        const bool context = occurs || sees;
+        // Vectors asked for so far: round `ask`, number `ask_g` of the group whose bits are
+        // in `ask_hits`, with the next group's behind them.  What is hit in the vectors
+        // under way queues in `queue`, N bits each.
+        int ask = 0, ask_g = 0;
+        uint32_t ask_hits = context ? hits_of(0) : 0, next_hits = context ? hits_of(G) : 0;
+        uint64_t queue = 0;
+        const uint32_t slot0 = smem_u32(ring);
+        auto place = [&](int k, int part, int bytes) {  // of a vector's part of the ring
+            return slot0 + (k % R) * (Slot::bytes * kPickThreads) + part * kPickThreads + tid * bytes;
+        };
+        auto fetch = [&] {
+            const int v = v_tid + ask * STEP;
+            uint32_t hit = 0;
+            if (context) {
+                hit = bits_of(ask_hits, ask_g);
+                if (++ask_g == G) {
+                    ask_g = 0;
+                    ask_hits = next_hits;
+                    next_hits = hits_of(ask + 1 + G);
+                }
+                if (v >= end) hit = 0;
+                queue = queue >> N | (uint64_t)hit << N * (R - 1);
+            }
+            if (v < end) {
+                cp_async16(place(ask, 0, 16), x + v);
+                if (BIAS && bias_vec) {
+#pragma unroll
+                    for (int k = 0; k < N; k += 4)
+                        cp_async16(place(ask, Slot::bias, 4 * N) + 4 * k, bias + v + k);
+                }
+            }
+            if (hit && occurs) {
+                const C *const z = counts + (v - skew);
+                const uint32_t to = place(ask, Slot::counts, 2 * Slot::window);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if (k && !skew) break;
+#pragma unroll
+                    for (int q = 0; q < Slot::window; q += 8)
+                        cp_async_small<8>(to + k * Slot::window + q, (const char *)(z + k * N) + q);
+                }
+            }
+            cp_async_commit();
+            ask++;
+        };
+#pragma unroll 1
+        for (int k = 0; k < R - 1; k++) fetch();
+        uint32_t may = may_of(0), next_may = may_of(G);
+        int g = 0;
+        float bound = -INFINITY;            // what the warp has seen is at least this
+#pragma unroll 1
+        for (int k = 0; k < rounds; k++) {
+            fetch();
+            const uint32_t hit = (uint32_t)queue & ((1u << N) - 1);
+            const uint32_t allow = ALLOWED ? bits_of(may, g) : 0;
+            cp_async_wait<R - 1>();
+            const int v = v_tid + k * STEP;
+            float f[N], most = -INFINITY;
+            if (v < end) {
+                PickVec<T> raw;
+                *(uint4 *)&raw = lds_u4(place(k, 0, 16));
+#pragma unroll
+                for (int q = 0; q < N; q++) f[q] = AttnType<T>::up(raw.x[q]);
+                if (hit) {
+                    const int d = (v - v0) >> 5;
+                    const uint32_t mine =
+                        sees ? __funnelshift_r(drafts[d], drafts[d + 1], v & 31) & hit : 0;
+                    bool plain = less.inverse != 0.f && !mine;
+#pragma unroll
+                    for (int q = 0; q < N; q++) plain &= pick_tame(f[q]);
+                    if (__builtin_expect(plain, 1)) {
+                        const C *const z = (const C *)(ring + (place(k, Slot::counts, 2 * Slot::window) -
+                                                               slot0));
+                        alignas(16) C c[N];
+                        if (!skew) {
+#pragma unroll
+                            for (int q = 0; q < Slot::window; q += 8)
+                                *(uint2 *)((char *)c + q) = *(const uint2 *)((const char *)z + q);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < N; q++) c[q] = z[q + skew];
+                        }
+#pragma unroll
+                        for (int q = 0; q < N; q++) {
+                            const float w = pick_less(f[q], pick_float(c[q]), less, false);
+                            f[q] = hit >> q & 1 ? w : f[q];
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < N; q++)
+                            if (hit >> q & 1) f[q] = adjusted(f[q], v + q);
+                    }
+                }
+                if (BIAS) {
+                    alignas(16) float w[N];
+                    if (bias_vec) {
+#pragma unroll
+                        for (int q = 0; q < N; q += 4)
+                            *(uint4 *)(w + q) = lds_u4(place(k, Slot::bias, 4 * N) + 4 * q);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < N; q++) w[q] = __ldg(bias + v + q);
+                    }
+#pragma unroll
+                    for (int q = 0; q < N; q++) f[q] = __fadd_rn(f[q], w[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < N; q++) {
+                    if (ALLOWED && !(allow >> q & 1)) f[q] = -INFINITY;
+                    most = fmaxf(most, f[q]);
+                }
+                if (KEEP) {
+                    PickVec<T> z;
+#pragma unroll
+                    for (int q = 0; q < N; q++) z.x[q] = AttnType<T>::down(f[q]);
+                    if (y_vec) {
+                        *(uint4 *)(y + v) = *(const uint4 *)&z;
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < N; q++) y[v + q] = z.x[q];
+                    }
+                }
+            }
+            if (__any_sync(~0u, most > bound)) {
+                if (most > top) {
+                    top = most;
+#pragma unroll
+                    for (int q = N - 1; q >= 0; q--)
+                        if (f[q] == most) at = v + q;
+                }
+                bound = warp_max(top);
+            }
+            if (ALLOWED && ++g == G) {
+                g = 0;
+                may = next_may;
+                next_may = may_of(k + 1 + G);
+            }
+        }
+        cp_async_wait<0>();
+        if (tid < a0 - v0) single(v0 + tid);
+        if (tid < v1 - end) single(end + tid);
+
+        unsigned long long key = at < 0 ? 0 : pick_key(top, at);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) key = max(key, __shfl_xor_sync(~0u, key, d));
+        __syncthreads();                    // the last part's are read
+        if (lane == 0) best[warp] = key;
+        __syncthreads();
+        if (tid) continue;
+#pragma unroll
+        for (int k = 1; k < kPickWarps; k++) key = max(key, best[k]);
+        if (v1 - v0 < a.vocab) {
+            // the last of the row's parts, whoever has it, says what is picked
+            const unsigned mine = (unsigned)(next - piece);
+            atomicMax(a.best + t, key);
+            __threadfence();
+            if (atomicAdd(a.done + t, mine) + mine < (unsigned)a.pieces) continue;
+            __threadfence();
+            key = atomicMax(a.best + t, 0ull);
+        }
+        a.picked[t] = key ? (int)~(uint32_t)key : -1;
+    }
+    if (!waited) pdl_wait();                // a grid is not complete before the one before it
+}
+
+// ------------------------------------------------------------ host side --
+
+// Scratch: the choices and how many pieces are done, the history's bits and counts.
+struct PickPlan {
+    int words, slice, slices, pieces;
+    bool wide;                              // counts of 32 bits
+    int64_t done_at, bits_at, counts_at, bytes;
+};
+
+static int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+static PickPlan pick_plan(const warp_pick_desc *d) {
+    PickPlan p = {};
+    p.words = (d->vocab + 31) / 32;
+    // 16 bits where no history is long enough to outgrow them
+    p.wide = d->history_wide >= 65536;
+    const int most = p.wide ? kPickSlice / 2 : kPickSlice;
+    p.slice = p.words < most ? p.words : most;
+    p.slices = (p.words + p.slice - 1) / p.slice;
+    p.pieces = (d->vocab + kPickPiece - 1) / kPickPiece;
+    int64_t at = align256((int64_t)d->tokens * 8);
+    p.done_at = at;
+    at += align256((int64_t)d->tokens * 4);
+    p.bits_at = at;
+    if (d->history) {
+        at += align256((int64_t)d->batch * p.words * 4);
+        p.counts_at = at;
+        // a vector's window may reach past the last word's
+        at += align256(((int64_t)d->batch * p.words + 1) * 32 * (p.wide ? 4 : 2));
+    } else if (p.pieces == 1) {
+        at = 0;
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <typename C>
+static int pick_history(const PickArgs &a, cudaStream_t st) {
     static std::atomic<uint64_t> done;
-    const int words = a.part / 32;
-    constexpr int most = (kPickPart + kPickPart / 32 * (1 + kPickRows)) * 4;
-    static_assert(most + kPickRows * kPickWarps * 8 <= 227 * 1024, "shared memory of a block");
-    cudaError_t e = attn_smem(pick_kernel<T>, most, done);
+    constexpr int most = kPickSlice * 32 * 2;
+    cudaError_t e = attn_smem(pick_history_kernel<C>, most, done);
     if (e != cudaSuccess) return cuda_fail(e, "pick smem attribute");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.batch * a.groups * size));
-    cfg.blockDim = dim3(kPickThreads);
-    cfg.dynamicSmemBytes = a.history || a.seen ? (a.part + words * (1 + a.rows)) * 4 : 0;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = size;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, pick_kernel<T>, a);
-    if (e != cudaSuccess) return cuda_fail(e, "pick_kernel");
+    e = attn_start(pick_history_kernel<C>,
+                   dim3(a.history ? (unsigned)a.batch * a.slices : cdiv(a.tokens, kPickCounters)),
+                   kPickCounters, a.history ? (size_t)a.slice * 32 * sizeof(C) : 0, st, true, a);
+    if (e != cudaSuccess) return cuda_fail(e, "pick_history_kernel");
     count_launch();
     return WARP_OK;
 }
 
-}  // namespace warp
+template <typename T, typename C, int OPT>
+static int pick_rows(const PickArgs &a, bool first, cudaStream_t st) {
+    static std::atomic<uint64_t> done;
+    constexpr int ring = PickSlot<T, C, OPT>::ring, fixed = kPickPart / 8 + 4 * kPickOwn + 256;
+    static_assert(ring + fixed <= 227 * 1024, "shared memory of a block");
+    cudaError_t e = attn_smem(pick_rows_kernel<T, C, OPT>, ring, done);
+    if (e != cudaSuccess) return cuda_fail(e, "pick smem attribute");
+    // as many blocks as fit, by their shared memory
+    constexpr int fit = 228 * 1024 / (ring + fixed + 1024);
+    const int64_t all = (int64_t)a.tokens * a.pieces, room = (fit < 4 ? fit : 4) * 148;
+    e = attn_start(pick_rows_kernel<T, C, OPT>, dim3((unsigned)(all < room ? all : room)),
+                   kPickThreads, ring, st, first, a);
+    if (e != cudaSuccess) return cuda_fail(e, "pick_rows_kernel");
+    count_launch();
+    return WARP_OK;
+}
 
-using namespace warp;
+template <typename T, typename C>
+static int pick_run(const PickArgs &a, cudaStream_t st) {
+    const bool alone = !a.history && a.pieces == 1;
+    if (!alone) {
+        const int rc = pick_history<C>(a, st);
+        if (rc) return rc;
+    }
+    switch ((a.bias ? kPickBias : 0) | (a.allowed ? kPickAllowed : 0) | (a.out ? kPickKeep : 0)) {
+    case 0: return pick_rows<T, C, 0>(a, alone, st);
+    case 1: return pick_rows<T, C, 1>(a, alone, st);
+    case 2: return pick_rows<T, C, 2>(a, alone, st);
+    case 3: return pick_rows<T, C, 3>(a, alone, st);
+    case 4: return pick_rows<T, C, 4>(a, alone, st);
+    case 5: return pick_rows<T, C, 5>(a, alone, st);
+    case 6: return pick_rows<T, C, 6>(a, alone, st);
+    default: return pick_rows<T, C, 7>(a, alone, st);
+    }
+}
 
-extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *stream) {
+static int pick_check(const warp_pick_desc *d) {
     const char *who = "warp_pick_tokens";
     WARP_ARG(d, "%s: NULL description", who);
     WARP_ARG(d->tokens >= 0 && d->batch >= 0 && d->max_q >= 0 && d->history_wide >= 0,
@@ -232,6 +608,23 @@ extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *stream) {
              "%s: negative stride", who);
     WARP_ARG(d->q_start || d->tokens == d->batch, "%s: %d rows of %d requests", who, d->tokens,
              d->batch);
+    WARP_ARG(d->batch <= (1 << 27), "%s: %d requests", who, d->batch);
+    return WARP_OK;
+}
+
+}  // namespace warp
+
+using namespace warp;
+
+extern "C" int64_t warp_pick_scratch(const warp_pick_desc *d) {
+    const int rc = pick_check(d);
+    return rc ? rc : pick_plan(d).bytes;
+}
+
+extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *scratch, void *stream) {
+    const char *who = "warp_pick_tokens";
+    int rc = pick_check(d);
+    if (rc) return rc;
     if (d->tokens == 0 || d->batch == 0 || (d->q_start && d->max_q == 0)) return WARP_OK;
     WARP_ARG(d->logits && d->picked, "%s: NULL pointer", who);
     WARP_ARG(!d->history == !d->history_len, "%s: history and history_len go together", who);
@@ -243,6 +636,10 @@ extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *stream) {
              "%s: logits are not aligned to their type", who);
     WARP_ARG(d->out != d->logits || d->out_row == d->row || d->tokens == 1,
              "%s: results in the logits' place have their layout", who);
+    const PickPlan p = pick_plan(d);
+    WARP_ARG(p.bytes == 0 || (scratch && ((uintptr_t)scratch & 255) == 0),
+             "%s: scratch must be 256-byte aligned", who);
+    WARP_ARG((int64_t)d->batch * p.slices < (int64_t)1 << 31, "%s: %d requests", who, d->batch);
     PickArgs a = {};
     a.logits = d->logits, a.out = d->out, a.picked = d->picked, a.q_start = d->q_start;
     a.history = d->history, a.history_len = d->history_len, a.drafted = d->drafted;
@@ -251,20 +648,18 @@ extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *stream) {
     a.row = d->row, a.out_row = d->out_row, a.history_row = d->history_row;
     a.bias_row = d->bias_row, a.allowed_row = d->allowed_row, a.seen_words = d->seen_words;
     a.tokens = d->tokens, a.batch = d->batch, a.vocab = d->vocab;
-    a.history_wide = d->history_wide;
-    a.max_q = d->q_start ? (d->max_q < d->tokens ? d->max_q : d->tokens) : 1;
-    const int rc = attn_err_word(&a.err);
+    a.history_wide = d->history_wide, a.max_q = d->max_q;
+    char *const s = (char *)scratch;
+    a.best = (unsigned long long *)s, a.done = (unsigned *)(s + p.done_at);
+    a.bits = (uint32_t *)(s + p.bits_at), a.counts = s + p.counts_at;
+    a.words = p.words, a.slice = p.slice, a.slices = p.slices, a.pieces = p.pieces;
+    rc = attn_err_word(&a.err);
     if (rc) return rc;
-    const int size = 8;
-    a.part = (int)((cdiv(d->vocab, size) + 31) / 32 * 32);
-    if (a.part > kPickPart) a.part = kPickPart;
-    a.passes = (int)cdiv(d->vocab, (size_t)a.part * size);
-    a.rows = a.max_q < 4 ? a.max_q : 4;
-    a.groups = (int)cdiv(a.max_q, a.rows);
-    WARP_ARG((int64_t)a.batch * a.groups * size < (int64_t)1 << 31, "%s: %d requests of %d rows",
-             who, a.batch, a.max_q);
     cudaStream_t st = (cudaStream_t)stream;
-    return d->type == WARP_T_F32   ? pick_launch<float>(a, size, st)
-           : d->type == WARP_T_F16 ? pick_launch<__half>(a, size, st)
-                                   : pick_launch<__nv_bfloat16>(a, size, st);
+    if (d->type == WARP_T_F32)
+        return p.wide ? pick_run<float, uint32_t>(a, st) : pick_run<float, uint16_t>(a, st);
+    if (d->type == WARP_T_F16)
+        return p.wide ? pick_run<__half, uint32_t>(a, st) : pick_run<__half, uint16_t>(a, st);
+    return p.wide ? pick_run<__nv_bfloat16, uint32_t>(a, st)
+                  : pick_run<__nv_bfloat16, uint16_t>(a, st);
 }

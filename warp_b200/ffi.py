@@ -52,7 +52,8 @@ SIGNATURES = {
     "warp_paged_attention": (I, [P, P, P, P]),
     "warp_step_plan": (I, [P, P]),
     "warp_tree_attention": (I, [P, P, P, I64, P, P]),
-    "warp_pick_tokens": (I, [P, P]),
+    "warp_pick_scratch": (I64, [P]),
+    "warp_pick_tokens": (I, [P, P, P]),
     "warp_tree_accept": (I, [P, P, I, P, P, P]),
     "warp_attn_status": (I, [I]),
     "warp_moe_layer_create": (I, [P, I, P]),

@@ -624,7 +624,12 @@ def pick_tokens(logits, q_start=None, max_q=1, history=None, history_len=None, r
     d = ffi.PICK_DESC.pack(T, B, V, _TYPES[dt], max_q, logits.data_ptr(), row, op, orow,
                            picked.data_ptr(), qp, hp, lp, hrow, wide, *scalars, bp, brow, ap, arow,
                            dp, sp, words)
-    ffi.check(ffi.load().warp_pick_tokens(d, _stream()))
+    lib = ffi.load()
+    need = lib.warp_pick_scratch(d)
+    if need < 0:
+        ffi.check(need)
+    scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    ffi.check(lib.warp_pick_tokens(d, scratch.data_ptr() if need else None, _stream()))
     return picked
 
 
