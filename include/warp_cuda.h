@@ -415,10 +415,12 @@ typedef struct {
 
 WARP_API int warp_step_plan(const warp_plan_desc *d, void *stream);
 
-/* warp_paged_attention where a request's queries are the nodes of a tree: the
+/* warp_paged_attention where a request's queries are the nodes of a tree, with a
+ * scratch of warp_tree_scratch(d, c) bytes: the
  * request's own keys before its last n (n its queries) are seen by all, and of
  * the last n node i sees those of its row of masks, seen[t * seen_words ..].
  * seen_words is at least ceil(max_q / 64).  d->causal is not used. */
+WARP_API int64_t warp_tree_scratch(const warp_attn_desc *d, const warp_kv_pages *c);
 WARP_API int warp_tree_attention(const warp_attn_desc *d, const warp_kv_pages *c,
                                  const uint64_t *seen, int64_t seen_words, void *scratch,
                                  void *stream);

@@ -377,6 +377,105 @@ def test_tree_behind_long_context(cuda, D, n):
     Trees(trees_of([n, n]), [20001, 4096 + n // 2], 8, 2, D, 64, torch.bfloat16, seed=n).check()
 
 
+# Batches whose keys the card's blocks take equal runs of: items that begin and end within
+# a run, runs within an item, requests without nodes or keys in between.
+RAGGED = [1500, 3, 0, 129, 700, 128, 40, 1, 1023]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nodes, Hq, Hk", [(8, 24, 4), (32, 16, 4), (21, 24, 4), (100, 8, 8)])
+def test_runs(cuda, dtype, D, nodes, Hq, Hk):
+    sizes = [max(0, min(nodes - 3 * (b % 4), k)) for b, k in enumerate(RAGGED)]
+    sizes[4] = 0
+    Trees(trees_of(sizes), RAGGED, Hq, Hk, D, 16, dtype, seed=nodes).check()
+
+
+@pytest.mark.parametrize("batch", [31, 33, 70])
+def test_runs_of_many_requests(cuda, batch):
+    """More requests than a warp has lanes; most items lie within one run."""
+    rng = random.Random(batch)
+    kv = [rng.choice([0, 20, 127, 128, 129, 300]) for _ in range(batch)]
+    sizes = [min(k, rng.randint(0, 9)) for k in kv]
+    sizes[0], kv[0] = 9, 300
+    Trees(trees_of(sizes), kv, 16, 4, 64, 32, torch.bfloat16, seed=batch).check()
+
+
+@pytest.mark.parametrize("kv, prefix", [([20011], 0), ([5000], 1001), ([33], 9000)])
+def test_runs_of_one_request(cuda, kv, prefix):
+    """Every block has a part of few items, a prefix in the same pass."""
+    c = Trees(trees_of([30]), kv, 8, 2, 128, 64, torch.bfloat16, prefix=prefix, seed=prefix)
+    c.check()
+
+
+@pytest.mark.parametrize("nodes", [9, 30])
+def test_runs_are_the_same_every_time(cuda, nodes):
+    sizes = [min(nodes, k) for k in RAGGED]
+    c = Trees(trees_of(sizes), RAGGED, 16, 4, 128, 16, torch.bfloat16, seed=7)
+    want = c.run()
+    for _ in range(5):
+        assert torch.equal(c.run(), want)
+
+
+def test_runs_with_more_nodes_than_keys_and_empty_masks(cuda):
+    sizes = [30, 20, 7, 30, 30, 12]
+    c = Trees(trees_of(sizes, "chain"), [1000, 9, 0, 15, 700, 1], 16, 4, 128, 16, torch.float16,
+              seed=3)
+    seen = c.seen.clone()
+    seen[80:90] = 0                         # of the fourth request, without a key before them
+    got = c.check(seen)
+    first = starts_of(sizes)
+    assert not got[first[2]:first[3]].any() and not got[first[1]:first[1] + 11].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_runs_keep_what_is_not_seen_apart(cuda, dtype, bad):
+    """Values that are not finite, in several requests at once, reach who sees them alone."""
+    sizes = [20, 31, 9, 30, 25, 1]
+    c = Trees(trees_of(sizes, seed=5), [900, 300, 9, 158, 700, 1], 16, 4, 64, 16, dtype, seed=5)
+    clean, first = c.run(), starts_of(sizes)
+    sees = torch.zeros(sum(sizes), dtype=torch.bool)
+    for b, m in ((0, 7), (1, 30), (3, 12), (4, 3)):
+        j = c.kv_lens[b] - sizes[b] + m
+        c.v[c.pages[b, j // 16].long(), j % 16][2, 5] = bad
+        for i in range(sizes[b]):
+            sees[first[b] + i] = bool(int(c.seen[first[b] + i, 0]) >> m & 1)
+    got = c.run()
+    assert torch.equal(got[~sees], clean[~sees])
+    mine = torch.zeros(16, dtype=torch.bool)
+    mine[8:12] = True                       # of kv head 2
+    assert torch.equal(got[sees][:, ~mine], clean[sees][:, ~mine])
+    hit = got[sees][:, mine][..., 5].float()
+    assert (hit.isnan() if math.isnan(bad) else hit == bad).all()
+
+
+def test_runs_replay_while_lengths_change(cuda):
+    """A captured call reads the lengths, the nodes and the masks of its replay."""
+    from warp_b200 import ops
+    sizes = [min(9, k) for k in RAGGED]
+    c = Trees(trees_of(sizes), RAGGED, 16, 4, 128, 16, torch.bfloat16, seed=9)
+    args = [c.q.cuda(), c.k.cuda(), c.v.cuda(), c.pages.cuda(), i32(c.kv_lens).cuda(),
+            i32(starts_of(sizes)).cuda(), c.seen.cuda()]
+    out = torch.zeros_like(args[0])
+
+    def call():
+        ops.tree_attention(*args, 9, 1500, out=out)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for shorter in (0, 5, 300, 1499):
+        kv = [max(n, k - shorter) for n, k in zip(sizes, RAGGED)]
+        args[4].copy_(i32(kv))
+        c.kv_lens = kv
+        out.fill_(7.0)
+        graph.replay()
+        c.run = lambda seen: out.cpu()
+        c.check()
+    ops.attn_status()
+
+
 @pytest.mark.parametrize("sizes, kv", [([5], [2]), ([40, 3], [33, 1]), ([200], [100]), ([2, 1], [0, 4])])
 def test_more_nodes_than_keys(cuda, sizes, kv):
     """Nodes whose key would lie before the first have none."""
@@ -433,11 +532,14 @@ def test_what_a_node_does_not_see_has_no_effect(cuda, dtype, n, group, bad):
 
 @pytest.mark.parametrize("sizes, kv", [([3, 5], [50, 5]), ([90, 40], [300, 40])])
 def test_a_chain_is_causal(cuda, sizes, kv):
+    """Attention of the same rows without a tree is as near to the tree's definition."""
     from warp_b200 import ops
     c = Trees(trees_of(sizes, "chain"), kv, 8, 2, 128, 16, torch.bfloat16, seed=8)
-    want = ops.paged_attention(c.q.cuda(), c.k.cuda(), c.v.cuda(), c.pages.cuda(), i32(kv).cuda(),
-                               i32(starts_of(sizes)).cuda(), c.max_q, max(kv))
-    assert torch.equal(c.run(), want.cpu())
+    c.check()
+    c.run = lambda seen: ops.paged_attention(
+        c.q.cuda(), c.k.cuda(), c.v.cuda(), c.pages.cuda(), i32(kv).cuda(),
+        i32(starts_of(sizes)).cuda(), c.max_q, max(kv)).cpu()
+    c.check()
 
 
 def test_tree_rows_of_no_request_and_bounds(cuda):

@@ -548,6 +548,80 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     join_store<T, D>(a, row, l, acc);
 }
 
+// Joins the parts of the items that several blocks of runs had, as the blocks told; the
+// other items were written by those that had all of them.  The blocks here are shared out
+// among these items, and an item's rows among its blocks' warps.  The rows of requests
+// without a key, which are no item's, are made zeros.
+constexpr int kJoinBlocks = 4 * 148;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int V = D / 32, U = 8;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    pdl_wait();
+    // the items, and the one of this block: number blockIdx.x % all
+    int all = 0, mine = -1;
+    unsigned has[5];                        // 148 blocks of runs at most
+#pragma unroll
+    for (int i = 0; i < 5; i++) {
+        const int c = i * 32 + lane;
+        has[i] = __ballot_sync(~0u, c < a.runs && a.splits[c].c1);
+        all += __popc(has[i]);
+    }
+    if (all) {
+        int k = blockIdx.x % all;
+#pragma unroll
+        for (int i = 0; i < 5; i++) {
+            const int n = __popc(has[i]);
+            if (mine < 0 && k < n) mine = i * 32 + __fns(has[i], 0, k + 1);
+            k -= n;
+        }
+        const AttnSplit s = a.splits[mine];
+        const int slices = (kJoinBlocks - (int)blockIdx.x % all + all - 1) / all;
+        auto place = [&](int p) { return ((int64_t)p * 2 + (p == s.c0 && s.late)) * kAttnRunRows; };
+        for (int x = blockIdx.x / all * 8 + warp; x < s.rows; x += slices * 8) {
+            float M = -INFINITY;
+#pragma unroll 8
+            for (int p = s.c0; p <= s.c1; p++) M = fmaxf(M, a.part_ml[place(p) + x].x);
+            const float z = M == -INFINITY ? 0.f : M;
+            float l = 0.f, acc[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] = 0.f;
+            for (int p0 = s.c0; p0 <= s.c1; p0 += U) {
+                float v[U][V];
+                float2 ml[U];
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    if (p0 + k > s.c1) continue;
+                    const int64_t at = place(p0 + k) + x;
+                    ml[k] = a.part_ml[at];
+                    const float *const src = a.part_o + at * D + lane * V;
+                    if (V == 4) *(float4 *)v[k] = *(const float4 *)src;
+                    else *(float2 *)v[k] = *(const float2 *)src;
+                }
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    if (p0 + k > s.c1) continue;
+                    const float w = ex2(ml[k].x - z);
+                    l += w * ml[k].y;
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[i] += w * v[k][i];
+                }
+            }
+            const int tok = x / a.group;
+            join_store<T, D>(a, (int64_t)(s.t0 + tok) * a.q_heads + s.kvh * a.group + x - tok * a.group,
+                             l, acc);
+        }
+    }
+    for (int i = blockIdx.x; i < a.batch; i += kJoinBlocks) {
+        const AttnReq rq = attn_req(a, i, false);
+        if (attn_item(a, rq.n, rq.len)) continue;
+        uint4 *const to = (uint4 *)((T *)a.out + (int64_t)rq.t0 * a.q_heads * D);
+        const int64_t n = (int64_t)rq.n * a.q_heads * (D / 8);
+        for (int64_t x = threadIdx.x; x < n; x += 256) to[x] = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // ------------------------------------------------------------ host side --
 
 struct AttnPlan {
@@ -557,6 +631,7 @@ struct AttnPlan {
     int wide_each, wide_parts;              // and attn_umma_kernel (0 parts: not run)
     int small_tiles;                        // row tiles a request, attn_rows_kernel (0: not run)
     int join;
+    int runs;                               // blocks that take runs (0: none)
     int64_t o_bytes, ml_bytes;
     int max_q, max_kv;                      // the host's bounds, no wider than tokens and pages
 };
@@ -624,7 +699,7 @@ static int split_prefix(int64_t tiles, int64_t ctas, double bytes, double rows, 
     return (int)best;
 }
 
-static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
+static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c, bool tree) {
     AttnPlan p = {};
     p.max_q = d->max_q < d->tokens ? d->max_q : d->tokens;
     const int64_t held = (int64_t)d->pages_per_row * c->page_size;
@@ -637,6 +712,18 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     p.packed = d->prefix_len > 0 && d->batch > 1 && d->tokens * group <= (int64_t)128 * d->batch;
     const int pre = p.packed ? 0 : d->prefix_len;
     const int64_t rows = p.max_q * group;
+    // One row tile a kv head: the card's blocks take equal runs of the batch's keys,
+    // whatever the requests' lengths (32 trees of up to 16 nodes, 56 heads over 8, behind
+    // keys of unequal length up to 8192: 141 us against 163; with two row tiles, 36 nodes, 204
+    // against 169, as these have no other at work while they write their results).
+    const int64_t all = (up(p.max_kv, keys) + up(pre, keys)) * d->kv_heads * d->batch;
+    if (tree && !p.packed && rows > kADRows && rows <= kAttnRunRows && all > 148 &&
+        all < (int64_t)1 << 31) {
+        p.runs = 148;
+        p.o_bytes = up((int64_t)p.runs * 2 * kAttnRunRows * d->head_dim * 4, 256) * 256;
+        p.ml_bytes = up((int64_t)p.runs * (2 * kAttnRunRows * 8 + sizeof(AttnSplit)), 256) * 256;
+        return p;
+    }
     // A single request's rows are known to be more than a few: all of them wide.
     p.rows_small = d->batch == 1 && rows > kADRows ? 0 : kADRows;
     if (rows > p.rows_small) {
@@ -666,9 +753,9 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c) {
     }
     const int own = p.parts > p.wide_parts ? p.parts : p.wide_parts;
     p.join = p.packed || own > 1;
-    const int64_t all = p.join ? p.prefix_parts + own : 0;
-    p.o_bytes = up(all * out * d->head_dim * 4, 256) * 256;
-    p.ml_bytes = up(all * out * 8, 256) * 256;
+    const int64_t parts = p.join ? p.prefix_parts + own : 0;
+    p.o_bytes = up(parts * out * d->head_dim * 4, 256) * 256;
+    p.ml_bytes = up(parts * out * 8, 256) * 256;
     return p;
 }
 
@@ -726,6 +813,11 @@ static int attn_launch(AttnArgs a, const AttnPlan &p, bool first, cudaStream_t s
         count_launch();
         first = false;
     }
+    if (p.runs) {
+        e = attn_start(attn_join_runs_kernel<T, D>, dim3(kJoinBlocks), 256, 0, st, first, a);
+        if (e != cudaSuccess) return cuda_fail(e, "attn_join_runs_kernel");
+        count_launch();
+    }
     if (p.join) {
         // a token's heads in one block, or shared out while the card has room, down
         // to a block a row
@@ -747,7 +839,14 @@ static int attn_launch(AttnArgs a, const AttnPlan &p, bool first, cudaStream_t s
 extern "C" int64_t warp_attn_scratch(const warp_attn_desc *d, const warp_kv_pages *c) {
     const int rc = warp::attn_check(d, c);
     if (rc) return rc;
-    const warp::AttnPlan p = warp::attn_plan(d, c);
+    const warp::AttnPlan p = warp::attn_plan(d, c, false);
+    return p.o_bytes + p.ml_bytes;
+}
+
+extern "C" int64_t warp_tree_scratch(const warp_attn_desc *d, const warp_kv_pages *c) {
+    const int rc = warp::attn_check(d, c, "warp_tree_attention");
+    if (rc) return rc;
+    const warp::AttnPlan p = warp::attn_plan(d, c, true);
     return p.o_bytes + p.ml_bytes;
 }
 
@@ -763,7 +862,7 @@ static int attn_run(const warp_attn_desc *d, const warp_kv_pages *c, const uint6
     WARP_ARG(((uintptr_t)d->q & 15) == 0 && ((uintptr_t)d->out & 15) == 0 && d->q_token % 8 == 0 &&
                  d->q_head % 8 == 0,
              "%s: queries and results must be 16-byte aligned, strides multiples of 16 bytes", who);
-    const AttnPlan p = attn_plan(d, c);
+    const AttnPlan p = attn_plan(d, c, seen);
     WARP_ARG(p.o_bytes + p.ml_bytes == 0 || (scratch && ((uintptr_t)scratch & 255) == 0),
              "%s: scratch must be 256-byte aligned", who);
     AttnArgs a = {};
@@ -790,13 +889,18 @@ static int attn_run(const warp_attn_desc *d, const warp_kv_pages *c, const uint6
     a.by_wide_parts = attn_div(p.wide_parts), a.by_wide_each = attn_div(p.wide_each);
     a.by_prefix_parts = attn_div(p.prefix_parts);
     a.by_prefix_each = attn_div(p.prefix_each);
-    a.seen = seen, a.seen_words = seen_words;
+    a.seen = seen, a.seen_words = seen_words, a.runs = p.runs;
+    a.splits = (AttnSplit *)((char *)a.part_ml + (int64_t)p.runs * 2 * kAttnRunRows * 8);
     rc = attn_err_word(&a.err);
     if (rc) return rc;
     bool first = true;
     if (p.packed_wide) {
         a.more = 1;
         rc = attn_umma(a, c, kAttnPacked, first, st), first = false;
+    }
+    if (!rc && p.runs) {
+        a.more = 1;
+        rc = attn_umma(a, c, kAttnTreeRuns, first, st), first = false;
     }
     if (!rc && p.wide_parts) {
         a.more = p.small_tiles || p.join;

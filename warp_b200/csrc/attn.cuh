@@ -80,25 +80,31 @@ struct AttnArgs {
     // Trees: the nodes that token t sees, bit m of seen[t * seen_words + m / 64] for node m.
     const uint64_t *seen;
     int64_t seen_words;
+    int runs;                               // blocks of attn_umma_kernel, where they take runs
+    struct AttnSplit *splits;               // [runs], what they leave to be joined
 };
+
+// An item that blocks c0 .. c1 had a part of each (c1 0: none).  `late`: c0's run begins
+// before the item, whose part is then in its second place.
+struct AttnSplit { int c0, c1, late, t0, rows, kvh; };
 
 // What a kernel's rows and keys are: those of one request (causal or not), all the
 // batch's rows and the shared prefix, or those of one request whose queries are the
-// nodes of a tree.
-enum AttnKind { kAttnOwn, kAttnPacked, kAttnTree };
+// nodes of a tree; and the same with the batch's work in equal runs (AttnRuns).
+enum AttnKind { kAttnOwn, kAttnPacked, kAttnTree, kAttnTreeRuns };
 
 // Request b as the host's bounds leave it: its first token, its queries and
 // its own keys.
 struct AttnReq { int t0, n, len; };
 
-__device__ __forceinline__ AttnReq attn_req(const AttnArgs &a, int b) {
+__device__ __forceinline__ AttnReq attn_req(const AttnArgs &a, int b, bool report = true) {
     AttnReq r;
     const int s = a.q_start[b], e = a.q_start[b + 1], l = a.kv_len[b];
     r.t0 = min(max(s, 0), a.tokens);
     r.n = min(min(max(e - s, 0), a.max_q), a.tokens - r.t0);
     r.len = (int)min((int64_t)min(max(l, 0), a.max_kv),
                      (int64_t)a.pages_per_row << a.page_shift);
-    if (threadIdx.x == 0 && (r.t0 != s || r.n != e - s || r.len != l))
+    if (report && threadIdx.x == 0 && (r.t0 != s || r.n != e - s || r.len != l))
         atomicOr(a.err, kAttnBadLen);
     return r;
 }
@@ -133,6 +139,67 @@ __device__ __forceinline__ uint64_t low_bits(int n) {
 constexpr int kAttnTile = 16;
 // Keys a tile of attn_umma_kernel.
 __host__ __device__ constexpr int attn_wide(int) { return 128; }
+
+// The batch's work as one line of units, which the blocks take equal runs of: units are
+// key tiles of an item, an item is a request's rows, one row tile at most, on one kv head,
+// and items lie request by request.  An item that one block has all of is written by it; the
+// parts of others go to the two places that each block has, one for what its run
+// begins with and one for what it ends with, and are joined.  A request without rows or
+// keys has no units.
+constexpr int kAttnRunRows = 128;
+struct AttnRuns {
+    int all, blocks;
+    __device__ __forceinline__ int begin(int block) const {
+        return (int)((int64_t)all * block / blocks);
+    }
+    __device__ __forceinline__ int block_of(int u) const {
+        return (int)((((int64_t)u + 1) * blocks - 1) / all);
+    }
+};
+// Units of an item of n tokens and len own keys.
+__device__ __forceinline__ int attn_item(const AttnArgs &a, int n, int len) {
+    return n ? (a.prefix_len + attn_wide(0) - 1) / attn_wide(0) +
+                   (len + attn_wide(0) - 1) / attn_wide(0)
+             : 0;
+}
+// Units of request b, 0 past the batch; all are below 2^31 (the host sees to that).
+__device__ __forceinline__ int attn_units_of(const AttnArgs &a, int b) {
+    if (b >= a.batch) return 0;
+    const AttnReq r = attn_req(a, b, false);
+    return attn_item(a, r.n, r.len) * a.kv_heads;
+}
+// Units of the requests before request b, by all lanes of a warp.
+__device__ __forceinline__ int attn_units_before(const AttnArgs &a, int b) {
+    int sum = 0;
+    for (int i = threadIdx.x % 32; i < b; i += 32) sum += attn_units_of(a, i);
+    return __reduce_add_sync(~0u, sum);
+}
+// No more blocks than units, so that each has one.
+__device__ __forceinline__ AttnRuns attn_runs(const AttnArgs &a) {
+    const int all = attn_units_before(a, a.batch);
+    return {all, min(all, a.runs)};
+}
+// The request that has unit u, and the units before it.
+__device__ __forceinline__ int attn_units_at(const AttnArgs &a, int u, int &b) {
+    const int lane = threadIdx.x % 32;
+    int before = 0;
+    for (b = 0;; b += 32) {
+        const int mine = attn_units_of(a, b + lane);
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += x;
+        }
+        const unsigned has = __ballot_sync(~0u, before + upto > u);
+        if (has || b + 32 >= a.batch) {
+            const int k = has ? __ffs(has) - 1 : 0;
+            b += k;
+            return before + __shfl_sync(~0u, upto - mine, k);
+        }
+        before += __shfl_sync(~0u, upto, 31);
+    }
+}
 
 // How many parts a range of `tiles` key tiles is split into, `each` tiles a part.
 __device__ __forceinline__ int attn_parts(int tiles, int each) {

@@ -51,6 +51,7 @@ SIGNATURES = {
     "warp_attn_scratch": (I64, [P, P]),
     "warp_paged_attention": (I, [P, P, P, P]),
     "warp_step_plan": (I, [P, P]),
+    "warp_tree_scratch": (I64, [P, P]),
     "warp_tree_attention": (I, [P, P, P, I64, P, P]),
     "warp_pick_scratch": (I64, [P]),
     "warp_pick_tokens": (I, [P, P, P]),

@@ -446,7 +446,7 @@ def _attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale
         out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), row, wide, max_q,
         max_kv, causal, (D or 1) ** -0.5 if scale is None else scale, pp, prefix_len)
     lib = ffi.load()
-    need = lib.warp_attn_scratch(d, c)
+    need = (lib.warp_attn_scratch if seen is None else lib.warp_tree_scratch)(d, c)
     if need < 0:
         ffi.check(need)
     # from torch's allocator: ordered by the stream, and private to a graph
