@@ -469,7 +469,7 @@ WARP_API int warp_pick_tokens(const warp_pick_desc *d, void *scratch, void *stre
 /* The drafted tokens checked.  Node i of a request agrees if it is node 0, or if
  * drafted[i] is picked[p] of its parent p (the last node before it that it sees)
  * and not negative.  Of the nodes whose whole path from node 0 agrees, the
- * deepest (the first of equals) ends the accepted path.  Written for
+ * deepest (the first of equals) ends the accepted path.  max_q is 4096 at most.  Written for
  * each request:
  *   count   nodes of the path (0 for a request without nodes)
  *   path    [max_q] their numbers, ascending, then -1

@@ -121,7 +121,7 @@ def test_pick_refuses_bad_scratch(lib):
 
 @pytest.mark.parametrize("kw, ckw, text", [
     (dict(batch=-1), {}, b"negative"), (dict(max_q=65), {}, b"words"),
-    (dict(max_q=64 * 513, seen_words=513), {}, b"words"), (dict(seen=None), {}, b"masks"),
+    (dict(max_q=4097, seen_words=65), {}, b"nodes"), (dict(seen=None), {}, b"masks"),
     (dict(seen=260), {}, b"8-byte"), (dict(drafted=None), {}, b"NULL"), (dict(path=None), {}, b"NULL"),
     (dict(count=None), {}, b"NULL"), (dict(kv_after=256), {}, b"kv_after"),
     (dict(pages=None), {}, b"pages"), ({}, dict(page_size=24), b"page_size"),

@@ -12,6 +12,10 @@ that the requests have in common.
     step = Step.plan(q_lens, kv_lens, pages, page_size)      # once a step
     for block, (k_pages, v_pages) in zip(blocks, caches):
         h = block.forward(h, k_pages, v_pages, step)
+
+A step of drafted tokens (Step.draft) is planned on the device, pages included, and
+its attention is that of trees.  Decoder runs such steps from tokens to tokens:
+plan, embedding, blocks, head, pick, accept.
 """
 from dataclasses import dataclass
 
@@ -43,7 +47,8 @@ class Trunk:
 class Step:
     """One step's batch: request b brings q_lens[b] tokens, the last of its
     kv_lens[b] own keys, and keeps its keys in the pages of pages[b].  With a
-    prefix, prefix_len keys of prefix_pages come before every request's own."""
+    prefix, prefix_len keys of prefix_pages come before every request's own.  seen:
+    the masks of a step whose requests bring trees of drafted tokens."""
     q_start: torch.Tensor
     kv_len: torch.Tensor
     pages: torch.Tensor
@@ -53,6 +58,7 @@ class Step:
     slots: torch.Tensor
     prefix_pages: torch.Tensor = None
     prefix_len: int = 0
+    seen: torch.Tensor = None
 
     @classmethod
     def plan(cls, q_lens, kv_lens, pages, page_size, prefix_pages=None, prefix_len=0):
@@ -79,6 +85,18 @@ class Step:
                                         base=prefix_len)
         return cls(q_start, kv_len, pages, max(q_lens), max(kv_lens), positions, slots,
                    prefix_pages, prefix_len)
+
+    @classmethod
+    def draft(cls, q_start, kv_len, pages, page_size, tokens, max_q, parents=None, held=None,
+              pool=None, prefix_pages=None, prefix_len=0):
+        """A step whose lengths are on the device (ops.step_plan, which hands out the
+        pages with held and pool): request b brings tokens q_start[b] ..
+        q_start[b+1]-1, max_q at most, of `tokens` in all.  With parents they are the
+        nodes of a tree, else they follow one another."""
+        planned = ops.step_plan(q_start, kv_len, pages, page_size, tokens, base=prefix_len,
+                                held=held, pool=pool, parents=parents, max_q=max_q)
+        return cls(q_start, kv_len, pages, max_q, pages.shape[1] * page_size, *planned[:2],
+                   prefix_pages, prefix_len, planned[2] if len(planned) > 2 else None)
 
 
 class DecoderBlock:
@@ -110,9 +128,13 @@ class DecoderBlock:
         q = ops.kv_append(q, k, v, k_pages, v_pages, step.slots, step.positions, self.inv_freq,
                           q_norm=self.q_norm, k_norm=self.k_norm, eps=self.eps,
                           interleaved=self.interleaved, rot_scale=self.rot_scale)
-        o = ops.paged_attention(q, k_pages, v_pages, step.pages, step.kv_len, step.q_start,
-                                step.max_q, step.max_kv, scale=self.scale,
-                                prefix_pages=step.prefix_pages, prefix_len=step.prefix_len)
+        over = (q, k_pages, v_pages, step.pages, step.kv_len, step.q_start)
+        how = dict(max_q=step.max_q, max_kv=step.max_kv, scale=self.scale,
+                   prefix_pages=step.prefix_pages, prefix_len=step.prefix_len)
+        if step.seen is None:
+            o = ops.paged_attention(*over, **how)
+        else:
+            o = ops.tree_attention(*over, step.seen, **how)
         o = o.view(T, -1)
         # the trunk takes bf16 or fp32
         return h + self.proj(o if o.dtype is torch.bfloat16 else o.float())
@@ -123,3 +145,65 @@ class DecoderBlock:
         if h.shape[0] <= self.moe.max_tokens:
             return self.moe.forward_block(h, torch.empty_like(h), self.norm2, self.eps)
         return self.moe.prefill(ops.rmsnorm(h, self.norm2, self.eps), residual=h)
+
+
+class Decoder:
+    """Blocks between an embedding and an output head, over the caches of all layers,
+    for a fixed number of requests whose pages come from one pool.
+
+    embed fp32 [vocabulary][hidden]; norm fp32 [hidden]; head: Trunk
+    [vocabulary][hidden]; k_pages / v_pages
+    [layers][pages][page_size][kv_heads][head_dim].  kv_len (int32 [requests], on the
+    device) is how many keys each request has: set it to 0 for one that ends, and its
+    pages go back with the next step.  Nothing here waits for the device."""
+
+    def __init__(self, blocks, embed, norm, head, k_pages, v_pages, requests,
+                 pages_per_request, eps=1e-6):
+        if k_pages.dim() != 5 or k_pages.shape != v_pages.shape or len(blocks) != len(k_pages):
+            raise ValueError("the caches must be [layers][pages][page_size][kv_heads][head_dim], "
+                             "a layer for each block")
+        if head.in_ != embed.shape[1] or head.out != embed.shape[0]:
+            raise ValueError("the head does not fit the embedding")
+        self.blocks, self.embed, self.norm, self.head, self.eps = blocks, embed, norm, head, eps
+        self.k_pages, self.v_pages, self.page_size = k_pages, v_pages, k_pages.shape[2]
+        dev = k_pages.device
+        self.pool = ops.page_pool(k_pages.shape[1], dev)
+        self.pages = torch.full((requests, pages_per_request), -1, dtype=torch.int32, device=dev)
+        self.held = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.kv_len = torch.zeros(requests, dtype=torch.int32, device=dev)
+
+    def _forward(self, tokens, q_start, max_q, parents=None):
+        """(states behind the last block, the step)."""
+        kv_len = self.kv_len + (q_start[1:] - q_start[:-1])
+        step = Step.draft(q_start, kv_len, self.pages, self.page_size, tokens.numel(), max_q,
+                          parents, self.held, self.pool)
+        h = self.embed[tokens.clamp(min=0)]
+        for block, k, v in zip(self.blocks, self.k_pages, self.v_pages):
+            h = block.forward(h, k, v, step)
+        return h, step
+
+    def _logits(self, h):
+        return self.head(ops.rmsnorm(h, self.norm, self.eps))
+
+    def extend(self, tokens, q_start, max_q, **choice):
+        """The requests' next tokens (int32, certain ones: a prompt, a chunk of one or a
+        single token), max_q a request at most, through the blocks; returns the
+        token picked behind each request's last, int32 [requests] (of no meaning where a
+        request brings none).  choice: what ops.pick_tokens weighs, a row a request."""
+        h, step = self._forward(tokens, q_start, max_q)
+        self.kv_len.copy_(step.kv_len)
+        return ops.pick_tokens(self._logits(h[(q_start[1:] - 1).clamp(min=0)]), **choice)
+
+    def verify(self, drafted, parents, q_start, max_q, **choice):
+        """A step of drafted trees: request b's nodes are tokens q_start[b] ..
+        q_start[b+1]-1, node 0 the last certain token, which is not in the cache yet.
+        Returns (count, chosen) of ops.tree_accept: chosen[b][:count[b]] are the
+        request's new tokens, the last of which is the next tree's node 0."""
+        h, step = self._forward(drafted, q_start, max_q, parents)
+        picked = ops.pick_tokens(self._logits(h), q_start, max_q, drafted=drafted, seen=step.seen,
+                                 **choice)
+        count, _, chosen, kv_len = ops.tree_accept(
+            drafted, picked, step.seen, q_start, step.kv_len, max_q,
+            caches=(self.k_pages, self.v_pages), pages=self.pages)
+        self.kv_len.copy_(kv_len)
+        return count, chosen

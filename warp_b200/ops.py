@@ -327,11 +327,15 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6,
     return q_out, k_out
 
 
-def _pages_pack(k_pages, v_pages, dev):
+def _pages_pack(k_pages, v_pages, dev, skip=0):
+    """The description of pages; `skip`: axes before theirs."""
     if k_pages.get_device() != dev or v_pages.get_device() != dev:
         _elsewhere(k_pages if k_pages.get_device() != dev else v_pages)
     shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
-    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or \
+    same = shape == v_pages.shape
+    if skip:
+        shape, ks, vs = shape[skip:], ks[skip:], vs[skip:]
+    if len(shape) != 4 or not same or k_pages.dtype is not v_pages.dtype or \
             (shape[3] > 1 and (ks[3] != 1 or vs[3] != 1)):
         raise ValueError("k_pages and v_pages must be [pages][page_size][kv_heads][head_dim] "
                          "of one shape and dtype with contiguous heads")
@@ -653,10 +657,6 @@ def tree_accept(drafted, picked, seen, q_start, kv_len, max_q, caches=(), pages=
     words = _seen_ok(seen, T, max_q, dev)
     if not _vec_ok(drafted, T, torch.int32, dev) or not _vec_ok(picked, T, torch.int32, dev):
         raise ValueError("drafted and picked must be contiguous int32 [tokens]")
-    if not _vec_ok(kv_len, B, torch.int32, dev):
-        raise ValueError("kv_len must be contiguous int32 [batch]")
-    if not _vec_ok(q_start, B + 1, torch.int32, dev):
-        raise ValueError("q_start must be contiguous int32 [batch + 1]")
     n = row = wide = tp = 0
     c = ks = vs = None
     if len(caches):
@@ -665,10 +665,13 @@ def tree_accept(drafted, picked, seen, q_start, kv_len, max_q, caches=(), pages=
         _, row, wide = _batch(q_start, kv_len, pages, dev)
         tp = pages.data_ptr()
         n, c, ks, vs = _caches_pack(caches, dev)
-    count = torch.empty(2, B, dtype=torch.int32, device=kv_len.device)
-    path = torch.empty(2, B, max_q, dtype=torch.int32, device=kv_len.device)
-    count, after = count.unbind()
-    path, chosen = path.unbind()
+    elif not _vec_ok(kv_len, B, torch.int32, dev):
+        raise ValueError("kv_len must be contiguous int32 [batch]")
+    elif not _vec_ok(q_start, B + 1, torch.int32, dev):
+        raise ValueError("q_start must be contiguous int32 [batch + 1]")
+    count, after = torch.empty_like(kv_len), torch.empty_like(kv_len)
+    path = kv_len.new_empty((B, max_q))
+    chosen = torch.empty_like(path)
     d = ffi.ACCEPT_DESC.pack(B, T, max_q, drafted.data_ptr(), picked.data_ptr(), seen.data_ptr(),
                              words, q_start.data_ptr(), kv_len.data_ptr(), tp, row, wide,
                              count.data_ptr(), path.data_ptr(), chosen.data_ptr(),
@@ -681,14 +684,17 @@ def _caches_pack(caches, dev):
     """(layers, their layout, addresses of their keys and of their values)."""
     if isinstance(caches[0], torch.Tensor):
         k, v = caches
-        if k.dim() != 5 or v.dim() != 5 or k.shape[0] != v.shape[0]:
+        if k.dim() != 5 or v.dim() != 5:
             raise ValueError("caches must be a pair [layers][pages][page_size][kv_heads][head_dim]")
         n = k.shape[0]
         if not n:
             return 0, None, None, None
-        c = _pages_pack(k[0], v[0], dev)
-        at = [struct.pack(f"@{n}P", *(x.data_ptr() + i * x.stride(0) * x.element_size()
-                                      for i in range(n))) for x in (k, v)]
+        c = _pages_pack(k, v, dev, 1)
+        at = []
+        for x in (k, v):
+            first, step = x.data_ptr(), x.stride(0) * x.element_size()
+            at.append(struct.pack(f"@{n}P", *(range(first, first + n * step, step) if step
+                                              else [first] * n)))
         return n, c, *at
     packed = [_pages_pack(k, v, dev) for k, v in caches]
     if any(x[16:] != packed[0][16:] for x in packed):
