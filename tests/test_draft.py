@@ -114,8 +114,10 @@ def test_pick_refusals(lib, kw, text):
 
 
 def test_pick_refuses_bad_scratch(lib):
+    many = pick_desc(tokens=600, max_q=600, vocab=4000, row=4000, seen_words=10)
+    assert lib.warp_pick_scratch(ctypes.byref(many)) > 0
     for at in (None, 264):
-        assert lib.warp_pick_tokens(ctypes.byref(pick_desc()), at, None) == -1
+        assert lib.warp_pick_tokens(ctypes.byref(many), at, None) == -1
         assert b"scratch" in lib.warp_last_error()
 
 

@@ -672,6 +672,112 @@ def test_pick_strides(cuda, dtype, offset, row, in_place):
         assert (room == 77).all()
 
 
+# Above a million logits a call goes the way of large ones.
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sizes, V", [([3, 0, 40, 1, 26], 16001), ([12], 100003), ([1] * 33, 32000),
+                                      ([2, 3], 262149), ([1] * 600, 2049)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_pick_many(cuda, dtype, sizes, V, keep):
+    Logits(sizes, V, dtype, seed=V, bias="each", masked=True, history=3000).check(keep)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(penalties=False, tree=False), dict(penalties=False), dict(tree=False), dict(),
+    dict(bias="all"), dict(masked=True), dict(far=True), dict(history=20000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pick_many_parts(cuda, dtype, kw):
+    Logits([30, 1, 40], 16004, dtype, seed=6, **kw).check()
+
+
+def test_pick_long_histories(cuda):
+    """Tokens that occur more often than 16 bits count, in a history that says so."""
+    from warp_b200 import ops
+    V, rep = 40000, torch.full((30,), 2.0, device="cuda")
+    x = torch.zeros(30, V, device="cuda")
+    x[:, 77], x[:, 5] = 9.0, 8.0
+    history = torch.full((30, 70001), 77, dtype=torch.int32, device="cuda")
+    history[:, ::3] = torch.arange(23334, device="cuda").int()
+    freq = torch.full((30,), 2.0 ** -14, device="cuda")
+    out = torch.empty_like(x)
+    lens = i32([70001 - 7 * b for b in range(30)]).cuda()
+    picked = ops.pick_tokens(x, history=history, history_len=lens, repetition=rep, frequency=freq,
+                             out=out)
+    ops.attn_status()
+    count = torch.stack([torch.bincount(h[:n].long(), minlength=V) for h, n in zip(history, lens)])
+    want = torch.where(count > 0, x / 2 - freq[:, None] * count.float(), x)
+    assert torch.equal(out, want) and count[:, 77].min() > 46000
+    assert picked.tolist() == want.argmax(1).tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset, row", [(0, 2003), (1, 2003), (3, 2048), (5, 2001), (8, 2008)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_pick_many_strides(cuda, dtype, offset, row, in_place):
+    base = []
+
+    def place(x):
+        room = torch.full((len(x) * row + 40,), 77.0, dtype=dtype, device="cuda")
+        y = torch.as_strided(room, x.shape, (row, 1), offset)
+        y.copy_(x)
+        base.append((room, y))
+        return y
+    Logits([300, 1, 299], 2000, dtype, seed=offset, bias="all").check(place=place,
+                                                                      in_place=in_place)
+    for room, y in base:
+        y.fill_(77.0)
+        assert (room == 77).all()
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e30, 3e38])
+@pytest.mark.parametrize("repetition", [1.0, 1.1, 3.0, 1e-7, 1e7, 1e30])
+def test_pick_divides_as_a_division(cuda, scale, repetition):
+    """At the numbers' ends, where a product by the reciprocal would be off."""
+    from warp_b200 import ops
+    g = torch.Generator().manual_seed(4)
+    x = (torch.randn(40, 30000, generator=g) * scale).cuda()
+    rep = torch.full((40,), repetition, device="cuda")
+    history = torch.arange(30000, dtype=torch.int32, device="cuda").expand(40, 30000).contiguous()
+    out = torch.empty_like(x)
+    ops.pick_tokens(x, history=history, repetition=rep, out=out,
+                    history_len=torch.full((40,), 30000, dtype=torch.int32, device="cuda"))
+    ops.attn_status()
+    assert torch.equal(out, torch.where(x > 0, x / rep[:, None], x * rep[:, None]))
+
+
+def test_pick_reciprocals_divide_exactly(cuda):
+    """The corrected product by a reciprocal against the division, over many divisors."""
+    from warp_b200 import ops
+    g = torch.Generator().manual_seed(8)
+    B, V = 4096, 4096
+    rep = (1 + torch.rand(B, generator=g)).cuda()
+    rep[:1024] = torch.exp2(torch.rand(1024, generator=g) * 40 - 20).cuda()
+    rep[0], rep[1], rep[2] = 1.0, 2 - 2.0 ** -23, 1 + 2.0 ** -23
+    x = (torch.randn(B, V, generator=g) * 8).abs().cuda()
+    history = torch.arange(V, dtype=torch.int32, device="cuda").expand(B, V).contiguous()
+    out = torch.empty_like(x)
+    ops.pick_tokens(x, history=history, repetition=rep, out=out,
+                    history_len=torch.full((B,), V, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out, x / rep[:, None])
+
+
+def test_pick_many_ties_and_what_is_not_finite(cuda):
+    from warp_b200 import ops
+    x = torch.zeros(300, 5000)
+    x[1, 4000] = x[1, 17] = x[1, 4999] = 2.0
+    x[2] = -math.inf
+    x[3] = -math.inf
+    x[3, 4321] = -1e30
+    x[4] = math.nan
+    x[5, ::2] = math.nan
+    x[6] = -0.0
+    x[6, 3000] = 0.0
+    x[7, 2500:] = math.inf
+    want = [0, 17, -1, 4321, -1, 1, 0, 2500] + [0] * 292
+    assert ops.pick_tokens(x.cuda()).tolist() == want
+    none = torch.zeros(157, dtype=torch.int32, device="cuda")
+    assert ops.pick_tokens(x.cuda(), allowed=none).tolist() == [-1] * 300
+
+
 def test_pick_without_requests(cuda):
     """A row a request, and no context: the plain largest."""
     from warp_b200 import ops
