@@ -247,7 +247,8 @@ class Trees:
     """Ragged requests whose queries are trees, over shuffled pages; what no request
     owns is NaN."""
 
-    def __init__(self, trees, kv_lens, Hq, Hk, D, page, dtype, heads_first=False, prefix=0, seed=0):
+    def __init__(self, trees, kv_lens, Hq, Hk, D, page, dtype, heads_first=False, prefix=0, seed=0,
+                 runs=False):
         g = torch.Generator().manual_seed(seed)
         self.trees, self.kv_lens, self.prefix, self.page = trees, kv_lens, prefix, page
         self.q_lens = [len(t) for t in trees]
@@ -270,7 +271,12 @@ class Trees:
         self.k, self.v = k.to(dtype), v.to(dtype)
         self.q = torch.randn(sum(self.q_lens), Hq, D, generator=g).to(dtype)
         self.heads_first = heads_first
-        self.max_q = max(self.q_lens)
+        self.max_q, self.max_kv = max(self.q_lens), max(kv_lens)
+        if runs:                            # by a bound, and a table for as many keys
+            assert B > 1 and 16 < self.max_q * Hq // Hk <= 128 and not prefix
+            self.max_kv = 128 * -(-8192 // (B * Hk))
+            more = self.max_kv // page - wide
+            self.pages = torch.cat((self.pages, torch.full((B, more), -7, dtype=torch.int32)), 1)
         self.seen = seen_of(trees, self.max_q)
 
     def place(self, x):
@@ -283,7 +289,7 @@ class Trees:
         out = ops.tree_attention(
             self.q.cuda(), self.place(self.k), self.place(self.v), self.pages.cuda(),
             i32(self.kv_lens).cuda(), i32(starts_of(self.q_lens)).cuda(),
-            (self.seen if seen is None else seen).cuda(), self.max_q, max(self.kv_lens),
+            (self.seen if seen is None else seen).cuda(), self.max_q, self.max_kv,
             prefix_pages=self.pp.cuda() if self.prefix else None, prefix_len=self.prefix, **kw)
         ops.attn_status()
         return out.cpu()
@@ -388,7 +394,7 @@ RAGGED = [1500, 3, 0, 129, 700, 128, 40, 1, 1023]
 def test_runs(cuda, dtype, D, nodes, Hq, Hk):
     sizes = [max(0, min(nodes - 3 * (b % 4), k)) for b, k in enumerate(RAGGED)]
     sizes[4] = 0
-    Trees(trees_of(sizes), RAGGED, Hq, Hk, D, 16, dtype, seed=nodes).check()
+    Trees(trees_of(sizes), RAGGED, Hq, Hk, D, 16, dtype, seed=nodes, runs=True).check()
 
 
 @pytest.mark.parametrize("batch", [31, 33, 70])
@@ -398,20 +404,21 @@ def test_runs_of_many_requests(cuda, batch):
     kv = [rng.choice([0, 20, 127, 128, 129, 300]) for _ in range(batch)]
     sizes = [min(k, rng.randint(0, 9)) for k in kv]
     sizes[0], kv[0] = 9, 300
-    Trees(trees_of(sizes), kv, 16, 4, 64, 32, torch.bfloat16, seed=batch).check()
+    Trees(trees_of(sizes), kv, 16, 4, 64, 32, torch.bfloat16, seed=batch, runs=True).check()
 
 
-@pytest.mark.parametrize("kv, prefix", [([20011], 0), ([5000], 1001), ([33], 9000)])
-def test_runs_of_one_request(cuda, kv, prefix):
-    """Every block has a part of few items, a prefix in the same pass."""
-    c = Trees(trees_of([30]), kv, 8, 2, 128, 64, torch.bfloat16, prefix=prefix, seed=prefix)
-    c.check()
+@pytest.mark.parametrize("sizes, kv", [([30, 0], [20011, 0]), ([0, 30], [50, 5000]),
+                                       ([9, 9], [40000, 1]), ([5, 9, 0], [0, 0, 0]),
+                                       ([30, 1], [100, 0])])
+def test_runs_of_few_items(cuda, sizes, kv):
+    """Every block has a part of the same items, or none has any."""
+    Trees(trees_of(sizes), kv, 8, 2, 128, 64, torch.bfloat16, seed=kv[0], runs=True).check()
 
 
 @pytest.mark.parametrize("nodes", [9, 30])
 def test_runs_are_the_same_every_time(cuda, nodes):
     sizes = [min(nodes, k) for k in RAGGED]
-    c = Trees(trees_of(sizes), RAGGED, 16, 4, 128, 16, torch.bfloat16, seed=7)
+    c = Trees(trees_of(sizes), RAGGED, 16, 4, 128, 16, torch.bfloat16, seed=7, runs=True)
     want = c.run()
     for _ in range(5):
         assert torch.equal(c.run(), want)
@@ -420,7 +427,7 @@ def test_runs_are_the_same_every_time(cuda, nodes):
 def test_runs_with_more_nodes_than_keys_and_empty_masks(cuda):
     sizes = [30, 20, 7, 30, 30, 12]
     c = Trees(trees_of(sizes, "chain"), [1000, 9, 0, 15, 700, 1], 16, 4, 128, 16, torch.float16,
-              seed=3)
+              seed=3, runs=True)
     seen = c.seen.clone()
     seen[80:90] = 0                         # of the fourth request, without a key before them
     got = c.check(seen)
@@ -433,7 +440,8 @@ def test_runs_with_more_nodes_than_keys_and_empty_masks(cuda):
 def test_runs_keep_what_is_not_seen_apart(cuda, dtype, bad):
     """Values that are not finite, in several requests at once, reach who sees them alone."""
     sizes = [20, 31, 9, 30, 25, 1]
-    c = Trees(trees_of(sizes, seed=5), [900, 300, 9, 158, 700, 1], 16, 4, 64, 16, dtype, seed=5)
+    c = Trees(trees_of(sizes, seed=5), [900, 300, 9, 158, 700, 1], 16, 4, 64, 16, dtype, seed=5,
+              runs=True)
     clean, first = c.run(), starts_of(sizes)
     sees = torch.zeros(sum(sizes), dtype=torch.bool)
     for b, m in ((0, 7), (1, 30), (3, 12), (4, 3)):
@@ -454,13 +462,13 @@ def test_runs_replay_while_lengths_change(cuda):
     """A captured call reads the lengths, the nodes and the masks of its replay."""
     from warp_b200 import ops
     sizes = [min(9, k) for k in RAGGED]
-    c = Trees(trees_of(sizes), RAGGED, 16, 4, 128, 16, torch.bfloat16, seed=9)
+    c = Trees(trees_of(sizes), RAGGED, 16, 4, 128, 16, torch.bfloat16, seed=9, runs=True)
     args = [c.q.cuda(), c.k.cuda(), c.v.cuda(), c.pages.cuda(), i32(c.kv_lens).cuda(),
             i32(starts_of(sizes)).cuda(), c.seen.cuda()]
     out = torch.zeros_like(args[0])
 
     def call():
-        ops.tree_attention(*args, 9, 1500, out=out)
+        ops.tree_attention(*args, 9, c.max_kv, out=out)
     call()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
@@ -561,7 +569,7 @@ def test_tree_rows_of_no_request_and_bounds(cuda):
 
 class Logits:
     def __init__(self, sizes, V, dtype, seed=0, history=50, penalties=True, bias=None,
-                 masked=False, tree=True, far=False):
+                 masked=False, tree=True, far=False, large=False):
         rng, g = random.Random(seed), torch.Generator().manual_seed(seed)
         self.sizes, self.V = sizes, V
         B, T = len(sizes), sum(sizes)
@@ -573,7 +581,8 @@ class Logits:
         self.drafted = [rng.choice([0, V - 1, rng.randint(-2 if far else 0, top)]) for _ in range(T)]
         self.trees = [random_parents(rng, n, "any") if n else [] for n in sizes]
         if penalties:
-            wide = max(1, max(map(len, self.history)))
+            # a history with more places than this goes the way of large calls
+            wide = 16400 if large else max(1, max(map(len, self.history)))
             self.kw.update(history=i32([h + [0] * (wide - len(h)) for h in self.history]),
                            history_len=i32([len(h) for h in self.history]),
                            repetition=1 + torch.rand(B, generator=g),
@@ -672,21 +681,21 @@ def test_pick_strides(cuda, dtype, offset, row, in_place):
         assert (room == 77).all()
 
 
-# Above a million logits a call goes the way of large ones.
+# Calls that go the way of large ones: by a history of many places, or by a vocabulary.
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("sizes, V", [([3, 0, 40, 1, 26], 16001), ([12], 100003), ([1] * 33, 32000),
                                       ([2, 3], 262149), ([1] * 600, 2049)])
 @pytest.mark.parametrize("keep", [False, True])
 def test_pick_many(cuda, dtype, sizes, V, keep):
-    Logits(sizes, V, dtype, seed=V, bias="each", masked=True, history=3000).check(keep)
+    Logits(sizes, V, dtype, seed=V, bias="each", masked=True, history=3000, large=True).check(keep)
 
 
 @pytest.mark.parametrize("kw", [
     dict(penalties=False, tree=False), dict(penalties=False), dict(tree=False), dict(),
-    dict(bias="all"), dict(masked=True), dict(far=True), dict(history=20000)])
+    dict(bias="all"), dict(masked=True), dict(far=True), dict(history=16000)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_pick_many_parts(cuda, dtype, kw):
-    Logits([30, 1, 40], 16004, dtype, seed=6, **kw).check()
+    Logits([5, 1, 3], 131204, dtype, seed=6, large=True, **kw).check()
 
 
 def test_pick_long_histories(cuda):
@@ -721,8 +730,8 @@ def test_pick_many_strides(cuda, dtype, offset, row, in_place):
         y.copy_(x)
         base.append((room, y))
         return y
-    Logits([300, 1, 299], 2000, dtype, seed=offset, bias="all").check(place=place,
-                                                                      in_place=in_place)
+    Logits([30, 1, 29], 2000, dtype, seed=offset, bias="all", large=True).check(
+        place=place, in_place=in_place)
     for room, y in base:
         y.fill_(77.0)
         assert (room == 77).all()
@@ -734,7 +743,7 @@ def test_pick_divides_as_a_division(cuda, scale, repetition):
     """At the numbers' ends, where a product by the reciprocal would be off."""
     from warp_b200 import ops
     g = torch.Generator().manual_seed(4)
-    x = (torch.randn(40, 30000, generator=g) * scale).cuda()
+    x = (torch.randn(40, 30000, generator=g) * scale).cuda()    # by the places of the history
     rep = torch.full((40,), repetition, device="cuda")
     history = torch.arange(30000, dtype=torch.int32, device="cuda").expand(40, 30000).contiguous()
     out = torch.empty_like(x)
@@ -762,7 +771,7 @@ def test_pick_reciprocals_divide_exactly(cuda):
 
 def test_pick_many_ties_and_what_is_not_finite(cuda):
     from warp_b200 import ops
-    x = torch.zeros(300, 5000)
+    x = torch.zeros(1300, 5000)
     x[1, 4000] = x[1, 17] = x[1, 4999] = 2.0
     x[2] = -math.inf
     x[3] = -math.inf
@@ -772,10 +781,10 @@ def test_pick_many_ties_and_what_is_not_finite(cuda):
     x[6] = -0.0
     x[6, 3000] = 0.0
     x[7, 2500:] = math.inf
-    want = [0, 17, -1, 4321, -1, 1, 0, 2500] + [0] * 292
+    want = [0, 17, -1, 4321, -1, 1, 0, 2500] + [0] * 1292
     assert ops.pick_tokens(x.cuda()).tolist() == want
     none = torch.zeros(157, dtype=torch.int32, device="cuda")
-    assert ops.pick_tokens(x.cuda(), allowed=none).tolist() == [-1] * 300
+    assert ops.pick_tokens(x.cuda(), allowed=none).tolist() == [-1] * 1300
 
 
 def test_pick_without_requests(cuda):

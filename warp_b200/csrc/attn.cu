@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_consta
     }
     for (int i = blockIdx.x; i < a.batch; i += kJoinBlocks) {
         const AttnReq rq = attn_req(a, i, false);
-        if (attn_item(a, rq.n, rq.len)) continue;
+        if (attn_item(rq.n, rq.len)) continue;
         uint4 *const to = (uint4 *)((T *)a.out + (int64_t)rq.t0 * a.q_heads * D);
         const int64_t n = (int64_t)rq.n * a.q_heads * (D / 8);
         for (int64_t x = threadIdx.x; x < n; x += 256) to[x] = make_uint4(0, 0, 0, 0);
@@ -712,13 +712,16 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c, bool 
     p.packed = d->prefix_len > 0 && d->batch > 1 && d->tokens * group <= (int64_t)128 * d->batch;
     const int pre = p.packed ? 0 : d->prefix_len;
     const int64_t rows = p.max_q * group;
-    // One row tile a kv head: the card's blocks take equal runs of the batch's keys,
-    // whatever the requests' lengths (32 trees of up to 16 nodes, 56 heads over 8, behind
-    // keys of unequal length up to 8192: 141 us against 163; with two row tiles, 36 nodes, 204
-    // against 169, as these have no other at work while they write their results).
-    const int64_t all = (up(p.max_kv, keys) + up(pre, keys)) * d->kv_heads * d->batch;
-    if (tree && !p.packed && rows > kADRows && rows <= kAttnRunRows && all > 148 &&
-        all < (int64_t)1 << 31) {
+    // One row tile a kv head and many keys of several requests: the card's blocks take
+    // equal runs of the batch's keys, whatever the requests' lengths.  56 heads over 8,
+    // lengths from a fifth of the largest up, against the parts below: 32 trees of up to 16
+    // nodes 141 us against 163 behind up to 8192 keys, 88.6 and 87.3 behind 4096, 63 and 52 behind
+    // 2048; 3 of 8 nodes behind 65536 101 and 137; one behind 131072 102 and 101; and with two
+    // row tiles (36 nodes, 8192 keys), which have no other at work while they write their results,
+    // 204 and 169.
+    const int64_t all = up(p.max_kv, keys) * d->kv_heads * d->batch;
+    if (tree && d->prefix_len == 0 && d->batch > 1 && rows > kADRows && rows <= kAttnRunRows &&
+        all >= 8192 && all < (int64_t)1 << 31) {
         p.runs = 148;
         p.o_bytes = up((int64_t)p.runs * 2 * kAttnRunRows * d->head_dim * 4, 256) * 256;
         p.ml_bytes = up((int64_t)p.runs * (2 * kAttnRunRows * 8 + sizeof(AttnSplit)), 256) * 256;

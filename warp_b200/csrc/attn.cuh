@@ -157,16 +157,14 @@ struct AttnRuns {
     }
 };
 // Units of an item of n tokens and len own keys.
-__device__ __forceinline__ int attn_item(const AttnArgs &a, int n, int len) {
-    return n ? (a.prefix_len + attn_wide(0) - 1) / attn_wide(0) +
-                   (len + attn_wide(0) - 1) / attn_wide(0)
-             : 0;
+__device__ __forceinline__ int attn_item(int n, int len) {
+    return n ? (len + attn_wide(0) - 1) / attn_wide(0) : 0;
 }
 // Units of request b, 0 past the batch; all are below 2^31 (the host sees to that).
 __device__ __forceinline__ int attn_units_of(const AttnArgs &a, int b) {
     if (b >= a.batch) return 0;
     const AttnReq r = attn_req(a, b, false);
-    return attn_item(a, r.n, r.len) * a.kv_heads;
+    return attn_item(r.n, r.len) * a.kv_heads;
 }
 // Units of the requests before request b, by all lanes of a warp.
 __device__ __forceinline__ int attn_units_before(const AttnArgs &a, int b) {

@@ -391,7 +391,7 @@ template <typename T, int D, AttnKind KIND> struct WideTasks {
                 AttnSplit x = {};
                 const int from = u - k.cnt - k.first, c0 = k.first ? runs.block_of(from) : 0;
                 if (k.first && c0 == (int)blockIdx.x - 1)
-                    x = {c0, runs.block_of(from + attn_item(a, k.rq.n, k.rq.len) - 1),
+                    x = {c0, runs.block_of(from + attn_item(k.rq.n, k.rq.len) - 1),
                          runs.begin(c0) < from, k.rq.t0, k.rows, k.kvh};
                 a.splits[blockIdx.x] = x;
             }
@@ -430,7 +430,7 @@ template <typename T, int D, AttnKind KIND> struct WideTasks {
         const int in = u - attn_units_at(a, u, k.b);
         k.rq = attn_req(a, k.b);
         k.rows = k.rq.n * a.group;
-        const int tiles = attn_item(a, k.rq.n, k.rq.len);
+        const int tiles = attn_item(k.rq.n, k.rq.len);
         k.kvh = in / tiles;
         k.first = in - k.kvh * tiles;
         k.row0 = 0;
@@ -455,7 +455,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     WideTasks<T, D, KIND> tasks{a};
     WideTask task;
     if (!tasks.begin(task)) return;
-    const int n_pre = PACKED || !a.packed ? a.prefix_len : 0;
+    const int n_pre = !RUNS && (PACKED || !a.packed) ? a.prefix_len : 0;
     const int pre_tiles = (n_pre + KEYS - 1) / KEYS;
 
     const uint32_t base = smem_u32(basep);
@@ -682,7 +682,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 note[kFirst] = task.first, note[kCnt] = task.cnt, note[kSteps] = task.steps;
                 note[kU] = tasks.u, note[kHi] = tasks.hi, note[kDone] = done;
                 note[kTile] = task.tile;
-                note[kMask] = pre_tiles + max(task.rq.len - task.rq.n, 0) / KEYS - task.first;
+                note[kMask] = max(task.rq.len - task.rq.n, 0) / KEYS - task.first;
             }
             if (RUNS) tile_sync(t);
             const bool live = task.has(t);
@@ -733,8 +733,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             };
             for (int j = 0; j < mine; j++) {
                 const bool masked =
-                    RUNS ? j >= note[kMask] || (n_pre % KEYS && j == pre_tiles - 1 - note[kFirst])
-                         : j >= masked_from || j == masked_pre;
+                    RUNS ? j >= note[kMask] : j >= masked_from || j == masked_pre;
                 int lim = 0;                    // keys of the step that this row sees
                 uint64_t bits = 0;              // and of this thread's half, one a bit
                 if (__builtin_expect(masked, 0)) {

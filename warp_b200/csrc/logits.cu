@@ -541,13 +541,14 @@ __device__ __forceinline__ unsigned long long cluster_u64(const void *p, uint32_
 
 constexpr int kPickCluster = 8;
 constexpr int kPickFewPart = 16384;         // tokens a block, at most
-constexpr int kPickFewValues = 1 << 20;     // and logits of a call
+constexpr int kPickFewValues = 6 << 20;     // and logits of a call
 constexpr int kPickFewHistory = 16384;      // and places of a history, which each block reads
 
 // A cluster has a row, each block a part of the vocabulary, whose tokens it counts for
-// itself: one launch and no scratch, where what is to be read takes less time than a
-// launch (a row of 32000 behind 700 tokens: 6.9 us on the device and 13.2 as a call,
-// against 9.5 and 17.5 by two kernels).
+// itself: one launch and no scratch, and better as long as rows are few (on the device,
+// against the two kernels: a row of 32000 behind 700 tokens 7.5 us and 9.7, 32 of 131072
+// behind 8000 tokens each 18.1 and 24.5, 7 million logits 27.1 and 30.9, but 14 million 69.4
+// and 49.7: each row counts its history anew).
 template <typename T>
 __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_constant__ PickArgs a) {
     extern __shared__ __align__(16) uint32_t counts[];  // [part]
