@@ -211,7 +211,7 @@ constexpr int kPickBias = 1, kPickAllowed = 2, kPickKeep = 4;
 constexpr int kPickThreads = 256;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickOwn = 256;               // nodes' tokens that a block keeps
-constexpr int kPickPart = 65536;            // tokens of a row at once, at most
+constexpr int kPickPart = 32768;            // tokens of a row at once, at most
 constexpr int kPickPiece = 2048;            // tokens of a row that one block takes, at least
 
 template <int BYTES>
@@ -229,8 +229,12 @@ template <typename T, typename C, int OPT> struct PickSlot {
     static constexpr int window = n * sizeof(C);        // bytes of a vector's counts
     static constexpr int counts = bias + (OPT & kPickBias ? n * 4 : 0);
     static constexpr int bytes = counts + 2 * window;
-    static constexpr int ahead = bytes <= 48 ? 8 : bytes <= 80 ? 6 : 4;  // vectors under way
-    static constexpr int ring = ahead * bytes * kPickThreads;
+    // vectors under way: what lets four blocks fit an SM, with biases and counts three.  The
+    // stream is as much arithmetic as memory, so more warps are worth more than deeper rings: 8
+    // masked trees of 26 in bf16 take 45 us so and 49 us with eight vectors and two blocks.
+    static constexpr int ahead = 192 / bytes > 3 ? 192 / bytes : 3;
+    static constexpr int round = bytes * kPickThreads, ring = ahead * round;
+    static_assert(n * ahead <= 32, "what is hit in them, a bit each, is one word");
 };
 
 // The rows lie one behind another in pieces of kPickPiece tokens, and the blocks take
@@ -242,7 +246,7 @@ template <typename T, typename C, int OPT> struct PickSlot {
 // known ahead: a warp's bits of G vectors are one register a lane (N words a vector, and one
 // more where they are not aligned), asked for G vectors before they are needed.
 template <typename T, typename C, int OPT>
-__global__ void __launch_bounds__(kPickThreads)
+__global__ void __launch_bounds__(kPickThreads, 4)
 pick_rows_kernel(const __grid_constant__ PickArgs a) {
     using Slot = PickSlot<T, C, OPT>;
     constexpr int N = Slot::n, STEP = kPickThreads * N, R = Slot::ahead;
@@ -358,10 +362,15 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
         // under way queues in `queue`, N bits each.
         int ask = 0, ask_g = 0;
         uint32_t ask_hits = context ? hits_of(0) : 0, next_hits = context ? hits_of(G) : 0;
-        uint64_t queue = 0;
-        const uint32_t slot0 = smem_u32(ring);
-        auto place = [&](int k, int part, int bytes) {  // of a vector's part of the ring
-            return slot0 + (k % R) * (Slot::bytes * kPickThreads) + part * kPickThreads + tid * bytes;
+        uint32_t queue = 0;
+        // places in the ring of what is asked for next, and of what is next in turn
+        const uint32_t ring0 = smem_u32(ring);
+        uint32_t ask_at = ring0, turn_at = ring0;
+        auto part_of = [&](uint32_t at, int part, int bytes) {
+            return at + part * kPickThreads + tid * bytes;
+        };
+        auto behind = [&](uint32_t at) {
+            return at + Slot::round == ring0 + Slot::ring ? ring0 : at + Slot::round;
         };
         auto fetch = [&] {
             const int v = v_tid + ask * STEP;
@@ -374,19 +383,19 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                     next_hits = hits_of(ask + 1 + G);
                 }
                 if (v >= end) hit = 0;
-                queue = queue >> N | (uint64_t)hit << N * (R - 1);
+                queue = queue >> N | hit << N * (R - 1);
             }
             if (v < end) {
-                cp_async16(place(ask, 0, 16), x + v);
+                cp_async16(part_of(ask_at, 0, 16), x + v);
                 if (BIAS && bias_vec) {
 #pragma unroll
                     for (int k = 0; k < N; k += 4)
-                        cp_async16(place(ask, Slot::bias, 4 * N) + 4 * k, bias + v + k);
+                        cp_async16(part_of(ask_at, Slot::bias, 4 * N) + 4 * k, bias + v + k);
                 }
             }
             if (hit && occurs) {
                 const C *const z = counts + (v - skew);
-                const uint32_t to = place(ask, Slot::counts, 2 * Slot::window);
+                const uint32_t to = part_of(ask_at, Slot::counts, 2 * Slot::window);
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     if (k && !skew) break;
@@ -397,6 +406,7 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
             }
             cp_async_commit();
             ask++;
+            ask_at = behind(ask_at);
         };
 #pragma unroll 1
         for (int k = 0; k < R - 1; k++) fetch();
@@ -406,14 +416,14 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
 #pragma unroll 1
         for (int k = 0; k < rounds; k++) {
             fetch();
-            const uint32_t hit = (uint32_t)queue & ((1u << N) - 1);
+            const uint32_t hit = queue & ((1u << N) - 1);
             const uint32_t allow = ALLOWED ? bits_of(may, g) : 0;
             cp_async_wait<R - 1>();
             const int v = v_tid + k * STEP;
             float f[N], most = -INFINITY;
             if (v < end) {
                 PickVec<T> raw;
-                *(uint4 *)&raw = lds_u4(place(k, 0, 16));
+                *(uint4 *)&raw = lds_u4(part_of(turn_at, 0, 16));
 #pragma unroll
                 for (int q = 0; q < N; q++) f[q] = AttnType<T>::up(raw.x[q]);
                 if (hit) {
@@ -424,8 +434,8 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
 #pragma unroll
                     for (int q = 0; q < N; q++) plain &= pick_tame(f[q]);
                     if (__builtin_expect(plain, 1)) {
-                        const C *const z = (const C *)(ring + (place(k, Slot::counts, 2 * Slot::window) -
-                                                               slot0));
+                        const C *const z = (const C *)(
+                            ring + (part_of(turn_at, Slot::counts, 2 * Slot::window) - ring0));
                         alignas(16) C c[N];
                         if (!skew) {
 #pragma unroll
@@ -451,7 +461,7 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                     if (bias_vec) {
 #pragma unroll
                         for (int q = 0; q < N; q += 4)
-                            *(uint4 *)(w + q) = lds_u4(place(k, Slot::bias, 4 * N) + 4 * q);
+                            *(uint4 *)(w + q) = lds_u4(part_of(turn_at, Slot::bias, 4 * N) + 4 * q);
                     } else {
 #pragma unroll
                         for (int q = 0; q < N; q++) w[q] = __ldg(bias + v + q);
@@ -490,6 +500,7 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                 may = next_may;
                 next_may = may_of(k + 1 + G);
             }
+            turn_at = behind(turn_at);
         }
         cp_async_wait<0>();
         if (tid < a0 - v0) single(v0 + tid);
