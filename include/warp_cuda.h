@@ -397,6 +397,7 @@ WARP_API int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *
  * request; nodes past it, and a parent that does not come before its node (taken as
  * none), are reported by warp_attn_status.
  * pages, held and pool are read and written in place: order the calls of one pool.
+ * Without a pool rows of pages may overlap.
  * tokens 0 is no work but the pages'. */
 typedef struct {
     int batch, tokens;
@@ -479,8 +480,8 @@ WARP_API int warp_pick_tokens(const warp_pick_desc *d, void *scratch, void *stre
  * and in each of n_caches caches (one a layer) the path's keys and values move to the
  * places behind the request's keys before the tree, so that the first
  * kv_after keys are the accepted ones.  The caches share the layout of c, whose own
- * k and v are not used; theirs are k[i] and v[i] (host arrays).  kv_after is not
- * kv_len. */
+ * k and v are not used; theirs are k[i] and v[i] (host arrays), all of them apart from one
+ * another.  kv_after and count are not kv_len. */
 typedef struct {
     int batch, tokens, max_q;
     const int32_t *drafted, *picked;        /* [tokens] */

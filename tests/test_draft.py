@@ -40,7 +40,7 @@ def pick_desc(**kw):
 def accept_desc(**kw):
     return filled(ffi.AcceptDesc, dict(
         batch=1, tokens=1, max_q=1, drafted=256, picked=256, seen=256, seen_words=1, q_start=256,
-        kv_len=256, pages=256, pages_row=4, pages_per_row=4, count=256, path=256, chosen=256,
+        kv_len=256, pages=256, pages_row=4, pages_per_row=4, count=768, path=256, chosen=256,
         kv_after=512), kw)
 
 
@@ -63,7 +63,7 @@ def test_packed_descriptions_match_the_structures(fmt, cls):
     (dict(batch=1 << 20, pages_per_row=1 << 12), b"2^31"), (dict(batch=0), b"no request"),
     (dict(kv_len=None), b"NULL"), (dict(pages=None), b"NULL"), (dict(q_start=None), b"NULL"),
     (dict(slots=None), b"NULL"), (dict(positions=None), b"NULL"), (dict(seen=None), b"masks"),
-    (dict(seen=260), b"8-byte")])
+    (dict(seen=260), b"8-byte"), (dict(batch=2, pages_row=3), b"overlap")])
 def test_plan_refusals(lib, kw, text):
     assert lib.warp_step_plan(ctypes.byref(plan_desc(**kw)), None) == -1
     assert text in lib.warp_last_error()
@@ -114,7 +114,7 @@ def test_pick_refusals(lib, kw, text):
 
 
 def test_pick_refuses_bad_scratch(lib):
-    many = pick_desc(tokens=600, max_q=600, vocab=4000, row=4000, seen_words=10)
+    many = pick_desc(tokens=600, max_q=600, vocab=40000, row=40000, seen_words=10)
     assert lib.warp_pick_scratch(ctypes.byref(many)) > 0
     for at in (None, 264):
         assert lib.warp_pick_tokens(ctypes.byref(many), at, None) == -1
@@ -125,7 +125,8 @@ def test_pick_refuses_bad_scratch(lib):
     (dict(batch=-1), {}, b"negative"), (dict(max_q=65), {}, b"words"),
     (dict(max_q=4097, seen_words=65), {}, b"nodes"), (dict(seen=None), {}, b"masks"),
     (dict(seen=260), {}, b"8-byte"), (dict(drafted=None), {}, b"NULL"), (dict(path=None), {}, b"NULL"),
-    (dict(count=None), {}, b"NULL"), (dict(kv_after=256), {}, b"kv_after"),
+    (dict(count=None), {}, b"NULL"), (dict(kv_after=256, count=768), {}, b"kv_after"),
+    (dict(kv_len=512, count=512, kv_after=768), {}, b"count"),
     (dict(pages=None), {}, b"pages"), ({}, dict(page_size=24), b"page_size"),
     ({}, dict(type=0), b"fp16 or bf16"), ({}, dict(k_slot=0), b"strides"),
     ({}, dict(head_dim=63), b"odd")])
@@ -146,6 +147,15 @@ def test_accept_refuses_each_cache(lib):
     assert lib.warp_tree_accept(ctypes.byref(accept_desc()), None, 1, good, good, None) == -1
     assert lib.warp_tree_accept(ctypes.byref(accept_desc()), ctypes.byref(kv_pages()), -1, good,
                                 good, None) == -1
+
+
+@pytest.mark.parametrize("k, v", [((256, 256), (512, 768)), ((512, 768), (256, 256)),
+                                  ((256, 512), (768, 256)), ((256, 512), (256, 512))])
+def test_accept_refuses_a_cache_twice(lib, k, v):
+    k, v = ((ctypes.c_void_p * 2)(*x) for x in (k, v))
+    assert lib.warp_tree_accept(ctypes.byref(accept_desc()), ctypes.byref(kv_pages()), 2, k, v,
+                                None) == -1
+    assert b"twice" in lib.warp_last_error()
 
 
 def test_pool_on_the_host():

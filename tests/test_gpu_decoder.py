@@ -211,3 +211,29 @@ def test_choices_are_weighed(model):
     bias[11] = 1e4
     count, chosen = d.verify(i32([229, 11]), i32([-1, 0]), starts([2]), 2, bias=bias)
     assert count.tolist() == [2] and chosen.tolist() == [[11, 11]]
+
+
+def test_numbers_outside_the_vocabulary(model):
+    """They are no fault: a drafted one is never accepted, a start out of place is said."""
+    from warp_b200 import ops
+    d = decoder(model, 1, WIDE)
+    first = d.extend(i32([V + 5, -1, 1 << 30]), starts([3]), 3)
+    again = decoder(model, 1, WIDE).extend(i32([V - 1, 0, V - 1]), starts([3]), 3)
+    assert torch.equal(first, again)
+    count, chosen = d.verify(torch.cat((first, i32([V, 1 << 30, -1]))), i32([-1, 0, 1, 0]),
+                             starts([4]), 4)
+    ops.attn_status()
+    assert count.tolist() == [1] and 0 <= chosen[0, 0] < V and d.kv_len.tolist() == [4]
+
+
+def test_steps_that_are_refused(model):
+    """Before anything is done, or with the requests as they were."""
+    d = decoder(model, 2, WIDE)
+    for call in (lambda: d.extend(i32([]), i32([0, 0, 0]), 1),
+                 lambda: d.verify(i32([]), i32([]), i32([0, 0, 0]), 1),
+                 lambda: d.extend(i32([1, 2]), i32([0, 2]), 2),
+                 lambda: d.verify(i32([1, 2]), i32([-1]), i32([0, 1, 2]), 1),
+                 lambda: d.extend(i32([1, 2]), i32([0, 1, 2]), 1, bias=torch.zeros(V - 1).cuda())):
+        with pytest.raises(ValueError):
+            call()
+        assert d.kv_len.tolist() == [0, 0]

@@ -240,6 +240,24 @@ def test_plan_of_bad_trees(cuda):
     assert seen.flatten().tolist() == [1, 3, 7, 0]
 
 
+@pytest.mark.parametrize("pooled", [False, True])
+def test_plan_of_a_start_before_the_tokens(cuda, pooled):
+    """Parents before the array are not asked for: the request's tokens have no place."""
+    from warp_b200 import ffi, ops
+    ops.attn_status()
+    pages = torch.arange(16, dtype=torch.int32, device="cuda").view(2, 8)
+    kw = dict(held=i32([8, 8]).cuda(), pool=ops.page_pool(0)) if pooled else {}
+    around = torch.full((12,), 1 << 20, dtype=torch.int32, device="cuda")
+    parents = around[4:10]
+    parents.copy_(i32([-1, 0, 1, -1, 0, 0]))
+    _, slots, seen = ops.step_plan(i32([-3, 3, 6]).cuda(), i32([128, 128]).cuda(), pages, 16, 6,
+                                   parents=parents, max_q=6, **kw)
+    with pytest.raises(ffi.WarpError, match="length"):
+        ops.attn_status()
+    assert slots.tolist() == [-1] * 3 + [8 * 16 + 125 + i for i in range(3)]
+    assert seen.flatten().tolist() == [0, 0, 0, 1, 3, 5]
+
+
 # ---- tree attention --------------------------------------------------------------------
 
 

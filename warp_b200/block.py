@@ -155,7 +155,8 @@ class Decoder:
     [vocabulary][hidden]; k_pages / v_pages
     [layers][pages][page_size][kv_heads][head_dim].  kv_len (int32 [requests], on the
     device) is how many keys each request has: set it to 0 for one that ends, and its
-    pages go back with the next step.  Nothing here waits for the device."""
+    pages go back with the next step.  Nothing here waits for the device.  A number
+    outside the vocabulary is read as the nearest in it (and is never accepted)."""
 
     def __init__(self, blocks, embed, norm, head, k_pages, v_pages, requests,
                  pages_per_request, eps=1e-6):
@@ -174,10 +175,12 @@ class Decoder:
 
     def _forward(self, tokens, q_start, max_q, parents=None):
         """(states behind the last block, the step)."""
+        if not tokens.numel():
+            raise ValueError("a step needs a token")
         kv_len = self.kv_len + (q_start[1:] - q_start[:-1])
         step = Step.draft(q_start, kv_len, self.pages, self.page_size, tokens.numel(), max_q,
                           parents, self.held, self.pool)
-        h = self.embed[tokens.clamp(min=0)]
+        h = self.embed[tokens.clamp(0, len(self.embed) - 1)]
         for block, k, v in zip(self.blocks, self.k_pages, self.v_pages):
             h = block.forward(h, k, v, step)
         return h, step
@@ -191,8 +194,10 @@ class Decoder:
         token picked behind each request's last, int32 [requests] (of no meaning where a
         request brings none).  choice: what ops.pick_tokens weighs, a row a request."""
         h, step = self._forward(tokens, q_start, max_q)
+        last = (q_start[1:] - 1).clamp(0, len(h) - 1)
+        picked = ops.pick_tokens(self._logits(h[last]), **choice)
         self.kv_len.copy_(step.kv_len)
-        return ops.pick_tokens(self._logits(h[(q_start[1:] - 1).clamp(min=0)]), **choice)
+        return picked
 
     def verify(self, drafted, parents, q_start, max_q, **choice):
         """A step of drafted trees: request b's nodes are tokens q_start[b] ..

@@ -184,7 +184,8 @@ __device__ __forceinline__ PlanToken plan_find(const PlanArgs &a, int t) {
     const int first = a.q_start[b], end = a.q_start[b + 1];
     uint64_t *const row = a.seen + (int64_t)t * a.words;
     int64_t j = -1, pos = 0;
-    if (t >= first && t < end) {
+    if (first < 0) atomicOr(a.err, kAttnBadLen);        // its parents would lie before the array
+    if (first >= 0 && t >= first && t < end) {
         const int64_t base = (int64_t)a.kv_len[b] - end;
         j = base + t;
         pos = a.base + j;
@@ -219,7 +220,9 @@ __device__ __forceinline__ void plan_slot(const PlanArgs &a, int t, PlanToken p)
     a.slots[t] = slot;
 }
 
-// Pages, and the tokens where they are few enough for one block.
+// Pages, and the tokens where they are few enough for one block: what a second launch saves on
+// the device (302 tokens 4.1 us a call against 4.7, 1774 tokens 4.2 against 6.1) is less than the
+// 2.5 us that it costs the host as long as the one block's part is a round or less.
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanArgs a, bool tokens) {
     pdl_trigger();
     if (a.pool) plan_pages(a);
@@ -266,7 +269,7 @@ __device__ __forceinline__ uint64_t upto(const uint64_t *row, int w, int i) {
 // The accepted path, and its keys and values behind the certain ones: node path[d]
 // to place d.  A block has a request and some of the caches, and finds the path itself: a
 // few loads, which a kernel before this one would only put in front of them (48 trees of up
-// to 61 nodes in 32 caches: 11.0 us against 13.7).  A thread moves the same piece of
+// to 61 nodes in 32 caches: 12.2 us against 13.7; one tree of 16 in two: 4.5 against 5.8).  A thread moves the same piece of
 // every key, d ascending: path[d] >= d ascends, so a place is read before it is
 // written.
 template <typename V>
@@ -391,6 +394,16 @@ accept_kernel(const __grid_constant__ AcceptArgs a) {
     }
 }
 
+// Whether an address occurs twice: a cache whose path moves twice is not in order.
+static bool cache_twice(int n, void *const *k, void *const *v) {
+    bool twice = false;
+    for (int i = 0; i < n; i++) {
+        for (int j = 0; j < i; j++) twice |= k[i] == k[j] || v[i] == v[j];
+        for (int j = 0; j < n; j++) twice |= k[i] == v[j];
+    }
+    return twice;
+}
+
 }  // namespace warp
 
 using namespace warp;
@@ -408,6 +421,8 @@ extern "C" int warp_step_plan(const warp_plan_desc *d, void *stream) {
              "%s: %lld pages in the pool", who, (long long)d->pool_pages);
     WARP_ARG((int64_t)d->batch * d->pages_per_row < (int64_t)1 << 31,
              "%s: a page table of 2^31 entries and more", who);
+    WARP_ARG(!d->pool || d->batch < 2 || d->pages_row >= d->pages_per_row,
+             "%s: rows of the page table overlap", who);
     if (d->batch == 0 && d->tokens == 0) return WARP_OK;
     WARP_ARG(d->batch >= 1 && d->kv_len && (d->pages || !d->pages_per_row),
              "%s: NULL pointer or no request", who);
@@ -456,7 +471,8 @@ extern "C" int warp_tree_accept(const warp_accept_desc *d, const warp_kv_pages *
     WARP_ARG(!d->max_q || (d->path && d->chosen), "%s: NULL pointer", who);
     WARP_ARG(!d->tokens || (d->drafted && d->picked && d->seen && ((uintptr_t)d->seen & 7) == 0),
              "%s: NULL pointer, or masks that are not 8-byte aligned", who);
-    WARP_ARG(d->kv_after != d->kv_len, "%s: kv_after may not be kv_len", who);
+    WARP_ARG(d->kv_after != d->kv_len && d->count != d->kv_len,
+             "%s: kv_after and count may not be kv_len", who);
     if (n_caches) {
         WARP_ARG(c && k && v && (d->pages || !d->pages_per_row), "%s: NULL pages", who);
         warp_kv_pages one = *c;
@@ -466,6 +482,7 @@ extern "C" int warp_tree_accept(const warp_accept_desc *d, const warp_kv_pages *
             if (rc) return rc;
         }
         WARP_ARG(c->head_dim % 2 == 0, "%s: head_dim %d is odd", who, c->head_dim);
+        WARP_ARG(!cache_twice(n_caches, k, v), "%s: a cache is there twice", who);
     }
     AcceptArgs a = {};
     a.drafted = d->drafted, a.picked = d->picked, a.q_start = d->q_start, a.kv_len = d->kv_len;

@@ -650,8 +650,9 @@ def tree_accept(drafted, picked, seen, q_start, kv_len, max_q, caches=(), pages=
     + count.
 
     caches: (k_pages, v_pages) of all layers, [layers][pages][page_size][Hk][D], or
-    a list of each layer's pair, all of one layout; their keys and values of the
-    path move behind the keys before the tree, pages int32 [B][n] being the page table."""
+    a list of each layer's pair, all of one layout and apart from one another; their keys
+    and values of the path move behind the keys before the tree, pages int32 [B][n] being
+    the page table."""
     dev = _device(kv_len)
     T, B = drafted.numel(), kv_len.numel()
     words = _seen_ok(seen, T, max_q, dev)
