@@ -31,6 +31,14 @@
 // half the keys of a step (with one, a scheduler has two warps, which do not hide
 // each other's latency); 16 issues the products, 17 loads keys and 18 values by TMA,
 // a box a page (its issue takes some 70 cycles), into a ring of tiles.
+//
+// Nodes of trees see the keys before their tree and the bits of their row of masks
+// (kAttnTree): only the last steps look at them, others cost what they cost without.
+// With few rows a request and lengths that differ, a block takes a run of the batch's
+// key tiles instead (kAttnTreeRuns; AttnRuns), which is bound by the keys' stream: the
+// two row tiles take the run's tasks in turn, one's rows are written while the other's keys
+// come, and the keys' ring goes on from task to task.  32 trees of up to 16 nodes, 56 heads
+// of 128 over 8, behind up to 8192 keys: 141 us, 4.7 TB/s.
 #pragma once
 #include "attn.cuh"
 #include "umma.cuh"
