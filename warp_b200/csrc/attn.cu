@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 // other items were written by those that had all of them.  The blocks here are shared out
 // among these items, and an item's rows among its blocks' warps.  The rows of requests
 // without a key, which are no item's, are made zeros.
-constexpr int kJoinBlocks = 4 * 148;
+constexpr int kJoinBlocks = 8 * 148;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_constant__ AttnArgs a) {
@@ -580,11 +580,7 @@ __global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_consta
         const int slices = (kJoinBlocks - (int)blockIdx.x % all + all - 1) / all;
         auto place = [&](int p) { return ((int64_t)p * 2 + (p == s.c0 && s.late)) * kAttnRunRows; };
         for (int x = blockIdx.x / all * 8 + warp; x < s.rows; x += slices * 8) {
-            float M = -INFINITY;
-#pragma unroll 8
-            for (int p = s.c0; p <= s.c1; p++) M = fmaxf(M, a.part_ml[place(p) + x].x);
-            const float z = M == -INFINITY ? 0.f : M;
-            float l = 0.f, acc[V];
+            float M = -INFINITY, l = 0.f, acc[V];
 #pragma unroll
             for (int i = 0; i < V; i++) acc[i] = 0.f;
             for (int p0 = s.c0; p0 <= s.c1; p0 += U) {
@@ -592,6 +588,7 @@ __global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_consta
                 float2 ml[U];
 #pragma unroll
                 for (int k = 0; k < U; k++) {
+                    ml[k] = make_float2(-INFINITY, 0.f);
                     if (p0 + k > s.c1) continue;
                     const int64_t at = place(p0 + k) + x;
                     ml[k] = a.part_ml[at];
@@ -599,6 +596,17 @@ __global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_consta
                     if (V == 4) *(float4 *)v[k] = *(const float4 *)src;
                     else *(float2 *)v[k] = *(const float2 *)src;
                 }
+                float most = M;
+#pragma unroll
+                for (int k = 0; k < U; k++) most = fmaxf(most, ml[k].x);
+                const float z = most == -INFINITY ? 0.f : most;
+                if (p0 > s.c0) {            // what is there, from the new maximum
+                    const float w = ex2(M - z);
+                    l *= w;
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[i] *= w;
+                }
+                M = most;
 #pragma unroll
                 for (int k = 0; k < U; k++) {
                     if (p0 + k > s.c1) continue;

@@ -158,28 +158,6 @@ __device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes) {
                  ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Two fp32 at a time: half the instructions, though each takes the pipe as long
-// as two.
-__device__ __forceinline__ uint64_t pair2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 both(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // Largest of three; a NaN wins.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;

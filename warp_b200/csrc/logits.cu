@@ -8,19 +8,21 @@
 // a row's parts by an atomic maximum of (logit, token) in one number, which any order
 // leaves the same.  A few rows are one kernel's, a cluster of blocks to a row.
 //
-// Measured: 160 rows of 131072 fp32 and their maximum 26 us, 3.2 TB/s; with masks, biases and
-// the adjusted logits written 43; with 64 histories of up to 30000 tokens 71.  What bounds it is
-// the arithmetic of each value as much as the stream, and with histories the counting (14 us)
-// that comes before it.  Tried and slower than two kernels for many rows: a cluster that
-// counts for itself (83 to 97), counts in the shared memory of others (200), tokens
-// sorted into buckets first (89), penalties spread out densely (86).
+// Measured: 160 rows of 131072 fp32 26 us, 3.2 TB/s; about as many (64 streams of 1 to 5) with
+// biases of each stream 40, and with histories of up to 30000 tokens 69; 104 rows of 100003 bf16
+// with histories of 8000 and masks, kept, 42.  What bounds it is the arithmetic of each value
+// (issue slots are used to two thirds and three quarters in the last two) more than the stream, and
+// the counting (15 and 6 us) that comes before it.  Tried and slower than two kernels for many
+// rows: a cluster that counts for itself (64 streams: 83 to 97), counts in the shared memory of
+// others (200), tokens sorted into buckets first (89), penalties spread out densely (86).
 //
-// Division: x / r for a row's many x and one r is q = x y with y = 1 / r rounded,
-// corrected twice by the remainder: q += y (x - q r), each step one fused
-// operation (Markstein, "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990: the last step rounds as a division does if y is rounded to nearest
-// and q is off by one place at most, which the first step sees to).  Where a quotient or
-// remainder could leave the normal numbers it divides.
+// Division: x / r for a row's many x and one r is by the reciprocal, kept in two words
+// y + z (z what y, rounded, is off by): q = x y + x z is one place off at most, and q + y (x - q r)
+// is the quotient rounded to nearest (Markstein, "Computation of elementary functions on
+// the IBM RISC System/6000 processor", 1990; the two words are those of Brisebarre, Muller and
+// Raina, "Accelerating correctly rounded floating-point division when the divisor is known
+// in advance", 2004).  The remainder is exact as long as no number here leaves the normal
+// ones; where one could, it divides.
 #include "attn.cuh"
 
 namespace warp {
@@ -161,27 +163,37 @@ template <typename T> struct alignas(16) PickVec {
 // The penalties of one request.
 struct PickLess {
     float repetition, frequency, presence;
-    float inverse;                          // of the first, rounded; 0 where it is divided by
+    float inverse, low;                     // of the first, in two words; 0 where it is divided by
 };
 
-__device__ __forceinline__ float pick_less(float x, float count, const PickLess &p, bool divide) {
-    float q;
-    if (divide) {
-        q = __fdiv_rn(x, p.repetition);
-    } else {
-        q = __fmul_rn(x, p.inverse);
-        q = __fmaf_rn(__fmaf_rn(-q, p.repetition, x), p.inverse, q);
-        q = __fmaf_rn(__fmaf_rn(-q, p.repetition, x), p.inverse, q);
-    }
-    x = x > 0.f ? q : __fmul_rn(x, p.repetition);
+__device__ __forceinline__ float pick_less(float x, float count, const PickLess &p) {
+    x = x > 0.f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
     x = __fsub_rn(x, __fmul_rn(p.frequency, count));
     return __fsub_rn(x, p.presence);
 }
-// Whether x is so far from the normal numbers' ends that the products above are exact
-// where they have to be; 2^-80 .. 2^80.
-__device__ __forceinline__ bool pick_tame(float x) {
-    constexpr uint32_t lo = (127u - 80u) << 24, hi = (127u + 80u) << 24;
-    return (__float_as_uint(x) << 1) - lo < hi - lo;
+// The same of two tame values, by the reciprocal.
+__device__ __forceinline__ float2 pick_less2(float x0, float x1, float count0, float count1,
+                                             const PickLess &p) {
+    const uint64_t x = pair2(x0, x1), inverse = pair2(p.inverse, p.inverse);
+    const uint64_t by = pair2(-p.repetition, -p.repetition);
+    uint64_t q = fma2(x, inverse, mul2(x, pair2(p.low, p.low)));
+    q = fma2(fma2(q, by, x), inverse, q);
+    const float2 over = both(q), times = both(mul2(x, by));
+    const uint64_t w = pair2(x0 > 0.f ? over.x : -times.x, x1 > 0.f ? over.y : -times.y);
+    // one by one: a product of two that is added to would not be rounded by itself
+    const uint64_t less = pair2(__fmul_rn(-p.frequency, count0), __fmul_rn(-p.frequency, count1));
+    return both(add2(add2(w, less), pair2(-p.presence, -p.presence)));
+}
+// Whether all x are so far from the normal numbers' ends that the products above are
+// exact where they have to be.  A NaN is one with either.
+template <int N> __device__ __forceinline__ bool pick_tame(const float (&x)[N]) {
+    float lo = fabsf(x[0]), hi = lo;
+#pragma unroll
+    for (int q = 1; q < N; q++) {
+        lo = fminf(lo, fabsf(x[q]));
+        hi = fmaxf(hi, fabsf(x[q]));
+    }
+    return lo >= 0x1p-80f && hi <= 0x1p80f;
 }
 // A count as a number: 16 bits below the last place of 2^23, and 2^23 taken off.
 __device__ __forceinline__ float pick_float(uint16_t c) {
@@ -293,12 +305,14 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
         const int v_tid = a0 + tid * N, skew = a0 % N;
         const bool y_vec = ((uintptr_t)(y + a0) & 15) == 0;
         const bool bias_vec = ((uintptr_t)(bias + a0) & 15) == 0;
-        PickLess less = {1.f, 0.f, 0.f, 0.f};
+        PickLess less = {1.f, 0.f, 0.f, 0.f, 0.f};
         if (a.repetition) less.repetition = a.repetition[b];
         if (a.frequency) less.frequency = a.frequency[b];
         if (a.presence) less.presence = a.presence[b];
-        if (less.repetition >= 0x1p-20f && less.repetition <= 0x1p20f)
+        if (less.repetition >= 0x1p-20f && less.repetition <= 0x1p20f) {
             less.inverse = __frcp_rn(less.repetition);
+            less.low = __fmul_rn(__fmaf_rn(-less.inverse, less.repetition, 1.f), less.inverse);
+        }
         if (sees) {
             __syncthreads();                // the last part's are read
             for (int w = tid; w < (v1 - v0 + 31) / 32 + 1; w += kPickThreads) drafts[w] = 0;
@@ -331,7 +345,7 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
             uint32_t count = 0;
             if (occurs && (occurs[v >> 5] >> (v & 31) & 1)) count = (uint32_t)counts[v];
             if (sees && (drafts[(v - v0) >> 5] >> (v & 31) & 1)) count += nodes_with(v);
-            return count ? pick_less(f, (float)count, less, true) : f;
+            return count ? pick_less(f, (float)count, less) : f;
         };
         auto single = [&](int v) {
             float f = adjusted(AttnType<T>::up(x[v]), v);
@@ -439,10 +453,7 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                     const int d = (v - v0) >> 5;
                     const uint32_t mine =
                         sees ? __funnelshift_r(drafts[d], drafts[d + 1], v & 31) & hit : 0;
-                    bool plain = less.inverse != 0.f && !mine;
-#pragma unroll
-                    for (int q = 0; q < N; q++) plain &= pick_tame(f[q]);
-                    if (__builtin_expect(plain, 1)) {
+                    if (__builtin_expect(less.inverse != 0.f && !mine && pick_tame(f), 1)) {
                         const C *const z = (const C *)(
                             ring + (part_of(turn_at, Slot::counts, 2 * Slot::window) - ring0));
                         alignas(16) C c[N];
@@ -455,9 +466,11 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                             for (int q = 0; q < N; q++) c[q] = z[q + skew];
                         }
 #pragma unroll
-                        for (int q = 0; q < N; q++) {
-                            const float w = pick_less(f[q], pick_float(c[q]), less, false);
-                            f[q] = hit >> q & 1 ? w : f[q];
+                        for (int q = 0; q < N; q += 2) {
+                            const float2 w = pick_less2(f[q], f[q + 1], pick_float(c[q]),
+                                                        pick_float(c[q + 1]), less);
+                            f[q] = hit >> q & 1 ? w.x : f[q];
+                            f[q + 1] = hit >> q & 2 ? w.y : f[q + 1];
                         }
                     } else {
 #pragma unroll
@@ -476,7 +489,10 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                         for (int q = 0; q < N; q++) w[q] = __ldg(bias + v + q);
                     }
 #pragma unroll
-                    for (int q = 0; q < N; q++) f[q] = __fadd_rn(f[q], w[q]);
+                    for (int q = 0; q < N; q += 2) {
+                        const float2 y = both(add2(pair2(f[q], f[q + 1]), pair2(w[q], w[q + 1])));
+                        f[q] = y.x, f[q + 1] = y.y;
+                    }
                 }
 #pragma unroll
                 for (int q = 0; q < N; q++) {
@@ -581,7 +597,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_con
     if (!pick_request(a, t, b, i, n, rank == 0)) return;        // all blocks of the cluster
     const int t0 = t - i;
     const bool context = a.history || a.seen;
-    PickLess less = {1.f, 0.f, 0.f, 0.f};
+    PickLess less = {1.f, 0.f, 0.f, 0.f, 0.f};
     if (a.repetition) less.repetition = a.repetition[b];
     if (a.frequency) less.frequency = a.frequency[b];
     if (a.presence) less.presence = a.presence[b];
@@ -629,7 +645,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_con
             const int v = base + u * kPickThreads;
             if (v >= v1) break;
             const uint32_t count = context ? counts[v - v0] : 0;
-            if (count) f[u] = pick_less(f[u], (float)count, less, true);
+            if (count) f[u] = pick_less(f[u], (float)count, less);
             if (bias) f[u] = __fadd_rn(f[u], __ldg(bias + v));
             if (allowed && !(__ldg(allowed + (v >> 5)) >> (v & 31) & 1)) f[u] = -INFINITY;
             if (f[u] > top) {
