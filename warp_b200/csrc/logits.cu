@@ -1,18 +1,17 @@
 // logits.cu — penalties for repeated tokens, biases and masks on logits, and the
 // largest of each row.
 //
-// The logits are read once (and, where they are kept, written once), which is what
-// bounds it.  Two kernels: the first counts each request's history, a block to a slice of
-// the vocabulary, and leaves a bit for each token that occurs, and the numbers where
-// there are such bits.  The second streams over the rows, in equal runs, and joins
+// The logits are read once (and, where they are kept, written once).  Two kernels: the
+// first counts each request's history, a block to a slice of the vocabulary, and leaves
+// a bit for each token that occurs, and the numbers where there are such bits.  The second streams over the rows, in equal runs, and joins
 // a row's parts by an atomic maximum of (logit, token) in one number, which any order
 // leaves the same.  A few rows are one kernel's, a cluster of blocks to a row.
 //
 // Measured: 160 rows of 131072 fp32 26 us, 3.2 TB/s; about as many (64 streams of 1 to 5) with
 // biases of each stream 40, and with histories of up to 30000 tokens 69; 104 rows of 100003 bf16
 // with histories of 8000 and masks, kept, 42.  What bounds it is the arithmetic of each value
-// (issue slots are used to two thirds and three quarters in the last two) more than the stream, and
-// the counting (15 and 6 us) that comes before it.  Tried and slower than two kernels for many
+// (issue slots are used to 73 and 65 % in the last two) more than the stream, and the
+// counting (15 and 6 us) that comes before it.  Tried and slower than two kernels for many
 // rows: a cluster that counts for itself (64 streams: 83 to 97), counts in the shared memory of
 // others (200), tokens sorted into buckets first (89), penalties spread out densely (86).
 //
