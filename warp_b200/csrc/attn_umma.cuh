@@ -966,7 +966,18 @@ struct WideLaunch {
 
     template <typename T, int D, AttnKind KIND> int go() const {
         static std::atomic<uint64_t> done;
-        cudaError_t e = attn_smem(attn_umma_kernel<T, D, KIND>, Lay<D>::bytes, done);
+        cudaError_t e = cudaSuccess;
+        if (KIND == kAttnTreeRuns && !done.load()) {
+            // fewer registers at the start than change hands, and a warp would wait for good
+            cudaFuncAttributes at;
+            e = cudaFuncGetAttributes(&at, attn_umma_kernel<T, D, KIND>);
+            if (e != cudaSuccess) return cuda_fail(e, "attention kernel attributes");
+            if (at.numRegs * threads_of(KIND) < 512 * kRowRegs + 128 * kOtherRegs) {
+                set_error("attn_umma_kernel: built with %d registers", at.numRegs);
+                return WARP_E_CUDA;
+            }
+        }
+        e = attn_smem(attn_umma_kernel<T, D, KIND>, Lay<D>::bytes, done);
         if (e != cudaSuccess) return cuda_fail(e, "attention smem attribute");
         e = attn_start(attn_umma_kernel<T, D, KIND>, grid, threads_of(KIND), Lay<D>::bytes, st, first,
                        a, km, vm);

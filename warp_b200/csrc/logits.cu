@@ -7,9 +7,9 @@
 // a row's parts by an atomic maximum of (logit, token) in one number, which any order
 // leaves the same.  A few rows are one kernel's, a cluster of blocks to a row.
 //
-// Measured: 160 rows of 131072 fp32 26 us, 3.2 TB/s; about as many (64 streams of 1 to 5) with
-// biases of each stream 40, and with histories of up to 30000 tokens 69; 104 rows of 100003 bf16
-// with histories of 8000 and masks, kept, 42.  What bounds it is the arithmetic of each value
+// Measured: 160 rows of 131072 fp32 22.5 us, 3.7 TB/s; about as many (64 streams of 1 to 5) with
+// biases of each stream 37, and with histories of up to 30000 tokens 66; 104 rows of 100003 bf16
+// with histories of 8000 and masks, kept, 39.  What bounds it is the arithmetic of each value
 // (issue slots are used to 73 and 65 % in the last two) more than the stream, and the
 // counting (15 and 6 us) that comes before it.  Tried and slower than two kernels for many
 // rows: a cluster that counts for itself (64 streams: 83 to 97), counts in the shared memory of
@@ -232,6 +232,10 @@ constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickOwn = 256;               // nodes' tokens that a block keeps
 constexpr int kPickPart = 49152;            // tokens of a row at once, where nodes' are marked
 constexpr int kPickPiece = 2048;            // tokens of a row that one block takes, at least
+// What a block's start on a row takes, in pieces: who has two rows gets fewer of them (160 rows
+// of 131072 22.5 us with 5 and 26 with 0, 8 trees of 26 39 and 42; with 9 and many penalties it is
+// slower again).
+constexpr int kPickLead = 5;
 
 template <int BYTES>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src) {
@@ -277,10 +281,15 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
     __shared__ unsigned long long best[kPickWarps];
     extern __shared__ __align__(16) uint8_t ring[];     // [vector][part of a slot][thread]
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    const int64_t all = (int64_t)a.tokens * a.pieces, blocks = gridDim.x;
-    const int64_t last = (blockIdx.x + 1) * all / blocks;
+    // this block's pieces
+    const int64_t span = a.pieces + kPickLead, all = a.tokens * span, blocks = gridDim.x;
+    auto piece_of = [&](int64_t u) {
+        const int64_t t = u / span;
+        return t * a.pieces + max((int)(u - t * span) - kPickLead, 0);
+    };
+    const int64_t last = piece_of((blockIdx.x + 1) * all / blocks);
     bool waited = false;
-    for (int64_t piece = blockIdx.x * all / blocks, next; piece < last; piece = next) {
+    for (int64_t piece = piece_of(blockIdx.x * all / blocks), next; piece < last; piece = next) {
         const int t = (int)(piece / a.pieces), first = (int)(piece - (int64_t)t * a.pieces);
         next = min(last, piece - first + a.pieces);
         if (a.seen) next = min(next, piece + kPickPart / kPickPiece);
@@ -288,20 +297,34 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
         const int v1 = (int)min((int64_t)a.vocab, v0 + (next - piece) * kPickPiece);
         const T *const x = (const T *)a.logits + t * a.row;
         T *const y = KEEP ? (T *)a.out + t * a.out_row : nullptr;
-        int b, i, n;
-        if (!pick_request(a, t, b, i, n, true)) continue;
-        const int t0 = t - i;
-        const uint64_t *const sees = a.seen ? a.seen + t * a.seen_words : nullptr;
-        const float *const bias = BIAS ? a.bias + b * a.bias_row : nullptr;
-        const uint32_t *const allowed = ALLOWED ? a.allowed + t * a.allowed_row : nullptr;
-        const uint32_t *const occurs = a.history ? a.bits + b * (int64_t)a.words : nullptr;
-        const C *const counts = (const C *)a.counts + b * (int64_t)a.words * 32;
         // Vectors are aligned in memory, from value a0 on; what is left over at the
         // part's ends goes one by one.
         const int a0 = min(v1, v0 + (int)(-((uintptr_t)(x + v0) / sizeof(T)) % N));
         const int vectors = (v1 - a0) / N, end = a0 + vectors * N;
         const int rounds = (vectors + kPickThreads - 1) / kPickThreads;
         const int v_tid = a0 + tid * N, skew = a0 % N;
+        // The first vectors are asked for before it is known whose row this is.
+        const uint32_t ring0 = smem_u32(ring);
+        auto part_of = [&](uint32_t at, int part, int bytes) {
+            return at + part * kPickThreads + tid * bytes;
+        };
+        auto ask_row = [&](uint32_t at, int v) {
+            if (v < end) cp_async16(part_of(at, 0, 16), x + v);
+        };
+#pragma unroll 1
+        for (int k = 0; k < R - 1; k++) ask_row(ring0 + k * Slot::round, v_tid + k * STEP);
+        int b, i, n;
+        if (!pick_request(a, t, b, i, n, true)) {
+            cp_async_commit();
+            cp_async_wait<0>();
+            continue;
+        }
+        const int t0 = t - i;
+        const uint64_t *const sees = a.seen ? a.seen + t * a.seen_words : nullptr;
+        const float *const bias = BIAS ? a.bias + b * a.bias_row : nullptr;
+        const uint32_t *const allowed = ALLOWED ? a.allowed + t * a.allowed_row : nullptr;
+        const uint32_t *const occurs = a.history ? a.bits + b * (int64_t)a.words : nullptr;
+        const C *const counts = (const C *)a.counts + b * (int64_t)a.words * 32;
         const bool y_vec = ((uintptr_t)(y + a0) & 15) == 0;
         const bool bias_vec = ((uintptr_t)(bias + a0) & 15) == 0;
         PickLess less = {1.f, 0.f, 0.f, 0.f, 0.f};
@@ -386,15 +409,11 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
         uint32_t ask_hits = context ? hits_of(0) : 0, next_hits = context ? hits_of(G) : 0;
         uint32_t queue = 0;
         // places in the ring of what is asked for next, and of what is next in turn
-        const uint32_t ring0 = smem_u32(ring);
         uint32_t ask_at = ring0, turn_at = ring0;
-        auto part_of = [&](uint32_t at, int part, int bytes) {
-            return at + part * kPickThreads + tid * bytes;
-        };
         auto behind = [&](uint32_t at) {
             return at + Slot::round == ring0 + Slot::ring ? ring0 : at + Slot::round;
         };
-        auto fetch = [&] {
+        auto fetch = [&](bool row) {
             const int v = v_tid + ask * STEP;
             uint32_t hit = 0;
             if (context) {
@@ -407,13 +426,11 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
                 if (v >= end) hit = 0;
                 queue = queue >> N | hit << N * (R - 1);
             }
-            if (v < end) {
-                cp_async16(part_of(ask_at, 0, 16), x + v);
-                if (BIAS && bias_vec) {
+            if (row) ask_row(ask_at, v);
+            if (BIAS && v < end && bias_vec) {
 #pragma unroll
-                    for (int k = 0; k < N; k += 4)
-                        cp_async16(part_of(ask_at, Slot::bias, 4 * N) + 4 * k, bias + v + k);
-                }
+                for (int k = 0; k < N; k += 4)
+                    cp_async16(part_of(ask_at, Slot::bias, 4 * N) + 4 * k, bias + v + k);
             }
             if (hit && occurs) {
                 const C *const z = counts + (v - skew);
@@ -431,13 +448,13 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
             ask_at = behind(ask_at);
         };
 #pragma unroll 1
-        for (int k = 0; k < R - 1; k++) fetch();
+        for (int k = 0; k < R - 1; k++) fetch(false);
         uint32_t may = may_of(0), next_may = may_of(G);
         int g = 0;
         float bound = -INFINITY;            // what the warp has seen is at least this
 #pragma unroll 1
         for (int k = 0; k < rounds; k++) {
-            fetch();
+            fetch(true);
             const uint32_t hit = queue & ((1u << N) - 1);
             const uint32_t allow = ALLOWED ? bits_of(may, g) : 0;
             cp_async_wait<R - 1>();
@@ -581,14 +598,14 @@ constexpr int kPickFewHistory = 16384;      // and places of a history, which ea
 
 // A cluster has a row, each block a part of the vocabulary, whose tokens it counts for
 // itself: one launch and no scratch, and better as long as rows are few (on the device,
-// against the two kernels: a row of 32000 behind 700 tokens 7.5 us and 9.7, 32 of 131072
-// behind 8000 tokens each 18.1 and 24.5, 7 million logits 27.1 and 30.9, but 14 million 69.4
-// and 49.7: each row counts its history anew).
-template <typename T>
-__global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_constant__ PickArgs a) {
+// against the two kernels: a row of 32000 behind 700 tokens 5.9 us and 9.7, 32 of 131072
+// with biases behind 8000 tokens each 19.3 and 23.3, 145 of 74835 28.3 and 27.3: each row counts
+// its history anew).
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) pick_few_kernel(const __grid_constant__ PickArgs a) {
     extern __shared__ __align__(16) uint32_t counts[];  // [part]
-    __shared__ unsigned long long best[kPickWarps];
-    constexpr int U = 8;
+    constexpr int U = 8, WARPS = THREADS / 32;
+    __shared__ unsigned long long best[WARPS];
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int rank = (int)cluster_rank(), t = blockIdx.x / kPickCluster;
     const int v0 = min(rank * a.part, a.vocab), v1 = min(v0 + a.part, a.vocab);
@@ -601,7 +618,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_con
     if (a.frequency) less.frequency = a.frequency[b];
     if (a.presence) less.presence = a.presence[b];
     if (context) {
-        for (int x = tid; x < a.part; x += kPickThreads) counts[x] = 0;
+        for (int x = 4 * tid; x < a.part; x += 4 * THREADS)
+            *(uint4 *)(counts + x) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         auto add = [&](int v) {
             if (v >= v0 && v < v1) atomicAdd(counts + (v - v0), 1u);
@@ -610,18 +628,18 @@ __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_con
             const int said = a.history_len[b], len = min(max(said, 0), a.history_wide);
             if (tid == 0 && said != len) atomicOr(a.err, kAttnBadLen);
             const int32_t *const past = a.history + b * a.history_row;
-            for (int x = tid; x < len; x += U * kPickThreads) {
+            for (int x = tid; x < len; x += U * THREADS) {
                 int v[U];
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    v[u] = x + u * kPickThreads < len ? __ldg(past + x + u * kPickThreads) : -1;
+                    v[u] = x + u * THREADS < len ? __ldg(past + x + u * THREADS) : -1;
 #pragma unroll
                 for (int u = 0; u < U; u++) add(v[u]);
             }
         }
         if (a.seen) {
             const uint64_t *const sees = a.seen + t * a.seen_words;
-            for (int m = tid; m < n && m < a.seen_words * 64; m += kPickThreads)
+            for (int m = tid; m < n && m < a.seen_words * 64; m += THREADS)
                 if (sees[m >> 6] >> (m & 63) & 1) add(a.drafted[t0 + m]);
         }
         __syncthreads();
@@ -632,21 +650,24 @@ __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_con
     const uint32_t *const allowed = a.allowed ? a.allowed + t * a.allowed_row : nullptr;
     float top = -INFINITY;
     int at = -1;
-    for (int base = v0 + tid; base < v1; base += U * kPickThreads) {
-        float f[U];
+    for (int base = v0 + tid; base < v1; base += U * THREADS) {
+        float f[U], w[U];
+        uint32_t may[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int v = base + u * kPickThreads;
+            const int v = base + u * THREADS;
             f[u] = v < v1 ? AttnType<T>::up(x[v]) : -INFINITY;
+            w[u] = bias && v < v1 ? __ldg(bias + v) : 0.f;
+            may[u] = allowed && v < v1 ? __ldg(allowed + (v >> 5)) : ~0u;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int v = base + u * kPickThreads;
+            const int v = base + u * THREADS;
             if (v >= v1) break;
             const uint32_t count = context ? counts[v - v0] : 0;
             if (count) f[u] = pick_less(f[u], (float)count, less);
-            if (bias) f[u] = __fadd_rn(f[u], __ldg(bias + v));
-            if (allowed && !(__ldg(allowed + (v >> 5)) >> (v & 31) & 1)) f[u] = -INFINITY;
+            if (bias) f[u] = __fadd_rn(f[u], w[u]);
+            if (!(may[u] >> (v & 31) & 1)) f[u] = -INFINITY;
             if (f[u] > top) {
                 top = f[u];
                 at = v;
@@ -661,8 +682,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_few_kernel(const __grid_con
     cluster_sync();
     if (rank == 0 && warp == 0) {
         key = 0;
-        for (int k = lane; k < kPickCluster * kPickWarps; k += 32)
-            key = max(key, cluster_u64(best + k % kPickWarps, k / kPickWarps));
+        for (int k = lane; k < kPickCluster * WARPS; k += 32)
+            key = max(key, cluster_u64(best + k % WARPS, k / WARPS));
 #pragma unroll
         for (int d = 16; d; d >>= 1) key = max(key, __shfl_xor_sync(~0u, key, d));
         if (lane == 0) a.picked[t] = key ? (int)~(uint32_t)key : -1;
@@ -745,13 +766,13 @@ static int pick_rows(const PickArgs &a, bool first, cudaStream_t st) {
     return WARP_OK;
 }
 
-template <typename T> static int pick_few(const PickArgs &a, cudaStream_t st) {
+template <typename T, int THREADS> static int pick_few(const PickArgs &a, cudaStream_t st) {
     static std::atomic<uint64_t> done;
-    cudaError_t e = attn_smem(pick_few_kernel<T>, kPickFewPart * 4, done);
+    cudaError_t e = attn_smem(pick_few_kernel<T, THREADS>, kPickFewPart * 4, done);
     if (e != cudaSuccess) return cuda_fail(e, "pick smem attribute");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.tokens * kPickCluster);
-    cfg.blockDim = dim3(kPickThreads);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = a.history || a.seen ? a.part * 4 : 0;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -760,7 +781,7 @@ template <typename T> static int pick_few(const PickArgs &a, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, pick_few_kernel<T>, a);
+    e = cudaLaunchKernelEx(&cfg, pick_few_kernel<T, THREADS>, a);
     if (e != cudaSuccess) return cuda_fail(e, "pick_few_kernel");
     count_launch();
     return WARP_OK;
@@ -768,7 +789,10 @@ template <typename T> static int pick_few(const PickArgs &a, cudaStream_t st) {
 
 template <typename T, typename C>
 static int pick_run(const PickArgs &a, cudaStream_t st) {
-    if (a.part) return pick_few<T>(a, st);
+    // more threads a block as long as the card holds all of them, two blocks an SM (16 rows of
+    // 131072 12.0 us and 14.2 with 256 threads, 166 of 59120 33.0 and 17.7)
+    if (a.part && a.tokens * kPickCluster <= 2 * 148) return pick_few<T, 512>(a, st);
+    if (a.part) return pick_few<T, 256>(a, st);
     const bool alone = !a.history && a.pieces == 1;
     if (!alone) {
         const int rc = pick_history<C>(a, st);
