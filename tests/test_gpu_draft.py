@@ -453,6 +453,16 @@ def test_runs_with_more_nodes_than_keys_and_empty_masks(cuda):
     assert not got[first[2]:first[3]].any() and not got[first[1]:first[1] + 11].any()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("short", [1, 60, 129])
+def test_runs_with_short_requests_between_long_ones(cuda, D, short):
+    """Several tasks a block: a short one's tile of keys, partly filled, is waited for while
+    the long one before it still goes through the ring."""
+    kv = [n for i in range(14) for n in (2600 - 90 * i, short + i // 4)]
+    sizes = [min(5, n) for n in kv]
+    Trees(trees_of(sizes), kv, 16, 4, D, 16, torch.bfloat16, seed=short, runs=True).check()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_runs_keep_what_is_not_seen_apart(cuda, dtype, bad):

@@ -736,6 +736,9 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                             bits &= tree_sight(sight_of(), a.seen_words,
                                                k0 + h * L::cols - see_first);
                     }
+                    // A task's warps may be here long before its turn in the ring, whose
+                    // barriers say nothing of uses that far ahead: its scores do.
+                    if (RUNS) wait(s_full + 8 * t, (turn + j) & 1, fail);
                     const int n = 2 * (kept(kSteps, task.steps) + j) + 1;   // the n-th tile in the ring
                     wait(kv_full + 8 * (n % NS), (n / NS) & 1, fail);
                     // two threads a key
