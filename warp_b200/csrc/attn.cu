@@ -723,7 +723,7 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c, bool 
     // One row tile a kv head and many keys of several requests: the card's blocks take
     // equal runs of the batch's keys, whatever the requests' lengths.  56 heads over 8,
     // lengths from a fifth of the largest up, against the parts below: 32 trees of up to 16
-    // nodes 141 us against 163 behind up to 8192 keys, 88.6 and 87.3 behind 4096, 63 and 52 behind
+    // nodes 138 us against 163 behind up to 8192 keys, 88.6 and 87.3 behind 4096, 63 and 52 behind
     // 2048; 3 of 8 nodes behind 65536 101 and 137; one behind 131072 102 and 101; and with two
     // row tiles (36 nodes, 8192 keys), which have no other at work while they write their results,
     // 204 and 169.
