@@ -10,8 +10,8 @@
 // Measured: 160 rows of 131072 fp32 22.5 us, 3.7 TB/s; about as many (64 streams of 1 to 5) with
 // biases of each stream 37, and with histories of up to 30000 tokens 66; 104 rows of 100003 bf16
 // with histories of 8000 and masks, kept, 39.  What bounds it is the arithmetic of each value
-// (issue slots are used to 73 and 65 % in the last two) more than the stream, and the
-// counting (15 and 6 us) that comes before it.  Tried and slower than two kernels for many
+// (issue slots are used to 69 and 65 % in the last two) more than the stream, and the
+// counting (15 and 7 us) that comes before it.  Tried and slower than two kernels for many
 // rows: a cluster that counts for itself (64 streams: 83 to 97), counts in the shared memory of
 // others (200), tokens sorted into buckets first (89), penalties spread out densely (86).
 //
