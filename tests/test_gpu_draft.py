@@ -292,7 +292,7 @@ class Trees:
         self.max_q, self.max_kv = max(self.q_lens), max(kv_lens)
         if runs:                            # by a bound, and a table for as many keys
             assert B > 1 and 16 < self.max_q * Hq // Hk <= 128 and not prefix
-            self.max_kv = 128 * -(-8192 // (B * Hk))
+            self.max_kv = 128 * max(32, -(-4096 // (B * Hk)))
             more = self.max_kv // page - wide
             self.pages = torch.cat((self.pages, torch.full((B, more), -7, dtype=torch.int32)), 1)
         self.seen = seen_of(trees, self.max_q)

@@ -722,14 +722,15 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c, bool 
     const int64_t rows = p.max_q * group;
     // One row tile a kv head and many keys of several requests: the card's blocks take
     // equal runs of the batch's keys, whatever the requests' lengths.  56 heads over 8,
-    // lengths from a fifth of the largest up, against the parts below: 32 trees of up to 16
-    // nodes 138 us against 163 behind up to 8192 keys, 88.6 and 87.3 behind 4096, 63 and 52 behind
-    // 2048; 3 of 8 nodes behind 65536 101 and 137; one behind 131072 102 and 101; and with two
-    // row tiles (36 nodes, 8192 keys), which have no other at work while they write their results,
-    // 204 and 169.
-    const int64_t all = up(p.max_kv, keys) * d->kv_heads * d->batch;
+    // lengths from a fifth of the largest up, runs against the parts below: 32 trees of up to 8
+    // nodes 131 us and 151 behind up to 8192 keys, 84 and 109 behind 4096; 32 of 16 nodes 90 and 88
+    // behind 4096, 67 and 52 behind 2048; 64 of 8 nodes behind 2048 100 and 96, 96 of them behind
+    // 1500 116 and 99; 8 of them behind 8192 48 and 56, behind 4096 35 and 35; 3 behind 65536 102
+    // and 138; one behind 131072 102 either way; and with two row tiles (36 nodes, 8192 keys), which
+    // have no other at work while they write their results, 204 and 169.
+    const int64_t each = up(p.max_kv, keys), all = each * d->kv_heads * d->batch;
     if (tree && d->prefix_len == 0 && d->batch > 1 && rows > kADRows && rows <= kAttnRunRows &&
-        all >= 8192 && all < (int64_t)1 << 31) {
+        each >= 32 && all >= 4096 && all < (int64_t)1 << 31) {
         p.runs = 148;
         p.o_bytes = up((int64_t)p.runs * 2 * kAttnRunRows * d->head_dim * 4, 256) * 256;
         p.ml_bytes = up((int64_t)p.runs * (2 * kAttnRunRows * 8 + sizeof(AttnSplit)), 256) * 256;
