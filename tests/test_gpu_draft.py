@@ -460,7 +460,21 @@ def test_runs_with_short_requests_between_long_ones(cuda, D, short):
     the long one before it still goes through the ring."""
     kv = [n for i in range(14) for n in (2600 - 90 * i, short + i // 4)]
     sizes = [min(5, n) for n in kv]
-    Trees(trees_of(sizes), kv, 16, 4, D, 16, torch.bfloat16, seed=short, runs=True).check()
+    c = Trees(trees_of(sizes), kv, 16, 4, D, 16, torch.bfloat16, seed=short, runs=True)
+    want = c.check()
+    for _ in range(20):
+        assert torch.equal(c.run(), want)
+
+
+def test_runs_of_many_short_requests(cuda):
+    """Tasks of one tile behind one another, and items that two blocks share: the same bits."""
+    kv = [(18, 20, 1017, 61, 17, 1, 2158, 243, 14, 1, 102, 2686, 68, 371, 210)[i % 15] + i // 15
+          for i in range(90)]
+    sizes = [min(3 + i * 7 % 16, n) for i, n in enumerate(kv)]
+    c = Trees(trees_of(sizes), kv, 56, 8, 64, 256, torch.bfloat16, seed=7, runs=True)
+    want = c.check()
+    for _ in range(20):
+        assert torch.equal(c.run(), want)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])

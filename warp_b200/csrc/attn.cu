@@ -723,9 +723,9 @@ static AttnPlan attn_plan(const warp_attn_desc *d, const warp_kv_pages *c, bool 
     // One row tile a kv head and many keys of several requests: the card's blocks take
     // equal runs of the batch's keys, whatever the requests' lengths.  56 heads over 8,
     // lengths from a fifth of the largest up, runs against the parts below: 32 trees of up to 8
-    // nodes 131 us and 151 behind up to 8192 keys, 84 and 109 behind 4096; 32 of 16 nodes 90 and 88
+    // nodes 133 us and 149 behind up to 8192 keys, 85 and 111 behind 4096; 32 of 16 nodes 90 and 88
     // behind 4096, 67 and 52 behind 2048; 64 of 8 nodes behind 2048 100 and 96, 96 of them behind
-    // 1500 116 and 99; 8 of them behind 8192 48 and 56, behind 4096 35 and 35; 3 behind 65536 102
+    // 1500 116 and 99; 8 of them behind 8192 49 and 56, behind 4096 35 and 35; 3 behind 65536 103
     // and 138; one behind 131072 102 either way; and with two row tiles (36 nodes, 8192 keys), which
     // have no other at work while they write their results, 204 and 169.
     const int64_t each = up(p.max_kv, keys), all = each * d->kv_heads * d->batch;

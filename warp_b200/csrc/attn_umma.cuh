@@ -37,10 +37,9 @@
 // With few rows a request and lengths that differ, a block takes a run of the batch's
 // key tiles instead (kAttnTreeRuns; AttnRuns), which is bound by the keys' stream: the
 // two row tiles take the run's tasks in turn, one's rows are written while the other's keys
-// come, and the keys' ring goes on from task to task.  The two places of scores are used
-// in turn too, so that a step's are there before the last one's weights are multiplied (with
-// all keys from the L2 120 us and 132 with a place a row tile).  32 trees of up to 16 nodes,
-// 56 heads of 128 over 8, behind up to 8192 keys: 138 us, 4.8 TB/s.
+// come, and the keys' ring goes on from task to task.  32 trees of up to 16 nodes, 56 heads
+// of 128 over 8, behind up to 8192 keys: 141 us, 4.7 TB/s; with two places of scores in turn,
+// the next ones there before a step's weights, 138, not worth its barriers.
 #pragma once
 #include "attn.cuh"
 #include "umma.cuh"
@@ -74,8 +73,7 @@ template <int D> struct Lay {
     static constexpr int kv_full = 0, kv_empty = kv_full + stages * 8,
                          q_full = kv_empty + stages * 8, s_full = q_full + 16,
                          p_full = s_full + 16, o_end = p_full + 32, drain = o_end + 16,
-                         s_begin = drain + 8, tmem = s_begin + 16, fail = tmem + 4,
-                         dirty = fail + 4;
+                         tmem = drain + 8, fail = tmem + 4, dirty = fail + 4;
     // a word for each of four tasks, as the row tiles' may be up to three apart; a row
     // tile's notes
     static constexpr int note = dirty + 16;
@@ -452,7 +450,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
     const uint32_t kv_full = bars + L::kv_full, kv_empty = bars + L::kv_empty,
                    q_full = bars + L::q_full, s_full = bars + L::s_full,
                    p_full = bars + L::p_full, o_end = bars + L::o_end, drain = bars + L::drain,
-                   s_begin = bars + L::s_begin, tmem_slot = bars + L::tmem;
+                   tmem_slot = bars + L::tmem;
     const uint32_t fail = bars + L::fail;
     volatile int *const failed = (volatile int *)(basep + L::bars + L::fail);
     volatile int *const dirty = (volatile int *)(basep + L::bars + L::dirty);
@@ -497,7 +495,6 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 umma::mbar_init(p_full + 16 * x, 8);
                 umma::mbar_init(p_full + 16 * x + 8, 8);
                 umma::mbar_init(o_end + 8 * x, 1);
-                umma::mbar_init(s_begin + 8 * x, 1);
             }
             umma::mbar_init(drain, 1);
             *failed = 0;
@@ -581,26 +578,25 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             const uint64_t q_desc = desc128(base, 16, 1024),
                            k_desc = desc128(base + L::ring, 16, 1024),
                            v_desc = desc128(base + L::ring, L::kv_half, 1024);
-            // (place of the scores and weights: a row tile's, or with runs in turn)
-            auto qk = [&](int t, int st, int at) {
+            auto qk = [&](int t, int st) {
                 const uint64_t q = q_desc + t * (L::q_tile >> 4),
                                k = k_desc + st * (L::kv_tile >> 4);
 #pragma unroll
                 for (int x = 0; x < D / 16; x++)
-                    mma_ss(leader, tmem + L::s(at), q + (((x / 4) * L::q_half + (x % 4) * 32) >> 4),
+                    mma_ss(leader, tmem + L::s(t), q + (((x / 4) * L::q_half + (x % 4) * 32) >> 4),
                            k + (((x / 4) * L::kv_half + (x % 4) * 32) >> 4), idesc<T>(KEYS, false),
                            x > 0);
-                commit(leader, s_full + 8 * at);
+                commit(leader, s_full + 8 * t);
             };
             // The weights of each half of the keys lie where its scores did, and come
             // in two parts: part w is keys w * cols/2 on of both halves.
-            auto pv = [&](int t, int st, int at, int w, bool acc) {
+            auto pv = [&](int t, int st, int w, bool acc) {
                 const uint64_t v = v_desc + st * (L::kv_tile >> 4);
                 constexpr int H = L::cols / 16, Q = H / 2;
 #pragma unroll
                 for (int i = 0; i < H; i++) {
                     const int x = i / Q * H + w * Q + i % Q;
-                    mma_ts(leader, tmem + L::o(t), tmem + L::s(at) + x / H * L::cols + x % H * 8,
+                    mma_ts(leader, tmem + L::o(t), tmem + L::s(t) + x / H * L::cols + x % H * 8,
                            v + x * (2048 >> 4), idesc<T>(D, true), acc || i > 0);
                 }
             };
@@ -614,38 +610,14 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                 const int s0 = n0 % NS;
                 wait(kv_full + 8 * s0, (n0 / NS) & 1, fail);
                 umma::fence_after();
-                if (cnt0 > 0) qk(0, s0, RUNS ? task.steps & 1 : 0);
-                if (cnt1 > 0) qk(1, s0, RUNS ? task.steps & 1 : 1);
-                if (RUNS) commit(leader, s_begin + 8 * task.tile);
+                if (cnt0 > 0) qk(0, s0);
+                if (cnt1 > 0) qk(1, s0);
                 if (n0 + NS < all) commit(leader, kv_empty + 8 * s0);
                 // ring tiles of V j and K j + 1, their parities
                 int sv = (n0 + 1) % NS, sk = (n0 + 2) % NS;
                 int fv = (n0 + 1) / NS & 1, fk = (n0 + 2) / NS & 1;
                 for (int j = 0; j < cnt; j++) {
                     if (__any_sync(~0u, *failed)) break;
-                    if (RUNS) {
-                        // the next scores, in the other place, before these weights are waited for
-                        const int t = task.tile, n = task.steps + j, at = n & 1, turn = n >> 1 & 1;
-                        if (j + 1 < cnt) {
-                            wait(kv_full + 8 * sk, fk, fail);
-                            umma::fence_after();
-                            qk(t, sk, at ^ 1);
-                            if (n0 + 2 * j + 2 + NS < all) commit(leader, kv_empty + 8 * sk);
-                        }
-                        wait(kv_full + 8 * sv, fv, fail);
-                        wait(p_full + 16 * at, turn, fail);
-                        umma::fence_after();
-                        pv(t, sv, at, 0, j > 0);
-                        wait(p_full + 16 * at + 8, turn, fail);
-                        umma::fence_after();
-                        pv(t, sv, at, 1, true);
-                        commit(leader, o_end + 8 * t);
-                        if (n0 + 2 * j + 1 + NS < all) commit(leader, kv_empty + 8 * sv);
-                        sv += 2, sk += 2;
-                        if (sv >= NS) sv -= NS, fv ^= 1;
-                        if (sk >= NS) sk -= NS, fk ^= 1;
-                        continue;
-                    }
                     wait(kv_full + 8 * sv, fv, fail);
                     if (j + 1 < cnt) wait(kv_full + 8 * sk, fk, fail);
 #pragma unroll
@@ -655,12 +627,12 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                         const int turn = (past[t] + j) & 1;
                         wait(p_full + 16 * t, turn, fail);
                         umma::fence_after();
-                        pv(t, sv, t, 0, j > 0);
+                        pv(t, sv, 0, j > 0);
                         wait(p_full + 16 * t + 8, turn, fail);
                         umma::fence_after();
-                        pv(t, sv, t, 1, true);
+                        pv(t, sv, 1, true);
                         // in order behind it: the next scores take the weights' place
-                        if (j + 1 < mine) qk(t, sk, t);
+                        if (j + 1 < mine) qk(t, sk);
                         else commit(leader, o_end + 8 * t);
                     }
                     // only what the loader will wait for
@@ -680,7 +652,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
         }
     } else {
         // ---- the rows ----------------------------------------------------------------
-        int turn = 0;                       // parity of this row tile's steps so far
+        int turn = 0;                       // parities: 1 of this row tile's steps, 2 of its tasks
         // What a task has to say after its steps is kept in shared memory in between, where the
         // registers are needed.
         volatile int *const note = (volatile int *)(basep + L::bars + L::note) + t * L::notes;
@@ -716,7 +688,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             }
             const uint32_t lanes = (uint32_t)quad * 32 << 16;
             // this thread's half of the scores and of the weights
-            const uint32_t ot = tmem + L::o(t) + lanes;
+            const uint32_t ot = tmem + L::o(t) + lanes, st = tmem + L::s(t) + h * L::cols + lanes;
             float *const swap = (float *)(basep + L::swap) + t * 2 * kRows;
             const bool warp_live = task.row_of(t) + quad * 32 < task.rows;
             const float c = a.scale_log2;
@@ -749,15 +721,6 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
             for (int j = 0; j < mine; j++) {
                 const bool masked =
                     RUNS ? j >= note[kMask] : j >= masked_from || j == masked_pre;
-                // the place of the scores, and the weights' barriers
-                const int unit = RUNS ? note[kSteps] + j : 0, at = RUNS ? unit & 1 : t;
-                const uint32_t st = tmem + L::s(at) + h * L::cols + lanes, ready = p_full + 16 * at;
-                // A task's first scores have a barrier of their own: its warps may be here
-                // long before its turn, and s_full says nothing of uses that far ahead.
-                auto ask_s = [&] {
-                    if (RUNS && j == 0) wait(s_begin + 8 * t, note[kDone] >> 1 & 1, fail);
-                    else wait(s_full + 8 * at, RUNS ? unit >> 1 & 1 : j & 1, fail);
-                };
                 int lim = 0;                    // keys of the step that this row sees
                 uint64_t bits = 0;              // and of this thread's half, one a bit
                 if (__builtin_expect(masked, 0)) {
@@ -774,8 +737,9 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                             bits &= tree_sight(sight_of(), a.seen_words,
                                                k0 + h * L::cols - see_first);
                     }
-                    // Nor do the ring's barriers, so the scores are waited for first.
-                    if (RUNS) ask_s();
+                    // A task's warps may be here long before its turn in the ring, whose
+                    // barriers say nothing of uses that far ahead: its scores do.
+                    if (RUNS) wait(s_full + 8 * t, (turn + j) & 1, fail);
                     const int n = 2 * (kept(kSteps, task.steps) + j) + 1;   // the n-th tile in the ring
                     wait(kv_full + 8 * (n % NS), (n / NS) & 1, fail);
                     // two threads a key
@@ -808,7 +772,7 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                     }
                     umma::fence_smem_async();
                 }
-                ask_s();
+                wait(s_full + 8 * t, (turn + j) & 1, fail);
                 umma::fence_after();
                 if (warp_live) {
                     float s[L::cols];
@@ -838,10 +802,6 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                         const float to = grow ? top : m;
                         const float w = !grow || to == -INFINITY ? 1.f : ex2(m * c - to * c);
                         if (j > 0) {
-                            if (RUNS) {         // the products before are in O
-                                wait(o_end + 8 * t, (turn + j - 1) & 1, fail);
-                                umma::fence_after();
-                            }
 #pragma unroll 1
                             for (int x = h * (D / 2); x < (h + 1) * (D / 2); x += 16) {
                                 float o[16];
@@ -860,16 +820,16 @@ __device__ __forceinline__ void attn_wide_rows(const AttnArgs &a, const CUtensor
                     const float mc = m == -INFINITY ? 0.f : m < INFINITY ? lowered(m) : NAN;
                     const uint64_t c2 = pair2(c, c), mc2 = pair2(-mc, -mc);
                     uint64_t l2 = pair2(l.x, l.y);
-                    if (__builtin_expect(masked, 0)) weights<T, 0>(s, c2, mc2, l2, st, ready);
-                    else weights<T, poly_pairs(D)>(s, c2, mc2, l2, st, ready);
+                    if (__builtin_expect(masked, 0)) weights<T, 0>(s, c2, mc2, l2, st, p_full + 16 * t);
+                    else weights<T, poly_pairs(D)>(s, c2, mc2, l2, st, p_full + 16 * t);
                     l = both(l2);
                 } else {
-                    hand_over(ready);
-                    hand_over(ready + 8);
+                    hand_over(p_full + 16 * t);
+                    hand_over(p_full + 16 * t + 8);
                 }
             }
-            if (mine > 0) wait(o_end + 8 * t, RUNS ? (turn + mine - 1) & 1 : 0, fail);
-            if (RUNS) turn ^= mine & 1;
+            if (mine > 0) wait(o_end + 8 * t, turn >> 1, fail);
+            if (RUNS && mine > 0) turn ^= 2 | (mine & 1);
             umma::fence_after();
             if (live) {
                 const int t0 = kept(kT0, task.rq.t0), row0 = kept(kRow0, task.row_of(t)),
