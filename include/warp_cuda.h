@@ -439,8 +439,9 @@ WARP_API int warp_tree_attention(const warp_attn_desc *d, const warp_kv_pages *c
  * outside the vocabulary count for nothing).  Masks: bit v % 32 of word v / 32 of
  * the row's words.  picked[t]: the lowest v of the largest x; -1 where nothing is
  * above -inf (a NaN never is).  out (NULL for none; may be logits) takes x,
- * rounded to `type`.  max_q bounds the rows of a request; rows past it are left
- * out and reported by warp_attn_status, rows of no request are not written.
+ * rounded to `type`.  max_q bounds the rows of a request (0 is no work); rows past it
+ * are reported by warp_attn_status, and their picked is -1 and their out stays as it
+ * is; rows of no request are not written.
  * scratch: warp_pick_scratch(d) bytes of device memory, 256-byte aligned, free
  * again when the stream has passed the call. */
 typedef struct {

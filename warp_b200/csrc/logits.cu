@@ -201,11 +201,13 @@ __device__ __forceinline__ float pick_float(uint16_t c) {
 __device__ __forceinline__ float pick_float(uint32_t c) { return (float)c; }
 
 // Row t's request b (the last one that starts at or before it), whose node i of n the
-// row is; false for a row of none, and for one past the bound, which is reported.
-__device__ __forceinline__ bool pick_request(const PickArgs &a, int t, int &b, int &i, int &n,
-                                             bool report) {
+// row is.  A row of none is kPickNone and stays as it is; one past the bound is
+// kPickPast, which is reported and has no choice.
+enum { kPickTaken, kPickNone, kPickPast };
+__device__ __forceinline__ int pick_request(const PickArgs &a, int t, int &b, int &i, int &n,
+                                            bool report) {
     b = t, i = 0, n = 1;
-    if (!a.q_start) return true;
+    if (!a.q_start) return kPickTaken;
     const int lane = threadIdx.x % 32;
     b = -1;
     for (int i0 = 0; i0 < a.batch; i0 += 32) {
@@ -213,15 +215,15 @@ __device__ __forceinline__ bool pick_request(const PickArgs &a, int t, int &b, i
         if (hit) b = i0 + 31 - __clz(hit);
         if (hit != ~0u) break;
     }
-    if (b < 0) return false;
+    if (b < 0) return kPickNone;
     const int s = a.q_start[b], e = a.q_start[b + 1];
-    if (t >= e) return false;
+    if (t >= e) return kPickNone;
     i = t - s;
     n = min(e - s, a.max_q);
     if (report && threadIdx.x == 0 && (s < 0 || e > a.tokens || i >= n)) atomicOr(a.err, kAttnBadLen);
-    if (s < 0 || i >= n) return false;
+    if (s < 0 || i >= n) return kPickPast;
     n = min(n, a.tokens - s);
-    return true;
+    return kPickTaken;
 }
 
 // What a kernel does besides the penalties: asked for each value, this would cost
@@ -314,7 +316,8 @@ pick_rows_kernel(const __grid_constant__ PickArgs a) {
 #pragma unroll 1
         for (int k = 0; k < R - 1; k++) ask_row(ring0 + k * Slot::round, v_tid + k * STEP);
         int b, i, n;
-        if (!pick_request(a, t, b, i, n, true)) {
+        if (const int not_taken = pick_request(a, t, b, i, n, true)) {
+            if (not_taken == kPickPast && tid == 0) a.picked[t] = -1;
             cp_async_commit();
             cp_async_wait<0>();
             continue;
@@ -610,7 +613,10 @@ __global__ void __launch_bounds__(THREADS) pick_few_kernel(const __grid_constant
     const int rank = (int)cluster_rank(), t = blockIdx.x / kPickCluster;
     const int v0 = min(rank * a.part, a.vocab), v1 = min(v0 + a.part, a.vocab);
     int b = t, i = 0, n = 1;
-    if (!pick_request(a, t, b, i, n, rank == 0)) return;        // all blocks of the cluster
+    if (const int not_taken = pick_request(a, t, b, i, n, rank == 0)) {     // in all of the cluster
+        if (not_taken == kPickPast && rank == 0 && tid == 0) a.picked[t] = -1;
+        return;
+    }
     const int t0 = t - i;
     const bool context = a.history || a.seen;
     PickLess less = {1.f, 0.f, 0.f, 0.f, 0.f};

@@ -552,16 +552,17 @@ def _table(x, name, rows, wide, dtype, dev):
     return strides[0] if len(shape) == 2 and rows > 1 else 0
 
 
-def pick_tokens(logits, q_start=None, max_q=1, history=None, history_len=None, repetition=None,
+def pick_tokens(logits, q_start=None, max_q=None, history=None, history_len=None, repetition=None,
                 frequency=None, presence=None, bias=None, allowed=None, drafted=None, seen=None,
                 out=None):
     """The token of the largest adjusted logit of each row, int32 [T]; -1 where
     none is above -inf (warp_pick_tokens).
 
     logits [T][V] fp32, fp16 or bf16, rows contiguous; row t belongs to request t,
-    or to the one with q_start[b] <= t < q_start[b+1] (int32 [B+1]; max_q rows a
-    request at most).  With c the number of times that a token is in the row's
-    context,
+    or to the one with q_start[b] <= t < q_start[b+1] (int32 [B+1]).  max_q bounds
+    the rows of a request; by default all of them are taken, with seen as many as its
+    words have bits.  A row past the bound gets -1, and attn_status raises.  With c the
+    number of times that a token is in the row's context,
 
         x > 0 ? x / repetition : x * repetition, then less frequency * c and
         presence, where c > 0 (float32 [B] each); plus bias (float32 [V] or
@@ -583,6 +584,8 @@ def pick_tokens(logits, q_start=None, max_q=1, history=None, history_len=None, r
     T, V = logits.shape
     row = logits.stride(0) if T > 1 else 0
     B = T
+    if max_q is None:
+        max_q = max(1, T if seen is None or seen.dim() != 2 else min(T, 64 * seen.shape[1]))
     qp = op = orow = hp = lp = hrow = wide = bp = brow = ap = arow = dp = sp = words = 0
     if q_start is not None:
         B = q_start.numel() - 1
@@ -624,6 +627,8 @@ def pick_tokens(logits, q_start=None, max_q=1, history=None, history_len=None, r
     if allowed is not None:
         arow = _table(allowed, "allowed", T, (V + 31) // 32, torch.int32, dev)
         ap = allowed.data_ptr()
+    if qp and not max_q:                    # which the kernels take for no work
+        return torch.full((T,), -1, dtype=torch.int32, device=logits.device)
     picked = torch.empty(T, dtype=torch.int32, device=logits.device)
     d = ffi.PICK_DESC.pack(T, B, V, _TYPES[dt], max_q, logits.data_ptr(), row, op, orow,
                            picked.data_ptr(), qp, hp, lp, hrow, wide, *scalars, bp, brow, ap, arow,
