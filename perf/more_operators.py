@@ -276,7 +276,7 @@ def prepare(case, seed):
     # [layer][keys, values][pages]...
     x = _pool_of_pages(g, 2 * case["layers"] * count, case)
     s["pools"] = x.unflatten(0, (case["layers"], 2, count))
-    s["caches"] = s["pools"][:, 0], s["pools"][:, 1]
+    s["caches"] = [(c[0], c[1]) for c in s["pools"].unbind()]
     drafted = torch.randint(0, TOKENS, (tokens,), generator=g, device="cuda", dtype=torch.int32)
     picked = torch.randint(0, TOKENS, (tokens,), generator=g, device="cuda", dtype=torch.int32)
     start, ups, downs = 0, [], []
@@ -343,8 +343,8 @@ def run(s):
                                       max_kv=s["kv_max"], prefix_pages=s["prefix_pages"],
                                       prefix_len=s["prefix"])
         if kind == "pick":
-            picked = ops.pick_tokens(s["logits"], s["q_start"], max_q=s["max_q"],
-                                     history=s["history"], history_len=s["history_len"], repetition=s["repetition"],
+            picked = ops.pick_tokens(s["logits"], s["q_start"], history=s["history"],
+                                     history_len=s["history_len"], repetition=s["repetition"],
                                      frequency=s["frequency"], presence=s["presence"],
                                      bias=s["bias"], allowed=s["allowed"], drafted=s["drafted"],
                                      seen=s["seen"], out=s["out"])
