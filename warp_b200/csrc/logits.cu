@@ -65,7 +65,9 @@ pick_history_kernel(const __grid_constant__ PickArgs a) {
     constexpr int PER = 4 / sizeof(C), U = 4;
     pdl_trigger();
     const int tid = threadIdx.x;
-    for (int t = blockIdx.x * kPickCounters + tid; t < a.tokens; t += gridDim.x * kPickCounters) {
+    // (2^21 requests and more have blocks whose product is past 31 bits)
+    for (int64_t t = (int64_t)blockIdx.x * kPickCounters + tid; t < a.tokens;
+         t += (int64_t)gridDim.x * kPickCounters) {
         a.best[t] = 0;
         a.done[t] = 0;
     }
