@@ -713,10 +713,11 @@ static int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 static PickPlan pick_plan(const warp_pick_desc *d) {
     PickPlan p = {};
+    const bool past = d->history || d->history_len;
     p.words = (d->vocab + 31) / 32;
     p.part = (p.words + kPickCluster - 1) / kPickCluster * 32;
     if ((int64_t)d->tokens * d->vocab <= kPickFewValues && p.part <= kPickFewPart &&
-        (!d->history || d->history_wide <= kPickFewHistory))
+        (!past || d->history_wide <= kPickFewHistory))
         return p;
     p.part = 0;
     // 16 bits where no history is long enough to outgrow them
@@ -731,7 +732,7 @@ static PickPlan pick_plan(const warp_pick_desc *d) {
     p.done_at = at;
     at += align256((int64_t)d->tokens * 4);
     p.bits_at = at;
-    if (d->history) {
+    if (past) {
         at += align256((int64_t)d->batch * p.words * 4);
         p.counts_at = at;
         // a vector's window may reach past the last word's
@@ -850,7 +851,9 @@ extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *scratch, void *st
     if (rc) return rc;
     if (d->tokens == 0 || d->batch == 0 || (d->q_start && d->max_q == 0)) return WARP_OK;
     WARP_ARG(d->logits && d->picked, "%s: NULL pointer", who);
-    WARP_ARG(!d->history == !d->history_len, "%s: history and history_len go together", who);
+    // no address is needed for a history without places
+    WARP_ARG(!d->history == !d->history_len || (d->history_len && d->history_wide == 0),
+             "%s: history and history_len go together", who);
     WARP_ARG(!d->drafted == !d->seen && (!d->seen || d->q_start),
              "%s: drafted, seen and q_start go together", who);
     WARP_ARG(((uintptr_t)d->seen & 7) == 0, "%s: the masks are not 8-byte aligned", who);
@@ -865,7 +868,9 @@ extern "C" int warp_pick_tokens(const warp_pick_desc *d, void *scratch, void *st
     WARP_ARG((int64_t)d->batch * p.slices < (int64_t)1 << 31, "%s: %d requests", who, d->batch);
     PickArgs a = {};
     a.logits = d->logits, a.out = d->out, a.picked = d->picked, a.q_start = d->q_start;
-    a.history = d->history, a.history_len = d->history_len, a.drafted = d->drafted;
+    // without places the lengths alone are looked at, and any address says that there are some
+    a.history = d->history ? d->history : d->history_len;
+    a.history_len = d->history_len, a.drafted = d->drafted;
     a.repetition = d->repetition, a.frequency = d->frequency, a.presence = d->presence;
     a.bias = d->bias, a.allowed = d->allowed, a.seen = d->seen;
     a.row = d->row, a.out_row = d->out_row, a.history_row = d->history_row;
