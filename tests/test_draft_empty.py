@@ -1,9 +1,9 @@
-"""A history without places needs no address: what comes behind that check is reached."""
+"""What needs no address where it has no place: a history without places, what no request holds."""
 import ctypes
 
 import pytest
 
-from test_draft import lib, pick_desc  # noqa: F401
+from test_draft import lib, pick_desc, plan_desc  # noqa: F401
 
 
 @pytest.mark.parametrize("history", [None, 256])
@@ -27,3 +27,14 @@ def test_scratch_by_either_of_the_two(lib):  # noqa: F811
             for kw in ({}, dict(history=None), dict(history_len=None),
                        dict(history=None, history_len=None))]
     assert need[0] == need[1] == need[2] > need[3] > 0
+
+
+@pytest.mark.parametrize("kw", [dict(held=None), dict(held=None, kv_len=None, pages=None), {}])
+def test_a_plan_of_no_request(lib, kw):  # noqa: F811
+    """Nothing to do, with a pool too: what [0] requests hold has no address."""
+    assert lib.warp_step_plan(ctypes.byref(plan_desc(batch=0, tokens=0, **kw)), None) == 0
+
+
+def test_tokens_of_no_request_are_refused(lib):  # noqa: F811
+    assert lib.warp_step_plan(ctypes.byref(plan_desc(batch=0, held=None)), None) == -1
+    assert b"no request" in lib.warp_last_error()

@@ -416,7 +416,8 @@ extern "C" int warp_step_plan(const warp_plan_desc *d, void *stream) {
              "%s: negative size", who);
     WARP_ARG(d->page_size >= 16 && d->page_size <= 4096 && !(d->page_size & (d->page_size - 1)),
              "%s: page_size %d is not a power of two in 16..4096", who, d->page_size);
-    WARP_ARG(!d->held == !d->pool, "%s: held and pool go together", who);
+    // held may have no address where there is no request
+    WARP_ARG(!d->held == !d->pool || d->batch == 0, "%s: held and pool go together", who);
     WARP_ARG(!d->pool || (d->pool_pages >= 0 && d->pool_pages < ((int64_t)1 << 31) - 1),
              "%s: %lld pages in the pool", who, (long long)d->pool_pages);
     WARP_ARG((int64_t)d->batch * d->pages_per_row < (int64_t)1 << 31,
