@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(256) attn_join_runs_kernel(const __grid_consta
         }
     }
     for (int i = blockIdx.x; i < a.batch; i += kJoinBlocks) {
-        const AttnReq rq = attn_req(a, i, false);
+        const AttnReq rq = attn_req(a, i);  // which reports those that no block of runs takes
         if (attn_item(rq.n, rq.len)) continue;
         uint4 *const to = (uint4 *)((T *)a.out + (int64_t)rq.t0 * a.q_heads * D);
         const int64_t n = (int64_t)rq.n * a.q_heads * (D / 8);
