@@ -155,8 +155,11 @@ class Decoder:
     [vocabulary][hidden]; k_pages / v_pages
     [layers][pages][page_size][kv_heads][head_dim].  kv_len (int32 [requests], on the
     device) is how many keys each request has: set it to 0 for one that ends, and its
-    pages go back with the next step.  Nothing here waits for the device.  A number
-    outside the vocabulary is read as the nearest in it (and is never accepted)."""
+    pages go back with the next step.  A request that a step leaves without pages for all
+    its keys (the pool ran empty, or its row of pages is full; ops.attn_status raises) stays
+    as it was, with -1 or a count of 0 for its result: bring the same tokens again when
+    there are pages.  Nothing here waits for the device.  A number outside the vocabulary is
+    read as the nearest in it (and is never accepted)."""
 
     def __init__(self, blocks, embed, norm, head, k_pages, v_pages, requests,
                  pages_per_request, eps=1e-6):
@@ -185,6 +188,10 @@ class Decoder:
             h = block.forward(h, k, v, step)
         return h, step
 
+    def _placed(self, step):
+        """Which requests have pages for all keys of the step, bool [requests]."""
+        return self.held * self.page_size >= step.kv_len
+
     def _logits(self, h):
         return self.head(ops.rmsnorm(h, self.norm, self.eps))
 
@@ -192,23 +199,27 @@ class Decoder:
         """The requests' next tokens (int32, certain ones: a prompt, a chunk of one or a
         single token), max_q a request at most, through the blocks; returns the
         token picked behind each request's last, int32 [requests] (of no meaning where a
-        request brings none).  choice: what ops.pick_tokens weighs, a row a request."""
+        request brings none, -1 where its keys have no place).  choice: what ops.pick_tokens
+        weighs, a row a request."""
         h, step = self._forward(tokens, q_start, max_q)
         last = (q_start[1:] - 1).clamp(0, len(h) - 1)
         picked = ops.pick_tokens(self._logits(h[last]), **choice)
-        self.kv_len.copy_(step.kv_len)
-        return picked
+        placed = self._placed(step)
+        torch.where(placed, step.kv_len, self.kv_len, out=self.kv_len)
+        return torch.where(placed, picked, -1)
 
     def verify(self, drafted, parents, q_start, max_q, **choice):
         """A step of drafted trees: request b's nodes are tokens q_start[b] ..
         q_start[b+1]-1, node 0 the last certain token, which is not in the cache yet.
         Returns (count, chosen) of ops.tree_accept: chosen[b][:count[b]] are the
-        request's new tokens, the last of which is the next tree's node 0."""
+        request's new tokens, the last of which is the next tree's node 0; count is 0 for a
+        request whose keys have no place."""
         h, step = self._forward(drafted, q_start, max_q, parents)
         picked = ops.pick_tokens(self._logits(h), q_start, max_q, drafted=drafted, seen=step.seen,
                                  **choice)
         count, _, chosen, kv_len = ops.tree_accept(
             drafted, picked, step.seen, q_start, step.kv_len, max_q,
             caches=(self.k_pages, self.v_pages), pages=self.pages)
-        self.kv_len.copy_(kv_len)
-        return count, chosen
+        placed = self._placed(step)
+        torch.where(placed, kv_len, self.kv_len, out=self.kv_len)
+        return torch.where(placed, count, 0), torch.where(placed[:, None], chosen, -1)
