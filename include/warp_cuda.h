@@ -434,10 +434,13 @@ WARP_API int warp_tree_attention(const warp_attn_desc *d, const warp_kv_pages *c
  *                 x = x - frequency[b] * c;  x = x - presence[b]
  *   x = x + bias[v];  where the row's mask does not allow v: x = -inf
  * each an fp32 operation rounded by itself; NULL leaves one out (1, 0, 0, 0, all
- * allowed).  The context: the first history_len[b] tokens of history[b] (NULL will do
+ * allowed).  The bias comes behind the penalties, which do not see it, and all three
+ * penalties have one context; where settings mean it otherwise (a bias in front of them, or
+ * frequency and presence over the answer alone) they are to be translated by the caller.
+ * The context: the first history_len[b] tokens of history[b] (NULL will do
  * where history_wide is 0), and with seen the drafted tokens of the nodes that the row
- * sees (as above; numbers outside the vocabulary count for nothing).  Masks: bit v % 32 of word v / 32 of
- * the row's words.  picked[t]: the lowest v of the largest x; -1 where nothing is
+ * sees (as above; numbers outside the vocabulary count for nothing).  Masks: bit v % 32
+ * of word v / 32 of the row's words.  picked[t]: the lowest v of the largest x; -1 where nothing is
  * above -inf (a NaN never is).  out (NULL for none; may be logits) takes x,
  * rounded to `type`.  max_q bounds the rows of a request (0 is no work); rows past it
  * are reported by warp_attn_status, and their picked is -1 and their out stays as it

@@ -38,8 +38,10 @@
 // key tiles instead (kAttnTreeRuns; AttnRuns), which is bound by the keys' stream: the
 // two row tiles take the run's tasks in turn, one's rows are written while the other's keys
 // come, and the keys' ring goes on from task to task.  32 trees of up to 16 nodes, 56 heads
-// of 128 over 8, behind up to 8192 keys: 141 us, 4.7 TB/s; with two places of scores in turn,
-// the next ones there before a step's weights, 138, not worth its barriers.
+// of 128 over 8, behind up to 8192 keys: 141 us, 4.7 TB/s.  Two places of scores in turn, the
+// next ones there before a step's weights, took 138 and were wrong: the barrier at a task's end
+// could be one use behind, so that results were read before the last products, and a wait put
+// before it was one use ahead and gave up.
 #pragma once
 #include "attn.cuh"
 #include "umma.cuh"

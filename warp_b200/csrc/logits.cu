@@ -8,7 +8,7 @@
 // leaves the same.  A few rows are one kernel's, a cluster of blocks to a row.
 //
 // Measured: 160 rows of 131072 fp32 22.5 us, 3.7 TB/s; about as many (64 streams of 1 to 5) with
-// biases of each stream 37, and with histories of up to 30000 tokens 66; 104 rows of 100003 bf16
+// biases of each stream 37, and with histories of up to 30000 tokens 66; 138 rows of 100003 bf16
 // with histories of 8000 and masks, kept, 39.  What bounds it is the arithmetic of each value
 // (issue slots are used to 69 and 65 % in the last two) more than the stream, and the
 // counting (15 and 7 us) that comes before it.  Tried and slower than two kernels for many
@@ -603,9 +603,9 @@ constexpr int kPickFewHistory = 16384;      // and places of a history, which ea
 
 // A cluster has a row, each block a part of the vocabulary, whose tokens it counts for
 // itself: one launch and no scratch, and better as long as rows are few (on the device,
-// against the two kernels: a row of 32000 behind 700 tokens 5.9 us and 9.7, 32 of 131072
-// with biases behind 8000 tokens each 19.3 and 23.3, 145 of 74835 28.3 and 27.3: each row counts
-// its history anew).
+// against the two kernels: a row of 32000 behind 700 tokens 5.3 us and 8.2, 32 of 131072
+// with biases behind 8000 tokens each 18.6 and 21.7, 100 of 60000 behind 700 21.7 and 22.3; 80 of
+// 75000 with biases behind 8000 34.0 and 30.4, as each row counts its history anew).
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) pick_few_kernel(const __grid_constant__ PickArgs a) {
     extern __shared__ __align__(16) uint32_t counts[];  // [part]
@@ -799,7 +799,7 @@ template <typename T, int THREADS> static int pick_few(const PickArgs &a, cudaSt
 template <typename T, typename C>
 static int pick_run(const PickArgs &a, cudaStream_t st) {
     // more threads a block as long as the card holds all of them, two blocks an SM (16 rows of
-    // 131072 12.0 us and 14.2 with 256 threads, 166 of 59120 33.0 and 17.7)
+    // 131072 9.0 us and 10.3 with 256 threads, 100 of 60000 20.1 and 13.8)
     if (a.part && a.tokens * kPickCluster <= 2 * 148) return pick_few<T, 512>(a, st);
     if (a.part) return pick_few<T, 256>(a, st);
     const bool alone = !a.history && a.pieces == 1;

@@ -467,9 +467,7 @@ def _attention(q, k_pages, v_pages, pages, kv_len, q_start, max_q, max_kv, scale
 def page_pool(pages, device="cuda"):
     """A pool with all of `pages` pages free, for step_plan: int32 [1 + pages], how
     many are free and their numbers, of which page 0 comes off first."""
-    pool = torch.arange(pages, -1, -1, dtype=torch.int32, device=device)
-    pool[1:] = pool[1:].clone()
-    return pool
+    return torch.arange(pages, -1, -1, dtype=torch.int32, device=device)
 
 
 def step_plan(q_start, kv_len, pages, page_size, tokens, base=0, held=None, pool=None,
@@ -569,6 +567,8 @@ def pick_tokens(logits, q_start=None, max_q=None, history=None, history_len=None
         [B][V]); -inf where allowed (int32 [T][ceil(V / 32)] or [ceil(V / 32)],
         a bit a token, the lowest first) has no bit.
 
+    The bias is added behind the penalties, which do not see it (a sampler that
+    penalises biased logits has it in front), and one context serves all three.
     The context: the first history_len[b] (int32 [B]) tokens of history[b] (int32
     [B][H]), and with drafted (int32 [T]) and seen (step_plan's) the drafted
     tokens of the nodes that the row's node sees.  out, of logits' shape and
