@@ -385,8 +385,8 @@ WARP_API int warp_paged_attention(const warp_attn_desc *d, const warp_kv_pages *
  * Surplus pages go back to the pool and their entries become -1; then missing
  * ones are taken from it, in order of the requests.  What is given back last comes off
  * first, so that requests that shrink and grow again get their pages back.
- * A pool that runs empty leaves entries as they are and held[b] short, and
- * warp_attn_status says so.
+ * A pool that runs empty leaves held[b] short and -1 in the entries that lack a page,
+ * and warp_attn_status says so.
  *   pool   int32 [1 + pool_pages]: how many pages are free, then their numbers
  *          (the last of them comes off first)
  * Then, for each of `tokens` tokens, positions and slots as warp_kv_slots makes

@@ -135,12 +135,12 @@ __device__ __forceinline__ void plan_pages(const PlanArgs &a) {
             __syncthreads();
             for (int k = tid; k < (int)lack; k += kPlanThreads) {
                 const int64_t place = (int64_t)top - 1 - (uint32_t)before - k;
-                if (place < 0) {
-                    atomicOr(a.err, kAttnNoPage);
-                    break;
-                }
+                // what was in the entry may be a page that another request has
+                int32_t page = -1;
+                if (place < 0) atomicOr(a.err, kAttnNoPage);
+                else page = a.pool[1 + place];
                 const int r = item_of(first, k);
-                a.pages[(b0 + r) * a.pages_row + entry[r] + (k - first[r])] = a.pool[1 + place];
+                a.pages[(b0 + r) * a.pages_row + entry[r] + (k - first[r])] = page;
             }
         }
         if (b0 + tid < a.batch) {
